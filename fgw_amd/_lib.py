@@ -100,6 +100,13 @@ SIGNATURES = {
                              ctypes.POINTER(Schedule), c_void_p),
 }
 
+# The entry points of include/fgw_kv.h, in the order in which fgw_amd._kv.bind takes them
+# (fgw_kv_abi_version is not among those).
+KV_ABI_VERSION = 1
+KV_ENTRIES = ("fgw_kv_last_error", "fgw_rotary_apply", "fgw_kv_append", "fgw_kv_extend_workspace",
+              "fgw_kv_extend", "fgw_pages_workspace", "fgw_pages_reserve", "fgw_pages_fork",
+              "fgw_pages_free", "fgw_pages_compact", "fgw_pages_copy")
+
 _lock = threading.Lock()
 _lib = None
 
@@ -125,6 +132,11 @@ def load() -> ctypes.CDLL:
         version = lib.fgw_mha_abi_version()
         if version != ABI_VERSION:
             raise RuntimeError(f"{LIBRARY} has ABI {version}, expected {ABI_VERSION}; rebuild it")
+        lib.fgw_kv_abi_version.restype = ctypes.c_int
+        kv_version = lib.fgw_kv_abi_version()
+        if kv_version != KV_ABI_VERSION:
+            raise RuntimeError(f"{LIBRARY} has cache ABI {kv_version}, expected {KV_ABI_VERSION}; "
+                               "rebuild it")
         _lib = lib
         return lib
 
@@ -142,6 +154,18 @@ def load_launch_module():
         raise RuntimeError("fgw_amd._launch is missing: build it with `python -m fgw_amd.build` "
                            "(the operator has no other launch path)") from exc
     return _launch
+
+
+def load_kv_module():
+    """The C++ calls of the operators around the cache (fgw_amd._kv), bound to the loaded
+    library; raises if the module was not built."""
+    try:
+        from fgw_amd import _kv
+    except ImportError as exc:
+        raise RuntimeError("fgw_amd._kv is missing: build it with `python -m fgw_amd.build` "
+                           "(the operators have no other launch path)") from exc
+    _kv.bind(*(entry_address(name) for name in KV_ENTRIES))
+    return _kv
 
 
 def check(status: int) -> None:
