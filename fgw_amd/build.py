@@ -58,12 +58,11 @@ def shim_path(module: str = "_launch") -> pathlib.Path:
     return PACKAGE / (module + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
-def _build_shim(module: str) -> pathlib.Path:
+def _build_shim(module: str, out: pathlib.Path, python_include: str) -> pathlib.Path:
     """Host-only C++ extension over the C ABI (torch headers for tensors,
     allocation and the current HIP stream). Built with g++: no device code."""
     import torch
     tdir = pathlib.Path(torch.__file__).resolve().parent
-    out = shim_path(module)
     tmp = out.with_name(out.name + ".tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-unused-function",
            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
@@ -71,7 +70,7 @@ def _build_shim(module: str) -> pathlib.Path:
            # passes the same define).
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            f"-I{tdir / 'include'}", f"-I{tdir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
-           "-I/opt/rocm/include", f"-I{sysconfig.get_paths()['include']}",
+           "-I/opt/rocm/include", f"-I{python_include}",
            str(SHIM_SOURCES[module]), "-o", str(tmp), f"-L{tdir / 'lib'}", f"-Wl,-rpath,{tdir / 'lib'}",
            "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
            "-L/opt/rocm/lib", "-Wl,-rpath,/opt/rocm/lib", "-lamdhip64"]
@@ -92,8 +91,11 @@ def build(jobs: int | None = None, verbose: bool = True) -> pathlib.Path:
         shutil.rmtree(BUILD)
     BUILD.mkdir(parents=True)
     jobs = jobs or min(len(sources) + len(SHIM_SOURCES), max(1, min(16, os.cpu_count() or 1)))
+    # (sysconfig fills its tables on first use, without a lock: read here, not in the workers.)
+    include = sysconfig.get_paths()["include"]
+    outs = {module: shim_path(module) for module in SHIM_SOURCES}
     with cf.ThreadPoolExecutor(max_workers=jobs) as pool:
-        shims = [pool.submit(_build_shim, module) for module in SHIM_SOURCES]
+        shims = [pool.submit(_build_shim, module, out, include) for module, out in outs.items()]
         objects = list(pool.map(_compile, sources))
         shim_libs = [shim.result().name for shim in shims]
     tmp = LIBRARY.with_suffix(".so.tmp")

@@ -8,36 +8,50 @@
 // Softmax and products are those of fmha_kernel.h (fp32 sums and statistics, P rounded to the
 // input type for the PV product).
 //
-// Work. Lengths and counts are on the device, so the programs make the plan themselves (find_item):
-// each reads the lengths of 64 requests at a time, one to a lane, and sums tiles and key blocks
-// over the wave. W = kv_heads * sum(tiles * blocks) block visits; with `target` programs to fill
-// the card a tile's keys are cut into ceil(blocks / chunk) splits, chunk = max(min_chunk, W /
-// target): long requests into many, short ones not at all, and never more than target + tiles *
-// kv_heads items in all, which bounds grid and workspace on the host without the lengths. The
-// surplus programs end after the sums. Split tiles go through partials (O / l, LSE) and a join.
-// Item w = ((request, tile, split), K/V head), the head fastest: workgroup w runs on XCD w % 8, so
-// with 8 heads an XCD holds one of them, and every XCD has its share of every request.
+// Work. Lengths and counts are on the device, so each program finds its item itself (find_item): it
+// reads the lengths of 64 requests at a time, one to a lane, and sums tiles and splits over the
+// wave. An item is a tile, or where tiles are fewer than the `target` programs that fill the card,
+// one of its splits: a tile of u units of keys has ceil(u / chunk) of them, with the smallest chunk
+// that leaves no more than `target` items (best_chunk). So all items run at once, the long requests
+// of a ragged batch in pieces; a CU reads at most 38 GB/s, 1.7 times its share of the memory, so
+// pieces of unequal length cost nothing until one has twice its share (B 32, Hq 32, Hkv 8, D 128,
+// lengths 1024-4096, us: split W / target evenly 76, even ranges over the tiles laid end to end
+// 75, whole tiles 72; see also extend_rows_kernel). Grid and workspace follow on the host from
+// sizes alone, programs without an item end after the sums. Split tiles go through partials (O / l,
+// LSE) and a join.
+// The K/V head is fastest in an item's number: workgroup w runs on XCD w % 8, so with 8 heads an XCD
+// holds one of them.
 #pragma once
-#include "fmha_kernel.h"
+#include "fmha_prefill.h"
 
 namespace fgw_kv {
 
 using namespace fgw_mha;
 
-// heads: K/V heads; work: items of the launch at most; sq, q_tiles, mode, splits: unused.
+// heads: K/V heads; work: places for partials; sq, q_tiles, mode, splits: unused.
 struct ExtendParams : FwdParams {
   const int32_t* cu;
   int64_t q_token, q_head;  // bytes
   int32_t tokens, q_heads, group, max_new, window;
   int32_t rows_from, rows_to;  // requests with n * group in (rows_from, rows_to] are this launch's
-  int32_t target, min_chunk;   // target 0: nothing is split
+  int32_t target, min_chunk;   // items that fill the card (0: nothing is split), units of a split at least
+  int32_t* counters;           // rows kernel: arrivals at the split tiles, by their first item, or nullptr
+  int32_t* notes;              // for the join: [work] JoinNote
 };
+
+// Tiles of ROWS rows, keys in blocks of BN, splits in units of UNIT blocks.
+template <int ROWS_, int BN_, int UNIT_>
+struct Tiling {
+  static constexpr int ROWS = ROWS_, BN = BN_, UNIT = UNIT_, KEYS = BN_ * UNIT_;
+};
+typedef Tiling<32, 32, 4> ShortTiling;   // extend_rows_kernel: a round of its four waves
+typedef Tiling<256, 64, 1> LongTiling;   // extend_long_kernel
 
 struct Request {
-  int first, n, len, tiles, blocks;
+  int first, n, len, tiles, units;
 };
 
-template <int ROWS, int BN>
+template <class T>
 __device__ __forceinline__ Request load_request(const ExtendParams& p, const int32_t* lengths,
                                                 const int32_t* cu, int b) {
   Request r{0, 0, 0, 0, 0};
@@ -51,63 +65,90 @@ __device__ __forceinline__ Request load_request(const ExtendParams& p, const int
   r.n = next - first < p.max_new ? next - first : p.max_new;
   const int64_t rows = (int64_t)r.n * p.group;
   if (rows <= p.rows_from || rows > p.rows_to) return r;
-  r.tiles = (int)((rows + ROWS - 1) / ROWS);
+  r.tiles = (int)((rows + T::ROWS - 1) / T::ROWS);
   int lo = p.window > 0 ? r.len - r.n - p.window + 1 : 0;
   lo = lo < 0 ? 0 : lo;
-  r.blocks = (r.len + BN - 1) / BN - lo / BN;
+  r.units = (r.len + T::KEYS - 1) / T::KEYS - lo / T::KEYS;
   return r;
 }
 
-// One item: tile `tile` of request `b`, split `split` of `splits`; its keys are the blocks
-// [blk_begin, blk_end) and of those the keys [lo, hi) that some row of the tile sees.
-struct Item {
-  int b, first, n, len, tile, head, split, splits;
-  int rows;                  // of the tile
-  int lo, hi;
-  int blk_begin, blk_end;
-  int slot, slot_step;       // partials of split s: slot0 + s * slot_step; slot is this split's
-};
-
+// Inclusive sums over the wave's lanes: by DPP within rows of 16 (shifts by 1, 2, 4, 8), then each
+// row's last lane onto the rows behind it.
 __device__ __forceinline__ int wave_incl_sum(int x, int lane) {
-  for (int off = 1; off < 64; off <<= 1) {
-    const int up = __shfl_up(x, off, 64);
-    x += lane >= off ? up : 0;
-  }
-  return x;
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  const int a = __builtin_amdgcn_readlane(x, 15), b = __builtin_amdgcn_readlane(x, 31);
+  const int c = __builtin_amdgcn_readlane(x, 47);
+  return x + (lane >= 16 ? a : 0) + (lane >= 32 ? b : 0) + (lane >= 48 ? c : 0);
+}
+__device__ __forceinline__ int wave_sum(int x, int lane) {
+  return __builtin_amdgcn_readlane(wave_incl_sum(x, lane), 63);
 }
 
-// Item w (BY_TILE: the first split of tile w / kv_heads, head w % kv_heads) of the launch; false
-// past the last one. Uniform over the wave; every wave of a workgroup computes the same.
-template <int ROWS, int BN, bool BY_TILE>
+__device__ __forceinline__ int splits_of(int units, int chunk) {
+  return units > chunk ? (units + chunk - 1) / chunk : 1;
+}
+
+// Units of a split: the smallest chunk, up to the steps of the search, of at least min_chunk units
+// with which all tiles of a head have at most target / heads splits together; kWhole where whole
+// tiles are as many. The sums saturate (kMany) so that they stay in 32 bits; the same in every
+// program.
+constexpr int kWhole = 0x40000000, kMany = 1 << 24;
+template <class T>
+__device__ __forceinline__ int best_chunk(const ExtendParams& p, const int32_t* lengths, const int32_t* cu,
+                                          const Request& r0, int lane) {
+  const int limit = (int)((u32)p.target / (u32)p.heads);
+  if (limit <= 1) return kWhole;
+  auto sum = [&](auto&& count) {
+    int total = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 64) {
+      const Request r = b0 == 0 ? r0 : load_request<T>(p, lengths, cu, b0 + lane);
+      const int64_t x = r.tiles ? count(r) : 0;
+      total += wave_sum((int)(x < kMany ? x : kMany), lane);
+      total = total < kMany ? total : kMany;
+    }
+    return total;
+  };
+  if (sum([](const Request& r) { return (int64_t)r.tiles; }) >= limit) return kWhole;
+  const int units = sum([](const Request& r) { return (int64_t)r.tiles * r.units; });
+  int chunk = (int)((u32)(units + limit - 1) / (u32)limit);
+  chunk = chunk < p.min_chunk ? p.min_chunk : chunk;
+  for (;;) {
+    const int items = sum([&](const Request& r) { return (int64_t)r.tiles * splits_of(r.units, chunk); });
+    if (items <= limit || chunk >= kMany) return chunk;
+    chunk += (chunk >> 3) + 1;  // (with whole tiles the items are fewer than the limit)
+  }
+}
+
+// One item: the blocks [blk_begin, blk_end) of tile `tile` of request `b`, and of those the keys
+// [lo, hi) that some row of the tile sees.
+struct Item {
+  int b, first, n, len, tile, head, split, splits;
+  int rows;  // of the tile
+  int lo, hi;
+  int blk_begin, blk_end;
+  int slot, slot0, slot_step;  // partials: of this split, of the first one; between splits
+};
+
+// Item w of the launch; false where there is none. Uniform over the wave; every wave of a workgroup
+// computes the same.
+template <class T>
 __device__ __forceinline__ bool find_item(const ExtendParams& p, const int32_t* lengths,
                                           const int32_t* cu, int w, int lane, Item& it) {
-  const Request r0 = load_request<ROWS, BN>(p, lengths, cu, lane);
-  int chunk = 0x40000000;
-  if (p.target > 0) {
-    float visits = 0.0f;  // (the same order in every program: the same sum)
-    for (int b0 = 0; b0 < p.batch; b0 += 64) {
-      const Request r = b0 == 0 ? r0 : load_request<ROWS, BN>(p, lengths, cu, b0 + lane);
-      visits += (float)r.tiles * (float)r.blocks;
-    }
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) visits += __shfl_xor(visits, x, 64);
-    // (The bound on the items allows for the rounding of this sum: items_bound.)
-    const float per = ceilf(visits * (float)p.heads / (float)p.target);
-    chunk = per < 1.0e9f ? (int)per : 1000000000;
-    chunk = __builtin_amdgcn_readfirstlane(chunk < p.min_chunk ? p.min_chunk : chunk);
-  }
-  const int g = w / p.heads;
+  const Request r0 = load_request<T>(p, lengths, cu, lane);
+  const int chunk = p.target > 0 ? best_chunk<T>(p, lengths, cu, r0, lane) : kWhole;
+  const int g = (int)((u32)w / (u32)p.heads);
   it.head = w - g * p.heads;
-  int tiles_before = 0, items_before = 0;
+  int items_before = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
-    const Request r = b0 == 0 ? r0 : load_request<ROWS, BN>(p, lengths, cu, b0 + lane);
-    const int splits = r.blocks > chunk ? (r.blocks + chunk - 1) / chunk : 1;
+    const Request r = b0 == 0 ? r0 : load_request<T>(p, lengths, cu, b0 + lane);
+    const int splits = splits_of(r.units, chunk);
     const int items = r.tiles * splits;
     const int items_to = wave_incl_sum(items, lane);
-    const int tiles_to = BY_TILE ? wave_incl_sum(r.tiles, lane) : 0;
-    const int own = BY_TILE ? r.tiles : items;
-    const int at = BY_TILE ? g - tiles_before - (tiles_to - own) : g - items_before - (items_to - own);
-    const uint64_t hit = __ballot(at >= 0 && at < own);
+    const int at = g - items_before - (items_to - items);
+    const uint64_t hit = __ballot(at >= 0 && at < items);
     if (hit) {
       const int l = __builtin_ctzll(hit);
       auto pick = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
@@ -117,14 +158,15 @@ __device__ __forceinline__ bool find_item(const ExtendParams& p, const int32_t* 
       it.n = pick(r.n);
       it.len = pick(r.len);
       // The last tiles first: causal, they are the longest.
-      const int place_tile = BY_TILE ? place : place / s;
+      const int place_tile = (int)((u32)place / (u32)s);
       it.tile = tiles - 1 - place_tile;
-      it.split = BY_TILE ? 0 : place - place_tile * s;
+      it.split = place - place_tile * s;
+      it.slot = w;
+      it.slot0 = w - it.split * p.heads;
       it.slot_step = p.heads;
-      it.slot = (items_before + pick(items_to) - pick(items) + place_tile * s + it.split) * p.heads + it.head;
 
-      const int row0 = it.tile * ROWS, all = it.n * p.group;
-      it.rows = all - row0 < ROWS ? all - row0 : ROWS;
+      const int row0 = it.tile * T::ROWS, all = it.n * p.group;
+      it.rows = all - row0 < T::ROWS ? all - row0 : T::ROWS;
       const int t0 = row0 / p.group, t1 = (row0 + it.rows - 1) / p.group;
       int hi = p.causal ? it.len - it.n + t1 + 1 : it.len;
       hi = hi < 0 ? 0 : hi;
@@ -132,15 +174,18 @@ __device__ __forceinline__ bool find_item(const ExtendParams& p, const int32_t* 
       lo = lo < 0 ? 0 : (lo > hi ? hi : lo);
       it.lo = lo;
       it.hi = hi;
-      const int from = lo / BN, blocks = (hi + BN - 1) / BN - from;
-      const int most = blocks > chunk ? (blocks + chunk - 1) / chunk : 1;
+      // The tile's own units, fewer than its request's where it ends earlier or begins later.
+      const int from = lo / T::KEYS, units = (hi + T::KEYS - 1) / T::KEYS - from;
+      const int most = splits_of(units, chunk);
       it.splits = most < s ? most : s;
-      it.blk_begin = from + split_bound(blocks, it.split, it.splits);
-      it.blk_end = from + split_bound(blocks, it.split + 1, it.splits);
-      return it.split < it.splits;
+      const int end = (hi + T::BN - 1) / T::BN;
+      it.blk_begin = (from + split_bound(units, it.split, it.splits)) * T::UNIT;
+      it.blk_end = (from + split_bound(units, it.split + 1, it.splits)) * T::UNIT;
+      it.blk_end = it.blk_end < end ? it.blk_end : end;
+      // (Offsets that fall and rise again make more items than there are places for partials.)
+      return it.split < it.splits && (it.splits == 1 || it.slot0 + (it.splits - 1) * it.slot_step < p.work);
     }
-    items_before += __shfl(items_to, 63, 64);
-    if (BY_TILE) tiles_before += __shfl(tiles_to, 63, 64);
+    items_before += __builtin_amdgcn_readlane(items_to, 63);
   }
   return false;
 }
@@ -169,75 +214,295 @@ __device__ __forceinline__ void mask_seen(f32x16 (&s)[C::ST], int pos0, const Se
     }
 }
 
-// Rows that few requests' tokens fill: 32 rows to a tile, four waves that each stream their own
-// 32-key blocks of the item through LDS and meet at its end (the key layout of fwd_kernel, whose
-// operand layouts and softmax these are).
-//
-// DMA: lane l (mod 32) resolves key l of the block through the table, one block ahead of its use,
-// and the load instructions fetch their rows' offsets from those lanes, so any page size takes the
-// same path. Keys outside [lo, hi), page ids outside the pool and dims past D read zeros.
-template <class C>
-__device__ __forceinline__ int32_t key_page(const ExtendParams& p, const int32_t* table_b, int pos) {
-  const u32 pg = div_page((u32)pos, p.page_magic, p.page_shift), last = (u32)p.width - 1u;
-  return table_b[pg < last ? pg : last];
+// Element offset of row `row` of a request's rows of a K/V head in the output.
+__device__ __forceinline__ int64_t out_row(const ExtendParams& p, const Item& it, int row) {
+  const int tk = row / p.group;
+  return ((int64_t)(it.first + tk) * p.q_heads + it.head * p.group + (row - tk * p.group)) * p.dim;
 }
 
-template <class C>
-__device__ __forceinline__ void issue_rows(const ExtendParams& p, const char* kb, const char* vb,
-                                           int64_t row_bytes, int pos, int32_t page_id, int lo, int hi,
-                                           unsigned char* stage, int lane) {
-  const u32 dst = (u32)opaque_uniform((int)lds_address(stage));
-  const u32 pg = div_page((u32)pos, p.page_magic, p.page_shift);
-  const int64_t row = (int64_t)page_id * p.page_size + ((u32)pos - pg * (u32)p.page_size);
-  const bool live = pos >= lo && pos < hi && row >= 0 && row < p.pool_rows;
-  const int64_t off = live ? row * row_bytes : -1;
-  const u32 off_lo = (u32)off, off_hi = (u32)((uint64_t)off >> 32);
-  const char* zero = reinterpret_cast<const char*>(kZeroChunk);
+// Partials that this launch joins itself go through buffer loads and stores at device scope (sc1,
+// 16 bytes to a lane): they pass by the L2s of the XCDs, which are not coherent with each other. A
+// launch's partials are below 2^31 bytes (plan_items in kv_extend.hip).
+constexpr int kDeviceScope = 17;  // sc0 | sc1
+__device__ __forceinline__ f32x4 device_load4(const float* base, u32 bytes) {
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), (short)0, 0x7fffffff, 0x00027000);
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)bytes, 0, kDeviceScope));
+}
+__device__ __forceinline__ float device_load1(const float* base, u32 bytes) {
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), (short)0, 0x7fffffff, 0x00027000);
+  return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)bytes, 0, kDeviceScope));
+}
+__device__ __forceinline__ void device_store4(float* base, u32 bytes, f32x4 x) {
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(base, (short)0, 0x7fffffff, 0x00027000);
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), rsrc, (int)bytes, 0, kDeviceScope);
+}
+__device__ __forceinline__ void device_store1(float* base, u32 bytes, float x) {
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(base, (short)0, 0x7fffffff, 0x00027000);
+  __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), rsrc, (int)bytes, 0, kDeviceScope);
+}
+
+// What a second launch has to know to join split tiles: every item's, in its own place (splits 0:
+// no split tile's).
+struct JoinNote {
+  int32_t first, tile, head, rows, splits, split, pad[2];
+};
+__device__ __forceinline__ void write_note(const ExtendParams& p, const Item& it, bool found) {
+  const int w = (int)blockIdx.x;
+  if (p.notes == nullptr || w >= p.work || threadIdx.x != 0) return;
+  JoinNote note{0, 0, 0, 0, 0, 0, {0, 0}};
+  if (found && it.splits > 1)
+    note = JoinNote{it.first, it.tile, it.head, it.rows, it.splits, it.split, {0, 0}};
+  reinterpret_cast<JoinNote*>(p.notes)[w] = note;
+}
+
+// The splits g, g + share, ... of one (row, 4 dims) into a state; CH of them are loaded before any is
+// used.
+template <int ROWS, bool COH, int CH>
+__device__ __forceinline__ void join_splits(const ExtendParams& p, const Item& it, int r, int c, int g, int share,
+                                            float& peak, float& tot, f32x4& acc) {
+  for (int s0 = g; s0 < it.splits; s0 += CH * share) {
+    float x[CH];
+    f32x4 v[CH];
 #pragma unroll
-  for (int i = 0; i < C::INSTR; ++i) {
-    const int r = C::RPI * i + lane / C::CPR, at = lane % C::CPR;
-    const u32 rl = (u32)__builtin_amdgcn_ds_bpermute(4 * r, (int)off_lo);
-    const u32 rh = (u32)__builtin_amdgcn_ds_bpermute(4 * r, (int)off_hi);
-    const int64_t ro = (int64_t)(((uint64_t)rh << 32) | rl);
-    const int kc = at ^ (r % C::KSW), vc = at ^ (4 * (r % C::VSW));
-    const char* ks = ro >= 0 && kc * 8 < p.dim ? kb + ro + kc * 16 : zero;
-    const char* vs = ro >= 0 && vc * 8 < p.dim ? vb + ro + vc * 16 : zero;
-    __builtin_amdgcn_global_load_lds(ks, FGW_LDS(void, (uintptr_t)(dst + 1024u * i)), 16, 0, 0);
-    __builtin_amdgcn_global_load_lds(vs, FGW_LDS(void, (uintptr_t)(dst + C::TILE_BYTES + 1024u * i)), 16,
-                                     0, 0);
+    for (int k = 0; k < CH; ++k) {
+      const int split = s0 + k * share < it.splits ? s0 + k * share : g;  // (weight 0 below)
+      const u32 at = (u32)(it.slot0 + split * it.slot_step) * ROWS + (u32)r;
+      if constexpr (COH) {
+        x[k] = device_load1(p.lse, 4u * at);
+        v[k] = device_load4(p.parts, 4u * (at * (u32)p.dim + 4u * (u32)c));
+      } else {
+        x[k] = p.lse[at];
+        v[k] = *reinterpret_cast<const f32x4*>(p.parts + (int64_t)at * p.dim + 4 * c);
+      }
+    }
+    float top = peak;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const bool live = s0 + k * share < it.splits && x[k] > -1.0e29f;
+      top = live ? fmaxf(top, x[k]) : top;
+    }
+    const float keep = expf(peak - top);
+    tot *= keep;
+    acc *= keep;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const bool live = s0 + k * share < it.splits && x[k] > -1.0e29f;
+      const float w = live ? expf(x[k] - top) : 0.0f;
+      tot += w;
+      acc += live ? v[k] * w : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    peak = top;
   }
 }
 
+// Rows [row_from, row_to) of a split tile from its partials, by the whole workgroup. A thread holds 4
+// dims of a row; where rows and dims leave threads over, they share its splits. Weights exp(LSE -
+// peak), empty splits (LSE -1e30) weigh nothing, an all-empty row is zero. COH: the partials were
+// written by this launch. Uses 24 bytes of LDS a thread.
+template <bool BF16, int ROWS, bool COH>
+__device__ __forceinline__ void join_rows(const ExtendParams& p, const Item& it, int row_from, int row_to,
+                                          unsigned char* lds, int tid, int threads) {
+  using E = Elem<BF16>;
+  f32x4* const sacc = reinterpret_cast<f32x4*>(lds);
+  float* const speak = reinterpret_cast<float*>(lds + threads * 16);
+  float* const stot = speak + threads;
+  const int d4n = p.dim / 4, pairs = (row_to - row_from) * d4n;
+  const int share = pairs < threads ? threads / pairs : 1;  // threads of a (row, 4 dims) pair
+  for (int base = 0; base < pairs; base += threads) {
+    const int pair = share > 1 ? tid % pairs : base + tid, g = share > 1 ? tid / pairs : 0;
+    const bool act = pair < pairs && g < share;
+    const int r = row_from + pair / d4n, c = pair % d4n;
+    float peak = kNegBig, tot = 0.0f;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (act) {
+      if (it.splits <= 2 * share)
+        join_splits<ROWS, COH, 2>(p, it, r, c, g, share, peak, tot, acc);
+      else if (it.splits <= 4 * share)
+        join_splits<ROWS, COH, 4>(p, it, r, c, g, share, peak, tot, acc);
+      else
+        join_splits<ROWS, COH, 8>(p, it, r, c, g, share, peak, tot, acc);
+    }
+    if (share > 1) {  // uniform
+      sacc[tid] = acc;
+      speak[tid] = peak;
+      stot[tid] = tot;
+      __syncthreads();
+      if (act && g == 0) {
+        float top = peak;
+        for (int k = 1; k < share; ++k) top = fmaxf(top, speak[k * pairs + pair]);
+        const float keep = expf(peak - top);
+        acc *= keep;
+        tot *= keep;
+        for (int k = 1; k < share; ++k) {
+          const float w = expf(speak[k * pairs + pair] - top);
+          acc += sacc[k * pairs + pair] * w;
+          tot += stot[k * pairs + pair] * w;
+        }
+      }
+    }
+    if (act && g == 0) {
+      const float inv = 1.0f / fmaxf(tot, 1.0e-30f);
+      u32x2 w;
+      w.x = E::pack2(acc[0] * inv, acc[1] * inv);
+      w.y = E::pack2(acc[2] * inv, acc[3] * inv);
+      *reinterpret_cast<u32x2*>(static_cast<u16*>(p.out) + out_row(p, it, it.tile * ROWS + r) + 4 * c) = w;
+    }
+  }
+}
+
+// ---- requests of few rows -----------------------------------------------------------------------
+
+// Rows that few requests' tokens fill: 32 rows to a tile, four waves that each stream their own
+// 32-key blocks of the tile through LDS and meet at its end (the key layout of fwd_kernel, whose
+// operand layouts and softmax these are).
+//
+// Each wave keeps kStages blocks of its own on the way: the K tile of block n + kStages is issued
+// as soon as the scores of block n are computed, its V tile after the products of block n, and the
+// waits count the half blocks issued since. The loads are inline assembly (dma_saddr, dma_flat): the
+// compiler would wait for all of them before each transposing read of V. Their row offsets come
+// from page ids that lane l holds for load instruction l % INSTR of block l / INSTR, four such
+// windows read at a time: a read in the loop would wait for the DMA in front of it.
+// Keys outside [lo, hi) or in pages outside the pool read zeros, and so do dims past D. Blocks with
+// an instruction whose keys straddle pages are resolved key by key.
+template <int DPAD>
+constexpr int kStages = DPAD >= 128 ? 1 : DPAD == 64 ? 2 : 4;
+
+// The K (IS_V false) or V tile of the keys [pos0, pos0 + 32), each through the table: lane l (mod 32)
+// resolves key l, the load instructions fetch their rows' offsets from those lanes.
+template <class C, bool IS_V>
+__device__ __forceinline__ void issue_block_keys(const ExtendParams& p, const int32_t* table_b, const char* base,
+                                                 int64_t row_bytes, int pos0, int lo, int hi, u32 dst, int lane) {
+  const int dim = opaque_uniform(p.dim);
+  lane = opaque_lane(lane);
+  const char* zero = reinterpret_cast<const char*>(kZeroChunk);
+  const int pos = pos0 + (lane & 31);
+  const bool in = pos >= lo && pos < hi;
+  const u32 pg = in ? div_page((u32)pos, p.page_magic, p.page_shift) : 0u;
+  const int64_t row = (int64_t)table_b[pg] * p.page_size + ((u32)pos - pg * (u32)p.page_size);
+  const int64_t off = in && row >= 0 && row < p.pool_rows ? row * row_bytes : -1;
+#pragma unroll
+  for (int q = 0; q < C::INSTR; ++q) {
+    const int r = C::RPI * q + lane / C::CPR, at = lane % C::CPR;
+    const u32 rl = (u32)__builtin_amdgcn_ds_bpermute(4 * r, (int)(u32)off);
+    const u32 rh = (u32)__builtin_amdgcn_ds_bpermute(4 * r, (int)((uint64_t)off >> 32));
+    const int64_t ro = (int64_t)(((uint64_t)rh << 32) | rl);
+    const int c = IS_V ? at ^ (4 * (r % C::VSW)) : at ^ (r % C::KSW);
+    dma_flat(ro >= 0 && c * 8 < dim ? base + ro + c * 16 : zero, dst + 1024u * q);
+  }
+}
+
+// Waits until K (V) of a block has landed with `rem` further blocks of the wave to come: behind K
+// are V and the halves of the next kStages - 1 blocks, behind V those and one K more.
+template <class C, bool IS_V, int R = 0>
+__device__ __forceinline__ void wait_half(int rem) {
+  constexpr int S = kStages<C::DPAD>;
+  if constexpr (R < S) {
+    if (rem == R) {
+      wait_vm<C::INSTR * (2 * R + (IS_V ? 0 : 1))>();
+      return;
+    }
+    wait_half<C, IS_V, R + 1>(rem);
+  } else {
+    wait_vm<C::INSTR * (2 * S - 1)>();
+  }
+}
+
+// LDS reads of this wave have returned: their tile may be written again.
+__device__ __forceinline__ void wait_lds() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  asm volatile("" ::: "memory");
+}
+
 template <class C>
-__global__ __launch_bounds__(C::THREADS) void extend_rows_kernel(ExtendParams p,
-                                                                 const int32_t* __restrict__ table,
-                                                                 const int32_t* __restrict__ lengths,
-                                                                 const int32_t* __restrict__ cu) {
-  constexpr int kBytes = CMax<C::TILES_BYTES, C::COMB_BYTES>::value;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[kBytes];
-  const int tid = threadIdx.x;
+__device__ __forceinline__ void extend_tile(const ExtendParams& p, const int32_t* table, const Item& it,
+                                            unsigned char* smem, int tid, bool fused) {
+  // (Opaque copies: what derives from the lane is computed here and at the end, not held across the
+  // caller's loop.)
+  tid = opaque_lane(tid);
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
   const int il = lane & 31, hh = lane >> 5;
-  Item it;
-  if (!find_item<C::ROWS_TILE, C::BN, false>(p, lengths, cu, (int)blockIdx.x, lane, it)) return;
-
   const Lanes<C> ln(lane);
   const int64_t row_bytes = (int64_t)p.heads * p.dim * 2;
+  const DmaLanes<C> dl(lane, 0, row_bytes);
   const int32_t* table_b = table + (int64_t)it.b * p.width;
   const char* kb = static_cast<const char*>(p.k) + (int64_t)it.head * p.dim * 2;
   const char* vb = static_cast<const char*>(p.v) + (int64_t)it.head * p.dim * 2;
-  unsigned char* const stages = smem + wave * C::GROUP_BYTES;
+  constexpr int S = kStages<C::DPAD>;
+  unsigned char* const stages = smem + wave * S * C::STAGE_BYTES;
+  const u32 stages_lds = lds_address(stages);
 
   // This wave's blocks: blk_begin + wave, + 4, ...
   constexpr int kStep = C::NWK * C::BN;
   const int cnt = it.blk_end - it.blk_begin;
   const int my_n = cnt > wave ? (cnt - wave + C::NWK - 1) / C::NWK : 0;
   const int first_pos = (it.blk_begin + wave) * C::BN;
-  int32_t id = my_n > 0 ? key_page<C>(p, table_b, first_pos + il) : 0;
-  int32_t next_id = my_n > 1 ? key_page<C>(p, table_b, first_pos + kStep + il) : 0;
-  if (my_n > 0)
-    issue_rows<C>(p, kb, vb, row_bytes, first_pos + il, id, it.lo, it.hi, stages, lane);
+  constexpr int kWindow = 64 / C::INSTR, kIds = 4;  // blocks of a window, windows read at a time
+  int32_t ids[kIds];
+  auto unit_pos = [&](int n) { return first_pos + kStep * n + C::RPI * (lane % C::INSTR); };
+  auto read_ids = [&](int n0) {
+#pragma unroll
+    for (int k = 0; k < kIds; ++k) {
+      const u32 pg = div_page((u32)unit_pos(n0 + k * kWindow + lane / C::INSTR), p.page_magic, p.page_shift);
+      const u32 last = (u32)p.width - 1u;
+      ids[k] = table_b[pg < last ? pg : last];
+    }
+  };
+  // The lane's unit in the current window: pool byte offset of its first key (-1: it straddles
+  // pages), and its live keys [live & 255, live >> 8).
+  constexpr int kAllLive = C::RPI << 8;
+  int64_t off = 0;
+  int live = 0;
+  auto set_window = [&](int n0) {
+    const int w = n0 / kWindow % kIds;
+    if (w == 0 && n0 > 0) read_ids(n0);
+    const int32_t id = w == 0 ? ids[0] : w == 1 ? ids[1] : w == 2 ? ids[2] : ids[3];
+    const int n = n0 + lane / C::INSTR, pos = unit_pos(n);
+    const u32 pg = div_page((u32)pos, p.page_magic, p.page_shift), in_page = (u32)pos - pg * (u32)p.page_size;
+    const int64_t row0 = (int64_t)id * p.page_size + in_page;
+    const int from = it.lo > pos ? it.lo - pos : 0, to = it.hi - pos < C::RPI ? it.hi - pos : C::RPI;
+    const bool any = n < my_n && to > from;
+    const bool inside = row0 >= 0 && row0 + C::RPI <= p.pool_rows;
+    const bool straddles = any && in_page + C::RPI > (u32)p.page_size;
+    off = straddles ? -1 : any && inside ? row0 * row_bytes : 0;
+    live = any && inside ? from | to << 8 : 0;
+  };
+  const bool full_dim = p.dim == C::DPAD;
+  // Half a block: its K (IS_V false) or V tile.
+  auto issue = [&](int n, auto is_v) {
+    constexpr bool IS_V = decltype(is_v)::value;
+    if (!IS_V && n % kWindow == 0) set_window(n);
+    const char* base = IS_V ? vb : kb;
+    const u32 dst = stages_lds + (u32)(n % S * C::STAGE_BYTES) + (IS_V ? (u32)C::TILE_BYTES : 0u);
+    const int first = n % kWindow * C::INSTR;
+    constexpr uint64_t kUnits = (1ull << C::INSTR) - 1ull;
+    if ((__ballot(live != kAllLive || off < 0) >> first & kUnits) == 0 && full_dim) {
+#pragma unroll
+      for (int q = 0; q < C::INSTR; ++q)
+        dma_saddr(base + readlane64(off, first + q), IS_V ? dl.vq(q, 0) : dl.kq(q, 0), dst + 1024u * q);
+      return;
+    }
+    if (__ballot(off < 0) >> first & kUnits) {
+      int pos0 = first_pos + kStep * n;
+      asm volatile("" : "+s"(pos0));
+      issue_block_keys<C, IS_V>(p, table_b, base, row_bytes, pos0, it.lo, it.hi, dst, lane);
+      return;
+    }
+    const char* zero = reinterpret_cast<const char*>(kZeroChunk);
+    const int lr = opaque_lane(lane) / C::CPR;
+#pragma unroll
+    for (int q = 0; q < C::INSTR; ++q) {
+      const char* const src = base + readlane64(off, first + q);
+      const int keys = __builtin_amdgcn_readlane(live, first + q);
+      const u32 at = IS_V ? dl.vq(q, 0) : dl.kq(q, 0);
+      const bool in = lr >= (keys & 255) && lr < keys >> 8 && at - dl.row_off < 2u * (u32)p.dim;
+      dma_flat(in ? src + at : zero, dst + 1024u * q);
+    }
+  };
+  constexpr std::false_type k_half{};
+  constexpr std::true_type v_half{};
+  if (my_n > 0) read_ids(0);
 
   const int row = it.tile * C::ROWS_TILE + il;
   const int token = row / p.group, in_group = row - token * p.group;
@@ -267,47 +532,77 @@ __global__ __launch_bounds__(C::THREADS) void extend_rows_kernel(ExtendParams p,
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[dt][v] = 0.0f;
 
+  // (The compiler's waits for page ids and Q, older than the DMA, come here and not in the loop.)
+  if (my_n > 0) asm volatile("" ::"v"(ids[0]), "v"(ids[1]), "v"(ids[2]), "v"(ids[3]));
+  for (int n = 0; n < S && n < my_n; ++n) {
+    issue(n, k_half);
+    issue(n, v_half);
+  }
+#pragma unroll
+  for (int kk = 0; kk < C::KK; ++kk) asm volatile("" ::"v"(qf[kk]));
   for (int n = 0; n < my_n; ++n) {
     const int pos0 = first_pos + kStep * n;
-    unsigned char* stage = stages + (n % C::NBUF) * C::STAGE_BYTES;
-    wait_dma();
-    group_sync<C>();
-    const int32_t id1 = next_id;
-    if (n + 2 < my_n) next_id = key_page<C>(p, table_b, pos0 + 2 * kStep + il);
-    if (n + 1 < my_n && C::NBUF == 2)
-      issue_rows<C>(p, kb, vb, row_bytes, pos0 + kStep + il, id1, it.lo, it.hi,
-                    stages + ((n + 1) % C::NBUF) * C::STAGE_BYTES, lane);
-    f32x16 s[C::ST];
-    u32x4 pf[C::KS];
-    qk_block<C>(stage, ln, qf, s);
+    const unsigned char* stage = stages + n % S * C::STAGE_BYTES;
+    const int rem = my_n - 1 - n;
+    // One wave to a SIMD: nothing hides a chain of LDS reads and products but the block's own work.
+    // So all operands of a product are read at once (there are registers for them), the scores come
+    // in two chains, K's next tile is issued while they run, and V is read under the softmax.
+    u32x4 ka[C::KK], va[C::KS * C::DT], pf[C::KS];
+    f32x16 s[1], t;
+    wait_half<C, false>(rem);
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int kk = 0; kk < C::KK; ++kk) ka[kk] = read_k<C>(stage, ln, 0, kk);
+    wait_lds();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int v = 0; v < 16; ++v) s[0][v] = t[v] = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < C::KK; kk += 2) {
+      s[0] = Elem<C::BF16>::mma(ka[kk], qf[kk], s[0]);
+      t = Elem<C::BF16>::mma(ka[kk + 1], qf[kk + 1], t);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (rem >= S) issue(n + S, k_half);
+    wait_half<C, true>(rem);
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int k2 = 0; k2 < C::KS; ++k2)
+#pragma unroll
+      for (int dt = 0; dt < C::DT; ++dt) va[k2 * C::DT + dt] = read_vt<C>(stage + C::TILE_BYTES, ln, dt, k2);
+    __builtin_amdgcn_sched_barrier(0);
+    s[0] += t;
     if (pos0 + C::BN > hi_min || pos0 < lo_max) mask_seen<C>(s, pos0, seen, hh);
     online_softmax<C>(s, m, l, o, p.scale_log2, pf);
-    pv_block<C>(stage + C::TILE_BYTES, ln, pf, o);
-    if (n + 1 < my_n && C::NBUF == 1) {
-      group_sync<C>();
-      issue_rows<C>(p, kb, vb, row_bytes, pos0 + kStep + il, id1, it.lo, it.hi, stage, lane);
-    }
+    wait_lds();
+    if (rem >= S) issue(n + S, v_half);
+#pragma unroll
+    for (int k2 = 0; k2 < C::KS; ++k2)
+#pragma unroll
+      for (int dt = 0; dt < C::DT; ++dt)
+        o[dt] = Elem<C::BF16>::mma(va[k2 * C::DT + dt], pf[k2], o[dt]);
   }
-  wait_dma();
 
   // The waves' states of the same rows, through LDS.
   __syncthreads();
+  tid = opaque_lane(tid);
+  const int cil = tid & 31, chh = (tid & 63) >> 5;
   float* cm = reinterpret_cast<float*>(smem);
   float* cl = cm + C::NWK * C::ROWS_WAVE;
   float* co = cl + C::NWK * C::ROWS_WAVE;
   const float tot = pair_sum(l);
-  if (hh == 0) {
-    cm[wave * C::ROWS_WAVE + il] = m;
-    cl[wave * C::ROWS_WAVE + il] = tot;
+  if (chh == 0) {
+    cm[wave * C::ROWS_WAVE + cil] = m;
+    cl[wave * C::ROWS_WAVE + cil] = tot;
   }
-  if (mine) {
+  if (cil < it.rows) {
 #pragma unroll
     for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
       for (int gq = 0; gq < 4; ++gq) {
         f32x4 val = {o[dt][4 * gq], o[dt][4 * gq + 1], o[dt][4 * gq + 2], o[dt][4 * gq + 3]};
-        *reinterpret_cast<f32x4*>(co + (wave * C::ROWS_WAVE + il) * C::OSTRIDE + 32 * dt + 8 * gq +
-                                  4 * hh) = val;
+        *reinterpret_cast<f32x4*>(co + (wave * C::ROWS_WAVE + cil) * C::OSTRIDE + 32 * dt + 8 * gq +
+                                  4 * chh) = val;
       }
   }
   __syncthreads();
@@ -329,79 +624,84 @@ __global__ __launch_bounds__(C::THREADS) void extend_rows_kernel(ExtendParams p,
     }
     const float inv = 1.0f / fmaxf(t2, 1.0e-30f);
     if (it.splits == 1) {
-      const int rr = it.tile * C::ROWS_TILE + r, tk = rr / p.group;
-      u16* dst = static_cast<u16*>(p.out) +
-                 ((int64_t)(it.first + tk) * p.q_heads + it.head * p.group + (rr - tk * p.group)) * p.dim + d0;
       u32x2 w;
       w.x = E::pack2(acc[0] * inv, acc[1] * inv);
       w.y = E::pack2(acc[2] * inv, acc[3] * inv);
-      *reinterpret_cast<u32x2*>(dst) = w;
+      *reinterpret_cast<u32x2*>(static_cast<u16*>(p.out) +
+                                out_row(p, it, it.tile * C::ROWS_TILE + r) + d0) = w;
+      continue;
+    }
+    const u32 at = (u32)it.slot * C::ROWS_TILE + (u32)r;
+    acc *= inv;
+    if (fused) {
+      device_store4(p.parts, 4u * (at * (u32)p.dim + (u32)d0), acc);
+      if (d0 == 0) device_store1(p.lse, 4u * at, lse_of(mm, t2));
     } else {
-      *reinterpret_cast<f32x4*>(p.parts + ((int64_t)it.slot * C::ROWS_TILE + r) * p.dim + d0) = acc * inv;
-      if (d0 == 0) p.lse[(int64_t)it.slot * C::ROWS_TILE + r] = lse_of(mm, t2);
+      *reinterpret_cast<f32x4*>(p.parts + (int64_t)at * p.dim + d0) = acc;
+      if (d0 == 0) p.lse[at] = lse_of(mm, t2);
     }
   }
 }
 
-// The join of split tiles: workgroup (tile and head, part of its rows). D / 4 threads hold a row;
-// the workgroup's kMergeThreads / (D / 4) such groups share a row's splits (WIDE: few rows, many
-// splits) or take a row each. Weights exp(LSE - peak), empty splits (LSE -1e30) weigh nothing, an
-// all-empty row is zero.
-template <bool BF16, int ROWS, int BN, bool WIDE>
-__global__ __launch_bounds__(kMergeThreads) void extend_join_kernel(ExtendParams p,
-                                                                    const int32_t* __restrict__ lengths,
-                                                                    const int32_t* __restrict__ cu) {
-  using E = Elem<BF16>;
-  __shared__ float speak[kMergeThreads], stot[kMergeThreads];
-  __shared__ f32x4 sacc[kMergeThreads];
-  const int t = threadIdx.x;
+// One item a program. With counters the program that writes the last split of a tile joins it (and
+// sets the tile's counter, that of its first item, back to zero); else a second launch does.
+template <class C>
+__global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void extend_rows_kernel(
+    ExtendParams p, const int32_t* __restrict__ table, const int32_t* __restrict__ lengths,
+    const int32_t* __restrict__ cu) {
+  constexpr int kBytes = CMax<C::NWK * kStages<C::DPAD> * C::STAGE_BYTES, C::COMB_BYTES>::value;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[kBytes];
+  const int tid = threadIdx.x;
   Item it;
-  if (!find_item<ROWS, BN, true>(p, lengths, cu, (int)blockIdx.x, t & 63, it)) return;
-  // (Offsets that overlap make more items than the workspace has places for.)
-  if (it.splits == 1 || (int64_t)it.slot + (int64_t)(it.splits - 1) * it.slot_step >= p.work) return;
-  const int d4n = p.dim / 4, G = kMergeThreads / d4n;
-  const int c = t % d4n, g = t / d4n;
-  const int64_t ls = (int64_t)it.slot_step * ROWS;
-  for (int r0 = blockIdx.y * (WIDE ? 1 : G); r0 < it.rows; r0 += gridDim.y * (WIDE ? 1 : G)) {
-    const int r = WIDE ? r0 : r0 + g;
-    const bool act = g < G && r < it.rows;
-    const float* lse = p.lse + (int64_t)it.slot * ROWS + r;
-    const float* parts = p.parts + ((int64_t)it.slot * ROWS + r) * p.dim + 4 * c;
-    float peak = kNegBig, tot = 0.0f;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (act) wide_group<8>(lse, parts, ls, ls * p.dim, WIDE ? g : 0, WIDE ? G : 1, it.splits, peak, tot, acc);
-    if constexpr (WIDE) {
-      if (act && c == 0) speak[g] = peak;
-      __syncthreads();
-      float top = kNegBig;
-      for (int k = 0; k < G; ++k) top = fmaxf(top, speak[k]);
-      if (act) {
-        const float scale = expf(peak - top);
-        sacc[t] = acc * scale;
-        if (c == 0) stot[g] = tot * scale;
-      }
-      __syncthreads();
-      if (g == 0) {
-        acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        tot = 0.0f;
-        for (int k = 0; k < G; ++k) {
-          acc += sacc[k * d4n + c];
-          tot += stot[k];
-        }
-      }
-    }
-    if (act && (!WIDE || g == 0)) {
-      const float inv = 1.0f / fmaxf(tot, 1.0e-30f);
-      const int rr = it.tile * ROWS + r, tk = rr / p.group;
-      u16* dst = static_cast<u16*>(p.out) +
-                 ((int64_t)(it.first + tk) * p.q_heads + it.head * p.group + (rr - tk * p.group)) * p.dim + 4 * c;
-      u32x2 w;
-      w.x = E::pack2(acc[0] * inv, acc[1] * inv);
-      w.y = E::pack2(acc[2] * inv, acc[3] * inv);
-      *reinterpret_cast<u32x2*>(dst) = w;
-    }
-    if constexpr (WIDE) __syncthreads();  // the LDS entries are written again
-  }
+  const bool found = find_item<ShortTiling>(p, lengths, cu, (int)blockIdx.x, tid & 63, it);
+  write_note(p, it, found);
+  if (!found) return;
+  const bool fused = p.counters != nullptr;
+  extend_tile<C>(p, table, it, smem, tid, fused);
+  if (it.splits == 1 || !fused) return;
+  wait_vm<0>();     // this wave's partials are complete at the device
+  __syncthreads();  // ... and every wave's
+  int* const flag = reinterpret_cast<int*>(smem);
+  int32_t* const counter = p.counters + (int64_t)it.slot0 * kArrivalStride;
+  if (tid == 0)
+    *flag = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == it.splits - 1;
+  __syncthreads();
+  const bool last = *flag != 0;
+  __syncthreads();  // LDS is written again
+  if (!last) return;
+  join_rows<C::BF16, C::ROWS_TILE, true>(p, it, 0, it.rows, smem, tid, C::THREADS);
+  if (tid == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The joins that the kernels leave: blockIdx.x items of the rows kernel, then of the long one. The
+// programs of a tile's splits share its rows, kJoinParts of them (blockIdx.y) to a split of a long
+// tile: few programs, since one takes 5 ns to dispatch.
+constexpr int kJoinParts = 4;
+template <bool BF16>
+__global__ __launch_bounds__(kMergeThreads) void extend_join_kernel(ExtendParams rows, ExtendParams longs,
+                                                                    int rows_items) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kMergeThreads * 24];
+  const bool is_long = (int)blockIdx.x >= rows_items;
+  if (!is_long && blockIdx.y > 0) return;
+  const ExtendParams& p = is_long ? longs : rows;
+  const int w = (int)blockIdx.x - (is_long ? rows_items : 0);
+  const JoinNote note = reinterpret_cast<const JoinNote*>(p.notes)[w];
+  if (note.splits < 2) return;
+  Item it;
+  it.first = note.first;
+  it.tile = note.tile;
+  it.head = note.head;
+  it.splits = note.splits;
+  it.slot0 = w - note.split * p.heads;
+  it.slot_step = p.heads;
+  const int parts = note.splits * (is_long ? kJoinParts : 1);
+  const int part = note.split * (is_long ? kJoinParts : 1) + (int)blockIdx.y;
+  const int from = note.rows * part / parts, to = note.rows * (part + 1) / parts;
+  if (from == to) return;
+  if (is_long)
+    join_rows<BF16, LongTiling::ROWS, false>(p, it, from, to, lds, threadIdx.x, kMergeThreads);
+  else
+    join_rows<BF16, ShortTiling::ROWS, false>(p, it, from, to, lds, threadIdx.x, kMergeThreads);
 }
 
 template <bool BF16, int DPAD>

@@ -6,8 +6,27 @@
 
 #include "kv_common.h"
 #include "kv_extend.h"
+#include "kv_extend_long.h"
 
 namespace fgw_kv {
+
+// Requests of up to kLongFrom rows (tokens times query heads of a K/V head) take the kernel of few
+// rows: it reads the keys once for every 32 of them, the long one once for 256. Hq 32, Hkv 8, D 128,
+// pages of 64, few rows / long, us: 128 rows B1 KV 1024 17.0 / 26.9, B4 KV 2048 24.3 / 36.6, B1 KV
+// 8192 26.4 / 37.2, B8 KV 8192 96.5 / 88.6; 192 rows 17.2 / 29.2, 29.9 / 39.3, 32.6 / 39.1,
+// 146 / 93.9. Above a head dim of 128 there is no long kernel.
+constexpr int kLongFrom = 128;
+// Units of a split at least (rounds of 128 keys, blocks of 64): below, a split's own cost outweighs
+// what it saves. Few rows, B1 Hq 32 Hkv 8 D 128 KV 4096, 1 / 2 / 4 rounds: 13.1 / 12.2 / 14.4 us;
+// long, B1 100 tokens KV 1000, 4 / 8 blocks: 26.1 / 32.4 us.
+constexpr int kRowsMinChunk = 2, kLongMinChunk = 4;
+
+#define FGW_KV_EXTERN_LONG(BF, DP)                                                                    \
+  extern template hipError_t launch_extend_long<BF, DP, kRowsBlock>(const ExtendParams&, int, hipStream_t); \
+  extern template hipError_t launch_extend_long<BF, DP, kRowsGroup>(const ExtendParams&, int, hipStream_t); \
+  extern template hipError_t launch_extend_long<BF, DP, kRowsPadded>(const ExtendParams&, int, hipStream_t);
+FGW_KV_EXTERN_LONG(true, 64) FGW_KV_EXTERN_LONG(true, 128)
+FGW_KV_EXTERN_LONG(false, 64) FGW_KV_EXTERN_LONG(false, 128)
 
 #define FGW_KV_EXTERN_ROWS(BF, DP) \
   extern template hipError_t launch_extend_rows<BF, DP>(const ExtendParams&, int, hipStream_t);
@@ -16,47 +35,90 @@ FGW_KV_EXTERN_ROWS(true, 128) FGW_KV_EXTERN_ROWS(true, 256)
 FGW_KV_EXTERN_ROWS(false, 32) FGW_KV_EXTERN_ROWS(false, 64)
 FGW_KV_EXTERN_ROWS(false, 128) FGW_KV_EXTERN_ROWS(false, 256)
 
-namespace {
+typedef hipError_t (*ExtendLaunch)(const ExtendParams&, int, hipStream_t);
 
-constexpr int kRowsTile = 32, kRowsBlock = 32;
-
-int dim_tile(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-
-// One launch of a kernel: its items at most, and whether tiles may be split.
-struct Launch {
-  int64_t tiles;  // at most, of one K/V head
-  int64_t items;  // at most: the grid
-  int target, min_chunk;
-  int64_t floats;  // of workspace
-  int rows_tile;
-};
-
-// find_item cuts a tile into at most blocks / chunk + 1 splits with chunk >= visits / target, so
-// there are at most target + tiles * kv_heads items (and two for the rounding of the sum), and no
-// more than every tile cut as far as the table's capacity allows.
-Launch plan_launch(const fgw_kv_extend_args& a, int64_t tiles, int64_t tiles_sure, int rows_tile,
-                   int block, int target, int min_chunk) {
-  const int64_t capacity = (int64_t)a.width * a.page_size;
-  int64_t keys = capacity;
-  if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + a.max_new);
-  const int64_t blocks = (keys + block - 1) / block + 1;
-  const int64_t most = (blocks + min_chunk - 1) / min_chunk;
-  Launch l{tiles, tiles * a.kv_heads, 0, min_chunk, 0, rows_tile};
-  if (most > 1 && tiles_sure * a.kv_heads < 4 * (int64_t)target) {
-    l.target = target;
-    l.items = std::min(tiles * a.kv_heads * most, target + target / 1024 + 2 + tiles * a.kv_heads);
-    l.floats = l.items * rows_tile * (a.dim + 1);
-  }
-  return l;
+template <bool BF16>
+static ExtendLaunch rows_entry(int dim) {
+  return dim <= 32    ? &launch_extend_rows<BF16, 32>
+         : dim <= 64  ? &launch_extend_rows<BF16, 64>
+         : dim <= 128 ? &launch_extend_rows<BF16, 128>
+                      : &launch_extend_rows<BF16, 256>;
 }
 
-Launch plan_rows(const fgw_kv_extend_args& a) {
-  const int64_t group = a.heads / a.kv_heads;
-  const int64_t most = std::min<int64_t>(a.max_new, a.tokens);
-  const int64_t tiles = std::min<int64_t>(a.batch * ((most * group + kRowsTile - 1) / kRowsTile),
-                                          a.tokens * group / kRowsTile + std::min(a.batch, a.tokens));
-  const int64_t sure = std::max<int64_t>(a.tokens * group / kRowsTile, a.tokens / most);
-  return plan_launch(a, tiles, sure, kRowsTile, kRowsBlock, 2 * a.num_cus, 8);
+// Head dims up to 128. Keys of one DMA instruction: 1024 bytes / (2 * head-dim tile).
+template <bool BF16>
+static ExtendLaunch long_entry(int dim, int page) {
+  if (dim == 128)
+    return page % LongTiling::BN == 0 ? &launch_extend_long<BF16, 128, kRowsBlock>
+           : page % 4 == 0        ? &launch_extend_long<BF16, 128, kRowsGroup>
+                                  : &launch_extend_long<BF16, 128, kRowsPadded>;
+  if (dim == 64)
+    return page % LongTiling::BN == 0 ? &launch_extend_long<BF16, 64, kRowsBlock>
+           : page % 8 == 0        ? &launch_extend_long<BF16, 64, kRowsGroup>
+                                  : &launch_extend_long<BF16, 64, kRowsPadded>;
+  return dim < 64 ? &launch_extend_long<BF16, 64, kRowsPadded> : &launch_extend_long<BF16, 128, kRowsPadded>;
+}
+
+namespace {
+
+// One launch of a kernel over the requests with rows_from < n * group <= rows_to.
+struct Launch {
+  int rows_from, rows_to;
+  int target, min_chunk;     // ExtendParams
+  int64_t tiles;             // at most, of one K/V head
+  int64_t items;             // at most: the grid; 0: no launch
+  int64_t slots;             // places for partials and notes
+  int64_t floats, counters;  // of workspace
+};
+
+// Splits of a tile at most: of the table's capacity, or the window's span.
+template <class T>
+int64_t most_splits(const fgw_kv_extend_args& a, int min_chunk) {
+  int64_t keys = (int64_t)a.width * a.page_size;
+  if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + a.max_new);
+  return ((keys + T::KEYS - 1) / T::KEYS + 1 + min_chunk - 1) / min_chunk;
+}
+
+// Grid and workspace of a launch: where tiles may be split (best_chunk) all items together are at
+// most one to a CU; else there are as many as tiles.
+template <class T>
+void plan_items(Launch& l, const fgw_kv_extend_args& a, bool may_split) {
+  l.items = l.tiles * a.kv_heads;
+  const int64_t most = most_splits<T>(a, l.min_chunk);
+  if (!may_split || most <= 1 || a.num_cus / a.kv_heads <= 1) return;
+  l.target = a.num_cus;
+  l.slots = std::min<int64_t>(l.target, l.items * most);
+  l.items = std::max(l.items, l.slots);
+  l.floats = l.slots * (T::ROWS * (a.dim + 1) + (int64_t)sizeof(JoinNote) / 4);
+}
+
+struct Plan {
+  Launch rows, longs;
+};
+
+Plan plan(const fgw_kv_extend_args& a) {
+  const int64_t group = a.heads / a.kv_heads, total = a.tokens * group;
+  const int64_t rows_most = std::min(a.max_new, a.tokens) * group, batch = std::min(a.batch, a.tokens);
+  const int border = a.dim > 128 ? 0x7fffffff : kLongFrom;
+  auto tiles = [&](int64_t requests, int64_t rows, int64_t tile) {  // of so many requests at most
+    return std::min(requests * ((rows + tile - 1) / tile), total / tile + requests);
+  };
+  Plan p = {};
+  p.rows.rows_to = border;
+  p.rows.min_chunk = kRowsMinChunk;
+  p.rows.tiles = tiles(batch, std::min<int64_t>(rows_most, border), ShortTiling::ROWS);
+  plan_items<ShortTiling>(p.rows, a, true);
+  p.rows.counters = p.rows.slots * fgw_mha::kArrivalStride;
+  if (rows_most > border) {
+    p.longs.rows_from = border;
+    p.longs.rows_to = 0x7fffffff;
+    p.longs.min_chunk = kLongMinChunk;
+    p.longs.tiles = tiles(std::min(batch, total / border), rows_most, LongTiling::ROWS);
+    // (So many tokens that whole tiles fill the card four times over, unless most of them are
+    // padding: no workspace, and no launch for joins.)
+    plan_items<LongTiling>(p.longs, a, total / LongTiling::ROWS * a.kv_heads < 4 * (int64_t)a.num_cus);
+  }
+  return p;
 }
 
 int check(const fgw_kv_extend_args* a) {
@@ -86,25 +148,33 @@ int check(const fgw_kv_extend_args* a) {
 
 }  // namespace
 
-// At most `tiles` tiles of a launch; joins take 16 rows' workgroups of a tile each.
 template <bool BF16>
-static int run_rows(const ExtendParams& p, const Launch& l, int dpad, hipStream_t stream) {
-  hipError_t e;
-  switch (dpad) {
-    case 32: e = launch_extend_rows<BF16, 32>(p, (int)l.items, stream); break;
-    case 64: e = launch_extend_rows<BF16, 64>(p, (int)l.items, stream); break;
-    case 128: e = launch_extend_rows<BF16, 128>(p, (int)l.items, stream); break;
-    default: e = launch_extend_rows<BF16, 256>(p, (int)l.items, stream); break;
-  }
+static int run(const ExtendParams& base, const Plan& plan, hipStream_t stream) {
+  ExtendParams rows = base, longs = base;
+  float* work = base.parts;
+  auto place = [&](ExtendParams& p, const Launch& l, int rows_tile) {
+    p.rows_from = l.rows_from;
+    p.rows_to = l.rows_to;
+    p.target = l.target;
+    p.min_chunk = l.min_chunk;
+    p.work = (int)l.slots;
+    p.notes = l.target > 0 && !p.counters ? reinterpret_cast<int32_t*>(work + l.slots * rows_tile * (p.dim + 1)) : nullptr;
+    p.parts = work;
+    p.lse = work + l.slots * rows_tile * p.dim;
+    work += l.floats;
+  };
+  longs.counters = nullptr;
+  place(rows, plan.rows, ShortTiling::ROWS);
+  place(longs, plan.longs, LongTiling::ROWS);
+  hipError_t e = hipSuccess;
+  if (plan.longs.items > 0) e = long_entry<BF16>(base.dim, base.page_size)(longs, (int)plan.longs.items, stream);
+  if (e == hipSuccess) e = rows_entry<BF16>(base.dim)(rows, (int)plan.rows.items, stream);
   if (e != hipSuccess) return fail(FGW_MHA_EHIP, "fgw_kv_extend: %s", hipGetErrorString(e));
-  if (l.target > 0) {
-    const int64_t rows = std::min<int64_t>(kRowsTile, (int64_t)std::min(p.max_new, p.tokens) * p.group);
-    extend_join_kernel<BF16, kRowsTile, kRowsBlock, true>
-        <<<dim3((unsigned)(l.tiles * p.heads), (unsigned)rows), dim3(kMergeThreads), 0, stream>>>(
-            p, p.lengths, p.cu);
-    return launched("fgw_kv_extend");
-  }
-  return FGW_MHA_OK;
+  const int rows_items = rows.notes ? rows.work : 0, long_items = longs.notes ? longs.work : 0;
+  if (rows_items + long_items == 0) return FGW_MHA_OK;
+  extend_join_kernel<BF16><<<dim3((unsigned)(rows_items + long_items), long_items > 0 ? kJoinParts : 1),
+                             dim3(kMergeThreads), 0, stream>>>(rows, longs, rows_items);
+  return launched("fgw_kv_extend");
 }
 
 }  // namespace fgw_kv
@@ -113,9 +183,13 @@ using namespace fgw_kv;
 
 extern "C" {
 
-int fgw_kv_extend_workspace(const fgw_kv_extend_args* args, int64_t* floats) {
+int fgw_kv_extend_workspace(const fgw_kv_extend_args* args, int64_t* floats, int64_t* counters) {
   if (int rc = check(args)) return rc;
-  *floats = args->tokens == 0 ? 0 : plan_rows(*args).floats;
+  *floats = *counters = 0;
+  if (args->tokens == 0) return FGW_MHA_OK;
+  const Plan l = plan(*args);
+  *floats = l.rows.floats + l.longs.floats;
+  *counters = l.rows.counters;
   return FGW_MHA_OK;
 }
 
@@ -128,9 +202,10 @@ int fgw_kv_extend(const fgw_kv_extend_args* args, hipStream_t stream) {
   if (!aligned16(a.q.data) || !aligned16(a.out) || !aligned16(a.k_cache) || !aligned16(a.v_cache) ||
       a.q.token_stride % 8 || a.q.head_stride % 8)
     return fail(FGW_MHA_EINVAL, "rows must be 16-byte aligned, their strides multiples of 16 bytes");
-  const Launch l = plan_rows(a);
-  if (l.items > 0x7fffffff) return fail(FGW_MHA_EUNSUPPORTED, "too many rows for one call");
-  if (l.floats > 0 && (!a.workspace || !aligned16(a.workspace)))
+  const Plan l = plan(a);
+  if (std::max(l.rows.items, l.longs.items) > 0x3fffffff)
+    return fail(FGW_MHA_EUNSUPPORTED, "too many rows for one call");
+  if (l.rows.floats + l.longs.floats > 0 && (!a.workspace || !aligned16(a.workspace)))
     return fail(FGW_MHA_EINVAL, "the workspace is missing");
   ExtendParams p = {};
   p.q = a.q.data;
@@ -143,7 +218,7 @@ int fgw_kv_extend(const fgw_kv_extend_args* args, hipStream_t stream) {
   p.cu = a.cu_seqlens;
   p.out = a.out;
   p.parts = a.workspace;
-  p.lse = a.workspace ? a.workspace + l.items * l.rows_tile * a.dim : nullptr;
+  p.counters = l.rows.counters > 0 ? a.counters : nullptr;
   p.pool_rows = a.pool_rows;
   p.batch = a.batch;
   p.heads = a.kv_heads;
@@ -158,13 +233,7 @@ int fgw_kv_extend(const fgw_kv_extend_args* args, hipStream_t stream) {
   p.group = a.heads / a.kv_heads;
   p.max_new = std::min(a.max_new, a.tokens);
   p.window = a.window;
-  p.rows_from = 0;
-  p.rows_to = 0x7fffffff;
-  p.work = (int)l.items;
-  p.target = l.target;
-  p.min_chunk = l.min_chunk;
-  return a.dtype == FGW_KV_BFLOAT16 ? run_rows<true>(p, l, dim_tile(a.dim), stream)
-                                    : run_rows<false>(p, l, dim_tile(a.dim), stream);
+  return a.dtype == FGW_KV_BFLOAT16 ? run<true>(p, l, stream) : run<false>(p, l, stream);
 }
 
 }  // extern "C"

@@ -11,8 +11,10 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <map>
 #include <stdexcept>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/fgw_kv.h"
@@ -280,6 +282,25 @@ PyObject* append(Args& a) {
   return THPVariable_Wrap(std::move(q_out));
 }
 
+// Arrival counters of the fused joins: one zeroed buffer per (device, stream), grown as calls need
+// more. Every call leaves its counters at zero, so calls in stream order share them; calls on other
+// streams have their own. A captured call takes none (its replays may run on any stream): its
+// tiles are joined by a second launch, with the same arithmetic. Buffers live until the process
+// ends, replaced ones too, since a kernel in flight may count in them.
+int32_t* arrival_counters(const c10::Device& device, hipStream_t stream, int64_t need) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream, &status) != hipSuccess || status != hipStreamCaptureStatusNone)
+    return nullptr;
+  static auto* buffers = new std::map<std::pair<int, uintptr_t>, at::Tensor>();
+  static auto* retired = new std::vector<at::Tensor>();
+  at::Tensor& buffer = (*buffers)[{device.index(), reinterpret_cast<uintptr_t>(stream)}];
+  if (!buffer.defined() || buffer.numel() < need) {
+    if (buffer.defined()) retired->push_back(buffer);
+    buffer = at::zeros({need}, at::TensorOptions().device(device).dtype(at::kInt));
+  }
+  return static_cast<int32_t*>(buffer.data_ptr());
+}
+
 // (q, k_cache, v_cache, table, lens, cu, max_new, page, heads, kv_heads, dim, bf16, device, causal,
 //  window, scale, num_cus, out | None) -> out
 PyObject* extend(Args& a) {
@@ -317,8 +338,8 @@ PyObject* extend(Args& a) {
   r.batch = size32(batch);
   r.width = size32(table.size(1));
   need(r.max_new > 0, "max_new must be positive");
-  int64_t floats = 0;
-  check(entries.extend_workspace(&r, &floats));
+  int64_t floats = 0, counters = 0;
+  check(entries.extend_workspace(&r, &floats, &counters));
   const c10::DeviceGuard guard(device);
   if (out.defined()) {
     need(same_sizes(out, q) && out.scalar_type() == q.scalar_type(), "out does not match the rows");
@@ -334,7 +355,9 @@ PyObject* extend(Args& a) {
     work = at::empty({floats}, q.options().dtype(at::kFloat));
     r.workspace = static_cast<float*>(work.data_ptr());
   }
-  check(entries.extend(&r, stream_of(device)));
+  const hipStream_t stream = stream_of(device);
+  if (counters > 0) r.counters = arrival_counters(device, stream, counters);
+  check(entries.extend(&r, stream));
   return THPVariable_Wrap(std::move(out));
 }
 

@@ -101,7 +101,10 @@ typedef struct {
   const int32_t* block_table;
   const int32_t* cache_seqlens;
   const int32_t* cu_seqlens;
-  float* workspace; /* fgw_kv_extend_workspace floats, or NULL if that is 0 */
+  float* workspace; /* the floats of fgw_kv_extend_workspace, or NULL if that is 0 */
+  int32_t* counters; /* NULL (parts of split tiles are joined by a second launch), or the counters of
+                        fgw_kv_extend_workspace, all zero: the last program of a tile joins it and
+                        leaves its counter at zero. Calls that may overlap need their own. */
   int64_t pool_rows;
   int32_t tokens, batch, heads, kv_heads, dim, width, page_size;
   int32_t max_new;  /* no request has more new tokens than this (more are not computed) */
@@ -111,8 +114,9 @@ typedef struct {
   float scale;      /* of the scores */
 } fgw_kv_extend_args;
 
-/* fp32 elements that a call with these sizes needs (pointers are not read); pure host function. */
-int fgw_kv_extend_workspace(const fgw_kv_extend_args* args, int64_t* floats);
+/* fp32 elements of workspace and int32 counters that a call with these sizes can use (pointers are
+ * not read; 0 counters: none of its joins is fused); pure host function. */
+int fgw_kv_extend_workspace(const fgw_kv_extend_args* args, int64_t* floats, int64_t* counters);
 int fgw_kv_extend(const fgw_kv_extend_args* args, hipStream_t stream);
 
 /* Books of the pages, on the device: refs [pages] int32 holders of each page (0: free), table

@@ -422,7 +422,7 @@ class _Rows(ctypes.Structure):
 
 class _Extend(ctypes.Structure):
     _fields_ = [("q", _Rows)] + [(n, ctypes.c_void_p) for n in (
-        "out", "k_cache", "v_cache", "block_table", "cache_seqlens", "cu_seqlens", "workspace")] + [
+        "out", "k_cache", "v_cache", "block_table", "cache_seqlens", "cu_seqlens", "workspace", "counters")] + [
         ("pool_rows", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in (
             "tokens", "batch", "heads", "kv_heads", "dim", "width", "page_size", "max_new", "causal", "window",
             "dtype", "num_cus")] + [("scale", ctypes.c_float)]
@@ -456,10 +456,11 @@ def test_c_entry_refusals(changes, message):
 
 def test_workspace_is_bounded_by_the_sizes():
     lib = _lib.load()
-    floats = ctypes.c_int64()
+    floats, counters = ctypes.c_int64(), ctypes.c_int64()
 
     def need(**changes):
-        assert lib.fgw_kv_extend_workspace(ctypes.byref(_extend_args(**changes)), ctypes.byref(floats)) == 0
+        assert lib.fgw_kv_extend_workspace(ctypes.byref(_extend_args(**changes)), ctypes.byref(floats),
+                                           ctypes.byref(counters)) == 0
         return floats.value
 
     assert need(width=8) == 0            # 128 keys: nothing to split
