@@ -46,6 +46,7 @@ struct Tiling {
 };
 typedef Tiling<32, 32, 4> ShortTiling;   // extend_rows_kernel: a round of its four waves
 typedef Tiling<256, 64, 1> LongTiling;   // extend_long_kernel
+typedef Tiling<128, 64, 1> WideTiling;   // extend_wide_kernel
 
 struct Request {
   int first, n, len, tiles, units;
@@ -257,8 +258,8 @@ __device__ __forceinline__ void write_note(const ExtendParams& p, const Item& it
 
 // The splits g, g + share, ... of one (row, 4 dims) into a state; CH of them are loaded before any is
 // used.
-template <int ROWS, bool COH, int CH>
-__device__ __forceinline__ void join_splits(const ExtendParams& p, const Item& it, int r, int c, int g, int share,
+template <bool COH, int CH>
+__device__ __forceinline__ void join_splits(const ExtendParams& p, const Item& it, int tile_rows, int r, int c, int g, int share,
                                             float& peak, float& tot, f32x4& acc) {
   for (int s0 = g; s0 < it.splits; s0 += CH * share) {
     float x[CH];
@@ -266,7 +267,7 @@ __device__ __forceinline__ void join_splits(const ExtendParams& p, const Item& i
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       const int split = s0 + k * share < it.splits ? s0 + k * share : g;  // (weight 0 below)
-      const u32 at = (u32)(it.slot0 + split * it.slot_step) * ROWS + (u32)r;
+      const u32 at = (u32)(it.slot0 + split * it.slot_step) * (u32)tile_rows + (u32)r;
       if constexpr (COH) {
         x[k] = device_load1(p.lse, 4u * at);
         v[k] = device_load4(p.parts, 4u * (at * (u32)p.dim + 4u * (u32)c));
@@ -299,8 +300,8 @@ __device__ __forceinline__ void join_splits(const ExtendParams& p, const Item& i
 // dims of a row; where rows and dims leave threads over, they share its splits. Weights exp(LSE -
 // peak), empty splits (LSE -1e30) weigh nothing, an all-empty row is zero. COH: the partials were
 // written by this launch. Uses 24 bytes of LDS a thread.
-template <bool BF16, int ROWS, bool COH>
-__device__ __forceinline__ void join_rows(const ExtendParams& p, const Item& it, int row_from, int row_to,
+template <bool BF16, bool COH>
+__device__ __forceinline__ void join_rows(const ExtendParams& p, const Item& it, int tile_rows, int row_from, int row_to,
                                           unsigned char* lds, int tid, int threads) {
   using E = Elem<BF16>;
   f32x4* const sacc = reinterpret_cast<f32x4*>(lds);
@@ -316,11 +317,11 @@ __device__ __forceinline__ void join_rows(const ExtendParams& p, const Item& it,
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     if (act) {
       if (it.splits <= 2 * share)
-        join_splits<ROWS, COH, 2>(p, it, r, c, g, share, peak, tot, acc);
+        join_splits<COH, 2>(p, it, tile_rows, r, c, g, share, peak, tot, acc);
       else if (it.splits <= 4 * share)
-        join_splits<ROWS, COH, 4>(p, it, r, c, g, share, peak, tot, acc);
+        join_splits<COH, 4>(p, it, tile_rows, r, c, g, share, peak, tot, acc);
       else
-        join_splits<ROWS, COH, 8>(p, it, r, c, g, share, peak, tot, acc);
+        join_splits<COH, 8>(p, it, tile_rows, r, c, g, share, peak, tot, acc);
     }
     if (share > 1) {  // uniform
       sacc[tid] = acc;
@@ -345,12 +346,154 @@ __device__ __forceinline__ void join_rows(const ExtendParams& p, const Item& it,
       u32x2 w;
       w.x = E::pack2(acc[0] * inv, acc[1] * inv);
       w.y = E::pack2(acc[2] * inv, acc[3] * inv);
-      *reinterpret_cast<u32x2*>(static_cast<u16*>(p.out) + out_row(p, it, it.tile * ROWS + r) + 4 * c) = w;
+      *reinterpret_cast<u32x2*>(static_cast<u16*>(p.out) + out_row(p, it, it.tile * tile_rows + r) + 4 * c) = w;
     }
   }
 }
 
 // ---- requests of few rows -----------------------------------------------------------------------
+
+// The DMA of the 32-key tiles that one wave helps to fetch, tile n at key first_pos + step n, in tiles
+// laid out as fwd_kernel's (C: its Cfg, of which the NWQ waves of a key group share a tile). The
+// loads are inline assembly (dma_saddr, dma_flat): the compiler would wait for all of them before
+// each transposing read of V; the kernels place the waits. Row offsets come from page ids that lane
+// l holds for the wave's load instruction l % U of tile l / U, four such windows read at a time: a
+// read in the main loop would wait for the DMA in front of it (AHEAD false, for loops that wait for
+// all of it anyway: one window, in fewer registers).
+// Keys outside [lo, hi) or in pages outside the pool read zeros, and so do dims past D. Tiles with
+// an instruction whose keys straddle pages are resolved key by key.
+template <class C, bool AHEAD = true>
+struct KeyStream {
+  static constexpr int U = C::INSTR_PER_WAVE;
+  static constexpr int kWindow = 64 / U;  // tiles of a window
+  static constexpr int kAllLive = C::RPI << 8;
+  static_assert(C::BN == 32, "tiles of 32 keys");
+  const int32_t* const table_b;
+  const char* const kb;
+  const char* const vb;
+  const int64_t row_bytes;
+  const int lane, wq, first_pos, step, my_n, lo, hi, dim;
+  const u32 page, page_magic, page_shift, last_page;
+  const int64_t pool_rows;
+  int32_t id0 = 0, id1 = 0, id2 = 0, id3 = 0;
+  // The lane's unit in the current window: pool byte offset of its first key (-1: it straddles
+  // pages), and its live keys [live & 255, live >> 8).
+  int64_t off = 0;
+  int live = 0;
+
+  __device__ __forceinline__ KeyStream(const ExtendParams& p, const int32_t* table, const Item& it, int lane_,
+                                       int wq_, int first_pos_, int step_, int my_n_)
+      : table_b(table + (int64_t)it.b * p.width),
+        kb(static_cast<const char*>(p.k) + (int64_t)it.head * p.dim * 2),
+        vb(static_cast<const char*>(p.v) + (int64_t)it.head * p.dim * 2),
+        row_bytes((int64_t)p.heads * p.dim * 2), lane(lane_),
+        wq(wq_), first_pos(first_pos_), step(step_), my_n(my_n_), lo(it.lo), hi(it.hi),
+        dim(p.dim), page((u32)p.page_size), page_magic(p.page_magic), page_shift(p.page_shift),
+        last_page((u32)p.width - 1u), pool_rows(p.pool_rows) {
+    if (my_n > 0) read_ids(0);
+  }
+  __device__ __forceinline__ int unit_pos(int n) const {
+    return first_pos + step * n + C::RPI * (lane % U * C::NWQ + wq);
+  }
+  __device__ __forceinline__ int32_t read_id(int n0) const {
+    const u32 pg = div_page((u32)unit_pos(n0 + lane / U), page_magic, page_shift);
+    return table_b[pg < last_page ? pg : last_page];
+  }
+  __device__ __forceinline__ void read_ids(int n0) {
+    id0 = read_id(n0);
+    if constexpr (!AHEAD) return;
+    id1 = read_id(n0 + kWindow);
+    id2 = read_id(n0 + 2 * kWindow);
+    id3 = read_id(n0 + 3 * kWindow);
+  }
+  // The compiler's wait for the page ids comes here.
+  __device__ __forceinline__ void ids_ready() const {
+    if (my_n <= 0) return;
+    asm volatile("" ::"v"(id0));
+    if constexpr (AHEAD) asm volatile("" ::"v"(id1), "v"(id2), "v"(id3));
+  }
+  __device__ __forceinline__ void set_window(int n0) {
+    const int w = AHEAD ? n0 / kWindow % 4 : 0;
+    if (w == 0 && n0 > 0) read_ids(n0);
+    const int32_t a = id0, b = id1, c = id2, d = id3;  // (values: a choice of members would keep them in memory)
+    const int32_t id = w == 0 ? a : w == 1 ? b : w == 2 ? c : d;
+    const int n = n0 + lane / U, pos = unit_pos(n);
+    const u32 pg = div_page((u32)pos, page_magic, page_shift), in_page = (u32)pos - pg * page;
+    const int64_t row0 = (int64_t)id * page + in_page;
+    const int from = lo > pos ? lo - pos : 0, to = hi - pos < C::RPI ? hi - pos : C::RPI;
+    const bool any = n < my_n && to > from;
+    const bool inside = row0 >= 0 && row0 + C::RPI <= pool_rows;
+    const bool straddles = any && in_page + C::RPI > page;
+    off = straddles ? -1 : any && inside ? row0 * row_bytes : 0;
+    live = any && inside ? from | to << 8 : 0;
+  }
+  // The wave's part of the K (IS_V false) or V tile n into LDS at dst; tiles in order, K before V.
+  template <bool IS_V>
+  __device__ __forceinline__ void issue(const DmaLanes<C>& dl, int n, u32 dst) {
+    if (!IS_V && n % kWindow == 0) set_window(n);
+    const char* base = IS_V ? vb : kb;
+    const int first = n % kWindow * U;
+    constexpr uint64_t kUnits = (1ull << U) - 1ull;
+    if ((__ballot(live != kAllLive || off < 0) >> first & kUnits) == 0 && dim == C::DPAD) {
+#pragma unroll
+      for (int q = 0; q < U; ++q)
+        dma_saddr(base + readlane64(off, first + q), IS_V ? dl.vq(q, wq) : dl.kq(q, wq),
+                  dst + 1024u * (u32)(q * C::NWQ + wq));
+      return;
+    }
+    if (__ballot(off < 0) >> first & kUnits) {
+      issue_keys<IS_V>(base, first_pos + step * n, dst);
+      return;
+    }
+    const char* zero = reinterpret_cast<const char*>(kZeroChunk);
+    const int lr = opaque_lane(lane) / C::CPR;
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      const char* const src = base + readlane64(off, first + q);
+      const int keys = __builtin_amdgcn_readlane(live, first + q);
+      const u32 at = IS_V ? dl.vq(q, wq) : dl.kq(q, wq);
+      const bool in = lr >= (keys & 255) && lr < keys >> 8 && at - dl.row_off < 2u * (u32)dim;
+      dma_flat(in ? src + at : zero, dst + 1024u * (u32)(q * C::NWQ + wq));
+    }
+  }
+  // The same, each key through the table: lane l (mod 32) resolves key l, the load instructions fetch
+  // their rows' offsets from those lanes.
+  template <bool IS_V>
+  __device__ __forceinline__ void issue_keys(const char* base, int pos0, u32 dst) {
+    const int ln = opaque_lane(lane);
+    const char* zero = reinterpret_cast<const char*>(kZeroChunk);
+    const int pos = pos0 + (ln & 31);
+    const bool in = pos >= lo && pos < hi;
+    const u32 pg = in ? div_page((u32)pos, page_magic, page_shift) : 0u;
+    const int64_t row = (int64_t)table_b[pg] * page + ((u32)pos - pg * page);
+    const int64_t ro_own = in && row >= 0 && row < pool_rows ? row * row_bytes : -1;
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      const int i = q * C::NWQ + wq, r = C::RPI * i + ln / C::CPR, at = ln % C::CPR;
+      const u32 rl = (u32)__builtin_amdgcn_ds_bpermute(4 * r, (int)(u32)ro_own);
+      const u32 rh = (u32)__builtin_amdgcn_ds_bpermute(4 * r, (int)((uint64_t)ro_own >> 32));
+      const int64_t ro = (int64_t)(((uint64_t)rh << 32) | rl);
+      const int c = IS_V ? at ^ (4 * (r % C::VSW)) : at ^ (r % C::KSW);
+      dma_flat(ro >= 0 && c * 8 < dim ? base + ro + c * 16 : zero, dst + 1024u * (u32)i);
+    }
+  }
+};
+
+// Q^T operands of the lane's row of an item's tile (row `in_tile` of it): dims 16 kk + 8 hh ..
+template <class C>
+__device__ __forceinline__ void load_q(const ExtendParams& p, const Item& it, int row, bool mine, int hh,
+                                       u32x4 (&qf)[C::KK]) {
+  const int token = row / p.group, in_group = row - token * p.group;
+  const char* qp = static_cast<const char*>(p.q) + (int64_t)(it.first + token) * p.q_token +
+                   (int64_t)(it.head * p.group + in_group) * p.q_head;
+#pragma unroll
+  for (int kk = 0; kk < C::KK; ++kk) {
+    const int d = 16 * kk + 8 * hh;
+    u32x4 val = {0u, 0u, 0u, 0u};
+    if (mine && d < p.dim) val = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(qp + 2 * d));
+    qf[kk] = val;
+  }
+}
 
 // Rows that few requests' tokens fill: 32 rows to a tile, four waves that each stream their own
 // 32-key blocks of the tile through LDS and meet at its end (the key layout of fwd_kernel, whose
@@ -358,38 +501,11 @@ __device__ __forceinline__ void join_rows(const ExtendParams& p, const Item& it,
 //
 // Each wave keeps kStages blocks of its own on the way: the K tile of block n + kStages is issued
 // as soon as the scores of block n are computed, its V tile after the products of block n, and the
-// waits count the half blocks issued since. The loads are inline assembly (dma_saddr, dma_flat): the
-// compiler would wait for all of them before each transposing read of V. Their row offsets come
-// from page ids that lane l holds for load instruction l % INSTR of block l / INSTR, four such
-// windows read at a time: a read in the loop would wait for the DMA in front of it.
-// Keys outside [lo, hi) or in pages outside the pool read zeros, and so do dims past D. Blocks with
-// an instruction whose keys straddle pages are resolved key by key.
+// waits count the half blocks issued since. One stage at head-dim tile 128 leaves room for two
+// workgroups on a CU, which pays where tiles are short (B 256, lengths 75-300: 51 us, 74 with two
+// stages and one workgroup) and costs nothing where they are long.
 template <int DPAD>
 constexpr int kStages = DPAD >= 128 ? 1 : DPAD == 64 ? 2 : 4;
-
-// The K (IS_V false) or V tile of the keys [pos0, pos0 + 32), each through the table: lane l (mod 32)
-// resolves key l, the load instructions fetch their rows' offsets from those lanes.
-template <class C, bool IS_V>
-__device__ __forceinline__ void issue_block_keys(const ExtendParams& p, const int32_t* table_b, const char* base,
-                                                 int64_t row_bytes, int pos0, int lo, int hi, u32 dst, int lane) {
-  const int dim = opaque_uniform(p.dim);
-  lane = opaque_lane(lane);
-  const char* zero = reinterpret_cast<const char*>(kZeroChunk);
-  const int pos = pos0 + (lane & 31);
-  const bool in = pos >= lo && pos < hi;
-  const u32 pg = in ? div_page((u32)pos, p.page_magic, p.page_shift) : 0u;
-  const int64_t row = (int64_t)table_b[pg] * p.page_size + ((u32)pos - pg * (u32)p.page_size);
-  const int64_t off = in && row >= 0 && row < p.pool_rows ? row * row_bytes : -1;
-#pragma unroll
-  for (int q = 0; q < C::INSTR; ++q) {
-    const int r = C::RPI * q + lane / C::CPR, at = lane % C::CPR;
-    const u32 rl = (u32)__builtin_amdgcn_ds_bpermute(4 * r, (int)(u32)off);
-    const u32 rh = (u32)__builtin_amdgcn_ds_bpermute(4 * r, (int)((uint64_t)off >> 32));
-    const int64_t ro = (int64_t)(((uint64_t)rh << 32) | rl);
-    const int c = IS_V ? at ^ (4 * (r % C::VSW)) : at ^ (r % C::KSW);
-    dma_flat(ro >= 0 && c * 8 < dim ? base + ro + c * 16 : zero, dst + 1024u * q);
-  }
-}
 
 // Waits until K (V) of a block has landed with `rem` further blocks of the wave to come: behind K
 // are V and the halves of the next kStages - 1 blocks, behind V those and one K more.
@@ -424,11 +540,6 @@ __device__ __forceinline__ void extend_tile(const ExtendParams& p, const int32_t
   const int lane = tid & 63;
   const int il = lane & 31, hh = lane >> 5;
   const Lanes<C> ln(lane);
-  const int64_t row_bytes = (int64_t)p.heads * p.dim * 2;
-  const DmaLanes<C> dl(lane, 0, row_bytes);
-  const int32_t* table_b = table + (int64_t)it.b * p.width;
-  const char* kb = static_cast<const char*>(p.k) + (int64_t)it.head * p.dim * 2;
-  const char* vb = static_cast<const char*>(p.v) + (int64_t)it.head * p.dim * 2;
   constexpr int S = kStages<C::DPAD>;
   unsigned char* const stages = smem + wave * S * C::STAGE_BYTES;
   const u32 stages_lds = lds_address(stages);
@@ -438,87 +549,17 @@ __device__ __forceinline__ void extend_tile(const ExtendParams& p, const int32_t
   const int cnt = it.blk_end - it.blk_begin;
   const int my_n = cnt > wave ? (cnt - wave + C::NWK - 1) / C::NWK : 0;
   const int first_pos = (it.blk_begin + wave) * C::BN;
-  constexpr int kWindow = 64 / C::INSTR, kIds = 4;  // blocks of a window, windows read at a time
-  int32_t ids[kIds];
-  auto unit_pos = [&](int n) { return first_pos + kStep * n + C::RPI * (lane % C::INSTR); };
-  auto read_ids = [&](int n0) {
-#pragma unroll
-    for (int k = 0; k < kIds; ++k) {
-      const u32 pg = div_page((u32)unit_pos(n0 + k * kWindow + lane / C::INSTR), p.page_magic, p.page_shift);
-      const u32 last = (u32)p.width - 1u;
-      ids[k] = table_b[pg < last ? pg : last];
-    }
+  KeyStream<C> keys(p, table, it, lane, 0, first_pos, kStep, my_n);
+  const DmaLanes<C> dl(lane, 0, keys.row_bytes);
+  auto issue_k = [&](int n) { keys.template issue<false>(dl, n, stages_lds + (u32)(n % S * C::STAGE_BYTES)); };
+  auto issue_v = [&](int n) {
+    keys.template issue<true>(dl, n, stages_lds + (u32)(n % S * C::STAGE_BYTES) + (u32)C::TILE_BYTES);
   };
-  // The lane's unit in the current window: pool byte offset of its first key (-1: it straddles
-  // pages), and its live keys [live & 255, live >> 8).
-  constexpr int kAllLive = C::RPI << 8;
-  int64_t off = 0;
-  int live = 0;
-  auto set_window = [&](int n0) {
-    const int w = n0 / kWindow % kIds;
-    if (w == 0 && n0 > 0) read_ids(n0);
-    const int32_t id = w == 0 ? ids[0] : w == 1 ? ids[1] : w == 2 ? ids[2] : ids[3];
-    const int n = n0 + lane / C::INSTR, pos = unit_pos(n);
-    const u32 pg = div_page((u32)pos, p.page_magic, p.page_shift), in_page = (u32)pos - pg * (u32)p.page_size;
-    const int64_t row0 = (int64_t)id * p.page_size + in_page;
-    const int from = it.lo > pos ? it.lo - pos : 0, to = it.hi - pos < C::RPI ? it.hi - pos : C::RPI;
-    const bool any = n < my_n && to > from;
-    const bool inside = row0 >= 0 && row0 + C::RPI <= p.pool_rows;
-    const bool straddles = any && in_page + C::RPI > (u32)p.page_size;
-    off = straddles ? -1 : any && inside ? row0 * row_bytes : 0;
-    live = any && inside ? from | to << 8 : 0;
-  };
-  const bool full_dim = p.dim == C::DPAD;
-  // Half a block: its K (IS_V false) or V tile.
-  auto issue = [&](int n, auto is_v) {
-    constexpr bool IS_V = decltype(is_v)::value;
-    if (!IS_V && n % kWindow == 0) set_window(n);
-    const char* base = IS_V ? vb : kb;
-    const u32 dst = stages_lds + (u32)(n % S * C::STAGE_BYTES) + (IS_V ? (u32)C::TILE_BYTES : 0u);
-    const int first = n % kWindow * C::INSTR;
-    constexpr uint64_t kUnits = (1ull << C::INSTR) - 1ull;
-    if ((__ballot(live != kAllLive || off < 0) >> first & kUnits) == 0 && full_dim) {
-#pragma unroll
-      for (int q = 0; q < C::INSTR; ++q)
-        dma_saddr(base + readlane64(off, first + q), IS_V ? dl.vq(q, 0) : dl.kq(q, 0), dst + 1024u * q);
-      return;
-    }
-    if (__ballot(off < 0) >> first & kUnits) {
-      int pos0 = first_pos + kStep * n;
-      asm volatile("" : "+s"(pos0));
-      issue_block_keys<C, IS_V>(p, table_b, base, row_bytes, pos0, it.lo, it.hi, dst, lane);
-      return;
-    }
-    const char* zero = reinterpret_cast<const char*>(kZeroChunk);
-    const int lr = opaque_lane(lane) / C::CPR;
-#pragma unroll
-    for (int q = 0; q < C::INSTR; ++q) {
-      const char* const src = base + readlane64(off, first + q);
-      const int keys = __builtin_amdgcn_readlane(live, first + q);
-      const u32 at = IS_V ? dl.vq(q, 0) : dl.kq(q, 0);
-      const bool in = lr >= (keys & 255) && lr < keys >> 8 && at - dl.row_off < 2u * (u32)p.dim;
-      dma_flat(in ? src + at : zero, dst + 1024u * q);
-    }
-  };
-  constexpr std::false_type k_half{};
-  constexpr std::true_type v_half{};
-  if (my_n > 0) read_ids(0);
 
   const int row = it.tile * C::ROWS_TILE + il;
-  const int token = row / p.group, in_group = row - token * p.group;
-  const bool mine = il < it.rows;
+  const int token = row / p.group;
   u32x4 qf[C::KK];
-  {
-    const char* qp = static_cast<const char*>(p.q) + (int64_t)(it.first + token) * p.q_token +
-                     (int64_t)(it.head * p.group + in_group) * p.q_head;
-#pragma unroll
-    for (int kk = 0; kk < C::KK; ++kk) {
-      const int d = 16 * kk + 8 * hh;
-      u32x4 val = {0u, 0u, 0u, 0u};
-      if (mine && d < p.dim) val = load16(qp + 2 * d);
-      qf[kk] = val;
-    }
-  }
+  load_q<C>(p, it, row, il < it.rows, hh, qf);
   const Seen seen = row_seen(p, it, token);
   // Blocks with keys that some row of the tile does not see: past the first token's last key, or
   // below the last token's first.
@@ -533,10 +574,10 @@ __device__ __forceinline__ void extend_tile(const ExtendParams& p, const int32_t
     for (int v = 0; v < 16; ++v) o[dt][v] = 0.0f;
 
   // (The compiler's waits for page ids and Q, older than the DMA, come here and not in the loop.)
-  if (my_n > 0) asm volatile("" ::"v"(ids[0]), "v"(ids[1]), "v"(ids[2]), "v"(ids[3]));
+  keys.ids_ready();
   for (int n = 0; n < S && n < my_n; ++n) {
-    issue(n, k_half);
-    issue(n, v_half);
+    issue_k(n);
+    issue_v(n);
   }
 #pragma unroll
   for (int kk = 0; kk < C::KK; ++kk) asm volatile("" ::"v"(qf[kk]));
@@ -544,9 +585,9 @@ __device__ __forceinline__ void extend_tile(const ExtendParams& p, const int32_t
     const int pos0 = first_pos + kStep * n;
     const unsigned char* stage = stages + n % S * C::STAGE_BYTES;
     const int rem = my_n - 1 - n;
-    // One wave to a SIMD: nothing hides a chain of LDS reads and products but the block's own work.
-    // So all operands of a product are read at once (there are registers for them), the scores come
-    // in two chains, K's next tile is issued while they run, and V is read under the softmax.
+    // One or two waves to a SIMD hide little of a chain of LDS reads and products. So all operands of
+    // a product are read at once (there are registers for them), the scores come in two chains, K's
+    // next tile is issued while they run, and V is read under the softmax.
     u32x4 ka[C::KK], va[C::KS * C::DT], pf[C::KS];
     f32x16 s[1], t;
     wait_half<C, false>(rem);
@@ -563,7 +604,7 @@ __device__ __forceinline__ void extend_tile(const ExtendParams& p, const int32_t
       t = Elem<C::BF16>::mma(ka[kk + 1], qf[kk + 1], t);
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (rem >= S) issue(n + S, k_half);
+    if (rem >= S) issue_k(n + S);
     wait_half<C, true>(rem);
     asm volatile("" ::: "memory");
 #pragma unroll
@@ -575,7 +616,7 @@ __device__ __forceinline__ void extend_tile(const ExtendParams& p, const int32_t
     if (pos0 + C::BN > hi_min || pos0 < lo_max) mask_seen<C>(s, pos0, seen, hh);
     online_softmax<C>(s, m, l, o, p.scale_log2, pf);
     wait_lds();
-    if (rem >= S) issue(n + S, v_half);
+    if (rem >= S) issue_v(n + S);
 #pragma unroll
     for (int k2 = 0; k2 < C::KS; ++k2)
 #pragma unroll
@@ -669,7 +710,7 @@ __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void extend_row
   const bool last = *flag != 0;
   __syncthreads();  // LDS is written again
   if (!last) return;
-  join_rows<C::BF16, C::ROWS_TILE, true>(p, it, 0, it.rows, smem, tid, C::THREADS);
+  join_rows<C::BF16, true>(p, it, C::ROWS_TILE, 0, it.rows, smem, tid, C::THREADS);
   if (tid == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
@@ -681,27 +722,24 @@ template <bool BF16>
 __global__ __launch_bounds__(kMergeThreads) void extend_join_kernel(ExtendParams rows, ExtendParams longs,
                                                                     int rows_items) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[kMergeThreads * 24];
-  const bool is_long = (int)blockIdx.x >= rows_items;
-  if (!is_long && blockIdx.y > 0) return;
-  const ExtendParams& p = is_long ? longs : rows;
-  const int w = (int)blockIdx.x - (is_long ? rows_items : 0);
-  const JoinNote note = reinterpret_cast<const JoinNote*>(p.notes)[w];
-  if (note.splits < 2) return;
-  Item it;
-  it.first = note.first;
-  it.tile = note.tile;
-  it.head = note.head;
-  it.splits = note.splits;
-  it.slot0 = w - note.split * p.heads;
-  it.slot_step = p.heads;
-  const int parts = note.splits * (is_long ? kJoinParts : 1);
-  const int part = note.split * (is_long ? kJoinParts : 1) + (int)blockIdx.y;
-  const int from = note.rows * part / parts, to = note.rows * (part + 1) / parts;
-  if (from == to) return;
-  if (is_long)
-    join_rows<BF16, LongTiling::ROWS, false>(p, it, from, to, lds, threadIdx.x, kMergeThreads);
-  else
-    join_rows<BF16, ShortTiling::ROWS, false>(p, it, from, to, lds, threadIdx.x, kMergeThreads);
+  auto join = [&](const ExtendParams& p, int w, int tile_rows, int per_split) {
+    const JoinNote note = reinterpret_cast<const JoinNote*>(p.notes)[w];
+    if (note.splits < 2) return;
+    Item it;
+    it.first = note.first;
+    it.tile = note.tile;
+    it.head = note.head;
+    it.splits = note.splits;
+    it.slot0 = w - note.split * p.heads;
+    it.slot_step = p.heads;
+    const int parts = note.splits * per_split, part = note.split * per_split + (int)blockIdx.y;
+    const int from = note.rows * part / parts, to = note.rows * (part + 1) / parts;
+    if (from < to) join_rows<BF16, false>(p, it, tile_rows, from, to, lds, threadIdx.x, kMergeThreads);
+  };
+  if ((int)blockIdx.x >= rows_items)
+    join(longs, (int)blockIdx.x - rows_items, longs.dim > 128 ? WideTiling::ROWS : LongTiling::ROWS, kJoinParts);
+  else if (blockIdx.y == 0)
+    join(rows, (int)blockIdx.x, ShortTiling::ROWS, 1);
 }
 
 template <bool BF16, int DPAD>

@@ -7,6 +7,7 @@
 #include "kv_common.h"
 #include "kv_extend.h"
 #include "kv_extend_long.h"
+#include "kv_extend_wide.h"
 
 namespace fgw_kv {
 
@@ -14,7 +15,7 @@ namespace fgw_kv {
 // rows: it reads the keys once for every 32 of them, the long one once for 256. Hq 32, Hkv 8, D 128,
 // pages of 64, few rows / long, us: 128 rows B1 KV 1024 17.0 / 26.9, B4 KV 2048 24.3 / 36.6, B1 KV
 // 8192 26.4 / 37.2, B8 KV 8192 96.5 / 88.6; 192 rows 17.2 / 29.2, 29.9 / 39.3, 32.6 / 39.1,
-// 146 / 93.9. Above a head dim of 128 there is no long kernel.
+// 146 / 93.9.
 constexpr int kLongFrom = 128;
 // Units of a split at least (rounds of 128 keys, blocks of 64): below, a split's own cost outweighs
 // what it saves. Few rows, B1 Hq 32 Hkv 8 D 128 KV 4096, 1 / 2 / 4 rounds: 13.1 / 12.2 / 14.4 us;
@@ -25,6 +26,8 @@ constexpr int kRowsMinChunk = 2, kLongMinChunk = 4;
   extern template hipError_t launch_extend_long<BF, DP, kRowsBlock>(const ExtendParams&, int, hipStream_t); \
   extern template hipError_t launch_extend_long<BF, DP, kRowsGroup>(const ExtendParams&, int, hipStream_t); \
   extern template hipError_t launch_extend_long<BF, DP, kRowsPadded>(const ExtendParams&, int, hipStream_t);
+extern template hipError_t launch_extend_wide<true>(const ExtendParams&, int, hipStream_t);
+extern template hipError_t launch_extend_wide<false>(const ExtendParams&, int, hipStream_t);
 FGW_KV_EXTERN_LONG(true, 64) FGW_KV_EXTERN_LONG(true, 128)
 FGW_KV_EXTERN_LONG(false, 64) FGW_KV_EXTERN_LONG(false, 128)
 
@@ -45,9 +48,10 @@ static ExtendLaunch rows_entry(int dim) {
                       : &launch_extend_rows<BF16, 256>;
 }
 
-// Head dims up to 128. Keys of one DMA instruction: 1024 bytes / (2 * head-dim tile).
+// Keys of one DMA instruction: 1024 bytes / (2 * head-dim tile).
 template <bool BF16>
 static ExtendLaunch long_entry(int dim, int page) {
+  if (dim > 128) return &launch_extend_wide<BF16>;
   if (dim == 128)
     return page % LongTiling::BN == 0 ? &launch_extend_long<BF16, 128, kRowsBlock>
            : page % 4 == 0        ? &launch_extend_long<BF16, 128, kRowsGroup>
@@ -99,24 +103,28 @@ struct Plan {
 Plan plan(const fgw_kv_extend_args& a) {
   const int64_t group = a.heads / a.kv_heads, total = a.tokens * group;
   const int64_t rows_most = std::min(a.max_new, a.tokens) * group, batch = std::min(a.batch, a.tokens);
-  const int border = a.dim > 128 ? 0x7fffffff : kLongFrom;
   auto tiles = [&](int64_t requests, int64_t rows, int64_t tile) {  // of so many requests at most
     return std::min(requests * ((rows + tile - 1) / tile), total / tile + requests);
   };
   Plan p = {};
-  p.rows.rows_to = border;
+  p.rows.rows_to = kLongFrom;
   p.rows.min_chunk = kRowsMinChunk;
-  p.rows.tiles = tiles(batch, std::min<int64_t>(rows_most, border), ShortTiling::ROWS);
+  p.rows.tiles = tiles(batch, std::min<int64_t>(rows_most, kLongFrom), ShortTiling::ROWS);
   plan_items<ShortTiling>(p.rows, a, true);
   p.rows.counters = p.rows.slots * fgw_mha::kArrivalStride;
-  if (rows_most > border) {
-    p.longs.rows_from = border;
+  if (rows_most > kLongFrom) {
+    p.longs.rows_from = kLongFrom;
     p.longs.rows_to = 0x7fffffff;
     p.longs.min_chunk = kLongMinChunk;
-    p.longs.tiles = tiles(std::min(batch, total / border), rows_most, LongTiling::ROWS);
     // (So many tokens that whole tiles fill the card four times over, unless most of them are
     // padding: no workspace, and no launch for joins.)
-    plan_items<LongTiling>(p.longs, a, total / LongTiling::ROWS * a.kv_heads < 4 * (int64_t)a.num_cus);
+    const int64_t requests = std::min(batch, total / kLongFrom);
+    auto longs = [&](auto tiling) {
+      using T = decltype(tiling);
+      p.longs.tiles = tiles(requests, rows_most, T::ROWS);
+      plan_items<T>(p.longs, a, total / T::ROWS * a.kv_heads < 4 * (int64_t)a.num_cus);
+    };
+    if (a.dim > 128) longs(WideTiling{}); else longs(LongTiling{});
   }
   return p;
 }
@@ -165,7 +173,7 @@ static int run(const ExtendParams& base, const Plan& plan, hipStream_t stream) {
   };
   longs.counters = nullptr;
   place(rows, plan.rows, ShortTiling::ROWS);
-  place(longs, plan.longs, LongTiling::ROWS);
+  place(longs, plan.longs, base.dim > 128 ? WideTiling::ROWS : LongTiling::ROWS);
   hipError_t e = hipSuccess;
   if (plan.longs.items > 0) e = long_entry<BF16>(base.dim, base.page_size)(longs, (int)plan.longs.items, stream);
   if (e == hipSuccess) e = rows_entry<BF16>(base.dim)(rows, (int)plan.rows.items, stream);

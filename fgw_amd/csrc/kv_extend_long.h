@@ -69,6 +69,53 @@ __device__ __forceinline__ void issue_keys(const ExtendParams& p, const int32_t*
   dma_flat(live && c * 8 < dim ? base + row * row_bytes + c * 16 : zero, dst + 1024u * i);
 }
 
+// The 32 rows from `first_row` of an item's tile that one wave holds in o, m, l: to the output, or to
+// the partials of a split tile, whole rows through the wave's LDS at `st` (32 kStagedRowBytes<C>).
+template <class C>
+__device__ __forceinline__ void store_wave_rows(const ExtendParams& p, const Item& it, int first_row,
+                                                unsigned char* st, int lane, const f32x16 (&o)[C::DT], float m,
+                                                float l) {
+  const float tot = pair_sum(l), inv = 1.0f / fmaxf(tot, 1.0e-30f);
+  const bool split = it.splits > 1;
+  const int rows = it.rows - first_row;  // of this wave, where fewer than 32
+  const int ln = opaque_lane(lane), lr = ln & 31, lh = ln >> 5;
+  auto row_at = [&](int r) {
+    return static_cast<u16*>(p.out) + out_row(p, it, it.tile * C::ROWS_TILE + first_row + r);
+  };
+  float* const parts = p.parts + ((int64_t)it.slot * C::ROWS_TILE + first_row) * p.dim;
+  if (p.dim == C::DPAD) {
+    if (split) {
+      store_rows_staged<C>(st, lane, o, inv, true, parts, nullptr, 0, rows);
+    } else {
+      constexpr int NCH = C::DPAD * 2 / 16, RPS = 64 / NCH;
+      write_staged_bf16<C>(st, lr, lh, o, inv);
+#pragma unroll
+      for (int k = 0; k < kStagedChunks<C>; ++k) {
+        const int r = RPS * k + ln / NCH;
+        const u32x4 v = read_staged_bf16<C>(st, ln, k);
+        if (r < rows) __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(row_at(r) + 8 * (ln % NCH)));
+      }
+    }
+  } else if (lr < rows) {
+    using E = Elem<C::BF16>;
+    u16* const dst = row_at(lr);
+#pragma unroll
+    for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+      for (int gq = 0; gq < 4; ++gq) {
+        const int d0 = 32 * dt + 8 * gq + 4 * lh;
+        if (d0 >= p.dim) continue;
+        const f32x4 val = f32x4{o[dt][4 * gq], o[dt][4 * gq + 1], o[dt][4 * gq + 2], o[dt][4 * gq + 3]} * inv;
+        if (split) {
+          *reinterpret_cast<f32x4*>(parts + lr * p.dim + d0) = val;
+        } else {
+          *reinterpret_cast<u32x2*>(dst + d0) = u32x2{E::pack2(val[0], val[1]), E::pack2(val[2], val[3])};
+        }
+      }
+  }
+  if (split && lh == 0 && lr < rows) p.lse[(int64_t)it.slot * C::ROWS_TILE + first_row + lr] = lse_of(m, tot);
+}
+
 template <class C>
 __global__ __attribute__((aligned(4096))) __launch_bounds__(C::THREADS) void extend_long_kernel(
     ExtendParams p, const int32_t* __restrict__ table, const int32_t* __restrict__ lengths,
@@ -95,20 +142,9 @@ __global__ __attribute__((aligned(4096))) __launch_bounds__(C::THREADS) void ext
   // The lane's row: of the tile, of the request's (token, head) pairs.
   const int in_tile = wave * C::ROWS_WAVE + il;
   const int row = it.tile * C::ROWS_TILE + in_tile;
-  const int token = row / p.group, in_group = row - token * p.group;
-  const bool mine = in_tile < it.rows;
+  const int token = row / p.group;
   u32x4 qf[C::KK];
-  {
-    const char* qp = static_cast<const char*>(p.q) + (int64_t)(it.first + token) * p.q_token +
-                     (int64_t)(it.head * p.group + in_group) * p.q_head;
-#pragma unroll
-    for (int kk = 0; kk < C::KK; ++kk) {
-      const int d = 16 * kk + 8 * hh;
-      u32x4 val = {0u, 0u, 0u, 0u};
-      if (mine && d < p.dim) val = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(qp + 2 * d));
-      qf[kk] = val;
-    }
-  }
+  load_q<C>(p, it, row, in_tile < it.rows, hh, qf);
   const Seen seen = row_seen(p, it, token);
   // Blocks that end past the wave's first token's last key, or begin below its last token's first
   // key, hold keys that some row does not see.
@@ -123,51 +159,11 @@ __global__ __attribute__((aligned(4096))) __launch_bounds__(C::THREADS) void ext
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[dt][v] = 0.0f;
 
-  // Rows of this wave: the output, or the partial of a split. Each wave stages its rows in its own
-  // part of the K ring (head-dim tile 64: of both rings); the caller sees to it that nothing else
-  // uses that meanwhile.
+  // Each wave stages its output rows in its own part of the K ring (head-dim tile 64: of both
+  // rings); the caller sees to it that nothing else uses that meanwhile.
   constexpr bool kStageInK = C::WAVES * 32 * kStagedRowBytes<C> <= C::NKSLOT * C::TILE_BYTES;
   auto store_output = [&]() {
-    const float tot = pair_sum(l), inv = 1.0f / fmaxf(tot, 1.0e-30f);
-    const bool split = it.splits > 1;
-    const int rows = it.rows - wave * C::ROWS_WAVE;  // of this wave, 32 or fewer
-    const int ln = opaque_lane(lane), lr = ln & 31, lh = ln >> 5;
-    auto row_at = [&](int r) { return static_cast<u16*>(p.out) + out_row(p, it, wave_row + r); };
-    float* const parts = p.parts + ((int64_t)it.slot * C::ROWS_TILE + wave * C::ROWS_WAVE) * p.dim;
-    if (p.dim == C::DPAD) {
-      unsigned char* st = smem + wave * 32 * kStagedRowBytes<C>;
-      if (split) {
-        store_rows_staged<C>(st, lane, o, inv, true, parts, nullptr, 0, rows);
-      } else {
-        constexpr int NCH = C::DPAD * 2 / 16, RPS = 64 / NCH;
-        write_staged_bf16<C>(st, lr, lh, o, inv);
-#pragma unroll
-        for (int k = 0; k < kStagedChunks<C>; ++k) {
-          const int r = RPS * k + ln / NCH;
-          const u32x4 v = read_staged_bf16<C>(st, ln, k);
-          if (r < rows)
-            __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(row_at(r) + 8 * (ln % NCH)));
-        }
-      }
-    } else if (lr < rows) {
-      using E = Elem<C::BF16>;
-      u16* const dst = row_at(lr);
-#pragma unroll
-      for (int dt = 0; dt < C::DT; ++dt)
-#pragma unroll
-        for (int gq = 0; gq < 4; ++gq) {
-          const int d0 = 32 * dt + 8 * gq + 4 * lh;
-          if (d0 >= p.dim) continue;
-          const f32x4 val = f32x4{o[dt][4 * gq], o[dt][4 * gq + 1], o[dt][4 * gq + 2], o[dt][4 * gq + 3]} * inv;
-          if (split) {
-            *reinterpret_cast<f32x4*>(parts + lr * p.dim + d0) = val;
-          } else {
-            *reinterpret_cast<u32x2*>(dst + d0) = u32x2{E::pack2(val[0], val[1]), E::pack2(val[2], val[3])};
-          }
-        }
-    }
-    if (split && lh == 0 && lr < rows)
-      p.lse[(int64_t)it.slot * C::ROWS_TILE + wave * C::ROWS_WAVE + lr] = lse_of(m, tot);
+    store_wave_rows<C>(p, it, wave * C::ROWS_WAVE, smem + wave * 32 * kStagedRowBytes<C>, lane, o, m, l);
   };
   if (N <= 0) {
     store_output();

@@ -77,6 +77,11 @@ CASES = {
     "chunk_few_rows_long": ([70], [6000], 2, 1, 128, 16, True, 0),
     "prompt": ([1000], [1000], 2, 1, 128, 64, True, 0),
     "prompt_dim_256": ([270], [400], 2, 1, 256, 64, True, 0),
+    "wide_window": ([300, 1], [700, 90], 4, 2, 256, 16, True, 129),
+    "wide_odd_pages": ([140, 70], [300, 71], 4, 2, 192, 7, True, 0),
+    "wide_split": ([200], [5000], 2, 1, 256, 64, True, 0),
+    "wide_not_causal": ([150, 3], [1000, 33], 6, 2, 144, 48, False, 0),
+    "wide_no_keys": ([200, 140], [100, 0], 4, 4, 256, 1, True, 0),
 }
 
 
