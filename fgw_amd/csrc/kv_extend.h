@@ -5,8 +5,8 @@
 // tile: row R of (request, K/V head) is token R / G, head R % G of the group, so a tile of 32 rows
 // reads each key once for all of them. Row R sees the keys [lo, hi) of its token:
 //   hi = len - n + token + 1 (causal; else len),  lo = hi - window (no window: 0).
-// Softmax and products are those of fmha_kernel.h (fp32 sums and statistics, P rounded to the
-// input type for the PV product).
+// Softmax and products are those of fmha_kernel.h (fp32 sums and statistics); for the PV product P is
+// rounded to the input type in the kernels of long tiles, and two numbers of it in the one of few rows.
 //
 // Work. Lengths and counts are on the device, so each program finds its item itself (find_item): it
 // reads the lengths of 64 requests at a time, one to a lane, and sums tiles and splits over the
@@ -16,7 +16,7 @@
 // of a ragged batch in pieces; a CU reads at most 38 GB/s, 1.7 times its share of the memory, so
 // pieces of unequal length cost nothing until one has twice its share (B 32, Hq 32, Hkv 8, D 128,
 // lengths 1024-4096, us: split W / target evenly 76, even ranges over the tiles laid end to end
-// 75, whole tiles 72; see also extend_rows_kernel). Grid and workspace follow on the host from
+// 75, whole tiles 73, each with P as one number; see also extend_rows_kernel). Grid and workspace follow on the host from
 // sizes alone, programs without an item end after the sums. Split tiles go through partials (O / l,
 // LSE) and a join.
 // The K/V head is fastest in an item's number: workgroup w runs on XCD w % 8, so with 8 heads an XCD
@@ -297,18 +297,19 @@ __device__ __forceinline__ void join_splits(const ExtendParams& p, const Item& i
 }
 
 // Rows [row_from, row_to) of a split tile from its partials, by the whole workgroup. A thread holds 4
-// dims of a row; where rows and dims leave threads over, they share its splits. Weights exp(LSE -
-// peak), empty splits (LSE -1e30) weigh nothing, an all-empty row is zero. COH: the partials were
-// written by this launch. Uses 24 bytes of LDS a thread.
+// dims of a row; where `share_rows` rows leave threads over, they share its splits (both joins of a
+// short tile pass all its rows there, and so add in the same order). Weights exp(LSE - peak), empty
+// splits (LSE -1e30) weigh nothing, an all-empty row is zero. COH: the partials were written by this
+// launch. Uses 24 bytes of LDS a thread.
 template <bool BF16, bool COH>
 __device__ __forceinline__ void join_rows(const ExtendParams& p, const Item& it, int tile_rows, int row_from, int row_to,
-                                          unsigned char* lds, int tid, int threads) {
+                                          int share_rows, unsigned char* lds, int tid, int threads) {
   using E = Elem<BF16>;
   f32x4* const sacc = reinterpret_cast<f32x4*>(lds);
   float* const speak = reinterpret_cast<float*>(lds + threads * 16);
   float* const stot = speak + threads;
   const int d4n = p.dim / 4, pairs = (row_to - row_from) * d4n;
-  const int share = pairs < threads ? threads / pairs : 1;  // threads of a (row, 4 dims) pair
+  const int share = share_rows * d4n < threads ? threads / (share_rows * d4n) : 1;  // threads of a (row, 4 dims) pair
   for (int base = 0; base < pairs; base += threads) {
     const int pair = share > 1 ? tid % pairs : base + tid, g = share > 1 ? tid / pairs : 0;
     const bool act = pair < pairs && g < share;
@@ -504,6 +505,15 @@ __device__ __forceinline__ void load_q(const ExtendParams& p, const Item& it, in
 // waits count the half blocks issued since. One stage at head-dim tile 128 leaves room for two
 // workgroups on a CU, which pays where tiles are short (B 256, lengths 75-300: 51 us, 74 with two
 // stages and one workgroup) and costs nothing where they are long.
+//
+// The weights P of the PV product are the sum of two numbers of the input type (softmax_exp_two), so
+// that an output is as exact as its own rounding: the memory bounds this kernel, and the second product
+// costs 1-2% (D 128, us, one number / two: B 32 lengths 1024-4096 73.1 / 74.2, B 1 KV 32768 33.2 / 33.3,
+// 8 x 8 tokens KV 2048-8192 45.1 / 45.2; 9% where 120 rows read 512-2048 keys, 30.0 / 32.9). With one,
+// where a few keys carry a row, its error was up to 1.8 times that of the output's rounding.
+// Bound: B 32, lengths 1024-4096, 4.5 TB/s, by what a CU reads of the longest tile (a uniform batch
+// 5.3); D 256 5.0 TB/s; one request of 32768 keys 4.0 TB/s; one of 4096, 9.9 us, by its launch, the
+// search for the item, one round of reads and the join.
 template <int DPAD>
 constexpr int kStages = DPAD >= 128 ? 1 : DPAD == 64 ? 2 : 4;
 
@@ -528,6 +538,37 @@ __device__ __forceinline__ void wait_lds() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0xC07F);
   asm volatile("" ::: "memory");
+}
+
+// The two numbers of a packed pair.
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+template <bool BF16>
+__device__ __forceinline__ f32x2 unpack2(u32 w) {
+  if constexpr (BF16) return f32x2{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+  const f16x2 h = __builtin_bit_cast(f16x2, w);
+  return f32x2{(float)h[0], (float)h[1]};
+}
+
+// p = exp2(s * scale_log2 - m) as the sum of two numbers of the input type, hi + lo (the rest, rounded),
+// operands of the PV product; returns the lane's part of the row sum.
+template <class C>
+__device__ __forceinline__ float softmax_exp_two(const f32x16& s, float m, float scale_log2, u32x4 (&hi)[C::KS],
+                                                 u32x4 (&lo)[C::KS]) {
+  using E = Elem<C::BF16>;
+  float e[16], rs[4];
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    e[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], scale_log2, -m));
+    rs[v % 4] = v < 4 ? e[v] : rs[v % 4] + e[v];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const u32 w = E::pack2(e[2 * i], e[2 * i + 1]);
+    const f32x2 back = unpack2<C::BF16>(w);
+    hi[i / 4][i % 4] = w;
+    lo[i / 4][i % 4] = E::pack2(e[2 * i] - back[0], e[2 * i + 1] - back[1]);
+  }
+  return (rs[0] + rs[1]) + (rs[2] + rs[3]);
 }
 
 template <class C>
@@ -588,7 +629,7 @@ __device__ __forceinline__ void extend_tile(const ExtendParams& p, const int32_t
     // One or two waves to a SIMD hide little of a chain of LDS reads and products. So all operands of
     // a product are read at once (there are registers for them), the scores come in two chains, K's
     // next tile is issued while they run, and V is read under the softmax.
-    u32x4 ka[C::KK], va[C::KS * C::DT], pf[C::KS];
+    u32x4 ka[C::KK], va[C::KS * C::DT], pf[C::KS], pl[C::KS];
     f32x16 s[1], t;
     wait_half<C, false>(rem);
     asm volatile("" ::: "memory");
@@ -614,14 +655,28 @@ __device__ __forceinline__ void extend_tile(const ExtendParams& p, const int32_t
     __builtin_amdgcn_sched_barrier(0);
     s[0] += t;
     if (pos0 + C::BN > hi_min || pos0 < lo_max) mask_seen<C>(s, pos0, seen, hh);
-    online_softmax<C>(s, m, l, o, p.scale_log2, pf);
+    float sum = softmax_exp_two<C>(s[0], m, p.scale_log2, pf, pl);
+    if (__ballot(!(sum <= kSoftmaxSumBound))) {
+      const float top = fmaxf(m, row_max<C>(s, p.scale_log2));
+      const float keep = __builtin_amdgcn_exp2f(m - top);
+      l *= keep;
+#pragma unroll
+      for (int dt = 0; dt < C::DT; ++dt) o[dt] *= keep;
+      m = top;
+      sum = softmax_exp_two<C>(s[0], m, p.scale_log2, pf, pl);
+    }
+    l += sum;
     wait_lds();
     if (rem >= S) issue_v(n + S);
 #pragma unroll
-    for (int k2 = 0; k2 < C::KS; ++k2)
+    for (int k2 = 0; k2 < C::KS; ++k2) {
 #pragma unroll
       for (int dt = 0; dt < C::DT; ++dt)
         o[dt] = Elem<C::BF16>::mma(va[k2 * C::DT + dt], pf[k2], o[dt]);
+#pragma unroll
+      for (int dt = 0; dt < C::DT; ++dt)
+        o[dt] = Elem<C::BF16>::mma(va[k2 * C::DT + dt], pl[k2], o[dt]);
+    }
   }
 
   // The waves' states of the same rows, through LDS.
@@ -710,7 +765,7 @@ __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void extend_row
   const bool last = *flag != 0;
   __syncthreads();  // LDS is written again
   if (!last) return;
-  join_rows<C::BF16, true>(p, it, C::ROWS_TILE, 0, it.rows, smem, tid, C::THREADS);
+  join_rows<C::BF16, true>(p, it, C::ROWS_TILE, 0, it.rows, it.rows, smem, tid, C::THREADS);
   if (tid == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
@@ -722,7 +777,7 @@ template <bool BF16>
 __global__ __launch_bounds__(kMergeThreads) void extend_join_kernel(ExtendParams rows, ExtendParams longs,
                                                                     int rows_items) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[kMergeThreads * 24];
-  auto join = [&](const ExtendParams& p, int w, int tile_rows, int per_split) {
+  auto join = [&](const ExtendParams& p, int w, int tile_rows, int per_split, bool whole) {
     const JoinNote note = reinterpret_cast<const JoinNote*>(p.notes)[w];
     if (note.splits < 2) return;
     Item it;
@@ -734,12 +789,13 @@ __global__ __launch_bounds__(kMergeThreads) void extend_join_kernel(ExtendParams
     it.slot_step = p.heads;
     const int parts = note.splits * per_split, part = note.split * per_split + (int)blockIdx.y;
     const int from = note.rows * part / parts, to = note.rows * (part + 1) / parts;
-    if (from < to) join_rows<BF16, false>(p, it, tile_rows, from, to, lds, threadIdx.x, kMergeThreads);
+    if (from < to)
+      join_rows<BF16, false>(p, it, tile_rows, from, to, whole ? note.rows : to - from, lds, threadIdx.x, kMergeThreads);
   };
   if ((int)blockIdx.x >= rows_items)
-    join(longs, (int)blockIdx.x - rows_items, longs.dim > 128 ? WideTiling::ROWS : LongTiling::ROWS, kJoinParts);
+    join(longs, (int)blockIdx.x - rows_items, longs.dim > 128 ? WideTiling::ROWS : LongTiling::ROWS, kJoinParts, false);
   else if (blockIdx.y == 0)
-    join(rows, (int)blockIdx.x, ShortTiling::ROWS, 1);
+    join(rows, (int)blockIdx.x, ShortTiling::ROWS, 1, true);
 }
 
 template <bool BF16, int DPAD>
