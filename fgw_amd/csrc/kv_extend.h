@@ -63,8 +63,8 @@ __device__ __forceinline__ Request load_request(const ExtendParams& p, const int
   r.len = len < 0 ? 0 : (len > capacity ? capacity : len);
   r.first = first;
   if (first < 0 || next > p.tokens || next <= first) return r;
-  r.n = next - first < p.max_new ? next - first : p.max_new;
-  const int64_t rows = (int64_t)r.n * p.group;
+  r.n = next - first;
+  const int64_t rows = (int64_t)(r.n < p.max_new ? r.n : p.max_new) * p.group;
   if (rows <= p.rows_from || rows > p.rows_to) return r;
   r.tiles = (int)((rows + T::ROWS - 1) / T::ROWS);
   int lo = p.window > 0 ? r.len - r.n - p.window + 1 : 0;
@@ -94,8 +94,10 @@ __device__ __forceinline__ int splits_of(int units, int chunk) {
 
 // Units of a split: the smallest chunk, up to the steps of the search, of at least min_chunk units
 // with which all tiles of a head have at most target / heads splits together; kWhole where whole
-// tiles are as many. The sums saturate (kMany) so that they stay in 32 bits; the same in every
-// program.
+// tiles are as many, however unequal: the partials of long tiles, 132 KB each at D 128, cost what the
+// balance gains (tiles above the average share cut in two, us, whole / cut: B 2, Hq 8, Hkv 8, 4096
+// tokens 111 / 111; B 4, 512 tokens, lengths 1024-4096, Hq 32, Hkv 8 106 / 136). The sums saturate
+// (kMany) so that they stay in 32 bits; the same in every program.
 constexpr int kWhole = 0x40000000, kMany = 1 << 24;
 template <class T>
 __device__ __forceinline__ int best_chunk(const ExtendParams& p, const int32_t* lengths, const int32_t* cu,
@@ -166,7 +168,7 @@ __device__ __forceinline__ bool find_item(const ExtendParams& p, const int32_t* 
       it.slot0 = w - it.split * p.heads;
       it.slot_step = p.heads;
 
-      const int row0 = it.tile * T::ROWS, all = it.n * p.group;
+      const int row0 = it.tile * T::ROWS, all = (it.n < p.max_new ? it.n : p.max_new) * p.group;
       it.rows = all - row0 < T::ROWS ? all - row0 : T::ROWS;
       const int t0 = row0 / p.group, t1 = (row0 + it.rows - 1) / p.group;
       int hi = p.causal ? it.len - it.n + t1 + 1 : it.len;

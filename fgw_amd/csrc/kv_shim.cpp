@@ -11,6 +11,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cstdlib>
 #include <map>
 #include <stdexcept>
 #include <string>
@@ -149,10 +150,35 @@ fgw_kv_rows rows(const at::Tensor& x, const c10::Device& device) {
 
 bool same_sizes(const at::Tensor& a, const at::Tensor& b) { return a.sizes() == b.sizes(); }
 
+// First byte of a tensor without negative strides, and the byte behind its last one.
+std::pair<const char*, const char*> extent(const at::Tensor& x) {
+  const char* first = static_cast<const char*>(x.data_ptr());
+  int64_t last = 0;
+  for (int64_t i = 0; i < x.dim(); ++i) last += (x.size(i) - 1) * x.stride(i);
+  return {first, x.numel() == 0 ? first : first + (last + 1) * (int64_t)x.element_size()};
+}
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  const auto x = extent(a), y = extent(b);
+  return x.first < y.second && y.first < x.second;
+}
+// Whether rows [T, H, D] of two tensors share memory: heads of one fused buffer lie in each other's
+// range without that, side by side in every token.
+bool rows_overlap(const at::Tensor& a, const at::Tensor& b) {
+  if (!overlap(a, b)) return false;
+  if (a.size(0) < 2 || a.sizes() != b.sizes() || a.strides() != b.strides()) return true;
+  const int64_t span = ((a.size(1) - 1) * a.stride(1) + a.size(2)) * (int64_t)a.element_size();
+  const int64_t token = a.stride(0) * (int64_t)a.element_size();
+  const int64_t apart = std::abs(static_cast<const char*>(a.data_ptr()) - static_cast<const char*>(b.data_ptr()));
+  return token <= 0 || apart % token < span || apart % token + span > token;
+}
+
 // An output given by the caller: no two of its rows share memory, and it is `from` itself or has
 // memory apart from it.
 void check_out(const at::Tensor& out, const at::Tensor& from) {
   need(same_sizes(out, from) && out.scalar_type() == from.scalar_type(), "out does not match the rows");
+  need(out.dim() == 3 && out.stride(0) >= 0 && out.stride(1) >= 0, "negative strides");
+  need(!rows_overlap(out, from) || (out.data_ptr() == from.data_ptr() && out.strides() == from.strides()),
+       "out must be the rows themselves or memory apart from them");
   const int64_t span = out.size(2);
   need(out.numel() == 0 || out.size(1) == 1 || out.stride(1) >= span, "the rows of out overlap");
   need(out.numel() == 0 || out.size(0) == 1 ||
@@ -256,6 +282,7 @@ PyObject* append(Args& a) {
   need(same_sizes(k, v) && k.size(0) == q.size(0) && k.size(2) == q.size(2), "K/V shape mismatch");
   check_pool(kc, vc, q.size(2), device);
   need(kc.size(1) == k.size(1), "K/V shape mismatch");
+  need(!overlap(kc, vc), "the K and V pools must be apart from each other");
   need(table.dim() == 2 && table.size(0) > 0 && table.size(1) > 0,
        "positive Q extents and rank-2 table required");
   const int64_t batch = table.size(0);
@@ -345,7 +372,7 @@ PyObject* extend(Args& a) {
     need(same_sizes(out, q) && out.scalar_type() == q.scalar_type(), "out does not match the rows");
     on(out, device);
     need(out.is_contiguous(), kSameGpu);
-    need(out.numel() == 0 || out.data_ptr() != q.data_ptr(), "out must not be q");
+    need(!rows_overlap(out, q), "out must not be q or share memory with it");
   } else {
     out = at::empty(q.sizes(), q.options());
   }

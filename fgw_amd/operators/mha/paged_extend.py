@@ -39,7 +39,8 @@ def mha_paged_append(q, k, v, k_cache, v_cache, block_table, cache_seqlens, cu_s
     not written where pos lies outside [0, W * page_size) or the page id outside the pool. rotary (a
     Rotary) turns q and k to their cache positions, or to positions [T] (int32 or int64); None
     writes k as it is and copies q. Returns q_out ([T, Hq, D]; q itself for in place) or a new
-    contiguous tensor. No two tokens may have the same cache position of one page.
+    contiguous tensor. No two tokens may have the same cache position of one page, and the two pools
+    no memory in common.
     """
     if rotary is None:
         if positions is not None:
@@ -65,7 +66,7 @@ class _ExtendKernel:
 
     def __call__(self, q, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens, max_new, out=None):
         """O [T, Hq, D] (a new tensor, or `out`, contiguous and apart from q). max_new: at least the
-        new tokens of every request; a request's tokens past it are left out."""
+        new tokens of every request; the rows of a request's tokens past it are left as they are."""
         return _kv.extend(q, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens, max_new,
                           *self._tail, out)
 
@@ -86,7 +87,9 @@ def build_extend_kernel(heads, kv_heads, dim, page_size, dtype, device_index=Non
     unless given. The callable takes (q, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens,
     max_new, out=None), shapes free from call to call, and reads nothing back: lengths outside
     [0, W * page_size] are clamped, tokens that see no key give zero rows, page ids outside the
-    pool read as zeros.
+    pool read as zeros. Keys that no token of a request sees do not matter, whatever they hold. One
+    whose V is not finite gives NaN or infinities to the tokens that see it, and may give NaN to
+    other new tokens of the same request and call (a weight of 0 times it).
     """
     name = _dtype_name(dtype)
     if dim < 16 or dim > 256 or dim % 16:

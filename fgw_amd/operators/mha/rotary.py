@@ -128,8 +128,9 @@ class _Rotate(torch.autograd.Function):
     def backward(ctx, grad):
         # The map is s times a rotation: its transpose is the same with the angle reversed.
         positions, = ctx.saved_tensors
-        if grad.stride(-1) != 1 or any(n % (16 // grad.element_size()) for n in grad.stride()[:-1]):
-            grad = grad.contiguous()
+        if (grad.stride(-1) != 1 or grad.data_ptr() % 16
+                or any(n % (16 // grad.element_size()) for n in grad.stride()[:-1])):
+            grad = grad.clone(memory_format=torch.contiguous_format)
         return apply_rotary(grad, positions, ctx.rotary, inverse=not ctx.inverse), None, None, None
 
 

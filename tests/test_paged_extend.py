@@ -156,6 +156,70 @@ def test_strided_queries_given_output_and_rows_behind_the_last_request():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 40, 200])
+def test_one_request_shorter_than_the_sizes(n):
+    """Padding behind the only request of a call that is sized for a long one."""
+    cache = _cache([n], [n + 130], 2, 64, 16, torch.bfloat16)
+    q = _queries(260, 4, 64, torch.bfloat16)
+    q[n:] = math.nan
+    kernel = P.build_extend_kernel(4, 2, 64, 16, "bfloat16", 0)
+    out = torch.full((260, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    _compare(kernel(q.cuda(), *[x.cuda() for x in cache], 260, out), q, cache, 16, n)
+    assert bool((out[n:] == 7.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [1, 5, 70])
+def test_tokens_past_the_bound_are_left(most):
+    """max_new below a request's tokens: the ones within it as ever, the rest untouched."""
+    news = [150, 3]
+    cache = _cache(news, [400, 30], 2, 128, 16, torch.bfloat16)
+    q = _queries(153, 8, 128, torch.bfloat16)
+    kernel = P.build_extend_kernel(8, 2, 128, 16, "bfloat16", 0, window=100)
+    full = kernel(q.cuda(), *[x.cuda() for x in cache], 150)
+    out = torch.full((153, 8, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    kernel(q.cuda(), *[x.cuda() for x in cache], most, out)
+    want, bound = K.extend_exact(q, *cache, 16, window=100)
+    for first, n in ((0, 150), (150, 3)):
+        kept = slice(first, first + min(most, n))
+        assert bool(((out[kept].cpu().double() - want[kept]).abs() <= bound[kept]).all())
+        assert bool((out[first + min(most, n):first + n] == 7.0).all())
+    _compare(full, q, cache, 16, "full", window=100)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [599, 600, 2**31 - 1])
+def test_windows_at_and_past_the_capacity(window):
+    news, lens = [300, 4], [100, 600]
+    cache = _cache(news, lens, 1, 64, 20, torch.bfloat16)
+    q = _queries(304, 2, 64, torch.bfloat16)
+    kernel = P.build_extend_kernel(2, 1, 64, 20, "bfloat16", 0, window=window)
+    _compare(kernel(q.cuda(), *[x.cuda() for x in cache], 300), q, cache, 20, window, window=window)
+
+
+@pytest.mark.gpu
+def test_memory_that_rows_and_outputs_share():
+    k, v, table, lens, cu = [x.cuda() for x in _cache([4], [40], 2, 64, 16, torch.bfloat16)]
+    fused = torch.zeros(5, 10, 64, dtype=torch.bfloat16, device="cuda")
+    fused.copy_(_queries(5, 10, 64, torch.bfloat16))
+    q, other, across = fused[:4, :4], fused[:4, 4:8], fused[:4, 2:6]
+    new_k, new_v = fused[:4, 8:10].clone(), fused[:4, 8:10].clone()
+    rotary = Rotary(64)
+    want = P.mha_paged_append(q, new_k, new_v, k, v, table, lens, cu, 16, rotary=rotary)
+    args = (new_k, new_v, k, v, table, lens, cu, 16)
+    assert torch.equal(P.mha_paged_append(q, *args, rotary=rotary, q_out=other), want)  # side by side
+    for bad in (across, fused[1:5, :4]):
+        with pytest.raises(ValueError, match="memory apart"):
+            P.mha_paged_append(q, *args, rotary=rotary, q_out=bad)
+    with pytest.raises(ValueError, match="apart from each other"):
+        P.mha_paged_append(q, new_k, new_v, k, k, table, lens, cu, 16)
+    kernel = P.build_extend_kernel(4, 2, 64, 16, "bfloat16", 0)
+    flat = want.clone()
+    with pytest.raises(ValueError, match="share memory"):
+        kernel(flat, k, v, table, lens, cu, 4, flat)
+
+
+@pytest.mark.gpu
 def test_same_bits_on_every_run_and_alone_or_in_a_batch():
     """No result depends on an order of atomics; rows whose plan is the same do not see the batch."""
     cache = _cache([1, 1, 1], [900, 5000, 37], 2, 128, 16, torch.bfloat16)

@@ -182,6 +182,17 @@ def test_gradient_through_expanded_rows_and_twice():
 
 
 @pytest.mark.gpu
+def test_gradient_that_starts_at_any_element():
+    r = R.Rotary(16)
+    pos = torch.arange(6, dtype=torch.int32).cuda()
+    x = torch.randn(6, 2, 16, device="cuda", requires_grad=True)
+    weights = torch.randn(1 + 6 * 2 * 16, device="cuda")
+    flat = torch.cat([torch.zeros(1, device="cuda"), R.apply_rotary(x, pos, r).flatten()])
+    flat.backward(weights)  # the rotation's gradient is a view of it, 4 bytes on
+    assert torch.equal(x.grad, R.apply_rotary(weights[1:].view(6, 2, 16).clone(), pos, r, inverse=True))
+
+
+@pytest.mark.gpu
 def test_replays_of_a_captured_rotation():
     r = R.Rotary(64)
     x, pos = _rows(9, 4, 64, torch.bfloat16).cuda(), torch.arange(9, dtype=torch.int32).cuda()
