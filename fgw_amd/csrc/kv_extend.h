@@ -35,6 +35,7 @@ struct ExtendParams : FwdParams {
   int32_t tokens, q_heads, group, max_new, window;
   int32_t rows_from, rows_to;  // requests with n * group in (rows_from, rows_to] are this launch's
   int32_t target, min_chunk;   // items that fill the card (0: nothing is split), units of a split at least
+  int32_t whole, many;         // units of a tile that is never split, that has splits of 2 min_chunk
   int32_t* counters;           // rows kernel: arrivals at the split tiles, by their first item, or nullptr
   int32_t* notes;              // for the join: [work] JoinNote
 };
@@ -88,8 +89,8 @@ __device__ __forceinline__ int wave_sum(int x, int lane) {
   return __builtin_amdgcn_readlane(wave_incl_sum(x, lane), 63);
 }
 
-__device__ __forceinline__ int splits_of(int units, int chunk) {
-  return units > chunk ? (units + chunk - 1) / chunk : 1;
+__device__ __forceinline__ int splits_of(const ExtendParams& p, int units, int chunk) {
+  return units > chunk && units > p.whole ? (units + chunk - 1) / chunk : 1;
 }
 
 // Units of a split: the smallest chunk, up to the steps of the search, of at least min_chunk units
@@ -114,12 +115,14 @@ __device__ __forceinline__ int best_chunk(const ExtendParams& p, const int32_t* 
     }
     return total;
   };
-  if (sum([](const Request& r) { return (int64_t)r.tiles; }) >= limit) return kWhole;
+  const int tiles = sum([](const Request& r) { return (int64_t)r.tiles; });
+  if (tiles >= limit) return kWhole;
   const int units = sum([](const Request& r) { return (int64_t)r.tiles * r.units; });
   int chunk = (int)((u32)(units + limit - 1) / (u32)limit);
-  chunk = chunk < p.min_chunk ? p.min_chunk : chunk;
+  const int least = units > p.many * tiles ? 2 * p.min_chunk : p.min_chunk;
+  chunk = chunk < least ? least : chunk;
   for (;;) {
-    const int items = sum([&](const Request& r) { return (int64_t)r.tiles * splits_of(r.units, chunk); });
+    const int items = sum([&](const Request& r) { return (int64_t)r.tiles * splits_of(p, r.units, chunk); });
     if (items <= limit || chunk >= kMany) return chunk;
     chunk += (chunk >> 3) + 1;  // (with whole tiles the items are fewer than the limit)
   }
@@ -147,7 +150,7 @@ __device__ __forceinline__ bool find_item(const ExtendParams& p, const int32_t* 
   int items_before = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
     const Request r = b0 == 0 ? r0 : load_request<T>(p, lengths, cu, b0 + lane);
-    const int splits = splits_of(r.units, chunk);
+    const int splits = splits_of(p, r.units, chunk);
     const int items = r.tiles * splits;
     const int items_to = wave_incl_sum(items, lane);
     const int at = g - items_before - (items_to - items);
@@ -179,7 +182,7 @@ __device__ __forceinline__ bool find_item(const ExtendParams& p, const int32_t* 
       it.hi = hi;
       // The tile's own units, fewer than its request's where it ends earlier or begins later.
       const int from = lo / T::KEYS, units = (hi + T::KEYS - 1) / T::KEYS - from;
-      const int most = splits_of(units, chunk);
+      const int most = splits_of(p, units, chunk);
       it.splits = most < s ? most : s;
       const int end = (hi + T::BN - 1) / T::BN;
       it.blk_begin = (from + split_bound(units, it.split, it.splits)) * T::UNIT;
@@ -514,8 +517,8 @@ __device__ __forceinline__ void load_q(const ExtendParams& p, const Item& it, in
 // 8 x 8 tokens KV 2048-8192 45.1 / 45.2; 9% where 120 rows read 512-2048 keys, 30.0 / 32.9). With one,
 // where a few keys carry a row, its error was up to 1.8 times that of the output's rounding.
 // Bound: B 32, lengths 1024-4096, 4.5 TB/s, by what a CU reads of the longest tile (a uniform batch
-// 5.3); D 256 5.0 TB/s; one request of 32768 keys 4.0 TB/s; one of 4096, 9.9 us, by its launch, the
-// search for the item, one round of reads and the join.
+// 5.3); D 256 5.0 TB/s; one request of 32768 keys 4.0 TB/s. One of 512 keys (Hq 8, Hkv 2, D 64) takes
+// 9.1 us: a chain of dependent reads (lengths, page ids, keys) and four rounds.
 template <int DPAD>
 constexpr int kStages = DPAD >= 128 ? 1 : DPAD == 64 ? 2 : 4;
 

@@ -18,9 +18,17 @@ namespace fgw_kv {
 // 146 / 93.9.
 constexpr int kLongFrom = 128;
 // Units of a split at least (rounds of 128 keys, blocks of 64): below, a split's own cost outweighs
-// what it saves. Few rows, B1 Hq 32 Hkv 8 D 128 KV 4096, 1 / 2 / 4 rounds: 13.1 / 12.2 / 14.4 us;
-// long, B1 100 tokens KV 1000, 4 / 8 blocks: 26.1 / 32.4 us.
-constexpr int kRowsMinChunk = 2, kLongMinChunk = 4;
+// what it saves. Few rows, B1 Hq 32 Hkv 8 D 128, splits of 1 / 2 / 4 rounds, us: KV 1024
+// 10.5 / 11.3 / 14.3, 2048 10.8 / 12.1 / 14.6; long, B1 100 tokens KV 1000, 4 / 8 blocks: 26.1 / 32.4.
+constexpr int kRowsMinChunk = 1, kLongMinChunk = 4;
+// Rounds of a tile of few rows that is never split: one takes 0.9 us at D 64, 1.35 at D 128, the join
+// 3 us. Whole / split, us: D 64 KV 384 7.6 / 9.2, 512 8.6 / 9.0, 768 10.4 / 9.4; D 128 KV 384 9.6 / 10.2,
+// 512 11.0 / 10.0.
+constexpr int kRowsWhole = 3, kRowsWholeNarrow = 4;  // (D <= 64)
+// Rounds of a tile above which a split has two: a join takes 0.14 us for every split of 4 rows, 0.3 of
+// 16. Splits of 1 / 2, us: 4 rows (the case above) 16 rounds 10.8 / 12.1, 32 rounds 13.9 / 13.1; 16 rows
+// (Hkv 2) 8 rounds 12.4 / 13.4, 16 rounds 14.8 / 13.9.
+constexpr int kRowsMany = 16, kRowsManyTall = 8;  // (requests of more than 8 rows)
 
 #define FGW_KV_EXTERN_LONG(BF, DP)                                                                    \
   extern template hipError_t launch_extend_long<BF, DP, kRowsBlock>(const ExtendParams&, int, hipStream_t); \
@@ -68,7 +76,7 @@ namespace {
 // One launch of a kernel over the requests with rows_from < n * group <= rows_to.
 struct Launch {
   int rows_from, rows_to;
-  int target, min_chunk;     // ExtendParams
+  int target, min_chunk, whole, many;  // ExtendParams
   int64_t tiles;             // at most, of one K/V head
   int64_t items;             // at most: the grid; 0: no launch
   int64_t slots;             // places for partials and notes
@@ -113,6 +121,8 @@ Plan plan(const fgw_kv_extend_args& a) {
   if (!only_long) {
     p.rows.rows_to = kLongFrom;
     p.rows.min_chunk = kRowsMinChunk;
+    p.rows.whole = a.dim <= 64 ? kRowsWholeNarrow : kRowsWhole;
+    p.rows.many = rows_most <= 8 ? kRowsMany : kRowsManyTall;
     p.rows.tiles = tiles(batch, std::min<int64_t>(rows_most, kLongFrom), ShortTiling::ROWS);
     plan_items<ShortTiling>(p.rows, a, true);
     p.rows.counters = p.rows.slots * fgw_mha::kArrivalStride;
@@ -121,6 +131,7 @@ Plan plan(const fgw_kv_extend_args& a) {
     p.longs.rows_from = only_long ? 0 : kLongFrom;
     p.longs.rows_to = 0x7fffffff;
     p.longs.min_chunk = kLongMinChunk;
+    p.longs.many = 1 << 20;
     // (So many tokens that whole tiles fill the card four times over, unless most of them are
     // padding: no workspace, and no launch for joins.)
     const int64_t requests = std::min(batch, only_long ? 1 : total / kLongFrom);
@@ -170,6 +181,8 @@ static int run(const ExtendParams& base, const Plan& plan, hipStream_t stream) {
     p.rows_to = l.rows_to;
     p.target = l.target;
     p.min_chunk = l.min_chunk;
+    p.whole = l.whole;
+    p.many = l.many;
     p.work = (int)l.slots;
     p.notes = l.target > 0 && !p.counters ? reinterpret_cast<int32_t*>(work + l.slots * rows_tile * (p.dim + 1)) : nullptr;
     p.parts = work;

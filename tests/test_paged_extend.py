@@ -77,6 +77,9 @@ CASES = {
     "chunk_few_rows_long": ([70], [6000], 2, 1, 128, 16, True, 0),
     "prompt": ([1000], [1000], 2, 1, 128, 64, True, 0),
     "prompt_dim_256": ([270], [400], 2, 1, 256, 64, True, 0),
+    "chunk_uneven_splits": ([700, 60, 1], [2500, 2000, 900], 8, 2, 128, 16, True, 0),
+    "chunk_uneven_short_cache": ([600, 300], [300, 290], 4, 1, 64, 64, True, 0),
+    "wide_uneven_splits": ([330, 200], [2100, 1500], 2, 2, 192, 64, True, 0),
     "wide_window": ([300, 1], [700, 90], 4, 2, 256, 16, True, 129),
     "wide_odd_pages": ([140, 70], [300, 71], 4, 2, 192, 7, True, 0),
     "wide_split": ([200], [5000], 2, 1, 256, 64, True, 0),
@@ -169,22 +172,23 @@ def test_one_request_shorter_than_the_sizes(n):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("most", [1, 5, 70])
-def test_tokens_past_the_bound_are_left(most):
+@pytest.mark.parametrize("window", [None, 100])
+@pytest.mark.parametrize("most", [1, 5, 70, 141])
+def test_tokens_past_the_bound_are_left(most, window):
     """max_new below a request's tokens: the ones within it as ever, the rest untouched."""
     news = [150, 3]
-    cache = _cache(news, [400, 30], 2, 128, 16, torch.bfloat16)
+    cache = _cache(news, [900, 30], 2, 128, 16, torch.bfloat16)
     q = _queries(153, 8, 128, torch.bfloat16)
-    kernel = P.build_extend_kernel(8, 2, 128, 16, "bfloat16", 0, window=100)
+    kernel = P.build_extend_kernel(8, 2, 128, 16, "bfloat16", 0, window=window)
     full = kernel(q.cuda(), *[x.cuda() for x in cache], 150)
     out = torch.full((153, 8, 128), 7.0, dtype=torch.bfloat16, device="cuda")
     kernel(q.cuda(), *[x.cuda() for x in cache], most, out)
-    want, bound = K.extend_exact(q, *cache, 16, window=100)
+    want, bound = K.extend_exact(q, *cache, 16, window=window or 0)
     for first, n in ((0, 150), (150, 3)):
         kept = slice(first, first + min(most, n))
         assert bool(((out[kept].cpu().double() - want[kept]).abs() <= bound[kept]).all())
         assert bool((out[first + min(most, n):first + n] == 7.0).all())
-    _compare(full, q, cache, 16, "full", window=100)
+    _compare(full, q, cache, 16, "full", window=window or 0)
 
 
 @pytest.mark.gpu
