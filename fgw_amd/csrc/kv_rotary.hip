@@ -11,7 +11,7 @@
 // thread owns one unit of a token's heads, 16 bytes (both halves of the pairs in the half layout,
 // so 32) at the same place of heads g, g + G, ...: it computes the unit's angles once and walks
 // the heads. Neighbouring lanes own neighbouring units, then heads, so a wave reads whole rows.
-// Heads per thread (per_thread): 1 while the threads do not fill the card, up to 8 beyond.
+// Heads per thread (per_thread): 1 while the threads do not fill the card, 2 beyond.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -85,6 +85,15 @@ __device__ __forceinline__ u32x4 pack(const float* f) {
       x[i] = Elem<KIND == FGW_KV_BFLOAT16>::pack2(f[2 * i], f[2 * i + 1]);
   }
   return x;
+}
+
+// 16 bytes of a row. Alone (ONCE) the rows pass the caches by: 268 MB in and out take 44 us, with ordinary
+// loads 49, with non-temporal stores too 46; on the way into the pages 70 MB take 16 us with ordinary
+// loads, 19 with these.
+template <bool ONCE>
+__device__ __forceinline__ u32x4 load_row(const char* at) {
+  if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at));
+  return fgw_mha::load16(at);
 }
 
 // scale cos and scale sin of turns * pos / 2^64 of a turn. The fraction is split into quarters
@@ -195,7 +204,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryParams p) {
       dst = (is_v ? p.v_cache : p.k_cache) + (row * p.kv_heads + h) * pool_head;
       plain |= is_v;
     }
-    const u32x4 xa = fgw_mha::load16(src + lo);
+    const u32x4 xa = load_row<!APPEND>(src + lo);
     if (!rotates) {
       *reinterpret_cast<u32x4*>(dst + lo) = xa;
       return;
@@ -210,7 +219,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryParams p) {
       }
       *reinterpret_cast<u32x4*>(dst + lo) = plain ? xa : pack<KIND>(g);
     } else {
-      const u32x4 xb = fgw_mha::load16(src + hi);
+      const u32x4 xb = load_row<!APPEND>(src + hi);
       float f[E], g[E], u[E], w[E];
       unpack<KIND>(xa, f);
       unpack<KIND>(xb, g);
@@ -235,10 +244,12 @@ void launch_rotary(const RotaryParams& p, bool interleaved, int64_t blocks, hipS
     rotary_kernel<KIND, false, APPEND><<<grid, threads, 0, stream>>>(p);
 }
 
-// Heads that one thread walks: enough threads for the card (256 CUs of 2048) come first.
+// Heads that one thread walks: enough threads for the card (256 CUs of 2048) come first. More than two
+// leave fewer loads in flight than the memory takes (16384 tokens of 32 heads, D 128, us, at most 1 / 2 /
+// 4 / 8 heads: 52 / 49 / 54 / 57, ordinary loads).
 static int per_thread(int64_t units, int64_t tokens, int heads) {
   const int64_t n = units * tokens * heads / (256 * 2048);
-  return n < 1 ? 1 : (n > 8 ? 8 : (int)n);
+  return n < 2 ? 1 : 2;
 }
 
 static int check_rotary(const fgw_kv_rotary& r, int dim) {
