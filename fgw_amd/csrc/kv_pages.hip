@@ -9,8 +9,11 @@
 // to move, and writes the books of rows and pages that need no long walk) and `move` (the whole
 // card: pools' pages, 16 bytes to a lane, and the rows of the table). The plan is bound by the
 // latency of its few dependent reads: every thread takes 16 holders with four independent loads,
-// 16384 pages to a step of one scan. The moves are bound by memory: each page read and written
-// once in every pool, eight 16-byte loads in flight a thread.
+// 16384 pages to a step of one scan. The moves are bound by memory: each page read and written once
+// in every pool, 32 bytes to a thread (compact 205 pages of 32 KB in 16 pools, fork 40 of 128 KB in 16,
+// us, 32 / 64 / 128 / 256 bytes: 44 / 46 / 49 / 50, 25.1 / 25.8 / 26.5 / 30). Reads go through the
+// caches, since the children of a row copy the same page (40 of 16 rows: 28 us, 44 with non-temporal reads);
+// what is written is not read soon.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -28,7 +31,8 @@ constexpr int kPlanWaves = kPlanThreads / 64;
 constexpr int kSlabPer = 16;                          // pages of a thread and step
 constexpr int kSlab = kPlanThreads * kSlabPer;
 constexpr int kMoveThreads = 256;
-constexpr int kMoveLoads = 8;                         // 16-byte chunks of a thread
+constexpr int kMoveLoads = 2;                         // 16-byte chunks of a thread
+constexpr int kMovers = 8192;                         // workgroups of moves counted on the device
 constexpr int kPart = kMoveThreads * kMoveLoads * 16;  // bytes of a page that one workgroup moves
 constexpr int kMaxPools = 64;                         // of one launch
 constexpr int kMaxPages = 1 << 20;
@@ -365,7 +369,7 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(Pools pools, int n_p
 #pragma unroll
     for (int k = 0; k < kMoveLoads; ++k) {
       const int64_t at = (int64_t)(k * kMoveThreads + (int)threadIdx.x) * 16;
-      if (at < left) x[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from + at));
+      if (at < left) x[k] = *reinterpret_cast<const u32x4*>(from + at);
     }
 #pragma unroll
     for (int k = 0; k < kMoveLoads; ++k) {
@@ -415,7 +419,9 @@ static int check_pools(const fgw_pages_pools* p) {
 }
 
 // The pools in launches of kMaxPools, the table with the first. Workgroups of a pool: its moves'
-// parts up to four a CU over all pools of the launch, and at least 64, walked in a loop beyond.
+// parts; where only the device knows how many moves there are, kMovers over all pools of the launch
+// and at least 64 a pool, which walk them in a loop (205 moves, us, 2048 / 4096 / 8192: 50 / 48 / 45; with
+// nothing to move the call takes no longer).
 static int launch_moves(const fgw_pages_pools* pools, Job job, const Books& b, const int32_t* src,
                         const int32_t* dst, int count, const int32_t* device_count,
                         const int32_t* parents, const int32_t* children, const int32_t* whole,
@@ -432,7 +438,7 @@ static int launch_moves(const fgw_pages_pools* pools, Job job, const Books& b, c
     }
     const bool table = done == 0 && job != kCopy;
     const int64_t wanted = std::max<int64_t>(1, (int64_t)count * parts);
-    const int64_t most = std::max<int64_t>(64, 2048 / std::max(1, n));
+    const int64_t most = device_count ? std::max(64, kMovers / std::max(1, n)) : 1 << 20;
     const unsigned x = (unsigned)std::min(wanted, most), y = (unsigned)(n + (table ? 1 : 0));
     if (y == 0) break;
     move_kernel<<<dim3(x, y), dim3(kMoveThreads), 0, stream>>>(arg, n, job, b, src, dst, count,
