@@ -65,12 +65,15 @@ __device__ __forceinline__ Request load_request(const ExtendParams& p, const int
   r.first = first;
   if (first < 0 || next > p.tokens || next <= first) return r;
   r.n = next - first;
-  const int64_t rows = (int64_t)(r.n < p.max_new ? r.n : p.max_new) * p.group;
+  const int count = r.n < p.max_new ? r.n : p.max_new;
+  const int64_t rows = (int64_t)count * p.group;
   if (rows <= p.rows_from || rows > p.rows_to) return r;
   r.tiles = (int)((rows + T::ROWS - 1) / T::ROWS);
   int lo = p.window > 0 ? r.len - r.n - p.window + 1 : 0;
   lo = lo < 0 ? 0 : lo;
-  r.units = (r.len + T::KEYS - 1) / T::KEYS - lo / T::KEYS;
+  int end = p.causal ? r.len - r.n + count : r.len;
+  end = end < 0 ? 0 : end;
+  r.units = (end + T::KEYS - 1) / T::KEYS - lo / T::KEYS;
   return r;
 }
 

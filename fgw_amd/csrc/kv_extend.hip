@@ -83,12 +83,14 @@ struct Launch {
   int64_t floats, counters;  // of workspace
 };
 
-// Splits of a tile at most: of the table's capacity, or the window's span.
+// Splits of a tile at most: of the table's capacity, or the window's span (which begins anywhere in a
+// unit).
 template <class T>
-int64_t most_splits(const fgw_kv_extend_args& a, int min_chunk) {
+int64_t most_splits(const fgw_kv_extend_args& a, int min_chunk, int whole) {
   int64_t keys = (int64_t)a.width * a.page_size;
   if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + a.max_new);
-  return ((keys + T::KEYS - 1) / T::KEYS + 1 + min_chunk - 1) / min_chunk;
+  const int64_t units = (keys + T::KEYS - 1) / T::KEYS + (a.window > 0);
+  return units <= whole ? 1 : (units + min_chunk - 1) / min_chunk;
 }
 
 // Grid and workspace of a launch: where tiles may be split (best_chunk) all items together are at
@@ -96,7 +98,7 @@ int64_t most_splits(const fgw_kv_extend_args& a, int min_chunk) {
 template <class T>
 void plan_items(Launch& l, const fgw_kv_extend_args& a, bool may_split) {
   l.items = l.tiles * a.kv_heads;
-  const int64_t most = most_splits<T>(a, l.min_chunk);
+  const int64_t most = most_splits<T>(a, l.min_chunk, l.whole);
   if (!may_split || most <= 1 || a.num_cus / a.kv_heads <= 1) return;
   l.target = a.num_cus;
   l.slots = std::min<int64_t>(l.target, l.items * most);

@@ -192,6 +192,19 @@ def test_tokens_past_the_bound_are_left(most, window):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("window", [1, 300])
+def test_one_token_of_many_behind_a_window(window):
+    """The split of a tile follows the tokens within the bound, not all of the request's."""
+    cache = _cache([5000], [6000], 1, 64, 16, torch.bfloat16)
+    q = _queries(5000, 1, 64, torch.bfloat16)
+    kernel = P.build_extend_kernel(1, 1, 64, 16, "bfloat16", 0, window=window)
+    out = torch.full((5000, 1, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    kernel(q.cuda(), *[x.cuda() for x in cache], 1, out)
+    want, bound = K.extend_exact(q, *cache, 16, window=window)
+    assert bool(((out[0].cpu().double() - want[0]).abs() <= bound[0]).all()) and bool((out[1:] == 7.0).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("window", [599, 600, 2**31 - 1])
 def test_windows_at_and_past_the_capacity(window):
     news, lens = [300, 4], [100, 600]
