@@ -1,5 +1,6 @@
 // C ABI of the attention over pages with grouped heads: checks, sizes and dispatch. The kernels
-// stand in kv_extend.h, their instantiations in kv_extend_bf16.hip and kv_extend_f16.hip.
+// stand in kv_extend.h, kv_extend_long.h and kv_extend_wide.h, their instantiations in the
+// kv_extend_*.hip files of each type.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
