@@ -16,7 +16,7 @@
 // of a ragged batch in pieces; a CU reads at most 38 GB/s, 1.7 times its share of the memory, so
 // pieces of unequal length cost nothing until one has twice its share (B 32, Hq 32, Hkv 8, D 128,
 // lengths 1024-4096, us: split W / target evenly 76, even ranges over the tiles laid end to end
-// 75, whole tiles 73, each with P as one number; see also extend_rows_kernel). Grid and workspace follow on the host from
+// 75, whole tiles 73, each with P as one number and ordinary loads; see also extend_rows_kernel). Grid and workspace follow on the host from
 // sizes alone, programs without an item end after the sums. Split tiles go through partials (O / l,
 // LSE) and a join.
 // The K/V head is fastest in an item's number: workgroup w runs on XCD w % 8, so with 8 heads an XCD
@@ -362,16 +362,33 @@ __device__ __forceinline__ void join_rows(const ExtendParams& p, const Item& it,
 
 // ---- requests of few rows -----------------------------------------------------------------------
 
+// dma_saddr with a non-temporal load, for keys that a call reads once: they take no place from others in
+// the 256 MB cache. Ordinary / non-temporal, us: B 32, lengths 1024-4096, D 128 74.4 / 69.0, D 256
+// 135 / 125; 64 requests of 8192 keys 362 / 328; one of 32768 33.4 / 31.0; small or shared pages alike (32
+// requests over the same 4096 keys 56.7 / 56.8, B 4 KV 4096 19.1 / 19.7).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma_once(const void* base, u32 voff, u32 lds) {
+  const uint64_t b = (uint64_t)base;
+  const uint64_t ub = ((uint64_t)uniform_u32((u32)(b >> 32)) << 32) | uniform_u32((u32)b);
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+               :
+               : "v"(voff), "s"(ub), "s"(uniform_u32(lds))
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
 // The DMA of the 32-key tiles that one wave helps to fetch, tile n at key first_pos + step n, in tiles
 // laid out as fwd_kernel's (C: its Cfg, of which the NWQ waves of a key group share a tile). The
 // loads are inline assembly (dma_saddr, dma_flat): the compiler would wait for all of them before
 // each transposing read of V; the kernels place the waits. Row offsets come from page ids that lane
 // l holds for the wave's load instruction l % U of tile l / U, four such windows read at a time: a
-// read in the main loop would wait for the DMA in front of it (AHEAD false, for loops that wait for
-// all of it anyway: one window, in fewer registers).
+// read in the main loop would wait for the DMA in front of it. ONCE: a request's keys are read by few
+// tiles (false: by many, in loops that wait for all of the DMA anyway: ordinary loads, and one window of
+// page ids, in fewer registers).
 // Keys outside [lo, hi) or in pages outside the pool read zeros, and so do dims past D. Tiles with
 // an instruction whose keys straddle pages are resolved key by key.
-template <class C, bool AHEAD = true>
+template <class C, bool ONCE = true>
 struct KeyStream {
   static constexpr int U = C::INSTR_PER_WAVE;
   static constexpr int kWindow = 64 / U;  // tiles of a window
@@ -410,7 +427,7 @@ struct KeyStream {
   }
   __device__ __forceinline__ void read_ids(int n0) {
     id0 = read_id(n0);
-    if constexpr (!AHEAD) return;
+    if constexpr (!ONCE) return;
     id1 = read_id(n0 + kWindow);
     id2 = read_id(n0 + 2 * kWindow);
     id3 = read_id(n0 + 3 * kWindow);
@@ -419,10 +436,10 @@ struct KeyStream {
   __device__ __forceinline__ void ids_ready() const {
     if (my_n <= 0) return;
     asm volatile("" ::"v"(id0));
-    if constexpr (AHEAD) asm volatile("" ::"v"(id1), "v"(id2), "v"(id3));
+    if constexpr (ONCE) asm volatile("" ::"v"(id1), "v"(id2), "v"(id3));
   }
   __device__ __forceinline__ void set_window(int n0) {
-    const int w = AHEAD ? n0 / kWindow % 4 : 0;
+    const int w = ONCE ? n0 / kWindow % 4 : 0;
     if (w == 0 && n0 > 0) read_ids(n0);
     const int32_t a = id0, b = id1, c = id2, d = id3;  // (values: a choice of members would keep them in memory)
     const int32_t id = w == 0 ? a : w == 1 ? b : w == 2 ? c : d;
@@ -445,9 +462,14 @@ struct KeyStream {
     constexpr uint64_t kUnits = (1ull << U) - 1ull;
     if ((__ballot(live != kAllLive || off < 0) >> first & kUnits) == 0 && dim == C::DPAD) {
 #pragma unroll
-      for (int q = 0; q < U; ++q)
-        dma_saddr(base + readlane64(off, first + q), IS_V ? dl.vq(q, wq) : dl.kq(q, wq),
-                  dst + 1024u * (u32)(q * C::NWQ + wq));
+      for (int q = 0; q < U; ++q) {
+        const char* const src = base + readlane64(off, first + q);
+        const u32 at = IS_V ? dl.vq(q, wq) : dl.kq(q, wq), to = dst + 1024u * (u32)(q * C::NWQ + wq);
+        if constexpr (ONCE)
+          dma_once(src, at, to);
+        else
+          dma_saddr(src, at, to);
+      }
       return;
     }
     if (__ballot(off < 0) >> first & kUnits) {
@@ -516,12 +538,11 @@ __device__ __forceinline__ void load_q(const ExtendParams& p, const Item& it, in
 //
 // The weights P of the PV product are the sum of two numbers of the input type (softmax_exp_two), so
 // that an output is as exact as its own rounding: the memory bounds this kernel, and the second product
-// costs 1-2% (D 128, us, one number / two: B 32 lengths 1024-4096 73.1 / 74.2, B 1 KV 32768 33.2 / 33.3,
-// 8 x 8 tokens KV 2048-8192 45.1 / 45.2; 9% where 120 rows read 512-2048 keys, 30.0 / 32.9). With one,
+// costs 1-2% (D 128, ordinary loads, us, one number / two: B 32 lengths 1024-4096 73.1 / 74.2, B 1 KV 32768
+// 33.2 / 33.3, 8 x 8 tokens KV 2048-8192 45.1 / 45.2; 9% where 120 rows read 512-2048 keys, 30.0 / 32.9). With one,
 // where a few keys carry a row, its error was up to 1.8 times that of the output's rounding.
-// Bound: B 32, lengths 1024-4096, 4.5 TB/s, by what a CU reads of the longest tile (a uniform batch
-// 5.3); D 256 5.0 TB/s; one request of 32768 keys 4.0 TB/s. One of 512 keys (Hq 8, Hkv 2, D 64) takes
-// 9.1 us: a chain of dependent reads (lengths, page ids, keys) and four rounds.
+// Bound: B 32, lengths 1024-4096, 4.9 TB/s, by what a CU reads of the longest tile (D 256 5.4); 64
+// requests of 8192 keys 6.5 TB/s; one of 32768 4.3 TB/s. One of 512 keys (Hq 8, Hkv 2, D 64) takes 8.8 us: a chain of dependent reads (lengths, page ids, keys) and four rounds.
 template <int DPAD>
 constexpr int kStages = DPAD >= 128 ? 1 : DPAD == 64 ? 2 : 4;
 
