@@ -11,8 +11,9 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include <cstdlib>
+#include <initializer_list>
 #include <map>
+#include <numeric>
 #include <stdexcept>
 #include <string>
 #include <utility>
@@ -150,26 +151,64 @@ fgw_kv_rows rows(const at::Tensor& x, const c10::Device& device) {
 
 bool same_sizes(const at::Tensor& a, const at::Tensor& b) { return a.sizes() == b.sizes(); }
 
-// First byte of a tensor without negative strides, and the byte behind its last one.
+// First byte of a tensor without negative strides, and the byte behind its last one (empty: none).
 std::pair<const char*, const char*> extent(const at::Tensor& x) {
+  if (x.numel() == 0) return {nullptr, nullptr};
   const char* first = static_cast<const char*>(x.data_ptr());
   int64_t last = 0;
   for (int64_t i = 0; i < x.dim(); ++i) last += (x.size(i) - 1) * x.stride(i);
-  return {first, x.numel() == 0 ? first : first + (last + 1) * (int64_t)x.element_size()};
+  return {first, first + (last + 1) * (int64_t)x.element_size()};
 }
 bool overlap(const at::Tensor& a, const at::Tensor& b) {
   const auto x = extent(a), y = extent(b);
   return x.first < y.second && y.first < x.second;
 }
-// Whether rows [T, H, D] of two tensors share memory: heads of one fused buffer lie in each other's
-// range without that, side by side in every token.
-bool rows_overlap(const at::Tensor& a, const at::Tensor& b) {
+// Whether two tensors without negative strides share memory; true where that is not ruled out. Views
+// of one buffer lie in each other's range without that: heads side by side in every token, or the
+// parts of a [T, H, 3, D] projection. Those are told apart modulo a length m: dims whose stride is a
+// multiple of m fall away, the others span a range, and two ranges that are apart on a circle of m
+// bytes are apart in memory. m is tried at every stride and at their greatest common divisor.
+bool shares_memory(const at::Tensor& a, const at::Tensor& b) {
   if (!overlap(a, b)) return false;
-  if (a.size(0) < 2 || a.sizes() != b.sizes() || a.strides() != b.strides()) return true;
-  const int64_t span = ((a.size(1) - 1) * a.stride(1) + a.size(2)) * (int64_t)a.element_size();
-  const int64_t token = a.stride(0) * (int64_t)a.element_size();
-  const int64_t apart = std::abs(static_cast<const char*>(a.data_ptr()) - static_cast<const char*>(b.data_ptr()));
-  return token <= 0 || apart % token < span || apart % token + span > token;
+  const int64_t apart = static_cast<const char*>(b.data_ptr()) - static_cast<const char*>(a.data_ptr());
+  auto stride = [](const at::Tensor& x, int64_t i) { return x.size(i) > 1 ? x.stride(i) * (int64_t)x.element_size() : 0; };
+  auto disjoint = [&](int64_t m) {
+    auto span = [&](const at::Tensor& x) {
+      int64_t bytes = x.element_size();
+      for (int64_t i = 0; i < x.dim(); ++i) bytes += stride(x, i) % m ? (x.size(i) - 1) * stride(x, i) : 0;
+      return bytes;
+    };
+    const int64_t at = (apart % m + m) % m;  // of b's range behind the start of a's
+    return at >= span(a) && at + span(b) <= m;
+  };
+  int64_t common = 0;
+  for (const at::Tensor* x : {&a, &b})
+    for (int64_t i = 0; i + 1 < x->dim(); ++i) {
+      const int64_t m = stride(*x, i);
+      if (m > 0 && disjoint(m)) return false;
+      common = std::gcd(common, m);
+    }
+  return common == 0 || !disjoint(common);
+}
+
+// What a call writes shares no memory with what it reads (undefined tensors: not given).
+typedef std::initializer_list<const at::Tensor*> Tensors;
+void apart(Tensors written, Tensors read, const char* message) {
+  std::pair<const char*, const char*> spans[4] = {};
+  size_t n = 0;
+  for (const at::Tensor* w : written) {
+    if (w->defined()) spans[n] = extent(*w);
+    ++n;
+  }
+  for (const at::Tensor* r : read) {
+    if (!r->defined()) continue;
+    const auto x = extent(*r);
+    n = 0;
+    for (const at::Tensor* w : written) {
+      const auto& y = spans[n++];
+      need(!(x.first < y.second && y.first < x.second) || !shares_memory(*w, *r), message);
+    }
+  }
 }
 
 // An output given by the caller: no two of its rows share memory, and it is `from` itself or has
@@ -177,7 +216,7 @@ bool rows_overlap(const at::Tensor& a, const at::Tensor& b) {
 void check_out(const at::Tensor& out, const at::Tensor& from) {
   need(same_sizes(out, from) && out.scalar_type() == from.scalar_type(), "out does not match the rows");
   need(out.dim() == 3 && out.stride(0) >= 0 && out.stride(1) >= 0, "negative strides");
-  need(!rows_overlap(out, from) || (out.data_ptr() == from.data_ptr() && out.strides() == from.strides()),
+  need(!shares_memory(out, from) || (out.data_ptr() == from.data_ptr() && out.strides() == from.strides()),
        "out must be the rows themselves or memory apart from them");
   const int64_t span = out.size(2);
   need(out.numel() == 0 || out.size(1) == 1 || out.stride(1) >= span, "the rows of out overlap");
@@ -237,10 +276,12 @@ PyObject* rotate(Args& a) {
   r.dim = size32(x.size(2));
   positions_of(positions, x.size(0), device, r.positions, r.positions64);
   const c10::DeviceGuard guard(device);
-  if (out.defined())
+  if (out.defined()) {
     check_out(out, x);
-  else
+    apart({&out}, {&positions}, "out must not share memory with the positions");
+  } else {
     out = at::empty(x.sizes(), x.options());
+  }
   r.out = rows(out, device);
   check(entries.rotary_apply(&r, stream_of(device)));
   return THPVariable_Wrap(std::move(out));
@@ -300,6 +341,10 @@ PyObject* append(Args& a) {
   r.width = size32(table.size(1));
   if (positions.defined()) positions_of(positions, q.size(0), device, r.positions, r.positions64);
   const c10::DeviceGuard guard(device);
+  // (Another thread's rows may be read after this one's are written.)
+  const char* const message = "q_out and the pools must not share memory with what the call reads";
+  apart({&kc, &vc}, {&q, &q_out}, message);
+  apart({&kc, &vc, &q_out}, {&k, &v, &table, &lens, &cu, &positions}, message);
   if (q_out.defined())
     check_out(q_out, q);
   else
@@ -372,7 +417,8 @@ PyObject* extend(Args& a) {
     need(same_sizes(out, q) && out.scalar_type() == q.scalar_type(), "out does not match the rows");
     on(out, device);
     need(out.is_contiguous(), kSameGpu);
-    need(!rows_overlap(out, q), "out must not be q or share memory with it");
+    need(!shares_memory(out, q), "out must not be q or share memory with it");
+    apart({&out}, {&kc, &vc, &table, &lens, &cu}, "out must not share memory with what the call reads");
   } else {
     out = at::empty(q.sizes(), q.options());
   }
@@ -507,6 +553,12 @@ PyObject* copy_pages(Args& a) {
   Py_RETURN_NONE;
 }
 
+// (a, b) -> bool: what the calls take for sharing memory, on any device.
+PyObject* shares_memory_of(Args& a) {
+  const at::Tensor x = a.tensor(), y = a.tensor();
+  return PyBool_FromLong(shares_memory(x, y));
+}
+
 // The addresses of the C entry points, in the order of Entries.
 PyObject* bind(Args& a) {
   void** const table = reinterpret_cast<void**>(&entries);
@@ -534,6 +586,7 @@ PyMethodDef methods[] = {
     {"free", FGW_FAST(free_rows), METH_FASTCALL, "fgw_pages_free"},
     {"compact", FGW_FAST(compact), METH_FASTCALL, "fgw_pages_compact"},
     {"copy", FGW_FAST(copy_pages), METH_FASTCALL, "fgw_pages_copy"},
+    {"shares_memory", FGW_FAST(shares_memory_of), METH_FASTCALL, "whether two tensors may share memory"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_kv", "C++ calls over the fgw_kv C ABI", -1, methods};

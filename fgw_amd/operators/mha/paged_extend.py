@@ -39,8 +39,9 @@ def mha_paged_append(q, k, v, k_cache, v_cache, block_table, cache_seqlens, cu_s
     not written where pos lies outside [0, W * page_size) or the page id outside the pool. rotary (a
     Rotary) turns q and k to their cache positions, or to positions [T] (int32 or int64); None
     writes k as it is and copies q. Returns q_out ([T, Hq, D]; q itself for in place) or a new
-    contiguous tensor. No two tokens may have the same cache position of one page, and the two pools
-    no memory in common.
+    contiguous tensor. No two tokens may have the same cache position of one page. The two pools and
+    q_out share no memory with each other or with anything the call reads (but q_out with q, as q
+    itself); heads side by side in one buffer do not.
     """
     if rotary is None:
         if positions is not None:
@@ -65,8 +66,9 @@ class _ExtendKernel:
                       window or 0, softmax_scale, _device_info(device_index).num_cus)
 
     def __call__(self, q, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens, max_new, out=None):
-        """O [T, Hq, D] (a new tensor, or `out`, contiguous and apart from q). max_new: at least the
-        new tokens of every request; the rows of a request's tokens past it are left as they are."""
+        """O [T, Hq, D] (a new tensor, or `out`, contiguous and apart from all inputs). max_new: at
+        least the new tokens of every request; the rows of a request's tokens past it are left as
+        they are."""
         return _kv.extend(q, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens, max_new,
                           *self._tail, out)
 

@@ -13,7 +13,8 @@
  * as zeros and is not written. New tokens are packed: request b has the rows
  * [cu[b], cu[b + 1]) of Q, K, V (cu [B + 1] int32, cu[0] = 0, never falling), and its cache length
  * counts them: its row cu[b] + j has the cache position len_b - n_b + j, n_b = cu[b + 1] - cu[b].
- * Rows at and behind cu[B] are neither read nor written.
+ * Rows at and behind cu[B] are neither read nor written. What a call writes shares no memory with
+ * what it reads, except where a rotated output may be the input itself.
  *
  * All functions return 0 or a negative fgw_mha_status; the message of the calling thread's last
  * failure is in fgw_kv_last_error(). Nothing allocates, frees or synchronises; launches are
@@ -85,7 +86,7 @@ typedef struct {
   fgw_kv_rotary rotary;
 } fgw_kv_append_args;
 
-/* Writes q_out = rotated q, and each new token's rotated K and its V to the pool row
+/* Writes q_out (which may be q itself) = rotated q, and each new token's rotated K and its V to the pool row
  * table[b, pos / page] * page + pos % page. Tokens whose position lies outside [0, W * page), or
  * whose page id lies outside the pool, are not written to the pool. */
 int fgw_kv_append(const fgw_kv_append_args* args, hipStream_t stream);
