@@ -250,6 +250,12 @@ __device__ __forceinline__ void device_store1(float* base, u32 bytes, float x) {
   __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), rsrc, (int)bytes, 0, kDeviceScope);
 }
 
+// LSE of a split's row; one that saw no key has kNegBig, one that met a NaN keeps it (lse_of calls that
+// empty), so that the join neither drops the split nor returns zeros for the row.
+__device__ __forceinline__ float part_lse(float m_log2, float total) {
+  return total != total ? total : lse_of(m_log2, total);
+}
+
 // What a second launch has to know to join split tiles: every item's, in its own place (splits 0:
 // no split tile's).
 struct JoinNote {
@@ -287,7 +293,7 @@ __device__ __forceinline__ void join_splits(const ExtendParams& p, const Item& i
     float top = peak;
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      const bool live = s0 + k * share < it.splits && x[k] > -1.0e29f;
+      const bool live = s0 + k * share < it.splits && !(x[k] <= -1.0e29f);
       top = live ? fmaxf(top, x[k]) : top;
     }
     const float keep = expf(peak - top);
@@ -295,7 +301,7 @@ __device__ __forceinline__ void join_splits(const ExtendParams& p, const Item& i
     acc *= keep;
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      const bool live = s0 + k * share < it.splits && x[k] > -1.0e29f;
+      const bool live = s0 + k * share < it.splits && !(x[k] <= -1.0e29f);
       const float w = live ? expf(x[k] - top) : 0.0f;
       tot += w;
       acc += live ? v[k] * w : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -760,10 +766,10 @@ __device__ __forceinline__ void extend_tile(const ExtendParams& p, const int32_t
     acc *= inv;
     if (fused) {
       device_store4(p.parts, 4u * (at * (u32)p.dim + (u32)d0), acc);
-      if (d0 == 0) device_store1(p.lse, 4u * at, lse_of(mm, t2));
+      if (d0 == 0) device_store1(p.lse, 4u * at, part_lse(mm, t2));
     } else {
       *reinterpret_cast<f32x4*>(p.parts + (int64_t)at * p.dim + d0) = acc;
-      if (d0 == 0) p.lse[at] = lse_of(mm, t2);
+      if (d0 == 0) p.lse[at] = part_lse(mm, t2);
     }
   }
 }

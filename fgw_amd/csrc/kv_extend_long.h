@@ -113,7 +113,7 @@ __device__ __forceinline__ void store_wave_rows(const ExtendParams& p, const Ite
         }
       }
   }
-  if (split && lh == 0 && lr < rows) p.lse[(int64_t)it.slot * C::ROWS_TILE + first_row + lr] = lse_of(m, tot);
+  if (split && lh == 0 && lr < rows) p.lse[(int64_t)it.slot * C::ROWS_TILE + first_row + lr] = part_lse(m, tot);
 }
 
 template <class C>

@@ -89,9 +89,10 @@ def build_extend_kernel(heads, kv_heads, dim, page_size, dtype, device_index=Non
     unless given. The callable takes (q, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens,
     max_new, out=None), shapes free from call to call, and reads nothing back: lengths outside
     [0, W * page_size] are clamped, tokens that see no key give zero rows, page ids outside the
-    pool read as zeros. Keys that no token of a request sees do not matter, whatever they hold. One
-    whose V is not finite gives NaN or infinities to the tokens that see it, and may give NaN to
-    other new tokens of the same request and call (a weight of 0 times it).
+    pool read as zeros. Keys that no token of a request sees do not matter, whatever they hold. A NaN
+    in a query or in a key that it sees gives a row of NaN. A key whose V is not finite gives NaN or
+    infinities to the tokens that see it, and may give NaN to other new tokens of the same request
+    and call (a weight of 0 times it).
     """
     name = _dtype_name(dtype)
     if dim < 16 or dim > 256 or dim % 16:
