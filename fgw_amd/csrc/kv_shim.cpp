@@ -226,6 +226,14 @@ void check_out(const at::Tensor& out, const at::Tensor& from) {
        "the rows of out overlap");
 }
 
+// A call has written to these tensors of its caller: their version moves, as after any operation in
+// place, so that a gradient that has saved what they held before is refused and not computed from
+// what they hold now (inference tensors have no version).
+void changed(Tensors written) {
+  for (const at::Tensor* x : written)
+    if (x->defined() && !x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+}
+
 hipStream_t stream_of(const c10::Device& device) {
   return c10::hip::getCurrentHIPStream(device.index()).stream();
 }
@@ -276,6 +284,7 @@ PyObject* rotate(Args& a) {
   r.dim = size32(x.size(2));
   positions_of(positions, x.size(0), device, r.positions, r.positions64);
   const c10::DeviceGuard guard(device);
+  const at::Tensor given = out;
   if (out.defined()) {
     check_out(out, x);
     apart({&out}, {&positions}, "out must not share memory with the positions");
@@ -284,6 +293,7 @@ PyObject* rotate(Args& a) {
   }
   r.out = rows(out, device);
   check(entries.rotary_apply(&r, stream_of(device)));
+  changed({&given});
   return THPVariable_Wrap(std::move(out));
 }
 
@@ -345,12 +355,14 @@ PyObject* append(Args& a) {
   const char* const message = "q_out and the pools must not share memory with what the call reads";
   apart({&kc, &vc}, {&q, &q_out}, message);
   apart({&kc, &vc, &q_out}, {&k, &v, &table, &lens, &cu, &positions}, message);
+  const at::Tensor given = q_out;
   if (q_out.defined())
     check_out(q_out, q);
   else
     q_out = at::empty(q.sizes(), q.options());
   r.q_out = rows(q_out, device);
   check(entries.append(&r, stream_of(device)));
+  changed({&kc, &vc, &given});
   return THPVariable_Wrap(std::move(q_out));
 }
 
@@ -413,6 +425,7 @@ PyObject* extend(Args& a) {
   int64_t floats = 0, counters = 0;
   check(entries.extend_workspace(&r, &floats, &counters));
   const c10::DeviceGuard guard(device);
+  const at::Tensor given = out;
   if (out.defined()) {
     need(same_sizes(out, q) && out.scalar_type() == q.scalar_type(), "out does not match the rows");
     on(out, device);
@@ -431,6 +444,7 @@ PyObject* extend(Args& a) {
   const hipStream_t stream = stream_of(device);
   if (counters > 0) r.counters = arrival_counters(device, stream, counters);
   check(entries.extend(&r, stream));
+  changed({&given});
   return THPVariable_Wrap(std::move(out));
 }
 
@@ -455,6 +469,10 @@ fgw_pages_books books_of(const at::Tensor& refs, const at::Tensor& table, const 
 struct PoolList {
   std::vector<void*> data;
   std::vector<int64_t> bytes;
+  std::vector<at::Tensor> tensors;
+  void changed() const {
+    for (const at::Tensor& x : tensors) ::changed({&x});
+  }
   fgw_pages_pools view() const { return {data.data(), bytes.data(), (int32_t)data.size()}; }
 };
 
@@ -472,6 +490,7 @@ PoolList pools_of(PyObject* seq, int64_t pages, int32_t page, const c10::Device&
     need(page > 0 && x.dim() >= 1 && x.size(0) == pages * page, "a pool must have pages * page_size rows");
     list.data.push_back(x.data_ptr());
     list.bytes.push_back(x.numel() / pages * x.element_size());
+    list.tensors.push_back(x);
   }
   return list;
 }
@@ -490,6 +509,7 @@ PyObject* reserve(Args& a) {
   const c10::DeviceGuard guard(device);
   at::Tensor status = ints(2, device), work = ints(entries.pages_workspace(b.pages, b.rows), device);
   check(entries.reserve(&b, c, ptr(status), ptr(work), stream_of(device)));
+  changed({&refs, &table, &lens});
   return THPVariable_Wrap(std::move(status));
 }
 
@@ -508,6 +528,8 @@ PyObject* fork_rows(Args& a) {
   at::Tensor status = ints(2, device), work = ints(entries.pages_workspace(b.pages, pairs), device);
   const fgw_pages_pools view = pools.view();
   check(entries.fork(&b, &view, p, c, pairs, ptr(status), ptr(work), stream_of(device)));
+  changed({&refs, &table, &lens});
+  pools.changed();
   return THPVariable_Wrap(std::move(status));
 }
 
@@ -519,6 +541,7 @@ PyObject* free_rows(Args& a) {
   const int32_t* r = metadata(rows, {-1}, device);
   const c10::DeviceGuard guard(device);
   check(entries.free_rows(&b, r, size32(rows.size(0)), stream_of(device)));
+  changed({&refs, &table, &lens});
   Py_RETURN_NONE;
 }
 
@@ -533,6 +556,8 @@ PyObject* compact(Args& a) {
   at::Tensor moved = ints(1, device), work = ints(entries.pages_workspace(b.pages, 0), device);
   const fgw_pages_pools view = pools.view();
   check(entries.compact(&b, &view, ptr(moved), ptr(work), stream_of(device)));
+  changed({&refs, &table, &lens});
+  pools.changed();
   return THPVariable_Wrap(std::move(moved));
 }
 
@@ -550,6 +575,7 @@ PyObject* copy_pages(Args& a) {
   const c10::DeviceGuard guard(device);
   const fgw_pages_pools view = pools.view();
   check(entries.copy(&view, pages, s, d, size32(src.size(0)), stream_of(device)));
+  pools.changed();
   Py_RETURN_NONE;
 }
 
