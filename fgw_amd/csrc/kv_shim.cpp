@@ -8,6 +8,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -234,6 +235,14 @@ void changed(Tensors written) {
     if (x->defined() && !x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
 }
 
+// Calls that write to tensors of their caller record no gradient: none of those may require one while
+// gradients are recorded.
+void writable(Tensors written) {
+  if (!c10::GradMode::is_enabled()) return;
+  for (const at::Tensor* x : written)
+    need(!x->defined() || !x->requires_grad(), "a tensor that the call writes requires a gradient, which is not recorded");
+}
+
 hipStream_t stream_of(const c10::Device& device) {
   return c10::hip::getCurrentHIPStream(device.index()).stream();
 }
@@ -285,6 +294,7 @@ PyObject* rotate(Args& a) {
   positions_of(positions, x.size(0), device, r.positions, r.positions64);
   const c10::DeviceGuard guard(device);
   const at::Tensor given = out;
+  writable({&given});
   if (out.defined()) {
     check_out(out, x);
     apart({&out}, {&positions}, "out must not share memory with the positions");
@@ -356,6 +366,7 @@ PyObject* append(Args& a) {
   apart({&kc, &vc}, {&q, &q_out}, message);
   apart({&kc, &vc, &q_out}, {&k, &v, &table, &lens, &cu, &positions}, message);
   const at::Tensor given = q_out;
+  writable({&kc, &vc, &given});
   if (q_out.defined())
     check_out(q_out, q);
   else
@@ -426,6 +437,7 @@ PyObject* extend(Args& a) {
   check(entries.extend_workspace(&r, &floats, &counters));
   const c10::DeviceGuard guard(device);
   const at::Tensor given = out;
+  writable({&given});
   if (out.defined()) {
     need(same_sizes(out, q) && out.scalar_type() == q.scalar_type(), "out does not match the rows");
     on(out, device);
@@ -485,6 +497,7 @@ PoolList pools_of(PyObject* seq, int64_t pages, int32_t page, const c10::Device&
     PyObject* item = PySequence_Fast_GET_ITEM(seq, i);
     if (!THPVariable_Check(item)) throw WrongType("pools must be a list or a tuple of tensors");
     const at::Tensor& x = THPVariable_Unpack(item);
+    writable({&x});
     on(x, device);
     need(x.is_contiguous(), kSameGpu);
     need(page > 0 && x.dim() >= 1 && x.size(0) == pages * page, "a pool must have pages * page_size rows");

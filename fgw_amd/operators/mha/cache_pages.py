@@ -9,10 +9,11 @@ The books of a pool are three int32 tensors on the GPU, changed in place:
 
 Row r holds the pages table[r, : ceil(lens[r] / page_size)]; new_books makes empty books. Pools are
 the K/V tensors [pages * page_size, ...] of all layers, contiguous and of any dtype, whose pages
-share the ids. Every decision is made on the GPU, lowest free page first and rows in order, so that
-the results are the same on every run and no call waits for the device: counts of what was refused
-come back as int32 tensors. Books that were changed by hand must stay consistent (every held page
-counted in refs, and a partly filled last page held by its row alone).
+share the ids; while gradients are recorded none may require one. Every decision is made on the GPU,
+lowest free page first and rows in order, so that the results are the same on every run and no call
+waits for the device: counts of what was refused come back as int32 tensors. Books that were changed
+by hand must stay consistent (every held page counted in refs, and a partly filled last page held by
+its row alone).
 """
 from __future__ import annotations
 

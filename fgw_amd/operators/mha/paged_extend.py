@@ -13,7 +13,8 @@ and behind cu_seqlens[B] (a padded batch) are neither read nor written. A servin
   o = kernel(q, k_cache, v_cache, ...)    build_extend_kernel's callable
 
 with nothing read back from the device: every call can be captured into a HIP graph and replayed
-after lengths, counts and tables were changed in place. Inference only: no gradient is recorded.
+after lengths, counts and tables were changed in place. Inference only: no gradient is recorded, and
+none of the pools and outputs that a call writes may require one (torch.no_grad() lifts that).
 """
 from __future__ import annotations
 

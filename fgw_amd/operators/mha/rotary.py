@@ -145,7 +145,7 @@ def apply_rotary(x, positions, rotary, *, inverse=False, out=None):
     x may have any strides that are multiples of 16 bytes, its last dim contiguous. inverse turns
     the other way: the transpose of the forward, so its gradient. Returns a new contiguous tensor,
     or out ([T, H, D], x itself for in place, else memory apart from x and positions). Differentiable
-    in x, twice too; out is for calls that record no gradient.
+    in x, twice too; out is for calls that record no gradient, and requires none.
     """
     if not isinstance(rotary, Rotary):
         raise TypeError("rotary must be a Rotary")
