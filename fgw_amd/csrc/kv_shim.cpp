@@ -236,8 +236,10 @@ void changed(Tensors written) {
 }
 
 // Calls that write to tensors of their caller record no gradient: none of those may require one while
-// gradients are recorded.
+// gradients are recorded, or have a tangent of forward mode.
 void writable(Tensors written) {
+  for (const at::Tensor* x : written)
+    need(!x->defined() || !x->_fw_grad(0).defined(), "a tensor that the call writes has a forward gradient, which is not recorded");
   if (!c10::GradMode::is_enabled()) return;
   for (const at::Tensor* x : written)
     need(!x->defined() || !x->requires_grad(), "a tensor that the call writes requires a gradient, which is not recorded");
@@ -592,6 +594,9 @@ PyObject* copy_pages(Args& a) {
   Py_RETURN_NONE;
 }
 
+// x -> bool: x is a dual tensor of forward-mode derivatives.
+PyObject* has_tangent(Args& a) { return PyBool_FromLong(a.tensor()._fw_grad(0).defined()); }
+
 // (a, b) -> bool: what the calls take for sharing memory, on any device.
 PyObject* shares_memory_of(Args& a) {
   const at::Tensor x = a.tensor(), y = a.tensor();
@@ -625,6 +630,7 @@ PyMethodDef methods[] = {
     {"free", FGW_FAST(free_rows), METH_FASTCALL, "fgw_pages_free"},
     {"compact", FGW_FAST(compact), METH_FASTCALL, "fgw_pages_compact"},
     {"copy", FGW_FAST(copy_pages), METH_FASTCALL, "fgw_pages_copy"},
+    {"has_tangent", FGW_FAST(has_tangent), METH_FASTCALL, "whether a tensor has a forward gradient"},
     {"shares_memory", FGW_FAST(shares_memory_of), METH_FASTCALL, "whether two tensors may share memory"},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -121,6 +121,7 @@ class _Rotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, positions, rotary, inverse):
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         ctx.rotary, ctx.inverse = rotary, inverse
         return _rotate(x, positions, rotary, inverse, None)
 
@@ -128,10 +129,20 @@ class _Rotate(torch.autograd.Function):
     def backward(ctx, grad):
         # The map is s times a rotation: its transpose is the same with the angle reversed.
         positions, = ctx.saved_tensors
-        if (grad.stride(-1) != 1 or grad.data_ptr() % 16
-                or any(n % (16 // grad.element_size()) for n in grad.stride()[:-1])):
-            grad = grad.clone(memory_format=torch.contiguous_format)
-        return apply_rotary(grad, positions, ctx.rotary, inverse=not ctx.inverse), None, None, None
+        return apply_rotary(_aligned(grad), positions, ctx.rotary, inverse=not ctx.inverse), None, None, None
+
+    @staticmethod
+    def jvp(ctx, tangent, *_):
+        positions, = ctx.saved_tensors
+        return apply_rotary(_aligned(tangent), positions, ctx.rotary, inverse=ctx.inverse)
+
+
+def _aligned(x):
+    """x as rows that the kernel takes: gradients and tangents come with any strides."""
+    if (x.stride(-1) != 1 or x.data_ptr() % 16
+            or any(n % (16 // x.element_size()) for n in x.stride()[:-1])):
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
 
 
 def _rotate(x, positions, rotary, inverse, out):
@@ -145,11 +156,11 @@ def apply_rotary(x, positions, rotary, *, inverse=False, out=None):
     x may have any strides that are multiples of 16 bytes, its last dim contiguous. inverse turns
     the other way: the transpose of the forward, so its gradient. Returns a new contiguous tensor,
     or out ([T, H, D], x itself for in place, else memory apart from x and positions). Differentiable
-    in x, twice too; out is for calls that record no gradient, and requires none.
+    in x, twice too, and in forward mode; out is for calls that record no gradient, and requires none.
     """
     if not isinstance(rotary, Rotary):
         raise TypeError("rotary must be a Rotary")
-    if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
+    if isinstance(x, torch.Tensor) and (x.requires_grad and torch.is_grad_enabled() or _kv.has_tangent(x)):
         if out is not None:
             raise ValueError("out cannot be given where a gradient is recorded")
         return _Rotate.apply(x, positions, rotary, bool(inverse))
