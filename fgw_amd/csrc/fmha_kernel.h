@@ -866,7 +866,7 @@ __device__ __forceinline__ float lse_of(float m_log2, float total) {
 }
 
 // floor(nblk * s / splits): the first key block of split s (0 <= s <= splits
-// <= 128). 32-bit arithmetic whenever the product fits, which avoids the
+// <= 256). 32-bit arithmetic whenever the product fits, which avoids the
 // 64-bit division routine.
 __device__ __forceinline__ int split_bound(int nblk, int s, int splits) {
   if (nblk < (1 << 24)) return (int)(((u32)nblk * (u32)s) / (u32)splits);

@@ -31,6 +31,11 @@ constexpr int kRowsWhole = 3, kRowsWholeNarrow = 4;  // (D <= 64)
 // (Hkv 2) 8 rounds 12.4 / 13.4, 16 rounds 14.8 / 13.9.
 constexpr int kRowsMany = 16, kRowsManyTall = 8;  // (requests of more than 8 rows)
 
+// Compute units that a call fills at most: those of the card. They bound splits and workspace (256
+// places of 132 KB), so that offsets of partials and the products of split_bound stay in 32 bits
+// whatever num_cus a caller gives.
+constexpr int kMostCus = 256;
+
 #define FGW_KV_EXTERN_LONG(BF, DP)                                                                    \
   extern template hipError_t launch_extend_long<BF, DP, kRowsBlock>(const ExtendParams&, int, hipStream_t); \
   extern template hipError_t launch_extend_long<BF, DP, kRowsGroup>(const ExtendParams&, int, hipStream_t); \
@@ -111,7 +116,8 @@ struct Plan {
   Launch rows, longs;
 };
 
-Plan plan(const fgw_kv_extend_args& a) {
+Plan plan(fgw_kv_extend_args a) {
+  a.num_cus = std::min(a.num_cus, kMostCus);
   const int64_t group = a.heads / a.kv_heads, total = a.tokens * group;
   const int64_t rows_most = std::min(a.max_new, a.tokens) * group, batch = std::min(a.batch, a.tokens);
   auto tiles = [&](int64_t requests, int64_t rows, int64_t tile) {  // of so many requests at most

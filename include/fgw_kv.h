@@ -111,7 +111,7 @@ typedef struct {
   int32_t max_new;  /* no request has more new tokens than this (more are not computed) */
   int32_t causal, window;
   int32_t dtype;    /* FGW_KV_FLOAT16 or FGW_KV_BFLOAT16 */
-  int32_t num_cus;  /* compute units to fill */
+  int32_t num_cus;  /* compute units to fill (above 256: 256) */
   float scale;      /* of the scores */
 } fgw_kv_extend_args;
 
