@@ -12,6 +12,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <map>
 #include <numeric>
@@ -462,9 +463,9 @@ PyObject* extend(Args& a) {
   return THPVariable_Wrap(std::move(out));
 }
 
-// refs, table, lens, page_size of a call.
+// refs, table, lens, page_size of a call, and the lists that it reads while the books change.
 fgw_pages_books books_of(const at::Tensor& refs, const at::Tensor& table, const at::Tensor& lens,
-                         int32_t page) {
+                         int32_t page, Tensors lists) {
   const c10::Device device = refs.device();
   need(device.is_cuda(), kSameGpu);
   need(refs.dim() == 1 && table.dim() == 2 && lens.dim() == 1 && refs.size(0) > 0 && table.size(0) > 0 &&
@@ -477,6 +478,10 @@ fgw_pages_books books_of(const at::Tensor& refs, const at::Tensor& table, const 
   b.rows = size32(table.size(0));
   b.width = size32(table.size(1));
   b.page_size = page;
+  const char* const message = "refs, table and lens must not share memory with each other or with what the call reads";
+  apart({&refs, &table, &lens}, lists, message);
+  apart({&refs}, {&table, &lens}, message);
+  apart({&table}, {&lens}, message);
   return b;
 }
 
@@ -490,8 +495,10 @@ struct PoolList {
   fgw_pages_pools view() const { return {data.data(), bytes.data(), (int32_t)data.size()}; }
 };
 
-// A tuple or list of pools [pages * page_size, ...], contiguous on the device.
-PoolList pools_of(PyObject* seq, int64_t pages, int32_t page, const c10::Device& device) {
+// A tuple or list of pools [pages * page_size, ...], contiguous on the device: each apart from the
+// lists and books of the call, and from the others (but for one given twice, which is copied twice
+// to the same contents).
+PoolList pools_of(PyObject* seq, int64_t pages, int32_t page, const c10::Device& device, Tensors others) {
   if (!PyTuple_Check(seq) && !PyList_Check(seq)) throw WrongType("pools must be a list or a tuple of tensors");
   PoolList list;
   const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
@@ -506,7 +513,14 @@ PoolList pools_of(PyObject* seq, int64_t pages, int32_t page, const c10::Device&
     list.data.push_back(x.data_ptr());
     list.bytes.push_back(x.numel() / pages * x.element_size());
     list.tensors.push_back(x);
+    apart({&x}, others, "pools must not share memory with the books or lists of the call");
   }
+  std::vector<std::pair<const char*, int64_t>> spans;
+  for (const at::Tensor& x : list.tensors) spans.emplace_back(static_cast<const char*>(x.data_ptr()), (int64_t)x.nbytes());
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    need(spans[i - 1].first + spans[i - 1].second <= spans[i].first || spans[i - 1] == spans[i],
+         "pools must not share memory with each other");
   return list;
 }
 
@@ -518,7 +532,11 @@ int32_t* ptr(const at::Tensor& x) { return static_cast<int32_t*>(x.data_ptr()); 
 // (refs, table, lens, counts, page) -> status
 PyObject* reserve(Args& a) {
   const at::Tensor refs = a.tensor(), table = a.tensor(), lens = a.tensor(), counts = a.tensor();
-  const fgw_pages_books b = books_of(refs, table, lens, a.int32());
+  const fgw_pages_books b = books_of(refs, table, lens, a.int32(), {});
+  // (The lengths themselves may be the counts: a row's are read before they change.)
+  const char* const message = "counts must not share memory with the books";
+  apart({&refs, &table}, {&counts}, message);
+  if (counts.data_ptr() != lens.data_ptr()) apart({&lens}, {&counts}, message);
   const c10::Device device = refs.device();
   const int32_t* c = metadata(counts, {b.rows}, device);
   const c10::DeviceGuard guard(device);
@@ -533,9 +551,9 @@ PyObject* fork_rows(Args& a) {
   PyObject* list = a.next();
   const at::Tensor refs = a.tensor(), table = a.tensor(), lens = a.tensor();
   const at::Tensor parents = a.tensor(), children = a.tensor();
-  const fgw_pages_books b = books_of(refs, table, lens, a.int32());
+  const fgw_pages_books b = books_of(refs, table, lens, a.int32(), {&parents, &children});
   const c10::Device device = refs.device();
-  const PoolList pools = pools_of(list, b.pages, b.page_size, device);
+  const PoolList pools = pools_of(list, b.pages, b.page_size, device, {&refs, &table, &lens, &parents, &children});
   const int32_t* p = metadata(parents, {-1}, device);
   const int32_t* c = metadata(children, {parents.size(0)}, device);
   const int32_t pairs = size32(parents.size(0));
@@ -551,7 +569,7 @@ PyObject* fork_rows(Args& a) {
 // (refs, table, lens, rows, page)
 PyObject* free_rows(Args& a) {
   const at::Tensor refs = a.tensor(), table = a.tensor(), lens = a.tensor(), rows = a.tensor();
-  const fgw_pages_books b = books_of(refs, table, lens, a.int32());
+  const fgw_pages_books b = books_of(refs, table, lens, a.int32(), {&rows});
   const c10::Device device = refs.device();
   const int32_t* r = metadata(rows, {-1}, device);
   const c10::DeviceGuard guard(device);
@@ -564,9 +582,9 @@ PyObject* free_rows(Args& a) {
 PyObject* compact(Args& a) {
   PyObject* list = a.next();
   const at::Tensor refs = a.tensor(), table = a.tensor(), lens = a.tensor();
-  const fgw_pages_books b = books_of(refs, table, lens, a.int32());
+  const fgw_pages_books b = books_of(refs, table, lens, a.int32(), {});
   const c10::Device device = refs.device();
-  const PoolList pools = pools_of(list, b.pages, b.page_size, device);
+  const PoolList pools = pools_of(list, b.pages, b.page_size, device, {&refs, &table, &lens});
   const c10::DeviceGuard guard(device);
   at::Tensor moved = ints(1, device), work = ints(entries.pages_workspace(b.pages, 0), device);
   const fgw_pages_pools view = pools.view();
@@ -584,7 +602,7 @@ PyObject* copy_pages(Args& a) {
   const c10::Device device = src.device();
   need(device.is_cuda(), kSameGpu);
   need(pages > 0, "positive pages required");
-  const PoolList pools = pools_of(list, pages, page, device);
+  const PoolList pools = pools_of(list, pages, page, device, {&src, &dst});
   const int32_t* s = metadata(src, {-1}, device);
   const int32_t* d = metadata(dst, {src.size(0)}, device);
   const c10::DeviceGuard guard(device);

@@ -13,7 +13,8 @@ share the ids; while gradients are recorded none may require one. Every decision
 lowest free page first and rows in order, so that the results are the same on every run and no call
 waits for the device: counts of what was refused come back as int32 tensors. Books that were changed
 by hand must stay consistent (every held page counted in refs, and a partly filled last page held by
-its row alone).
+its row alone). Books, lists and pools of a call share no memory with each other (but lens may be
+its own counts).
 """
 from __future__ import annotations
 

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from fgw_amd import _lib
-from fgw_amd.operators.mha import paged_extend as P
+from fgw_amd.operators.mha import cache_pages as C, paged_extend as P
 from fgw_amd.operators.mha.rotary import Rotary, apply_rotary
 
 shares = _lib.load_kv_module().shares_memory
@@ -126,3 +126,40 @@ def test_attention_and_rotation_refuse_outputs_over_their_inputs(step):
     pos = torch.zeros(1280, dtype=torch.int32, device="cuda")
     with pytest.raises(ValueError, match="share memory"):
         apply_rotary(fused, pos[:5], Rotary(64), out=pos.view(torch.bfloat16).view(5, 8, 64))
+
+
+@pytest.mark.gpu
+def test_books_lists_and_pools_must_be_apart():
+    pages, rows, width, page = 8, 4, 6, 4
+    books = C.new_books(pages, rows, width)
+    refs, table, lens = books
+    pools = [torch.zeros(pages * page, 8, device="cuda") for _ in range(2)]
+    ids = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device="cuda")
+    buffer = torch.zeros(pages * page + page, 8, device="cuda")
+    within = buffer.view(torch.int32).view(-1)
+    table2 = torch.full((rows, width), -1, dtype=torch.int32, device="cuda")
+    calls = [
+        lambda: C.reserve_rows(*books, table[0, :4], page), lambda: C.reserve_rows(*books, refs[2:6], page),
+        lambda: C.reserve_rows(refs, table2, table2.view(-1)[:rows], ids, page),
+        lambda: C.reserve_rows(table2.view(-1)[:pages], table2, lens, ids, page),
+        lambda: C.free_rows(*books, table[1], page), lambda: C.free_rows(*books, lens, page),
+        lambda: C.fork_rows(pools, *books, ids[:2], table[0, 2:4], page), lambda: C.fork_rows(pools, *books, lens, ids, page),
+        lambda: C.fork_rows([buffer[:-page], buffer[page:]], *books, ids[:1], ids[1:2], page),
+        lambda: C.fork_rows([pools[0], buffer[:-page]], *books, within[5:6], ids[1:2], page),
+        lambda: C.compact_pages([buffer[1:1 - page], pools[0], buffer[:-page]], *books, page),
+        lambda: C.compact_pages([buffer[:-page]], within[:pages], table, lens, page),
+        lambda: C.copy_pages([buffer[:-page]], within[:2], ids[:2], page),
+        lambda: C.copy_pages([buffer[page:], buffer[:-page]], ids[:1], ids[1:2], page),
+    ]
+    for call in calls:
+        with pytest.raises(ValueError, match="share memory"):
+            call()
+    assert not refs.any() and not lens.any() and bool((table == -1).all())
+    # Neighbours in one buffer, parts of one pool's layers, and one pool twice are taken.
+    layers = torch.randn(2, 2, pages * page, 8, device="cuda")
+    want = layers.clone()
+    want.view(4, pages, -1)[:, 5] = want.view(4, pages, -1)[:, 2]
+    C.copy_pages([*layers[0], *layers[1], layers[0, 0]], ids[2:3], ids[2:3] + 3, page)
+    assert torch.equal(layers, want)
+    assert C.reserve_rows(*books, ids, page).tolist() == [0, 0] and lens.tolist() == [0, 1, 2, 3]
+    assert C.reserve_rows(*books, lens, page).tolist() == [0, 0] and lens.tolist() == [0, 2, 4, 6]
