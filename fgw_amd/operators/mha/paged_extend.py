@@ -37,12 +37,12 @@ def mha_paged_append(q, k, v, k_cache, v_cache, block_table, cache_seqlens, cu_s
     q [T, Hq, D], k and v [T, Hkv, D]: FP16 or BF16 rows, strides multiples of 16 bytes (views of
     one fused projection will do). Row cu_seqlens[b] + j goes to the pool row
     block_table[b, pos // page_size] * page_size + pos % page_size of its cache position pos; it is
-    not written where pos lies outside [0, W * page_size) or the page id outside the pool. rotary (a
-    Rotary) turns q and k to their cache positions, or to positions [T] (int32 or int64); None
-    writes k as it is and copies q. Returns q_out ([T, Hq, D]; q itself for in place) or a new
-    contiguous tensor. No two tokens may have the same cache position of one page. The two pools and
-    q_out share no memory with each other or with anything the call reads (but q_out with q, as q
-    itself); heads side by side in one buffer do not.
+    not written where pos lies outside [0, W * page_size) or the page id outside the pool (lengths are
+    taken as given here; the attention clamps them). rotary (a Rotary) turns q and k to their cache
+    positions, or to positions [T] (int32 or int64); None writes k as it is and copies q. Returns
+    q_out ([T, Hq, D]; q itself for in place) or a new contiguous tensor. No two tokens may have the
+    same cache position of one page. The two pools and q_out share no memory with each other or with
+    anything the call reads (but q_out with q, as q itself); heads side by side in one buffer do not.
     """
     if rotary is None:
         if positions is not None:
@@ -88,12 +88,13 @@ def build_extend_kernel(heads, kv_heads, dim, page_size, dtype, device_index=Non
     sees the keys 0 .. p, with window (>= 1) only the last `window` of them, itself among them; not
     causal: every live key (attention over an encoder's cached states). softmax_scale: D ** -0.5
     unless given. The callable takes (q, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens,
-    max_new, out=None), shapes free from call to call, and reads nothing back: lengths outside
-    [0, W * page_size] are clamped, tokens that see no key give zero rows, page ids outside the
-    pool read as zeros. Keys that no token of a request sees do not matter, whatever they hold. A NaN
-    in a query or in a key that it sees gives a row of NaN. A key whose V is not finite gives NaN or
-    infinities to the tokens that see it, and may give NaN to other new tokens of the same request
-    and call (a weight of 0 times it).
+    max_new, out=None), shapes free from call to call, and reads nothing back. Lengths outside
+    [0, W * page_size] are clamped (positions then follow from the clamped length, other ones than
+    mha_paged_append wrote); tokens that see no key give zero rows; page ids outside the pool read as
+    zeros. Keys that no token of a request sees do not matter, whatever they hold. A NaN in a query or
+    in a key that it sees gives a row of NaN. A key whose V is not finite gives NaN or infinities to
+    the tokens that see it, and may give NaN to other new tokens of the same request and call (a
+    weight of 0 times it).
     """
     name = _dtype_name(dtype)
     if dim < 16 or dim > 256 or dim % 16:

@@ -13,6 +13,9 @@
  * as zeros and is not written. New tokens are packed: request b has the rows
  * [cu[b], cu[b + 1]) of Q, K, V (cu [B + 1] int32, cu[0] = 0, never falling), and its cache length
  * counts them: its row cu[b] + j has the cache position len_b - n_b + j, n_b = cu[b + 1] - cu[b].
+ * Lengths lie in [0, W * page_size], where fgw_pages_reserve keeps them. Of others fgw_kv_append
+ * writes the tokens whose position has a place, while fgw_kv_extend takes the nearer end for the
+ * length, and so sees other positions than those written.
  * Rows at and behind cu[B] are neither read nor written. What a call writes shares no memory with
  * what it reads, except where a rotated output may be the input itself.
  *
