@@ -5,20 +5,25 @@
 // tile: row R of (request, K/V head) is token R / G, head R % G of the group, so a tile of 32 rows
 // reads each key once for all of them. Row R sees the keys [lo, hi) of its token:
 //   hi = len - n + token + 1 (causal; else len),  lo = hi - window (no window: 0).
-// Softmax and products are those of fmha_kernel.h (fp32 sums and statistics); for the PV product P is
-// rounded to the input type in the kernels of long tiles, and two numbers of it in the one of few rows.
+// Softmax and products are those of fmha_kernel.h (fp32 sums and statistics). For the PV product P is
+// two numbers of the input type in the kernel of few rows, which memory bounds, and one (rounded) in
+// the kernels of long tiles: there the second product would be half as many matrix operations again
+// where those are the bound. Error against 64 bits relative to the output (q of standard deviation 2,
+// the rest 1; the output's own rounding alone 0.0017 in BF16, 0.00021 in FP16): one number
+// 0.0022-0.0023 and 0.00027, two as the rounding alone; 4096 tokens, Hq 32, Hkv 8, D 256 take 424 us
+// with one, 796 with two.
 //
 // Work. Lengths and counts are on the device, so each program finds its item itself (find_item): it
 // reads the lengths of 64 requests at a time, one to a lane, and sums tiles and splits over the
 // wave. An item is a tile, or where tiles are fewer than the `target` programs that fill the card,
 // one of its splits: a tile of u units of keys has ceil(u / chunk) of them, with the smallest chunk
 // that leaves no more than `target` items (best_chunk). So all items run at once, the long requests
-// of a ragged batch in pieces; a CU reads at most 38 GB/s, 1.7 times its share of the memory, so
-// pieces of unequal length cost nothing until one has twice its share (B 32, Hq 32, Hkv 8, D 128,
-// lengths 1024-4096, us: split W / target evenly 76, even ranges over the tiles laid end to end
-// 75, whole tiles 73, each with P as one number and ordinary loads; see also extend_rows_kernel). Grid and workspace follow on the host from
-// sizes alone, programs without an item end after the sums. Split tiles go through partials (O / l,
-// LSE) and a join.
+// of a ragged batch in pieces. A CU that reads alone takes 32 GB/s at D 64, 42 at D 128 and 48 at D
+// 256, where its share of the memory is 20: pieces of unequal length cost little until one has twice
+// its share (B 32, Hq 32, Hkv 8, D 128, lengths 1024-4096, one tile to a CU, us: whole tiles 68.7,
+// split evenly by W / target 74.6; see also extend_rows_kernel). Grid and workspace follow on the host
+// from sizes alone, programs without an item end after the sums. Split tiles go through partials
+// (O / l, LSE) and a join.
 // The K/V head is fastest in an item's number: workgroup w runs on XCD w % 8, so with 8 heads an XCD
 // holds one of them.
 #pragma once
@@ -100,8 +105,10 @@ __device__ __forceinline__ int splits_of(const ExtendParams& p, int units, int c
 // with which all tiles of a head have at most target / heads splits together; kWhole where whole
 // tiles are as many, however unequal: the partials of long tiles, 132 KB each at D 128, cost what the
 // balance gains (tiles above the average share cut in two, us, whole / cut: B 2, Hq 8, Hkv 8, 4096
-// tokens 111 / 111; B 4, 512 tokens, lengths 1024-4096, Hq 32, Hkv 8 106 / 136). The sums saturate
-// (kMany) so that they stay in 32 bits; the same in every program.
+// tokens 111 / 111; B 4, 512 tokens, lengths 1024-4096, Hq 32, Hkv 8 106 / 136). One chunk serves
+// all tiles, so items jump by the number of long tiles: 17 tiles with places for 32 stay whole, 16 are
+// cut in two (a prompt of 1088 tokens, Hq 32, Hkv 8: the longest item 17 blocks; of 1024: 8). The sums
+// saturate (kMany) so that they stay in 32 bits; the same in every program.
 constexpr int kWhole = 0x40000000, kMany = 1 << 24;
 template <class T>
 __device__ __forceinline__ int best_chunk(const ExtendParams& p, const int32_t* lengths, const int32_t* cu,
@@ -371,7 +378,9 @@ __device__ __forceinline__ void join_rows(const ExtendParams& p, const Item& it,
 // dma_saddr with a non-temporal load, for keys that a call reads once: they take no place from others in
 // the 256 MB cache. Ordinary / non-temporal, us: B 32, lengths 1024-4096, D 128 74.4 / 69.0, D 256
 // 135 / 125; 64 requests of 8192 keys 362 / 328; one of 32768 33.4 / 31.0; small or shared pages alike (32
-// requests over the same 4096 keys 56.7 / 56.8, B 4 KV 4096 19.1 / 19.7).
+// requests over the same 4096 keys 56.7 / 56.8, B 4 KV 4096 19.1 / 19.7), and where several tiles read
+// the same keys it goes either way (8 requests of 8192 keys, 36 / 64 / 128 rows: 68.7 / 73.8, 70.9 / 67.7,
+// 112.5 / 111.3).
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void dma_once(const void* base, u32 voff, u32 lds) {
@@ -544,11 +553,14 @@ __device__ __forceinline__ void load_q(const ExtendParams& p, const Item& it, in
 //
 // The weights P of the PV product are the sum of two numbers of the input type (softmax_exp_two), so
 // that an output is as exact as its own rounding: the memory bounds this kernel, and the second product
-// costs 1-2% (D 128, ordinary loads, us, one number / two: B 32 lengths 1024-4096 73.1 / 74.2, B 1 KV 32768
-// 33.2 / 33.3, 8 x 8 tokens KV 2048-8192 45.1 / 45.2; 9% where 120 rows read 512-2048 keys, 30.0 / 32.9). With one,
-// where a few keys carry a row, its error was up to 1.8 times that of the output's rounding.
+// costs 0-2% (D 128, us, one number / two: B 32 lengths 1024-4096 68.0 / 69.4, B 1 KV 32768 30.5 /
+// 30.9, 8 x 8 tokens KV 2048-8192 41.9 / 42.0, 120 rows of 2048 keys 19.3 / 19.7). With one, where a
+// few keys carry a row, its error was up to 1.8 times that of the output's rounding.
 // Bound: B 32, lengths 1024-4096, 4.9 TB/s, by what a CU reads of the longest tile (D 256 5.4); 64
-// requests of 8192 keys 6.5 TB/s; one of 32768 4.3 TB/s. One of 512 keys (Hq 8, Hkv 2, D 64) takes 8.8 us: a chain of dependent reads (lengths, page ids, keys) and four rounds.
+// requests of 8192 keys 6.5 TB/s; one of 32768 4.4 TB/s. One of 512 keys (Hq 8, Hkv 2, D 64) takes
+// 8.4 us: a chain of dependent reads (lengths, page ids, keys) and four rounds. At D 64 a round moves
+// half the bytes of D 128 through the same chain, hence the lower rate of a CU; at D 80 and 96 every
+// instruction selects an address to a lane, since the tile has dims past D.
 template <int DPAD>
 constexpr int kStages = DPAD >= 128 ? 1 : DPAD == 64 ? 2 : 4;
 

@@ -14,9 +14,8 @@ namespace fgw_kv {
 
 // Requests of up to kLongFrom rows (tokens times query heads of a K/V head) take the kernel of few
 // rows: it reads the keys once for every 32 of them, the long one once for 256. Hq 32, Hkv 8, D 128,
-// pages of 64, few rows / long, us: 128 rows B1 KV 1024 17.0 / 26.9, B4 KV 2048 24.3 / 36.6, B1 KV
-// 8192 26.4 / 37.2, B8 KV 8192 96.5 / 88.6; 192 rows 17.2 / 29.2, 29.9 / 39.3, 32.6 / 39.1,
-// 146 / 93.9.
+// pages of 64, few rows / long, us: 128 rows B1 KV 1024 17.7 / 17.6, B4 KV 2048 27.6 / 30.6, B1 KV
+// 8192 29.3 / 27.0, B8 KV 8192 112 / 88; 192 rows 18.3 / 19.6, 34.0 / 32.3, 36.2 / 29.4, 184 / 92.
 constexpr int kLongFrom = 128;
 // Units of a split at least (rounds of 128 keys, blocks of 64): below, a split's own cost outweighs
 // what it saves. Few rows, B1 Hq 32 Hkv 8 D 128, splits of 1 / 2 / 4 rounds, us: KV 1024

@@ -6,7 +6,8 @@
 // blocks come by DMA into rings of four slots, two blocks ahead. What differs: a program runs one
 // item, found from the lengths on the device (find_item); a lane's row is a (token, head) pair, so
 // its keys end at its own token and, with a window, begin at it; output rows are written by token.
-// An item reads its keys once for the G heads of a group: at G 4 and 64 tokens a tile, a block of
+// P is rounded once to the input type for the PV product (kv_extend.h gives the error and the cost of
+// more). An item reads its keys once for the G heads of a group: at G 4 and 64 tokens a tile, a block of
 // 32 KB feeds 4.3 MFLOP.
 //
 // ROWS as in fmha_prefill.h: blocks in one page (page_size a multiple of 64), row groups (a page

@@ -4,10 +4,11 @@
 // The K/V ring of extend_long_kernel does not fit a CU's LDS at this head-dim tile, nor do its
 // operands fit the registers; this is fwd_kernel's kDual arrangement (fmha_kernel.h): two sets of
 // four waves hold the same 128 rows, each takes 32 keys of every 64-key block through two stages of
-// its own, and their states meet in LDS at the end, so that one set's softmax runs beside the
-// other's products. Bound by the chain of a block (two waves to a SIMD at 256 registers). Hq 32,
-// Hkv 8, 4096 tokens causal: D 256 427 us (644 TFLOP/s), D 192 439; 512 tokens behind 7680 cached
-// ones, D 256, 223. The kernel of few rows takes 787, 841 and 327 for them.
+// its own, and their states meet in LDS at the end, so that one set's softmax runs beside the other's
+// products (P rounded once, as in extend_long_kernel). Bound by the chain of a block (two waves to a
+// SIMD at 256 registers). Hq 32, Hkv 8, 4096 tokens causal: D 256 424 us (649 TFLOP/s), D 192 433;
+// 512 tokens behind 7680 cached ones, D 256, 210. The kernel of few rows takes 787, 841 and 327 for
+// them.
 #pragma once
 #include "kv_extend_long.h"
 

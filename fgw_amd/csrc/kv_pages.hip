@@ -5,15 +5,16 @@
 // out by its rank among the free pages in order of id, to rows in order: the same books and pools
 // on every run, with atomics only where sums of integers meet.
 //
-// Two launches: `plan` (one workgroup: scans the holders of all pages, ranks what is free or has
-// to move, and writes the books of rows and pages that need no long walk) and `move` (the whole
-// card: pools' pages, 16 bytes to a lane, and the rows of the table). The plan is bound by the
-// latency of its few dependent reads: every thread takes 16 holders with four independent loads,
-// 16384 pages to a step of one scan. The moves are bound by memory: each page read and written once
-// in every pool, 32 bytes to a thread (compact 205 pages of 32 KB in 16 pools, fork 40 of 128 KB in 16,
-// us, 32 / 64 / 128 / 256 bytes: 44 / 46 / 49 / 50, 25.1 / 25.8 / 26.5 / 30). Reads go through the
-// caches, since the children of a row copy the same page (40 of 16 rows: 28 us, 44 with non-temporal reads);
-// what is written is not read soon.
+// Two launches: `plan` (one workgroup: scans the holders of all pages, ranks what is free or has to
+// move, and writes the books of rows and pages that need no long walk) and `move` (the whole card:
+// pools' pages, 16 bytes to a lane, and the rows of the table). The plan is bound by the latency of
+// its few dependent reads: every thread takes 16 holders with four independent loads, 16384 pages to
+// a step of one scan. A reservation is that plan alone (a call with its launch: 32 rows of 512 pages
+// 5.1 us, 256 of 4096 5.6, 1024 of 65536 9.6). The moves are bound by memory: each page read and
+// written once in every pool, 32 bytes to a thread (compact 205 pages of 32 KB in 16 pools, fork 40
+// of 128 KB in 16, us, 32 / 64 / 128 / 256 bytes: 44 / 46 / 49 / 50, 25.1 / 25.8 / 26.5 / 30). Reads
+// go through the caches, since the children of a row copy the same page (40 of 16 rows: 28 us, 44
+// with non-temporal reads); what is written is not read soon.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
