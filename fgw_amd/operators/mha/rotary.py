@@ -157,6 +157,8 @@ def apply_rotary(x, positions, rotary, *, inverse=False, out=None):
     the other way: the transpose of the forward, so its gradient. Returns a new contiguous tensor,
     or out ([T, H, D], x itself for in place, else memory apart from x and positions). Differentiable
     in x, twice too, and in forward mode; out is for calls that record no gradient, and requires none.
+    A backward pass can be captured into a HIP graph like any of torch's, while no eager graph of the
+    same leaves lives.
     """
     if not isinstance(rotary, Rotary):
         raise TypeError("rotary must be a Rotary")
