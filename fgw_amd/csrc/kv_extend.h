@@ -45,6 +45,31 @@ struct ExtendParams : FwdParams {
   int32_t* notes;              // for the join: [work] JoinNote
 };
 
+// Requests in groups that share a prefix (fgw_kv_shared; kv_shared.hip has the two passes). The first
+// pass attends over the groups' prefixes, each a request of the kernels below whose rows are those of all
+// its group's tokens, and leaves partials; the second over the rest of each request's keys, and joins.
+struct SharedParams : ExtendParams {
+  const int32_t* groups;    // [n_groups + 1]
+  const int32_t* prefixes;  // [n_groups]
+  int32_t n_groups;
+  int32_t prefix_slots, prefix_rows;  // places of the first pass's partials, rows of a place
+  const float* prefix_parts;
+  const float* prefix_lse;
+  int32_t* group_notes;     // [n_groups] GroupNote
+};
+struct PrefixParams : SharedParams {};
+struct SuffixParams : SharedParams {};
+template <class P>
+constexpr bool kIsPrefix = std::is_same<P, PrefixParams>::value;
+template <class P>
+constexpr bool kIsSuffix = std::is_same<P, SuffixParams>::value;
+
+// Where a group's partials are: those of its first item (a place for each K/V head), the splits of its
+// tiles, how many tiles, and the group's first token. Written by the first pass.
+struct GroupNote {
+  int32_t base, splits, tiles, first;
+};
+
 // Tiles of ROWS rows, keys in blocks of BN, splits in units of UNIT blocks.
 template <int ROWS_, int BN_, int UNIT_>
 struct Tiling {
@@ -56,12 +81,20 @@ typedef Tiling<128, 64, 1> WideTiling;   // extend_wide_kernel
 
 struct Request {
   int first, n, len, tiles, units;
+  int row;          // prefix pass: of the block table
+  int from, group;  // suffix pass: keys [0, from) are in the prefix of `group` (-1: none shared)
 };
+
+template <class P>
+__device__ __forceinline__ int requests_of(const P& p) {
+  if constexpr (kIsPrefix<P>) return p.n_groups;
+  else return p.batch;
+}
 
 template <class T>
 __device__ __forceinline__ Request load_request(const ExtendParams& p, const int32_t* lengths,
                                                 const int32_t* cu, int b) {
-  Request r{0, 0, 0, 0, 0};
+  Request r{0, 0, 0, 0, 0, 0, 0, -1};
   if (b >= p.batch) return r;
   const int first = cu[b], next = cu[b + 1];
   int len = lengths[b];
@@ -79,6 +112,78 @@ __device__ __forceinline__ Request load_request(const ExtendParams& p, const int
   int end = p.causal ? r.len - r.n + count : r.len;
   end = end < 0 ? 0 : end;
   r.units = (end + T::KEYS - 1) / T::KEYS - lo / T::KEYS;
+  return r;
+}
+
+// Requests [f0, f1) of group g and the keys that they share: as many as the first of them, whose table
+// row holds them, has before its new tokens (none for a request alone: it reads its keys itself).
+struct Group {
+  int f0, f1, keys;
+};
+__device__ __forceinline__ Group load_group(const SharedParams& p, const int32_t* lengths, const int32_t* cu, int g) {
+  Group x{0, 0, 0};
+  if (g >= p.n_groups) return x;
+  const int f0 = p.groups[g], f1 = p.groups[g + 1], wanted = p.prefixes[g];
+  if (f0 < 0 || f1 > p.batch || f1 <= f0 + 1) return x;
+  const int n = cu[f0 + 1] - cu[f0], capacity = p.width * p.page_size;
+  int len = lengths[f0];
+  len = len < 0 ? 0 : (len > capacity ? capacity : len);
+  const int before = n >= 0 && n < len ? len - n : 0;
+  x.f0 = f0;
+  x.f1 = f1;
+  x.keys = wanted < before ? wanted : before;
+  x.keys = x.keys < 0 ? 0 : x.keys;
+  return x;
+}
+
+template <class T>
+__device__ __forceinline__ Request load_request(const PrefixParams& p, const int32_t* lengths, const int32_t* cu, int g) {
+  Request r{0, 0, 0, 0, 0, 0, 0, -1};
+  const Group x = load_group(p, lengths, cu, g);
+  if (x.keys == 0) return r;
+  const int first = cu[x.f0], next = cu[x.f1];
+  r.row = x.f0;
+  r.len = x.keys;
+  r.first = first;
+  if (first < 0 || next > p.tokens || next <= first) return r;
+  r.n = next - first;
+  r.tiles = (int)(((int64_t)r.n * p.group + T::ROWS - 1) / T::ROWS);
+  r.units = (r.len + T::KEYS - 1) / T::KEYS;
+  return r;
+}
+
+// The group of each lane's request: up to 64 groups are held one to a lane and passed around, more are
+// searched for in memory (their first requests never fall).
+template <class T>
+__device__ __forceinline__ Request load_request(const SuffixParams& p, const int32_t* lengths, const int32_t* cu, int b) {
+  Group x{0, 0, 0};
+  int group = -1;
+  if (p.n_groups <= 64) {
+    const Group mine = load_group(p, lengths, cu, (int)(threadIdx.x & 63u));
+    for (int g = 0; g < p.n_groups; ++g) {
+      const int f0 = __builtin_amdgcn_readlane(mine.f0, g), f1 = __builtin_amdgcn_readlane(mine.f1, g);
+      const int keys = __builtin_amdgcn_readlane(mine.keys, g);
+      if (b >= f0 && b < f1) {
+        x.keys = keys;
+        group = g;
+      }
+    }
+  } else {
+    int lo = 0, hi = p.n_groups;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (p.groups[mid] <= b) lo = mid; else hi = mid;
+    }
+    x = load_group(p, lengths, cu, lo);
+    group = lo;
+    if (b < x.f0 || b >= x.f1) x.keys = 0;
+  }
+  Request r = load_request<T>(static_cast<const ExtendParams&>(p), lengths, cu, b);
+  if (x.keys > 0 && r.n > 0 && r.len - r.n >= x.keys) {
+    r.from = x.keys;
+    r.group = group;
+    r.units -= r.units > 0 ? r.from / T::KEYS : 0;
+  }
   return r;
 }
 
@@ -110,14 +215,14 @@ __device__ __forceinline__ int splits_of(const ExtendParams& p, int units, int c
 // cut in two (a prompt of 1088 tokens, Hq 32, Hkv 8: the longest item 17 blocks; of 1024: 8). The sums
 // saturate (kMany) so that they stay in 32 bits; the same in every program.
 constexpr int kWhole = 0x40000000, kMany = 1 << 24;
-template <class T>
-__device__ __forceinline__ int best_chunk(const ExtendParams& p, const int32_t* lengths, const int32_t* cu,
+template <class T, class P>
+__device__ __forceinline__ int best_chunk(const P& p, const int32_t* lengths, const int32_t* cu,
                                           const Request& r0, int lane) {
   const int limit = (int)((u32)p.target / (u32)p.heads);
   if (limit <= 1) return kWhole;
   auto sum = [&](auto&& count) {
     int total = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += 64) {
+    for (int b0 = 0; b0 < requests_of(p); b0 += 64) {
       const Request r = b0 == 0 ? r0 : load_request<T>(p, lengths, cu, b0 + lane);
       const int64_t x = r.tiles ? count(r) : 0;
       total += wave_sum((int)(x < kMany ? x : kMany), lane);
@@ -146,19 +251,21 @@ struct Item {
   int lo, hi;
   int blk_begin, blk_end;
   int slot, slot0, slot_step;  // partials: of this split, of the first one; between splits
+  int from, group;             // suffix pass: as Request's
+  int place, tiles;            // prefix pass: among the request's items of a head, its tiles
 };
 
 // Item w of the launch; false where there is none. Uniform over the wave; every wave of a workgroup
 // computes the same.
-template <class T>
-__device__ __forceinline__ bool find_item(const ExtendParams& p, const int32_t* lengths,
+template <class T, class P>
+__device__ __forceinline__ bool find_item(const P& p, const int32_t* lengths,
                                           const int32_t* cu, int w, int lane, Item& it) {
   const Request r0 = load_request<T>(p, lengths, cu, lane);
   const int chunk = p.target > 0 ? best_chunk<T>(p, lengths, cu, r0, lane) : kWhole;
   const int g = (int)((u32)w / (u32)p.heads);
   it.head = w - g * p.heads;
   int items_before = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 64) {
+  for (int b0 = 0; b0 < requests_of(p); b0 += 64) {
     const Request r = b0 == 0 ? r0 : load_request<T>(p, lengths, cu, b0 + lane);
     const int splits = splits_of(p, r.units, chunk);
     const int items = r.tiles * splits;
@@ -169,7 +276,11 @@ __device__ __forceinline__ bool find_item(const ExtendParams& p, const int32_t* 
       const int l = __builtin_ctzll(hit);
       auto pick = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
       const int s = pick(splits), place = pick(at), tiles = pick(r.tiles);
-      it.b = b0 + l;
+      it.b = kIsPrefix<P> ? pick(r.row) : b0 + l;
+      it.from = kIsSuffix<P> ? pick(r.from) : 0;
+      it.group = kIsSuffix<P> ? pick(r.group) : kIsPrefix<P> ? b0 + l : -1;
+      it.place = place;
+      it.tiles = tiles;
       it.first = pick(r.first);
       it.n = pick(r.n);
       it.len = pick(r.len);
@@ -186,7 +297,7 @@ __device__ __forceinline__ bool find_item(const ExtendParams& p, const int32_t* 
       const int t0 = row0 / p.group, t1 = (row0 + it.rows - 1) / p.group;
       int hi = p.causal ? it.len - it.n + t1 + 1 : it.len;
       hi = hi < 0 ? 0 : hi;
-      int lo = p.window > 0 ? it.len - it.n + t0 - p.window + 1 : 0;
+      int lo = kIsSuffix<P> ? it.from : p.window > 0 ? it.len - it.n + t0 - p.window + 1 : 0;
       lo = lo < 0 ? 0 : (lo > hi ? hi : lo);
       it.lo = lo;
       it.hi = hi;
@@ -199,7 +310,7 @@ __device__ __forceinline__ bool find_item(const ExtendParams& p, const int32_t* 
       it.blk_end = (from + split_bound(units, it.split + 1, it.splits)) * T::UNIT;
       it.blk_end = it.blk_end < end ? it.blk_end : end;
       // (Offsets that fall and rise again make more items than there are places for partials.)
-      return it.split < it.splits && (it.splits == 1 || it.slot0 + (it.splits - 1) * it.slot_step < p.work);
+      return it.split < it.splits && ((it.splits == 1 && !kIsPrefix<P>) || it.slot0 + (it.splits - 1) * it.slot_step < p.work);
     }
     items_before += __builtin_amdgcn_readlane(items_to, 63);
   }
@@ -210,9 +321,11 @@ __device__ __forceinline__ bool find_item(const ExtendParams& p, const int32_t* 
 struct Seen {
   int lo, hi;
 };
-__device__ __forceinline__ Seen row_seen(const ExtendParams& p, const Item& it, int token) {
+template <class P>
+__device__ __forceinline__ Seen row_seen(const P& p, const Item& it, int token) {
   int hi = p.causal ? it.len - it.n + token + 1 : it.len;
   hi = hi < 0 ? 0 : hi;
+  if constexpr (kIsSuffix<P>) return Seen{it.from, hi};
   int lo = p.window > 0 ? it.len - it.n + token - p.window + 1 : 0;
   lo = lo < 0 ? 0 : lo;
   return Seen{lo, hi};
@@ -266,15 +379,41 @@ __device__ __forceinline__ float part_lse(float m_log2, float total) {
 // What a second launch has to know to join split tiles: every item's, in its own place (splits 0:
 // no split tile's).
 struct JoinNote {
-  int32_t first, tile, head, rows, splits, split, pad[2];
+  int32_t first, tile, head, rows, splits, split, group, pad;
 };
-__device__ __forceinline__ void write_note(const ExtendParams& p, const Item& it, bool found) {
+template <class P>
+__device__ __forceinline__ void write_note(const P& p, const Item& it, bool found) {
   const int w = (int)blockIdx.x;
+  if constexpr (kIsPrefix<P>) {
+    if (found && it.place == 0 && it.head == 0 && threadIdx.x == 0)
+      reinterpret_cast<GroupNote*>(p.group_notes)[it.group] = GroupNote{w / p.heads, it.splits, it.tiles, it.first};
+    return;
+  }
   if (p.notes == nullptr || w >= p.work || threadIdx.x != 0) return;
-  JoinNote note{0, 0, 0, 0, 0, 0, {0, 0}};
+  JoinNote note{0, 0, 0, 0, 0, 0, 0, 0};
   if (found && it.splits > 1)
-    note = JoinNote{it.first, it.tile, it.head, it.rows, it.splits, it.split, {0, 0}};
+    note = JoinNote{it.first, it.tile, it.head, it.rows, it.splits, it.split, it.group, 0};
   reinterpret_cast<JoinNote*>(p.notes)[w] = note;
+}
+
+// The partials that the first pass left for a row of a request: split s at place `slot` + s * step, row
+// `row` of it.
+struct PrefixRow {
+  int slot, step, splits, row;
+};
+__device__ __forceinline__ PrefixRow prefix_row(const SharedParams& p, const GroupNote& note, int first, int head, int row) {
+  const int r = (first - note.first) * p.group + row, tile = (int)((u32)r / (u32)p.prefix_rows);
+  PrefixRow x;
+  x.slot = (note.base + (note.tiles - 1 - tile) * note.splits) * p.heads + head;
+  x.step = p.heads;
+  x.row = r - tile * p.prefix_rows;
+  // (Places that a group of broken offsets would not have are not read.)
+  const int64_t last = (int64_t)x.slot + (int64_t)(note.splits - 1) * x.step;
+  x.splits = r >= 0 && note.splits > 0 && x.slot >= 0 && last < p.prefix_slots ? note.splits : 0;
+  return x;
+}
+__device__ __forceinline__ GroupNote group_note(const SharedParams& p, int group) {
+  return reinterpret_cast<const GroupNote*>(p.group_notes)[group];
 }
 
 // The splits g, g + share, ... of one (row, 4 dims) into a state; CH of them are loaded before any is
@@ -317,13 +456,43 @@ __device__ __forceinline__ void join_splits(const ExtendParams& p, const Item& i
   }
 }
 
+// The splits g, g + share, ... of a row's prefix into a state of 4 dims, as above.
+template <int CH>
+__device__ __forceinline__ void join_prefix(const SharedParams& p, const PrefixRow& x, int c, int g, int share, float& peak,
+                                            float& tot, f32x4& acc) {
+  for (int s0 = g; s0 < x.splits; s0 += CH * share) {
+    float lse[CH];
+    f32x4 v[CH];
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const int split = s0 + k * share < x.splits ? s0 + k * share : g;
+      const int64_t at = (int64_t)(x.slot + split * x.step) * p.prefix_rows + x.row;
+      lse[k] = p.prefix_lse[at];
+      v[k] = *reinterpret_cast<const f32x4*>(p.prefix_parts + at * p.dim + 4 * c);
+    }
+    float top = peak;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) top = s0 + k * share < x.splits ? fmaxf(top, lse[k]) : top;
+    const float keep = expf(peak - top);
+    tot *= keep;
+    acc *= keep;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const float w = s0 + k * share < x.splits ? expf(lse[k] - top) : 0.0f;
+      tot += w;
+      acc += s0 + k * share < x.splits ? v[k] * w : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    peak = top;
+  }
+}
+
 // Rows [row_from, row_to) of a split tile from its partials, by the whole workgroup. A thread holds 4
 // dims of a row; where `share_rows` rows leave threads over, they share its splits (both joins of a
 // short tile pass all its rows there, and so add in the same order). Weights exp(LSE - peak), empty
 // splits (LSE -1e30) weigh nothing, an all-empty row is zero. COH: the partials were written by this
 // launch. Uses 24 bytes of LDS a thread.
-template <bool BF16, bool COH>
-__device__ __forceinline__ void join_rows(const ExtendParams& p, const Item& it, int tile_rows, int row_from, int row_to,
+template <bool BF16, bool COH, class P>
+__device__ __forceinline__ void join_rows(const P& p, const Item& it, int tile_rows, int row_from, int row_to,
                                           int share_rows, unsigned char* lds, int tid, int threads) {
   using E = Elem<BF16>;
   f32x4* const sacc = reinterpret_cast<f32x4*>(lds);
@@ -344,6 +513,11 @@ __device__ __forceinline__ void join_rows(const ExtendParams& p, const Item& it,
         join_splits<COH, 4>(p, it, tile_rows, r, c, g, share, peak, tot, acc);
       else
         join_splits<COH, 8>(p, it, tile_rows, r, c, g, share, peak, tot, acc);
+      if constexpr (kIsSuffix<P>) {
+        if (it.group >= 0)
+          join_prefix<4>(p, prefix_row(p, group_note(p, it.group), it.first, it.head, it.tile * tile_rows + r), c, g,
+                         share, peak, tot, acc);
+      }
     }
     if (share > 1) {  // uniform
       sacc[tid] = acc;
@@ -618,8 +792,71 @@ __device__ __forceinline__ float softmax_exp_two(const f32x16& s, float m, float
   return (rs[0] + rs[1]) + (rs[2] + rs[3]);
 }
 
+// The rows of an unsplit tile of a request with a prefix: the four waves' states (cm, cl, co of
+// extend_tile) and the prefix's partials. Threads that rows times dims leave over share a row's partials.
 template <class C>
-__device__ __forceinline__ void extend_tile(const ExtendParams& p, const int32_t* table, const Item& it,
+__device__ __forceinline__ void finish_shared(const SuffixParams& p, const Item& it, const float* cm, const float* cl,
+                                              const float* co, unsigned char* lds, int tid) {
+  using E = Elem<C::BF16>;
+  constexpr int threads = C::THREADS;
+  const GroupNote note = group_note(p, it.group);
+  const int d4n = p.dim / 4, pairs = it.rows * d4n;
+  const int share = pairs < threads ? threads / pairs : 1;
+  for (int base = 0; base < pairs; base += threads) {
+    const int pair = share > 1 ? tid % pairs : base + tid, g = share > 1 ? tid / pairs : 0;
+    const bool act = pair < pairs && g < share;
+    const int r = pair / d4n, c = pair % d4n;
+    float peak = kNegBig, tot = 0.0f;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (act) {
+      if (g == 0) {
+        float mm = kNegBig;
+#pragma unroll
+        for (int k = 0; k < C::NWK; ++k) mm = fmaxf(mm, cm[k * C::ROWS_WAVE + r]);
+#pragma unroll
+        for (int k = 0; k < C::NWK; ++k) {
+          const float wt = __builtin_amdgcn_exp2f(cm[k * C::ROWS_WAVE + r] - mm);
+          tot += cl[k * C::ROWS_WAVE + r] * wt;
+          acc += *reinterpret_cast<const f32x4*>(co + (k * C::ROWS_WAVE + r) * C::OSTRIDE + 4 * c) * wt;
+        }
+        peak = mm * kLn2;
+      }
+      join_prefix<8>(p, prefix_row(p, note, it.first, it.head, it.tile * C::ROWS_TILE + r), c, g, share, peak, tot, acc);
+    }
+    if (share > 1) {  // uniform; one pass
+      f32x4* const sacc = reinterpret_cast<f32x4*>(lds);
+      float* const speak = reinterpret_cast<float*>(lds + threads * 16);
+      float* const stot = speak + threads;
+      __syncthreads();  // the waves' states are read
+      sacc[tid] = acc;
+      speak[tid] = peak;
+      stot[tid] = tot;
+      __syncthreads();
+      if (act && g == 0) {
+        float top = peak;
+        for (int k = 1; k < share; ++k) top = fmaxf(top, speak[k * pairs + pair]);
+        const float keep = expf(peak - top);
+        acc *= keep;
+        tot *= keep;
+        for (int k = 1; k < share; ++k) {
+          const float w = expf(speak[k * pairs + pair] - top);
+          acc += sacc[k * pairs + pair] * w;
+          tot += stot[k * pairs + pair] * w;
+        }
+      }
+    }
+    if (act && g == 0) {
+      const float inv = 1.0f / fmaxf(tot, 1.0e-30f);
+      u32x2 w;
+      w.x = E::pack2(acc[0] * inv, acc[1] * inv);
+      w.y = E::pack2(acc[2] * inv, acc[3] * inv);
+      *reinterpret_cast<u32x2*>(static_cast<u16*>(p.out) + out_row(p, it, it.tile * C::ROWS_TILE + r) + 4 * c) = w;
+    }
+  }
+}
+
+template <class C, class P>
+__device__ __forceinline__ void extend_tile(const P& p, const int32_t* table, const Item& it,
                                             unsigned char* smem, int tid, bool fused) {
   // (Opaque copies: what derives from the lane is computed here and at the end, not held across the
   // caller's loop.)
@@ -750,6 +987,12 @@ __device__ __forceinline__ void extend_tile(const ExtendParams& p, const int32_t
   }
   __syncthreads();
   using E = Elem<C::BF16>;
+  if constexpr (kIsSuffix<P>) {
+    if (it.splits == 1 && it.group >= 0) {
+      finish_shared<C>(p, it, cm, cl, co, smem, tid);
+      return;
+    }
+  }
   constexpr int D4 = C::DPAD / 4;
   for (int idx = tid; idx < it.rows * D4; idx += C::THREADS) {
     const int r = idx / D4, d0 = 4 * (idx % D4);
@@ -766,7 +1009,7 @@ __device__ __forceinline__ void extend_tile(const ExtendParams& p, const int32_t
       acc += *reinterpret_cast<const f32x4*>(co + (k * C::ROWS_WAVE + r) * C::OSTRIDE + d0) * wt;
     }
     const float inv = 1.0f / fmaxf(t2, 1.0e-30f);
-    if (it.splits == 1) {
+    if (it.splits == 1 && !kIsPrefix<P>) {
       u32x2 w;
       w.x = E::pack2(acc[0] * inv, acc[1] * inv);
       w.y = E::pack2(acc[2] * inv, acc[3] * inv);
@@ -788,9 +1031,9 @@ __device__ __forceinline__ void extend_tile(const ExtendParams& p, const int32_t
 
 // One item a program. With counters the program that writes the last split of a tile joins it (and
 // sets the tile's counter, that of its first item, back to zero); else a second launch does.
-template <class C>
+template <class C, class P>
 __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void extend_rows_kernel(
-    ExtendParams p, const int32_t* __restrict__ table, const int32_t* __restrict__ lengths,
+    P p, const int32_t* __restrict__ table, const int32_t* __restrict__ lengths,
     const int32_t* __restrict__ cu) {
   constexpr int kBytes = CMax<C::NWK * kStages<C::DPAD> * C::STAGE_BYTES, C::COMB_BYTES>::value;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[kBytes];
@@ -799,8 +1042,9 @@ __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void extend_row
   const bool found = find_item<ShortTiling>(p, lengths, cu, (int)blockIdx.x, tid & 63, it);
   write_note(p, it, found);
   if (!found) return;
-  const bool fused = p.counters != nullptr;
+  const bool fused = p.counters != nullptr && !kIsPrefix<P>;
   extend_tile<C>(p, table, it, smem, tid, fused);
+  if constexpr (kIsPrefix<P>) return;
   if (it.splits == 1 || !fused) return;
   wait_vm<0>();     // this wave's partials are complete at the device
   __syncthreads();  // ... and every wave's
@@ -820,11 +1064,10 @@ __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void extend_row
 // programs of a tile's splits share its rows, kJoinParts of them (blockIdx.y) to a split of a long
 // tile: few programs, since one takes 5 ns to dispatch.
 constexpr int kJoinParts = 4;
-template <bool BF16>
-__global__ __launch_bounds__(kMergeThreads) void extend_join_kernel(ExtendParams rows, ExtendParams longs,
-                                                                    int rows_items) {
+template <bool BF16, class P>
+__global__ __launch_bounds__(kMergeThreads) void extend_join_kernel(P rows, P longs, int rows_items) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[kMergeThreads * 24];
-  auto join = [&](const ExtendParams& p, int w, int tile_rows, int per_split, bool whole) {
+  auto join = [&](const P& p, int w, int tile_rows, int per_split, bool whole) {
     const JoinNote note = reinterpret_cast<const JoinNote*>(p.notes)[w];
     if (note.splits < 2) return;
     Item it;
@@ -834,6 +1077,7 @@ __global__ __launch_bounds__(kMergeThreads) void extend_join_kernel(ExtendParams
     it.splits = note.splits;
     it.slot0 = w - note.split * p.heads;
     it.slot_step = p.heads;
+    it.group = note.group;
     const int parts = note.splits * per_split, part = note.split * per_split + (int)blockIdx.y;
     const int from = note.rows * part / parts, to = note.rows * (part + 1) / parts;
     if (from < to)
@@ -845,10 +1089,10 @@ __global__ __launch_bounds__(kMergeThreads) void extend_join_kernel(ExtendParams
     join(rows, (int)blockIdx.x, ShortTiling::ROWS, 1, true);
 }
 
-template <bool BF16, int DPAD>
-hipError_t launch_extend_rows(const ExtendParams& p, int grid, hipStream_t stream) {
+template <bool BF16, int DPAD, class P>
+hipError_t launch_extend_rows(const P& p, int grid, hipStream_t stream) {
   using C = Cfg<BF16, DPAD, kLayoutKey, DPAD == 128 ? 1 : 0>;
-  extend_rows_kernel<C><<<dim3(grid), dim3(C::THREADS), 0, stream>>>(p, p.table, p.lengths, p.cu);
+  extend_rows_kernel<C, P><<<dim3(grid), dim3(C::THREADS), 0, stream>>>(p, p.table, p.lengths, p.cu);
   return hipGetLastError();
 }
 

@@ -72,12 +72,38 @@ __device__ __forceinline__ void issue_keys(const ExtendParams& p, const int32_t*
 
 // The 32 rows from `first_row` of an item's tile that one wave holds in o, m, l: to the output, or to
 // the partials of a split tile, whole rows through the wave's LDS at `st` (32 kStagedRowBytes<C>).
-template <class C>
-__device__ __forceinline__ void store_wave_rows(const ExtendParams& p, const Item& it, int first_row,
-                                                unsigned char* st, int lane, const f32x16 (&o)[C::DT], float m,
+// Suffix pass, unsplit: with the prefix's partials of the row first, each lane those of its dims.
+template <class C, class P>
+__device__ __forceinline__ void store_wave_rows(const P& p, const Item& it, int first_row,
+                                                unsigned char* st, int lane, f32x16 (&o)[C::DT], float m,
                                                 float l) {
-  const float tot = pair_sum(l), inv = 1.0f / fmaxf(tot, 1.0e-30f);
-  const bool split = it.splits > 1;
+  float tot = pair_sum(l);
+  const bool split = it.splits > 1 || kIsPrefix<P>;
+  if constexpr (kIsSuffix<P>) {
+    const int ln = opaque_lane(lane), lr = ln & 31, lh = ln >> 5;
+    if (!split && it.group >= 0 && lr < it.rows - first_row) {
+      const PrefixRow x = prefix_row(p, group_note(p, it.group), it.first, it.head, it.tile * C::ROWS_TILE + first_row + lr);
+      for (int s = 0; s < x.splits; ++s) {
+        const int64_t at = (int64_t)(x.slot + s * x.step) * p.prefix_rows + x.row;
+        const float* const part = p.prefix_parts + at * p.dim;
+        const float y = p.prefix_lse[at] * 1.4426950408889634f, top = fmaxf(m, y);
+        const float a = __builtin_amdgcn_exp2f(m - top), b = __builtin_amdgcn_exp2f(y - top);
+        tot = tot * a + b;
+#pragma unroll
+        for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+          for (int gq = 0; gq < 4; ++gq) {
+            const int d0 = 32 * dt + 8 * gq + 4 * lh;
+            if (p.dim != C::DPAD && d0 >= p.dim) continue;
+            const f32x4 v = *reinterpret_cast<const f32x4*>(part + d0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[dt][4 * gq + i] = o[dt][4 * gq + i] * a + v[i] * b;
+          }
+        m = top;
+      }
+    }
+  }
+  const float inv = 1.0f / fmaxf(tot, 1.0e-30f);
   const int rows = it.rows - first_row;  // of this wave, where fewer than 32
   const int ln = opaque_lane(lane), lr = ln & 31, lh = ln >> 5;
   auto row_at = [&](int r) {
@@ -117,9 +143,9 @@ __device__ __forceinline__ void store_wave_rows(const ExtendParams& p, const Ite
   if (split && lh == 0 && lr < rows) p.lse[(int64_t)it.slot * C::ROWS_TILE + first_row + lr] = part_lse(m, tot);
 }
 
-template <class C>
+template <class C, class P>
 __global__ __attribute__((aligned(4096))) __launch_bounds__(C::THREADS) void extend_long_kernel(
-    ExtendParams p, const int32_t* __restrict__ table, const int32_t* __restrict__ lengths,
+    P p, const int32_t* __restrict__ table, const int32_t* __restrict__ lengths,
     const int32_t* __restrict__ cu) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[C::RING_BYTES];
   const u32 kring_lds = lds_address(smem);
@@ -312,10 +338,10 @@ __global__ __attribute__((aligned(4096))) __launch_bounds__(C::THREADS) void ext
   }
 }
 
-template <bool BF16, int DPAD, int ROWS>
-hipError_t launch_extend_long(const ExtendParams& p, int grid, hipStream_t stream) {
+template <bool BF16, int DPAD, int ROWS, class P>
+hipError_t launch_extend_long(const P& p, int grid, hipStream_t stream) {
   using C = PCfg<BF16, DPAD, ROWS>;
-  extend_long_kernel<C><<<dim3(grid), dim3(C::THREADS), 0, stream>>>(p, p.table, p.lengths, p.cu);
+  extend_long_kernel<C, P><<<dim3(grid), dim3(C::THREADS), 0, stream>>>(p, p.table, p.lengths, p.cu);
   return hipGetLastError();
 }
 

@@ -14,8 +14,8 @@
 
 namespace fgw_kv {
 
-template <class C>
-__global__ __launch_bounds__(C::THREADS) void extend_wide_kernel(ExtendParams p, const int32_t* __restrict__ table,
+template <class C, class P>
+__global__ __launch_bounds__(C::THREADS) void extend_wide_kernel(P p, const int32_t* __restrict__ table,
                                                                  const int32_t* __restrict__ lengths,
                                                                  const int32_t* __restrict__ cu) {
   static_assert(C::DUAL && C::NBUF == 2 && C::ROWS_TILE == WideTiling::ROWS && C::BLOCK == WideTiling::BN,
@@ -104,10 +104,10 @@ __global__ __launch_bounds__(C::THREADS) void extend_wide_kernel(ExtendParams p,
     store_wave_rows<C>(p, it, wq * C::ROWS_WAVE, smem + wq * 32 * kStagedRowBytes<C>, lane, o, m, l);
 }
 
-template <bool BF16>
-hipError_t launch_extend_wide(const ExtendParams& p, int grid, hipStream_t stream) {
+template <bool BF16, class P>
+hipError_t launch_extend_wide(const P& p, int grid, hipStream_t stream) {
   using C = Cfg<BF16, 256, kLayoutQuery, 0, kDual>;
-  extend_wide_kernel<C><<<dim3(grid), dim3(C::THREADS), 0, stream>>>(p, p.table, p.lengths, p.cu);
+  extend_wide_kernel<C, P><<<dim3(grid), dim3(C::THREADS), 0, stream>>>(p, p.table, p.lengths, p.cu);
   return hipGetLastError();
 }
 

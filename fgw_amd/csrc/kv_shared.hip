@@ -1,0 +1,152 @@
+// C ABI of the attention over pages where groups of requests share a prefix (fgw_kv_shared).
+//
+// With the keys of a row cut in two, its prefix's and its own, and o, lse of each part alone,
+//   w = exp(lse - max lse),  o = (w_prefix o_prefix + w_own o_own) / (w_prefix + w_own).
+// Two passes of the kernels of fgw_kv_extend, each of which finds its requests on the device:
+//   1. A group is one request: its rows are those of all its tokens (they lie side by side in q), its keys
+//      the prefix, read through the first request's row of the table, with nothing to mask. Every item
+//      leaves partials (O / l, LSE).
+//   2. Each request over the keys behind its prefix; an unsplit tile takes the prefix's partials at its
+//      end and writes the output, a split one's join takes them with its own.
+// A request that does not reach past the prefix with all its new tokens, or is alone in its group, reads
+// all its keys itself in the second pass.
+#include <hip/hip_runtime.h>
+
+#include "kv_extend_plan.h"
+
+namespace fgw_kv {
+
+#define FGW_KV_EXTERN(BF, P)                                                                       \
+  extern template hipError_t launch_extend_rows<BF, 32, P>(const P&, int, hipStream_t);            \
+  extern template hipError_t launch_extend_rows<BF, 64, P>(const P&, int, hipStream_t);            \
+  extern template hipError_t launch_extend_rows<BF, 128, P>(const P&, int, hipStream_t);           \
+  extern template hipError_t launch_extend_rows<BF, 256, P>(const P&, int, hipStream_t);           \
+  extern template hipError_t launch_extend_long<BF, 64, kRowsBlock, P>(const P&, int, hipStream_t);   \
+  extern template hipError_t launch_extend_long<BF, 64, kRowsGroup, P>(const P&, int, hipStream_t);   \
+  extern template hipError_t launch_extend_long<BF, 64, kRowsPadded, P>(const P&, int, hipStream_t);  \
+  extern template hipError_t launch_extend_long<BF, 128, kRowsBlock, P>(const P&, int, hipStream_t);  \
+  extern template hipError_t launch_extend_long<BF, 128, kRowsGroup, P>(const P&, int, hipStream_t);  \
+  extern template hipError_t launch_extend_long<BF, 128, kRowsPadded, P>(const P&, int, hipStream_t); \
+  extern template hipError_t launch_extend_wide<BF, P>(const P&, int, hipStream_t);
+FGW_KV_EXTERN(true, PrefixParams) FGW_KV_EXTERN(true, SuffixParams)
+FGW_KV_EXTERN(false, PrefixParams) FGW_KV_EXTERN(false, SuffixParams)
+
+namespace {
+
+struct SharedPlan {
+  Launch prefix;
+  int prefix_rows;  // of a place
+  bool longs;       // long tiles in the first pass
+  int64_t notes;    // floats of the groups' notes
+  Plan suffix;
+};
+
+template <class T>
+void plan_prefix(SharedPlan& s, const fgw_kv_extend_args& a, int64_t groups) {
+  Launch& l = s.prefix;
+  const int64_t total = (int64_t)a.tokens * (a.heads / a.kv_heads);
+  s.prefix_rows = T::ROWS;
+  l.many = 1 << 20;
+  l.tiles = total / T::ROWS + std::min<int64_t>(groups, a.tokens);
+  plan_items<T>(l, a, true);
+  l.slots = l.items;  // every item leaves partials
+  l.floats = l.slots * T::ROWS * (a.dim + 1);
+}
+
+// The kernel of the first pass: long tiles where a group has more than kLongFrom rows on average.
+SharedPlan plan_shared(const fgw_kv_shared_args& args) {
+  fgw_kv_extend_args a = args.attend;
+  SharedPlan s = {};
+  s.suffix = plan(a);
+  if (args.groups == 0) return s;
+  a.num_cus = std::min(a.num_cus, kMostCus);
+  s.longs = (int64_t)a.tokens * (a.heads / a.kv_heads) > (int64_t)kLongFrom * args.groups;
+  s.prefix.min_chunk = s.longs ? kLongMinChunk : kRowsMinChunk;
+  if (!s.longs)
+    plan_prefix<ShortTiling>(s, a, args.groups);
+  else if (a.dim > 128)
+    plan_prefix<WideTiling>(s, a, args.groups);
+  else
+    plan_prefix<LongTiling>(s, a, args.groups);
+  s.notes = (int64_t)args.groups * (int64_t)sizeof(GroupNote) / 4;
+  return s;
+}
+
+int check_shared(const fgw_kv_shared_args* args) {
+  if (!args) return fail(FGW_MHA_EINVAL, "arguments are missing");
+  if (int rc = check(&args->attend)) return rc;
+  if (!args->attend.causal || args->attend.window != 0)
+    return fail(FGW_MHA_EUNSUPPORTED, "attention with shared prefixes is causal and has no window");
+  if (args->groups < 0) return fail(FGW_MHA_EINVAL, "the number of groups must not be negative");
+  return FGW_MHA_OK;
+}
+
+template <bool BF16>
+int run_shared(const fgw_kv_shared_args& args, const SharedPlan& s, hipStream_t stream) {
+  const fgw_kv_extend_args& a = args.attend;
+  SuffixParams own = params_of<SuffixParams>(a);
+  float* work = a.workspace;
+  own.groups = args.cu_groups;
+  own.prefixes = args.prefix_lens;
+  own.n_groups = args.groups;
+  if (s.prefix.items > 0) {
+    PrefixParams p = params_of<PrefixParams>(a);
+    static_cast<SharedParams&>(p) = own;
+    p.causal = 0;
+    p.max_new = p.tokens;
+    p.target = s.prefix.target;
+    p.min_chunk = s.prefix.min_chunk;
+    p.whole = s.prefix.whole;
+    p.many = s.prefix.many;
+    p.work = (int)s.prefix.slots;
+    p.group_notes = reinterpret_cast<int32_t*>(work);
+    p.parts = work + s.notes;
+    p.lse = p.parts + s.prefix.slots * s.prefix_rows * a.dim;
+    own.group_notes = p.group_notes;
+    own.prefix_parts = p.parts;
+    own.prefix_lse = p.lse;
+    own.prefix_slots = p.work;
+    own.prefix_rows = s.prefix_rows;
+    work = p.parts + s.prefix.floats;
+    const auto entry = s.longs ? long_entry<BF16, PrefixParams>(a.dim, a.page_size) : rows_entry<BF16, PrefixParams>(a.dim);
+    const hipError_t e = entry(p, (int)s.prefix.items, stream);
+    if (e != hipSuccess) return fail(FGW_MHA_EHIP, "fgw_kv_shared: %s", hipGetErrorString(e));
+  }
+  own.parts = work;
+  own.counters = s.suffix.rows.counters > 0 ? a.counters : nullptr;
+  return run<BF16>(own, s.suffix, "fgw_kv_shared", stream);
+}
+
+}  // namespace
+
+}  // namespace fgw_kv
+
+using namespace fgw_kv;
+
+extern "C" {
+
+int fgw_kv_shared_workspace(const fgw_kv_shared_args* args, int64_t* floats, int64_t* counters) {
+  if (int rc = check_shared(args)) return rc;
+  *floats = *counters = 0;
+  if (args->attend.tokens == 0) return FGW_MHA_OK;
+  const SharedPlan s = plan_shared(*args);
+  *floats = s.notes + s.prefix.floats + s.suffix.rows.floats + s.suffix.longs.floats;
+  *counters = s.suffix.rows.counters;
+  return FGW_MHA_OK;
+}
+
+int fgw_kv_shared(const fgw_kv_shared_args* args, hipStream_t stream) {
+  if (int rc = check_shared(args)) return rc;
+  const fgw_kv_extend_args& a = args->attend;
+  if (a.tokens == 0) return FGW_MHA_OK;
+  if (int rc = check_tensors(a)) return rc;
+  if (args->groups > 0 && (!args->cu_groups || !args->prefix_lens)) return fail(FGW_MHA_EINVAL, "tensors are missing");
+  const SharedPlan s = plan_shared(*args);
+  if (std::max(s.prefix.items, std::max(s.suffix.rows.items, s.suffix.longs.items)) > 0x3fffffff)
+    return fail(FGW_MHA_EUNSUPPORTED, "too many rows for one call");
+  if (s.notes + s.prefix.floats + s.suffix.rows.floats + s.suffix.longs.floats > 0 && (!a.workspace || !aligned16(a.workspace)))
+    return fail(FGW_MHA_EINVAL, "the workspace is missing");
+  return a.dtype == FGW_KV_BFLOAT16 ? run_shared<true>(*args, s, stream) : run_shared<false>(*args, s, stream);
+}
+
+}  // extern "C"

@@ -37,6 +37,8 @@ struct Entries {
   decltype(&fgw_pages_free) free_rows;
   decltype(&fgw_pages_compact) compact;
   decltype(&fgw_pages_copy) copy;
+  decltype(&fgw_kv_shared_workspace) shared_workspace;
+  decltype(&fgw_kv_shared) shared;
 } entries = {};
 
 struct Refused : std::runtime_error {  // ValueError
@@ -399,67 +401,101 @@ int32_t* arrival_counters(const c10::Device& device, hipStream_t stream, int64_t
   return static_cast<int32_t*>(buffer.data_ptr());
 }
 
+// What the attention entries share: (max_new, page, heads, kv_heads, dim, bf16, device, causal, window,
+// scale, num_cus, out | None) and the checks of their tensors.
+struct Attention {
+  at::Tensor q, kc, vc, table, lens, cu, out;
+  c10::Device device{c10::kCPU};
+  fgw_kv_extend_args r = {};
+  explicit Attention(Args& a) : q(a.tensor()), kc(a.tensor()), vc(a.tensor()), table(a.tensor()), lens(a.tensor()), cu(a.tensor()) {}
+  void parse(Args& a) {
+    r.max_new = a.int32();
+    r.page_size = a.int32();
+    r.heads = a.int32();
+    r.kv_heads = a.int32();
+    r.dim = a.int32();
+    const bool bf16 = a.int32() != 0;
+    device = c10::Device(c10::kCUDA, (c10::DeviceIndex)a.int32());
+    r.causal = a.int32();
+    r.window = a.int32();
+    r.scale = (float)a.real();
+    r.num_cus = a.int32();
+    out = a.maybe();
+    r.q = rows(q, device);
+    need(q.size(1) == r.heads && q.size(2) == r.dim, "tensor shapes do not match the built kernel");
+    r.dtype = cache_dtype(q, kc, vc);
+    need((r.dtype == FGW_KV_BFLOAT16) == bf16, "matching FP16/BF16 Q/K/V required");
+    check_pool(kc, vc, r.dim, device);
+    need(kc.size(1) == r.kv_heads, "tensor shapes do not match the built kernel");
+    need(table.dim() == 2 && table.size(0) > 0 && table.size(1) > 0,
+         "positive Q extents and rank-2 table required");
+    const int64_t batch = table.size(0);
+    r.block_table = metadata(table, {batch, -1}, device);
+    r.cache_seqlens = metadata(lens, {batch}, device);
+    r.cu_seqlens = metadata(cu, {batch + 1}, device);
+    r.k_cache = kc.data_ptr();
+    r.v_cache = vc.data_ptr();
+    r.pool_rows = kc.size(0);
+    r.tokens = size32(q.size(0));
+    r.batch = size32(batch);
+    r.width = size32(table.size(1));
+    need(r.max_new > 0, "max_new must be positive");
+  }
+  // The output, the workspace (whose tensor the caller holds) and the counters; on the device's guard.
+  at::Tensor place(fgw_kv_extend_args& to, int64_t floats, int64_t counters, Tensors more) {
+    writable({&out});
+    if (out.defined()) {
+      need(same_sizes(out, q) && out.scalar_type() == q.scalar_type(), "out does not match the rows");
+      on(out, device);
+      need(out.is_contiguous(), kSameGpu);
+      need(!shares_memory(out, q), "out must not be q or share memory with it");
+      const char* const message = "out must not share memory with what the call reads";
+      apart({&out}, {&kc, &vc, &table, &lens, &cu}, message);
+      apart({&out}, more, message);
+    }
+    at::Tensor result = out.defined() ? out : at::empty(q.sizes(), q.options());
+    to.out = result.data_ptr();
+    if (floats > 0) {
+      work = at::empty({floats}, q.options().dtype(at::kFloat));
+      to.workspace = static_cast<float*>(work.data_ptr());
+    }
+    if (counters > 0) to.counters = arrival_counters(device, stream_of(device), counters);
+    return result;
+  }
+  at::Tensor work;
+};
+
 // (q, k_cache, v_cache, table, lens, cu, max_new, page, heads, kv_heads, dim, bf16, device, causal,
 //  window, scale, num_cus, out | None) -> out
 PyObject* extend(Args& a) {
-  const at::Tensor q = a.tensor(), kc = a.tensor(), vc = a.tensor();
-  const at::Tensor table = a.tensor(), lens = a.tensor(), cu = a.tensor();
-  fgw_kv_extend_args r = {};
-  r.max_new = a.int32();
-  r.page_size = a.int32();
-  r.heads = a.int32();
-  r.kv_heads = a.int32();
-  r.dim = a.int32();
-  const bool bf16 = a.int32() != 0;
-  const c10::Device device(c10::kCUDA, (c10::DeviceIndex)a.int32());
-  r.causal = a.int32();
-  r.window = a.int32();
-  r.scale = (float)a.real();
-  r.num_cus = a.int32();
-  at::Tensor out = a.maybe();
-  r.q = rows(q, device);
-  need(q.size(1) == r.heads && q.size(2) == r.dim, "tensor shapes do not match the built kernel");
-  r.dtype = cache_dtype(q, kc, vc);
-  need((r.dtype == FGW_KV_BFLOAT16) == bf16, "matching FP16/BF16 Q/K/V required");
-  check_pool(kc, vc, r.dim, device);
-  need(kc.size(1) == r.kv_heads, "tensor shapes do not match the built kernel");
-  need(table.dim() == 2 && table.size(0) > 0 && table.size(1) > 0,
-       "positive Q extents and rank-2 table required");
-  const int64_t batch = table.size(0);
-  r.block_table = metadata(table, {batch, -1}, device);
-  r.cache_seqlens = metadata(lens, {batch}, device);
-  r.cu_seqlens = metadata(cu, {batch + 1}, device);
-  r.k_cache = kc.data_ptr();
-  r.v_cache = vc.data_ptr();
-  r.pool_rows = kc.size(0);
-  r.tokens = size32(q.size(0));
-  r.batch = size32(batch);
-  r.width = size32(table.size(1));
-  need(r.max_new > 0, "max_new must be positive");
+  Attention x(a);
+  x.parse(a);
   int64_t floats = 0, counters = 0;
-  check(entries.extend_workspace(&r, &floats, &counters));
-  const c10::DeviceGuard guard(device);
-  const at::Tensor given = out;
-  writable({&given});
-  if (out.defined()) {
-    need(same_sizes(out, q) && out.scalar_type() == q.scalar_type(), "out does not match the rows");
-    on(out, device);
-    need(out.is_contiguous(), kSameGpu);
-    need(!shares_memory(out, q), "out must not be q or share memory with it");
-    apart({&out}, {&kc, &vc, &table, &lens, &cu}, "out must not share memory with what the call reads");
-  } else {
-    out = at::empty(q.sizes(), q.options());
-  }
-  r.out = out.data_ptr();
-  at::Tensor work;
-  if (floats > 0) {
-    work = at::empty({floats}, q.options().dtype(at::kFloat));
-    r.workspace = static_cast<float*>(work.data_ptr());
-  }
-  const hipStream_t stream = stream_of(device);
-  if (counters > 0) r.counters = arrival_counters(device, stream, counters);
-  check(entries.extend(&r, stream));
-  changed({&given});
+  check(entries.extend_workspace(&x.r, &floats, &counters));
+  const c10::DeviceGuard guard(x.device);
+  at::Tensor out = x.place(x.r, floats, counters, {});
+  check(entries.extend(&x.r, stream_of(x.device)));
+  changed({&x.out});
+  return THPVariable_Wrap(std::move(out));
+}
+
+// (q, k_cache, v_cache, table, lens, cu, cu_groups, prefix_lens, max_new, ... as extend) -> out
+PyObject* shared(Args& a) {
+  Attention x(a);
+  const at::Tensor groups = a.tensor(), prefixes = a.tensor();
+  x.parse(a);
+  fgw_kv_shared_args r = {};
+  r.cu_groups = metadata(groups, {-1}, x.device);
+  need(groups.size(0) > 0, "metadata shape mismatch");
+  r.groups = size32(groups.size(0) - 1);
+  r.prefix_lens = metadata(prefixes, {r.groups}, x.device);
+  r.attend = x.r;
+  int64_t floats = 0, counters = 0;
+  check(entries.shared_workspace(&r, &floats, &counters));
+  const c10::DeviceGuard guard(x.device);
+  at::Tensor out = x.place(r.attend, floats, counters, {&groups, &prefixes});
+  check(entries.shared(&r, stream_of(x.device)));
+  changed({&x.out});
   return THPVariable_Wrap(std::move(out));
 }
 
@@ -643,6 +679,7 @@ PyMethodDef methods[] = {
     {"rotate", FGW_FAST(rotate), METH_FASTCALL, "fgw_rotary_apply"},
     {"append", FGW_FAST(append), METH_FASTCALL, "fgw_kv_append"},
     {"extend", FGW_FAST(extend), METH_FASTCALL, "fgw_kv_extend"},
+    {"shared", FGW_FAST(shared), METH_FASTCALL, "fgw_kv_shared"},
     {"reserve", FGW_FAST(reserve), METH_FASTCALL, "fgw_pages_reserve"},
     {"fork", FGW_FAST(fork_rows), METH_FASTCALL, "fgw_pages_fork"},
     {"free", FGW_FAST(free_rows), METH_FASTCALL, "fgw_pages_free"},

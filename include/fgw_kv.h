@@ -5,6 +5,7 @@
  *   fgw_rotary_apply   rotary positions of [T, H, D] rows (and their inverse)
  *   fgw_kv_append      new tokens into the pages, Q and K rotated on the way
  *   fgw_kv_extend      attention of packed ragged new tokens over the pages, grouped K/V heads
+ *   fgw_kv_shared      the same where groups of requests share a prefix, which is read once for a group
  *   fgw_pages_*        fork, free, reserve, compact and copy pages; books on the device
  * None has a counterpart in the reference, which reads a cache that its caller has written.
  *
@@ -122,6 +123,21 @@ typedef struct {
  * not read; 0 counters: none of its joins is fused); pure host function. */
 int fgw_kv_extend_workspace(const fgw_kv_extend_args* args, int64_t* floats, int64_t* counters);
 int fgw_kv_extend(const fgw_kv_extend_args* args, hipStream_t stream);
+
+/* The same, causal and without a window, where group g, the requests [cu_groups[g], cu_groups[g + 1]) (from
+ * 0, never falling; later requests are in no group), shares its first prefix_lens[g] keys: they are read
+ * through the table row of its first request f, once for the group, and are as many as f has before its
+ * new tokens (len_f - n_f) at most. Each request's own row holds the same keys (or is not read there):
+ * one whose new tokens begin within the prefix, or that is alone in its group, reads its own. */
+typedef struct {
+  fgw_kv_extend_args attend;  /* workspace and counters: those of fgw_kv_shared_workspace */
+  const int32_t* cu_groups;   /* [groups + 1], device */
+  const int32_t* prefix_lens; /* [groups], device */
+  int32_t groups;             /* 0: nothing is shared */
+} fgw_kv_shared_args;
+
+int fgw_kv_shared_workspace(const fgw_kv_shared_args* args, int64_t* floats, int64_t* counters);
+int fgw_kv_shared(const fgw_kv_shared_args* args, hipStream_t stream);
 
 /* Books of the pages, on the device: refs [pages] int32 holders of each page (0: free), table
  * [rows, width] int32, lens [rows] int32. Row r holds the pages table[r, 0 .. ceil(lens[r] /
