@@ -63,6 +63,8 @@ template <class P>
 constexpr bool kIsPrefix = std::is_same<P, PrefixParams>::value;
 template <class P>
 constexpr bool kIsSuffix = std::is_same<P, SuffixParams>::value;
+template <class P>
+constexpr bool kPicksFrom = kIsSuffix<P>;  // items with Request::from
 
 // Where a group's partials are: those of its first item (a place for each K/V head), the splits of its
 // tiles, how many tiles, and the group's first token. Written by the first pass.
@@ -83,6 +85,7 @@ struct Request {
   int first, n, len, tiles, units;
   int row;          // prefix pass: of the block table
   int from, group;  // suffix pass: keys [0, from) are in the prefix of `group` (-1: none shared)
+                    // (attention weight, kv_weights.h: keys [0, from) were there before the new tokens)
 };
 
 template <class P>
@@ -252,16 +255,18 @@ struct Item {
   int blk_begin, blk_end;
   int slot, slot0, slot_step;  // partials: of this split, of the first one; between splits
   int from, group;             // suffix pass: as Request's
-  int place, tiles;            // prefix pass: among the request's items of a head, its tiles
+  int place, place_splits, tiles;  // among the request's items of a head; splits of its tiles at most, tiles
 };
 
 // Item w of the launch; false where there is none. Uniform over the wave; every wave of a workgroup
 // computes the same.
 template <class T, class P>
 __device__ __forceinline__ bool find_item(const P& p, const int32_t* lengths,
-                                          const int32_t* cu, int w, int lane, Item& it) {
+                                          const int32_t* cu, int w, int lane, Item& it,
+                                          int* used_chunk = nullptr) {
   const Request r0 = load_request<T>(p, lengths, cu, lane);
   const int chunk = p.target > 0 ? best_chunk<T>(p, lengths, cu, r0, lane) : kWhole;
+  if (used_chunk) *used_chunk = chunk;
   const int g = (int)((u32)w / (u32)p.heads);
   it.head = w - g * p.heads;
   int items_before = 0;
@@ -277,9 +282,10 @@ __device__ __forceinline__ bool find_item(const P& p, const int32_t* lengths,
       auto pick = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
       const int s = pick(splits), place = pick(at), tiles = pick(r.tiles);
       it.b = kIsPrefix<P> ? pick(r.row) : b0 + l;
-      it.from = kIsSuffix<P> ? pick(r.from) : 0;
+      it.from = kPicksFrom<P> ? pick(r.from) : 0;
       it.group = kIsSuffix<P> ? pick(r.group) : kIsPrefix<P> ? b0 + l : -1;
       it.place = place;
+      it.place_splits = s;
       it.tiles = tiles;
       it.first = pick(r.first);
       it.n = pick(r.n);

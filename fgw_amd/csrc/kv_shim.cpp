@@ -39,6 +39,8 @@ struct Entries {
   decltype(&fgw_pages_copy) copy;
   decltype(&fgw_kv_shared_workspace) shared_workspace;
   decltype(&fgw_kv_shared) shared;
+  decltype(&fgw_kv_weights_workspace) weights_workspace;
+  decltype(&fgw_kv_weights) weights;
 } entries = {};
 
 struct Refused : std::runtime_error {  // ValueError
@@ -499,6 +501,55 @@ PyObject* shared(Args& a) {
   return THPVariable_Wrap(std::move(out));
 }
 
+// (scores, q, k_cache, table, lens, cu, page, last, scale, decay, num_cus)
+PyObject* weights(Args& a) {
+  const at::Tensor scores = a.tensor(), q = a.tensor(), kc = a.tensor(), table = a.tensor(), lens = a.tensor(), cu = a.tensor();
+  const c10::Device device = q.device();
+  need(device.is_cuda(), kSameGpu);
+  fgw_kv_weights_args r = {};
+  r.page_size = a.int32();
+  r.last = a.int32();
+  r.scale = (float)a.real();
+  r.decay = (float)a.real();
+  r.num_cus = a.int32();
+  r.q = rows(q, device);
+  r.dtype = cache_dtype(q, kc, kc);
+  check_pool(kc, kc, q.size(2), device);
+  need(table.dim() == 2 && table.size(0) > 0 && table.size(1) > 0,
+       "positive Q extents and rank-2 table required");
+  const int64_t batch = table.size(0);
+  r.block_table = metadata(table, {batch, -1}, device);
+  r.cache_seqlens = metadata(lens, {batch}, device);
+  r.cu_seqlens = metadata(cu, {batch + 1}, device);
+  need(scores.scalar_type() == at::kFloat && scores.dim() == 3 && scores.size(0) == batch && scores.size(1) == kc.size(1),
+       "expected FP32 scores [B, Hkv, S]");
+  on(scores, device);
+  need(scores.is_contiguous(), kSameGpu);
+  r.scores = static_cast<float*>(scores.data_ptr());
+  r.scores_stride = scores.size(2);
+  r.k_cache = kc.data_ptr();
+  r.pool_rows = kc.size(0);
+  r.tokens = size32(q.size(0));
+  r.batch = size32(batch);
+  r.heads = size32(q.size(1));
+  r.kv_heads = size32(kc.size(1));
+  r.dim = size32(q.size(2));
+  r.width = size32(table.size(1));
+  const int64_t floats = entries.weights_workspace(&r);
+  if (floats < 0) check((int)floats);
+  const c10::DeviceGuard guard(device);
+  writable({&scores});
+  apart({&scores}, {&q, &kc, &table, &lens, &cu}, "the scores must not share memory with what the call reads");
+  at::Tensor work;
+  if (floats > 0) {
+    work = at::empty({floats}, scores.options());
+    r.workspace = static_cast<float*>(work.data_ptr());
+  }
+  check(entries.weights(&r, stream_of(device)));
+  changed({&scores});
+  Py_RETURN_NONE;
+}
+
 // refs, table, lens, page_size of a call, and the lists that it reads while the books change.
 fgw_pages_books books_of(const at::Tensor& refs, const at::Tensor& table, const at::Tensor& lens,
                          int32_t page, Tensors lists) {
@@ -680,6 +731,7 @@ PyMethodDef methods[] = {
     {"append", FGW_FAST(append), METH_FASTCALL, "fgw_kv_append"},
     {"extend", FGW_FAST(extend), METH_FASTCALL, "fgw_kv_extend"},
     {"shared", FGW_FAST(shared), METH_FASTCALL, "fgw_kv_shared"},
+    {"weights", FGW_FAST(weights), METH_FASTCALL, "fgw_kv_weights"},
     {"reserve", FGW_FAST(reserve), METH_FASTCALL, "fgw_pages_reserve"},
     {"fork", FGW_FAST(fork_rows), METH_FASTCALL, "fgw_pages_fork"},
     {"free", FGW_FAST(free_rows), METH_FASTCALL, "fgw_pages_free"},

@@ -1,0 +1,162 @@
+// C ABI of the attention weight of cached keys (fgw_kv_weights): checks, sizes and dispatch. The kernels
+// stand in kv_weights.h, their instantiations in the kv_weights_*.hip files of each type.
+#include <hip/hip_runtime.h>
+
+#include "kv_extend_plan.h"
+#include "kv_weights.h"
+
+namespace fgw_kv {
+
+#define FGW_KV_EXTERN_WEIGHTS(BF, DP) \
+  extern template hipError_t launch_weights<BF, DP>(const WeightParams&, bool, int, int, hipStream_t);
+FGW_KV_EXTERN_WEIGHTS(true, 64) FGW_KV_EXTERN_WEIGHTS(true, 128) FGW_KV_EXTERN_WEIGHTS(true, 256)
+FGW_KV_EXTERN_WEIGHTS(false, 64) FGW_KV_EXTERN_WEIGHTS(false, 128) FGW_KV_EXTERN_WEIGHTS(false, 256)
+
+namespace {
+
+struct WeightPlan {
+  bool many;       // rows of a request and K/V head, at most, past kKeptRows
+  Launch launch;   // of the first pass
+  int columns, sums;  // grids of the persistent kernels; 0: no launch
+  int64_t keys_pad, kept_rows, parts;
+  int64_t kept, lse, notes, floats;  // of workspace
+};
+
+// Workgroups of a persistent kernel: as many as the card holds, or as there are items.
+int persistent(int64_t items, int num_cus, int each) { return (int)std::min<int64_t>(items, (int64_t)num_cus * each); }
+
+// The extents that plan_items reads.
+fgw_kv_extend_args extents(const fgw_kv_weights_args& a) {
+  fgw_kv_extend_args e = {};
+  e.tokens = a.tokens;
+  e.batch = a.batch;
+  e.heads = a.heads;
+  e.kv_heads = a.kv_heads;
+  e.dim = a.dim;
+  e.width = a.width;
+  e.page_size = a.page_size;
+  e.pool_rows = a.pool_rows;
+  e.max_new = a.last;
+  e.causal = 1;
+  e.dtype = a.dtype;
+  e.num_cus = std::min(a.num_cus, kMostCus);
+  e.scale = a.scale;
+  e.q = a.q;
+  e.k_cache = a.k_cache;
+  e.block_table = a.block_table;
+  e.cache_seqlens = a.cache_seqlens;
+  e.cu_seqlens = a.cu_seqlens;
+  return e;
+}
+
+WeightPlan plan_weights(const fgw_kv_weights_args& a) {
+  const fgw_kv_extend_args e = extents(a);
+  WeightPlan p = {};
+  const int64_t group = a.heads / a.kv_heads, total = a.tokens * group, capacity = (int64_t)a.width * a.page_size;
+  const int64_t rows = std::min(a.last, a.tokens) * group, requests = std::min(a.batch, a.tokens);
+  auto blocks = [&](int64_t size) { return std::min(requests * ((rows + size - 1) / size), total / size + requests); };
+  p.keys_pad = (capacity + kColumnKeys - 1) / kColumnKeys * kColumnKeys;
+  p.many = rows > kKeptRows;
+  if (!p.many) {
+    p.launch.min_chunk = kRowsMinChunk;
+    p.launch.whole = a.dim <= 64 ? kRowsWholeNarrow : kRowsWhole;
+    p.launch.many = rows <= 8 ? kRowsMany : kRowsManyTall;
+    p.launch.tiles = requests;
+    plan_items<ShortTiling>(p.launch, e, true);
+    p.kept_rows = rows;
+    p.kept = (int64_t)a.batch * a.kv_heads * rows * p.keys_pad;
+    p.lse = p.launch.slots * kKeptRows;
+  } else {
+    p.launch.min_chunk = kLongMinChunk;
+    p.launch.many = 1 << 20;
+    p.launch.tiles = blocks(StatsTiling::ROWS);
+    plan_items<StatsTiling>(p.launch, e, true);
+    p.launch.slots = p.launch.items;  // every item leaves statistics
+    p.lse = p.launch.slots * StatsTiling::ROWS;
+    p.notes = (int64_t)a.batch * (int64_t)sizeof(WeightNote) / 4;
+    const int64_t parts = blocks(kColumnRows), keys = p.keys_pad / kColumnKeys;
+    p.columns = persistent(parts * keys * a.kv_heads, e.num_cus, 3);
+    if (rows > kColumnRows) {
+      p.parts = parts;
+      p.kept = parts * a.kv_heads * p.keys_pad;
+      p.sums = persistent(requests * ((p.keys_pad + kSumKeys - 1) / kSumKeys) * a.kv_heads, e.num_cus, 4);
+    }
+  }
+  p.floats = p.kept + (p.lse + 3) / 4 * 4 + p.notes;
+  return p;
+}
+
+int check_weights(const fgw_kv_weights_args* args) {
+  if (!args) return fail(FGW_MHA_EINVAL, "arguments are missing");
+  if (args->last <= 0) return fail(FGW_MHA_EINVAL, "the number of tokens that count must be positive");
+  const fgw_kv_extend_args e = extents(*args);
+  if (int rc = check(&e)) return rc;
+  if (!(args->decay >= 0.0f) || args->decay > 3.0e38f)
+    return fail(FGW_MHA_EINVAL, "the decay must be finite and not negative");
+  if (args->scores_stride < (int64_t)args->width * args->page_size)
+    return fail(FGW_MHA_EINVAL, "the scores must have a place for every key of the table");
+  const int64_t rows = (int64_t)args->tokens * (args->heads / args->kv_heads);
+  const int64_t keys = (int64_t)args->width * args->page_size / kColumnKeys + 1;
+  if ((rows / kColumnRows + args->batch) * keys > 0x3fffffff)
+    return fail(FGW_MHA_EUNSUPPORTED, "too many rows for one call");
+  return FGW_MHA_OK;
+}
+
+template <bool BF16>
+hipError_t launch(const WeightParams& w, const WeightPlan& p, hipStream_t stream) {
+  return w.dim <= 64    ? launch_weights<BF16, 64>(w, p.many, (int)p.launch.items, p.columns, stream)
+         : w.dim <= 128 ? launch_weights<BF16, 128>(w, p.many, (int)p.launch.items, p.columns, stream)
+                        : launch_weights<BF16, 256>(w, p.many, (int)p.launch.items, p.columns, stream);
+}
+
+}  // namespace
+
+}  // namespace fgw_kv
+
+using namespace fgw_kv;
+
+extern "C" {
+
+int64_t fgw_kv_weights_workspace(const fgw_kv_weights_args* args) {
+  if (int rc = check_weights(args)) return rc;
+  return args->tokens == 0 ? 0 : plan_weights(*args).floats;
+}
+
+int fgw_kv_weights(const fgw_kv_weights_args* args, hipStream_t stream) {
+  if (int rc = check_weights(args)) return rc;
+  const fgw_kv_weights_args& a = *args;
+  if (a.tokens == 0) return FGW_MHA_OK;
+  if (!a.q.data || !a.scores || !a.k_cache || !a.block_table || !a.cache_seqlens || !a.cu_seqlens)
+    return fail(FGW_MHA_EINVAL, "tensors are missing");
+  if (!aligned16(a.q.data) || !aligned16(a.k_cache) || a.q.token_stride % 8 || a.q.head_stride % 8)
+    return fail(FGW_MHA_EINVAL, "rows must be 16-byte aligned, their strides multiples of 16 bytes");
+  const WeightPlan p = plan_weights(a);
+  if (p.launch.items > 0x3fffffff) return fail(FGW_MHA_EUNSUPPORTED, "too many rows for one call");
+  if (p.floats > 0 && (!a.workspace || !aligned16(a.workspace))) return fail(FGW_MHA_EINVAL, "the workspace is missing");
+  WeightParams w = params_of<WeightParams>(extents(a));
+  w.max_new = w.tokens;
+  w.scores = a.scores;
+  w.stride = a.scores_stride;
+  w.last = a.last;
+  w.decay = a.decay;
+  w.keys_pad = (int32_t)p.keys_pad;
+  w.kept_rows = (int32_t)p.kept_rows;
+  w.parts_most = (int32_t)p.parts;
+  w.target = p.launch.target;
+  w.min_chunk = p.launch.min_chunk;
+  w.whole = p.launch.whole;
+  w.many = p.launch.many;
+  w.work = (int32_t)p.launch.slots;
+  w.kept = w.sums = a.workspace;
+  w.lse = a.workspace + p.kept;
+  w.request_notes = reinterpret_cast<int32_t*>(w.lse + (p.lse + 3) / 4 * 4);
+  const hipError_t e = a.dtype == FGW_KV_BFLOAT16 ? launch<true>(w, p, stream) : launch<false>(w, p, stream);
+  if (e != hipSuccess) return fail(FGW_MHA_EHIP, "fgw_kv_weights: %s", hipGetErrorString(e));
+  if (!p.many && p.launch.target > 0)
+    weights_finish_kernel<<<dim3((unsigned)p.launch.items), dim3(kFinishThreads), 0, stream>>>(w, w.lengths, w.cu);
+  if (p.sums > 0)
+    weights_sum_kernel<<<dim3((unsigned)p.sums), dim3(kFinishThreads), 0, stream>>>(w, w.lengths, w.cu);
+  return launched("fgw_kv_weights");
+}
+
+}  // extern "C"

@@ -1,0 +1,47 @@
+"""Attention weight of cached keys, and rows shortened to those that carry the most of it (no reference
+counterpart: the reference's operator reads a cache that its caller keeps).
+
+A decoder that bounds its cache keeps, for each layer, FP32 sums scores [rows, Hkv, S] (S at least
+W * page_size): how much attention weight every cached key got, entry j of a row for its cache position
+j. add_weights adds that of a step's new tokens; evict_rows drops the keys with the least of it.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from fgw_amd import _lib
+from fgw_amd.operators.mha.kernels.mha_paged_decode_hip import _device_info
+
+_kv = _lib.load_kv_module()
+
+
+def add_weights(scores, q, k_cache, block_table, cache_seqlens, cu_seqlens, page_size, last, *, decay=1.0,
+                softmax_scale=None):
+    """Add the attention weight that cached keys get from new tokens to scores, in place.
+
+    q, the pool, table and metadata are those of build_extend_kernel's callable (causal, no window), the
+    new tokens' keys written already. For request b with n new tokens, K/V head h and key j < len,
+
+      scores[b, h, j] = (decay * scores[b, h, j] if j < len - n else 0) + sum of softmax(scale q k^T)_j
+
+    over the query heads of h and the last `last` of the new tokens (all, where they are fewer): 1 in a
+    decode step, the prompt's length for all of a prompt, some tens for what its end looks back at. The
+    keys of new tokens thus begin at zero without being cleared; decay 0 forgets all that was there.
+    Requests without new tokens, and entries from len on, are left. Lengths and page ids out of range are
+    taken as there; rows that see no key add nothing; a NaN in a query or in a key that it sees gives NaN
+    to all keys that it sees. Sums are fp32, in the same order on every run. Nothing is read back: the call
+    can be captured into a HIP graph. Records no gradient, and scores may require none.
+    """
+    if last < 1:
+        raise ValueError("the number of tokens that count must be positive")
+    if not (decay >= 0 and math.isfinite(decay)):
+        raise ValueError("the decay must be finite and not negative")
+    scale = q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError("the scale of the scores must be positive and finite")
+    if q.device.type != "cuda":
+        raise ValueError("contiguous inputs on the same GPU required")
+    _kv.weights(scores, q, k_cache, block_table, cache_seqlens, cu_seqlens, page_size, min(last, 2**31 - 1), scale,
+                decay, _device_info(q.device.index).num_cus)

@@ -6,6 +6,7 @@
  *   fgw_kv_append      new tokens into the pages, Q and K rotated on the way
  *   fgw_kv_extend      attention of packed ragged new tokens over the pages, grouped K/V heads
  *   fgw_kv_shared      the same where groups of requests share a prefix, which is read once for a group
+ *   fgw_kv_weights     the attention weight that cached keys get from new tokens, added to running sums
  *   fgw_pages_*        fork, free, reserve, compact and copy pages; books on the device
  * None has a counterpart in the reference, which reads a cache that its caller has written.
  *
@@ -138,6 +139,32 @@ typedef struct {
 
 int fgw_kv_shared_workspace(const fgw_kv_shared_args* args, int64_t* floats, int64_t* counters);
 int fgw_kv_shared(const fgw_kv_shared_args* args, hipStream_t stream);
+
+/* Attention weight of cached keys: for request b, K/V head h and key j < len_b,
+ *   scores[b, h, j] = (j < len_b - n_b ? decay * scores[b, h, j] : 0) + sum of softmax(scale q k^T)_j
+ * over the query heads of h and the last min(n_b, last) new tokens of b, each of which sees the keys up to
+ * its own position. Requests without new tokens, and entries at and behind len_b, are left as they are.
+ * decay 0 forgets what was there, whatever it is. Sums are taken in the same order on every run. */
+typedef struct {
+  fgw_kv_rows q;
+  float* scores;         /* [batch, kv_heads, scores_stride] */
+  int64_t scores_stride; /* at least width * page_size */
+  const void* k_cache;
+  const int32_t* block_table;
+  const int32_t* cache_seqlens;
+  const int32_t* cu_seqlens;
+  float* workspace;      /* the floats of fgw_kv_weights_workspace, or NULL if that is 0 */
+  int64_t pool_rows;
+  int32_t tokens, batch, heads, kv_heads, dim, width, page_size;
+  int32_t last;
+  int32_t dtype;         /* FGW_KV_FLOAT16 or FGW_KV_BFLOAT16 */
+  int32_t num_cus;
+  float scale, decay;
+} fgw_kv_weights_args;
+
+/* fp32 elements of workspace (pointers are not read), or a negative status. */
+int64_t fgw_kv_weights_workspace(const fgw_kv_weights_args* args);
+int fgw_kv_weights(const fgw_kv_weights_args* args, hipStream_t stream);
 
 /* Books of the pages, on the device: refs [pages] int32 holders of each page (0: free), table
  * [rows, width] int32, lens [rows] int32. Row r holds the pages table[r, 0 .. ceil(lens[r] /
