@@ -106,7 +106,8 @@ KV_ABI_VERSION = 1
 KV_ENTRIES = ("fgw_kv_last_error", "fgw_rotary_apply", "fgw_kv_append", "fgw_kv_extend_workspace",
               "fgw_kv_extend", "fgw_pages_workspace", "fgw_pages_reserve", "fgw_pages_fork",
               "fgw_pages_free", "fgw_pages_compact", "fgw_pages_copy", "fgw_kv_shared_workspace",
-              "fgw_kv_shared", "fgw_kv_weights_workspace", "fgw_kv_weights")
+              "fgw_kv_shared", "fgw_kv_weights_workspace", "fgw_kv_weights",
+              "fgw_pages_evict_workspace", "fgw_pages_evict")
 
 _lock = threading.Lock()
 _lib = None

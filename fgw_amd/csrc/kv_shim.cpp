@@ -41,6 +41,8 @@ struct Entries {
   decltype(&fgw_kv_shared) shared;
   decltype(&fgw_kv_weights_workspace) weights_workspace;
   decltype(&fgw_kv_weights) weights;
+  decltype(&fgw_pages_evict_workspace) evict_workspace;
+  decltype(&fgw_pages_evict) evict;
 } entries = {};
 
 struct Refused : std::runtime_error {  // ValueError
@@ -653,6 +655,75 @@ PyObject* fork_rows(Args& a) {
   return THPVariable_Wrap(std::move(status));
 }
 
+// (k_pools, v_pools, scores, refs, table, lens, keep, page, first, recent) -> status
+PyObject* evict(Args& a) {
+  PyObject *k_list = a.next(), *v_list = a.next(), *score_list = a.next();
+  const at::Tensor refs = a.tensor(), table = a.tensor(), lens = a.tensor(), keep = a.tensor();
+  const fgw_pages_books b = books_of(refs, table, lens, a.int32(), {&keep});
+  const c10::Device device = refs.device();
+  fgw_evict_args r = {};
+  r.first = a.int32();
+  r.recent = a.int32();
+  const Tensors books = {&refs, &table, &lens, &keep};
+  r.keep = metadata(keep, {b.rows}, device);
+  const PoolList k = pools_of(k_list, b.pages, b.page_size, device, books);
+  const PoolList v = pools_of(v_list, b.pages, b.page_size, device, books);
+  if (!PyTuple_Check(score_list) && !PyList_Check(score_list)) throw WrongType("scores must be a list or a tuple of tensors");
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(score_list);
+  need(n > 0 && k.tensors.size() == (size_t)n && v.tensors.size() == (size_t)n, "as many K pools, V pools and scores, at least one of each, required");
+  std::vector<at::Tensor> scores;
+  std::vector<float*> score_data;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* item = PySequence_Fast_GET_ITEM(score_list, i);
+    if (!THPVariable_Check(item)) throw WrongType("scores must be a list or a tuple of tensors");
+    const at::Tensor& x = THPVariable_Unpack(item);
+    writable({&x});
+    need(x.scalar_type() == at::kFloat && x.dim() == 3 && x.size(0) == b.rows && x.size(1) > 0, "expected FP32 scores [rows, Hkv, S]");
+    if (i == 0) {
+      r.heads = size32(x.size(1));
+      r.scores_stride = x.size(2);
+    }
+    need(x.size(1) == r.heads && x.size(2) == r.scores_stride, "the scores of all layers must have the same shape");
+    on(x, device);
+    need(x.is_contiguous(), kSameGpu);
+    apart({&x}, books, "scores must not share memory with the books or lists of the call");
+    scores.push_back(x);
+    score_data.push_back(static_cast<float*>(x.data_ptr()));
+  }
+  std::vector<int64_t> k_bytes, v_bytes;
+  auto heads_of = [&](const PoolList& list, std::vector<int64_t>& bytes) {
+    for (const at::Tensor& x : list.tensors) {
+      need(x.dim() >= 2 && x.size(1) == r.heads, "pools must be [pages * page_size, Hkv, ...] with the heads of the scores");
+      bytes.push_back(x.numel() / x.size(0) / r.heads * (int64_t)x.element_size());
+    }
+  };
+  heads_of(k, k_bytes);
+  heads_of(v, v_bytes);
+  // Every pool and every layer's scores are written on their own: none twice, none within another.
+  std::vector<std::pair<const char*, int64_t>> spans;
+  for (const std::vector<at::Tensor>* list : {&k.tensors, &v.tensors, (const std::vector<at::Tensor>*)&scores})
+    for (const at::Tensor& x : *list) spans.emplace_back(static_cast<const char*>(x.data_ptr()), (int64_t)x.nbytes());
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    need(spans[i - 1].first + spans[i - 1].second <= spans[i].first, "pools and scores must not share memory with each other");
+  r.k_pools = k.data.data();
+  r.v_pools = v.data.data();
+  r.k_head_bytes = k_bytes.data();
+  r.v_head_bytes = v_bytes.data();
+  r.scores = score_data.data();
+  r.layers = size32(n);
+  const int64_t ints_needed = entries.evict_workspace(&b, &r);
+  if (ints_needed < 0) check((int)ints_needed);
+  const c10::DeviceGuard guard(device);
+  at::Tensor status = ints(2, device), work = ints(ints_needed, device);
+  check(entries.evict(&b, &r, ptr(status), ptr(work), stream_of(device)));
+  changed({&refs, &table, &lens});
+  k.changed();
+  v.changed();
+  for (const at::Tensor& x : scores) changed({&x});
+  return THPVariable_Wrap(std::move(status));
+}
+
 // (refs, table, lens, rows, page)
 PyObject* free_rows(Args& a) {
   const at::Tensor refs = a.tensor(), table = a.tensor(), lens = a.tensor(), rows = a.tensor();
@@ -734,6 +805,7 @@ PyMethodDef methods[] = {
     {"weights", FGW_FAST(weights), METH_FASTCALL, "fgw_kv_weights"},
     {"reserve", FGW_FAST(reserve), METH_FASTCALL, "fgw_pages_reserve"},
     {"fork", FGW_FAST(fork_rows), METH_FASTCALL, "fgw_pages_fork"},
+    {"evict", FGW_FAST(evict), METH_FASTCALL, "fgw_pages_evict"},
     {"free", FGW_FAST(free_rows), METH_FASTCALL, "fgw_pages_free"},
     {"compact", FGW_FAST(compact), METH_FASTCALL, "fgw_pages_compact"},
     {"copy", FGW_FAST(copy_pages), METH_FASTCALL, "fgw_pages_copy"},

@@ -45,3 +45,24 @@ def add_weights(scores, q, k_cache, block_table, cache_seqlens, cu_seqlens, page
         raise ValueError("contiguous inputs on the same GPU required")
     _kv.weights(scores, q, k_cache, block_table, cache_seqlens, cu_seqlens, page_size, min(last, 2**31 - 1), scale,
                 decay, _device_info(q.device.index).num_cus)
+
+
+def evict_rows(k_pools, v_pools, scores, refs, table, lens, keep, page_size, *, first=0, recent=0):
+    """Shorten rows to the keys that carry the most attention weight, in every layer's pools.
+
+    k_pools and v_pools [pages * page_size, Hkv, ...] and scores [rows, Hkv, S] are lists with an entry for
+    each layer, refs, table and lens the books of cache_pages, keep int32 [rows]. Row r with lens[r] >
+    keep[r] >= 0 keeps keep[r] tokens (others stay as they are): the first `first`, the last `recent` and,
+    of those between, the ones with the largest scores, equal ones from the lowest position on and NaN as
+    minus infinity. Each layer and K/V head chooses for itself; the kept tokens stay in order and move, with
+    their scores, to the positions 0 .. keep[r] - 1, and lens[r] = keep[r]. Scores from there on are left,
+    and so are the keys' rotary positions: later tokens take theirs from the caller (mha_paged_append's
+    positions), no longer from the cache length.
+
+    The tokens move to fresh pages, lowest id first and rows in order, from the page that holds token
+    `first` on; whole pages before that stay, shared or not, and the pages that a row leaves lose a holder.
+    Returns int32 [2]: rows refused for want of pages (that call for more, with the rows before them, than
+    are free: what this call gives back is free for the next one), rows refused because keep is less than
+    first + recent. Every decision is made on the GPU, the same on every run; nothing is read back.
+    """
+    return _kv.evict(k_pools, v_pools, scores, refs, table, lens, keep, page_size, first, recent)

@@ -7,7 +7,8 @@
  *   fgw_kv_extend      attention of packed ragged new tokens over the pages, grouped K/V heads
  *   fgw_kv_shared      the same where groups of requests share a prefix, which is read once for a group
  *   fgw_kv_weights     the attention weight that cached keys get from new tokens, added to running sums
- *   fgw_pages_*        fork, free, reserve, compact and copy pages; books on the device
+ *   fgw_pages_*        fork, free, reserve, compact and copy pages, and shorten rows to the keys that carry
+ *                      the most attention weight; books on the device
  * None has a counterpart in the reference, which reads a cache that its caller has written.
  *
  * Shared conventions (those of fgw_mha.h): pool rows K, V [N, Hkv, D] contiguous, N = pages *
@@ -217,6 +218,30 @@ int fgw_pages_compact(const fgw_pages_books* books, const fgw_pages_pools* pools
  * skipped. No page may be a destination twice, or a destination and a source. */
 int fgw_pages_copy(const fgw_pages_pools* pools, int32_t pages, const int32_t* src,
                    const int32_t* dst, int32_t count, hipStream_t stream);
+
+/* Rows that are shortened: row r with lens[r] > keep[r] >= 0 keeps, in every layer and K/V head, its first
+ * `first` tokens, its last `recent` ones and, of those between, the keep[r] - first - recent with the largest
+ * scores (equal ones: the lowest position; NaN as minus infinity), in order of position; their scores move
+ * with them, and lens[r] = keep[r]. The tokens from the page of token `first` on go to fresh pages, lowest id
+ * first, rows in order; the old pages lose a holder. A row is left where keep[r] < first + recent
+ * (status[1]), and where its pages, with those of the rows before it, are more than the free ones
+ * (status[0]): the pages that a call gives back are free for the next one. */
+typedef struct {
+  const int32_t* keep;        /* [rows], device; negative: the row stays */
+  void* const* k_pools;       /* [layers], host; each [pages * page_size, heads, head bytes] */
+  void* const* v_pools;
+  const int64_t* k_head_bytes; /* [layers], host; multiples of 16 */
+  const int64_t* v_head_bytes;
+  float* const* scores;       /* [layers], host; each [rows, heads, scores_stride] */
+  int64_t scores_stride;      /* at least width * page_size */
+  int32_t layers, heads;
+  int32_t first, recent;
+} fgw_evict_args;
+
+/* int32 elements of the workspace (pointers are not read), or a negative status. */
+int64_t fgw_pages_evict_workspace(const fgw_pages_books* books, const fgw_evict_args* args);
+int fgw_pages_evict(const fgw_pages_books* books, const fgw_evict_args* args, int32_t* status,
+                    int32_t* workspace, hipStream_t stream);
 
 #ifdef __cplusplus
 }

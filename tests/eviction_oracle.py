@@ -60,3 +60,45 @@ def weights_exact(scores, q, k, table, lens, cu, page, last, decay=1.0, scale=No
             row[:length] = before + total
             bound[b, h, :length] = slack + unit * (g * used / 8 + 32) * total + 2 * unit * (before.abs() + total)
     return out, bound
+
+
+def evict_exact(k_pools, v_pools, scores, refs, table, lens, keep, page, first=0, recent=0):
+    """Books, pools and scores (all on the CPU, changed in place) after an eviction; returns the status."""
+    pages, (rows, width) = refs.numel(), table.shape
+    still = first // page
+    free = [i for i in range(pages) if int(refs[i]) == 0]
+    left, short, bad, given, todo = len(free), 0, 0, 0, []
+    for r in range(rows):
+        length, budget = min(max(int(lens[r]), 0), width * page), int(keep[r])
+        if budget < 0 or budget >= length:
+            continue
+        if budget < first + recent:
+            bad += 1
+            continue
+        need = -(-budget // page) - still
+        if need and given + need > left:
+            short += 1
+        else:
+            todo.append((r, length, budget, free[given:given + need]))
+        given += need
+    old = table.clone()
+    for r, length, budget, fresh in todo:
+        for at, pools in enumerate(zip(scores, k_pools, v_pools)):
+            x, ks, vs = pools
+            for h in range(x.shape[1]):
+                value = [float(y) if not math.isnan(float(y)) else -math.inf for y in x[r, h, first:length - recent]]
+                order = sorted(range(len(value)), key=lambda i: (-value[i], i))[:budget - first - recent]
+                kept = list(range(first)) + [first + i for i in sorted(order)] + list(range(length - recent, length))
+                x[r, h, :budget] = x[r, h, kept].clone()
+                for d in range(still * page, budget):
+                    s = kept[d]
+                    src, dst = int(old[r, s // page]) * page + s % page, fresh[d // page - still] * page + d % page
+                    ks[dst, h], vs[dst, h] = ks[src, h], vs[src, h]
+        for j in range(still, -(-length // page)):
+            refs[int(old[r, j])] -= 1
+        for i in fresh:
+            refs[i] = 1
+        table[r, still:] = -1
+        table[r, still:still + len(fresh)] = torch.tensor(fresh, dtype=torch.int32)
+        lens[r] = budget
+    return [short, bad]
