@@ -573,7 +573,7 @@ __device__ __forceinline__ void dma_once(const void* base, u32 voff, u32 lds) {
 }
 #pragma clang diagnostic pop
 
-// The DMA of the 32-key tiles that one wave helps to fetch, tile n at key first_pos + step n, in tiles
+// The DMA of the tiles (of 32 keys, or BN) that one wave helps to fetch, tile n at key first_pos + step n, in tiles
 // laid out as fwd_kernel's (C: its Cfg, of which the NWQ waves of a key group share a tile). The
 // loads are inline assembly (dma_saddr, dma_flat): the compiler would wait for all of them before
 // each transposing read of V; the kernels place the waits. Row offsets come from page ids that lane
@@ -588,7 +588,7 @@ struct KeyStream {
   static constexpr int U = C::INSTR_PER_WAVE;
   static constexpr int kWindow = 64 / U;  // tiles of a window
   static constexpr int kAllLive = C::RPI << 8;
-  static_assert(C::BN == 32, "tiles of 32 keys");
+  static_assert(C::BN == 32 || C::BN == 64, "a lane for every key of a tile");
   const int32_t* const table_b;
   const char* const kb;
   const char* const vb;
@@ -682,13 +682,13 @@ struct KeyStream {
       dma_flat(in ? src + at : zero, dst + 1024u * (u32)(q * C::NWQ + wq));
     }
   }
-  // The same, each key through the table: lane l (mod 32) resolves key l, the load instructions fetch
+  // The same, each key through the table: lane l (mod BN) resolves key l, the load instructions fetch
   // their rows' offsets from those lanes.
   template <bool IS_V>
   __device__ __forceinline__ void issue_keys(const char* base, int pos0, u32 dst) {
     const int ln = opaque_lane(lane);
     const char* zero = reinterpret_cast<const char*>(kZeroChunk);
-    const int pos = pos0 + (ln & 31);
+    const int pos = pos0 + (ln & (C::BN - 1));
     const bool in = pos >= lo && pos < hi;
     const u32 pg = in ? div_page((u32)pos, page_magic, page_shift) : 0u;
     const int64_t row = (int64_t)table_b[pg] * page + ((u32)pos - pg * page);

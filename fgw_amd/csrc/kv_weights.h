@@ -13,19 +13,22 @@
 //                          the split's L. A tile of one split is finished at once.
 //   weights_finish_kernel  L of the row from its splits', and the kept scores' exponentials.
 // More rows. K is read twice, which costs little beside the products:
-//   weights_stats_kernel   L: tiles of 128 rows, four waves with 32 rows each, all keys past them;
-//   weights_columns_kernel the other way round: four waves hold 32 keys each, and up to kColumnRows rows of
+//   weights_stats_kernel   L: tiles of 256 rows, four waves with 64 rows each, all keys past them;
+//   weights_columns_kernel the other way round: four waves hold 64 keys each, and up to kColumnRows rows of
 //                          Q go past them, so a lane adds up its own key's weights;
 //   weights_sum_kernel     where a request has more rows than that: the parts' sums.
 #pragma once
 #include "kv_extend.h"
 
+#include "fmha_prefill.h"
+
 namespace fgw_kv {
 
 constexpr int kKeptRows = 16;
 constexpr int kColumnRows = 1024;  // rows of a part
-constexpr int kColumnKeys = 128;   // keys of an item
-constexpr int kSumKeys = 1024;
+constexpr int kSumKeys = 256;
+constexpr int kColumnKeys = 256;   // keys of an item
+constexpr int kWaveSimd = 2;       // waves to a SIMD
 
 struct WeightParams : ExtendParams {
   float* scores;    // [batch, heads, stride]
@@ -45,7 +48,7 @@ struct WeightNote {
   int32_t base, splits, tiles, chunk;
 };
 
-typedef Tiling<128, 64, 1> StatsTiling;
+typedef Tiling<256, 64, 1> StatsTiling;
 
 // The request's last tokens alone are its rows; `from` says where its new keys begin.
 template <class T>
@@ -244,123 +247,229 @@ static __global__ __launch_bounds__(kFinishThreads) void weights_finish_kernel(W
 
 // ---- more rows ----------------------------------------------------------------------------------
 
-// Four waves that share 32-row tiles of K or Q in LDS, two tiles to a step.
+// Waves that share tiles of 64 keys or rows in LDS, each with NR times 32 rows or keys of its own, 256 in all.
 template <bool BF16_, int DPAD_>
 struct WCfg {
   static constexpr bool BF16 = BF16_;
-  static constexpr int DPAD = DPAD_, NWQ = 4, NWK = 1, BN = 32, THREADS = 256, ROWS_WAVE = 32, ROWS_TILE = 128;
-  static constexpr int KK = DPAD / 16, ST = 1, KS = 2, CPR = DPAD / 8, ROW_BYTES = DPAD * 2;
+  static constexpr int DPAD = DPAD_, NWQ = DPAD == 256 ? 8 : 4, NWK = 1, BN = 64, THREADS = 64 * NWQ;
+  static constexpr int NR = DPAD == 256 ? 1 : 2, ROWS_WAVE = 32 * NR, ROWS_TILE = NWQ * ROWS_WAVE;
+  static constexpr int KK = DPAD / 16, ST = BN / 32, CPR = DPAD / 8, ROW_BYTES = DPAD * 2;
   static constexpr int TILE_BYTES = BN * ROW_BYTES, INSTR = TILE_BYTES / 1024, INSTR_PER_WAVE = INSTR / NWQ;
   static constexpr int KSW = CMin<16, CPR>::value, VSW = CPR / 4, RPI = 64 / CPR;
-  static constexpr int STEP_BYTES = 2 * TILE_BYTES;
-  static constexpr int STAGES = DPAD == 256 ? 2 : 3;
-  static_assert(DPAD >= 64 && INSTR_PER_WAVE >= 1, "DMA granularity");
+  static constexpr int STAGES = 3;
+  static_assert(ROWS_TILE == 256 && DPAD >= 64 && INSTR_PER_WAVE >= 1 && ST * NR % 2 == 0, "DMA granularity");
+};
+template <class C>
+struct OneTile {  // of mask_seen and row_max: 32 rows
+  static constexpr int ST = 1;
 };
 
-// The step loop of both kernels: step j's two tiles have landed for all waves when work(j, stage) runs.
-template <class C, class Issue, class Work>
-__device__ __forceinline__ void stream_steps(int steps, Issue&& issue, Work&& work) {
-  constexpr int kAhead = C::STAGES - 1, kBatch = 2 * C::INSTR_PER_WAVE;
-  for (int j = 0; j < kAhead && j < steps; ++j) issue(j, j);
+// The loop of both kernels. A step is a tile of 64 in LDS against the wave's own 32 NR: ST * NR products of
+// 32 x 32, phase (t, r) its rows 32 t .. against the wave's 32 r .. . The matrix and the vector unit run side
+// by side only where their instructions come by turns (16 products 222 ns, the 32 exponentials of a lane with
+// their sums 221 ns; by turns 277 to 333, one after the other 443), so between a phase's products stand the
+// exponentials of the phase before: use(s, t, r, e) takes element e of it; begin(j, s, t, r) and end(s, t, r)
+// come before and after. issue(j, lds offset) starts tile j's DMA. begin says whether the phase takes the
+// common path; if not, rare(s, t, r) stands for all its elements.
+template <class C, class Issue, class Begin, class Use, class Rare, class End>
+__device__ __forceinline__ void stream_tiles(int tiles, u32 lds, const Lanes<C>& ln, const u32x4 (&held)[C::NR][C::KK],
+                                             Issue&& issue, Begin&& begin, Use&& use, Rare&& rare, End&& end) {
+  using E = Elem<C::BF16>;
+  constexpr int kAhead = C::STAGES - 1, PH = C::ST * C::NR;
+  if (tiles <= 0) return;
+  u32 addr[C::KK];
+#pragma unroll
+  for (int kk = 0; kk < C::KK; ++kk) addr[kk] = lds + (u32)(ln.k_base + 32 * (kk ^ ln.ky));
+  u32x4 a[C::KK];
+  f32x16 s[2][1];
+  auto read = [&](auto t, auto kk, u32 at) {
+    constexpr int T = decltype(t)::value, K = decltype(kk)::value;
+    a[K] = *(const __attribute__((address_space(3))) u32x4*)(lds_at(addr[K]) + at + T * 32 * C::ROW_BYTES);
+  };
+  for (int j = 0; j < kAhead && j < tiles; ++j) issue(j, j * C::TILE_BYTES);
   int stage = 0;
-  for (int j = 0; j < steps; ++j) {
-    if (kAhead > 1 && j + 1 < steps)
-      wait_vm<(kAhead - 1) * kBatch>();
+  for (int j = 0; j < tiles; ++j) {
+    if (kAhead > 1 && j + 1 < tiles)
+      wait_vm<(kAhead - 1) * C::INSTR_PER_WAVE>();
     else
       wait_vm<0>();
-    __syncthreads();
-    if (j + kAhead < steps) issue(j + kAhead, stage == 0 ? C::STAGES - 1 : stage - 1);
-    work(j, stage);
+    __syncthreads();  // tile j has landed for all waves, tile j - 1 is read
+    const u32 at = (u32)(stage * C::TILE_BYTES);
+    static_for<C::KK>([&](auto kk) { read(std::integral_constant<int, 0>{}, kk, at); });
+    if (j + kAhead < tiles) issue(j + kAhead, (stage == 0 ? C::STAGES - 1 : stage - 1) * C::TILE_BYTES);
+    static_for<PH>([&](auto ph) {
+      constexpr int P = decltype(ph)::value, T = P / C::NR, R = P % C::NR, Q = (P + PH - 1) % PH, QT = Q / C::NR, QR = Q % C::NR;
+      f32x16(&next)[1] = s[P % 2];
+      f32x16(&cur)[1] = s[(P + 1) % 2];
+      auto products = [&](auto&& between) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) next[0][v] = 0.0f;
+        static_for<C::KK>([&](auto kk) {
+          constexpr int K = decltype(kk)::value;
+          between(K);
+          next[0] = E::mma(a[K], held[R][K], next[0]);
+          if constexpr (R == C::NR - 1 && T + 1 < C::ST) read(std::integral_constant<int, T + 1>{}, kk, at);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      };
+      if (P > 0 || j > 0) {
+        if (begin(P > 0 ? j : j - 1, cur, QT, QR)) {
+          products([&](int k) {
+#pragma unroll
+            for (int e = 16 * k / C::KK; e < 16 * (k + 1) / C::KK; ++e) use(cur[0], QT, QR, e);
+          });
+        } else {
+          products([](int) {});
+          rare(cur[0], QT, QR);
+        }
+        end(cur, QT, QR);
+      } else {
+        products([](int) {});
+      }
+    });
     stage = stage + 1 == C::STAGES ? 0 : stage + 1;
   }
+  f32x16(&cur)[1] = s[1];
+  if (begin(tiles - 1, cur, C::ST - 1, C::NR - 1)) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) use(cur[0], C::ST - 1, C::NR - 1, e);
+  } else {
+    rare(cur[0], C::ST - 1, C::NR - 1);
+  }
+  end(cur, C::ST - 1, C::NR - 1);
 }
 
 template <class C>
-__global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 2 : 3) void weights_stats_kernel(
+__global__ __launch_bounds__(C::THREADS, kWaveSimd) void weights_stats_kernel(
     WeightParams p, const int32_t* __restrict__ table, const int32_t* __restrict__ lengths, const int32_t* __restrict__ cu) {
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[C::STAGES * C::STEP_BYTES];
+  typedef StatsTiling T;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[C::STAGES * C::TILE_BYTES];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int il = lane & 31, hh = lane >> 5;
   Item it;
   int chunk;
-  if (!find_item<StatsTiling>(p, lengths, cu, (int)blockIdx.x, lane, it, &chunk)) return;
+  if (!find_item<T>(p, lengths, cu, (int)blockIdx.x, lane, it, &chunk)) return;
   if (it.place == 0 && it.head == 0 && tid == 0)
     reinterpret_cast<WeightNote*>(p.request_notes)[it.b] = WeightNote{(int)blockIdx.x / p.heads, it.place_splits, it.tiles, chunk};
-  const int first_pos = it.blk_begin * StatsTiling::BN, tiles = 2 * (it.blk_end - it.blk_begin);
+  const int first_pos = it.blk_begin * T::BN, tiles = it.blk_end - it.blk_begin;
   KeyStream<C, false> keys(p, table, it, lane, wave, first_pos, C::BN, tiles);
   const DmaLanes<C> dl(lane, wave, keys.row_bytes);
   const u32 lds = lds_address(smem);
-  const int in_tile = wave * C::ROWS_WAVE + il, row = it.tile * C::ROWS_TILE + in_tile;
-  u32x4 qf[C::KK];
-  load_q<C>(p, it, row, in_tile < it.rows, hh, qf);
-  const Seen seen = row_seen(p, it, row / p.group);
-  const int hi_min = row_seen(p, it, (it.tile * C::ROWS_TILE + wave * C::ROWS_WAVE) / p.group).hi;
   const Lanes<C> ln(lane);
-  float m = kNegBig, l = 0.0f;
+  u32x4 qf[C::NR][C::KK];
+  int in_tile[C::NR], hi_min[C::NR];
+  Seen seen[C::NR];
+  float m[C::NR], l[C::NR], rs[4];
+#pragma unroll
+  for (int r = 0; r < C::NR; ++r) {
+    in_tile[r] = wave * C::ROWS_WAVE + 32 * r + il;
+    const int row = it.tile * C::ROWS_TILE + in_tile[r];
+    load_q<C>(p, it, row, in_tile[r] < it.rows, hh, qf[r]);
+    seen[r] = row_seen(p, it, row / p.group);
+    hi_min[r] = row_seen(p, it, (it.tile * C::ROWS_TILE + wave * C::ROWS_WAVE + 32 * r) / p.group).hi;
+    m[r] = kNegBig;
+    l[r] = 0.0f;
+  }
   keys.ids_ready();
 #pragma unroll
-  for (int kk = 0; kk < C::KK; ++kk) asm volatile("" ::"v"(qf[kk]));
-  stream_steps<C>(
-      tiles / 2,
-      [&](int j, int stage) {
-        keys.template issue<false>(dl, 2 * j, lds + (u32)(stage * C::STEP_BYTES));
-        keys.template issue<false>(dl, 2 * j + 1, lds + (u32)(stage * C::STEP_BYTES + C::TILE_BYTES));
-      },
-      [&](int j, int stage) {
+  for (int r = 0; r < C::NR; ++r)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int pos0 = first_pos + 64 * j + 32 * h;
-          f32x16 s[1];
-          qk_block<C>(smem + stage * C::STEP_BYTES + h * C::TILE_BYTES, ln, qf, s);
-          if (pos0 + C::BN > hi_min) mask_seen<C>(s, pos0, seen, hh);
-          float sum = exp_sum(s[0], m, p.scale_log2);
-          if (__ballot(!(sum <= kSoftmaxSumBound))) {
-            const float top = fmaxf(m, row_max<C>(s, p.scale_log2));
-            l *= __builtin_amdgcn_exp2f(m - top);
-            m = top;
-            sum = exp_sum(s[0], m, p.scale_log2);
-          }
-          l += sum;
+    for (int kk = 0; kk < C::KK; ++kk) asm volatile("" ::"v"(qf[r][kk]));
+  stream_tiles<C>(
+      tiles, lds, ln, qf, [&](int j, int at) { keys.template issue<false>(dl, j, lds + (u32)at); },
+      [&](int j, f32x16(&s)[1], int t, int r) {
+        const int pos0 = first_pos + C::BN * j + 32 * t;
+        if (pos0 + 32 > hi_min[r]) mask_seen<OneTile<C>>(s, pos0, seen[r], hh);
+        return true;
+      },
+      [&](const f32x16& s, int, int r, int e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], p.scale_log2, -m[r]));
+        rs[e % 4] = e < 4 ? x : rs[e % 4] + x;
+      },
+      [](const f32x16&, int, int) {},
+      [&](const f32x16(&s)[1], int, int r) {
+        float sum = (rs[0] + rs[1]) + (rs[2] + rs[3]);
+        if (__ballot(!(sum <= kSoftmaxSumBound))) {
+          const float top = fmaxf(m[r], row_max<OneTile<C>>(s, p.scale_log2));
+          l[r] *= __builtin_amdgcn_exp2f(m[r] - top);
+          m[r] = top;
+          sum = exp_sum(s[0], top, p.scale_log2);
         }
+        l[r] += sum;
       });
-  const float tot = pair_sum(l);
-  if (hh == 0 && in_tile < it.rows) p.lse[(int64_t)it.slot * C::ROWS_TILE + in_tile] = lse2_of(m, tot);
+#pragma unroll
+  for (int r = 0; r < C::NR; ++r) {
+    const float tot = pair_sum(l[r]);
+    if (hh == 0 && in_tile[r] < it.rows) p.lse[(int64_t)it.slot * C::ROWS_TILE + in_tile[r]] = lse2_of(m[r], tot);
+  }
 }
 
-// Items of the other two kernels: key blocks times parts of the rows of each request and head, and
+// Items of the other two kernels. weights_columns_kernel: the parts of a request's rows, the last first,
+// each with the blocks of keys that some row of it sees (the more, the later the part). weights_sum_kernel:
 // blocks of keys of the requests with several parts.
 struct Column {
   int b, head, first, n, len, from, block, part, parts, part0;
 };
+// Blocks of kColumnKeys keys that the rows of a part see: up to its last row's token.
+__device__ __forceinline__ int blocks_seen(const WeightParams& p, int n, int len, int part) {
+  const int64_t rows = (int64_t)n * p.group, end = (int64_t)(part + 1) * kColumnRows;
+  const int last = (int)((u32)((end < rows ? end : rows) - 1) / (u32)p.group), hi = len - n + last + 1;
+  return hi > 0 ? (hi + kColumnKeys - 1) / kColumnKeys : 0;
+}
+struct ColumnRequest {
+  Request r;
+  int parts, items;
+};
+template <bool SUM>
+__device__ __forceinline__ ColumnRequest column_request(const WeightParams& p, const int32_t* lengths, const int32_t* cu, int b) {
+  ColumnRequest x;
+  x.r = load_request<StatsTiling>(p, lengths, cu, b);
+  x.parts = x.r.tiles ? (int)(((int64_t)x.r.n * p.group + kColumnRows - 1) / kColumnRows) : 0;
+  x.items = 0;
+  if (SUM)
+    x.items = x.parts > 1 ? (x.r.len + kSumKeys - 1) / kSumKeys : 0;
+  else
+    for (int c = 0; c < x.parts; ++c) x.items += blocks_seen(p, x.r.n, x.r.len, c);
+  return x;
+}
 template <bool SUM>
 __device__ __forceinline__ bool find_column(const WeightParams& p, const int32_t* lengths, const int32_t* cu, int64_t w,
-                                            int lane, const Request& r0, Column& it) {
-  const int64_t g64 = w / p.heads;
-  it.head = (int)(w - g64 * p.heads);
+                                            int lane, const ColumnRequest& x0, Column& it) {
+  const int64_t g = w / p.heads;
+  it.head = (int)(w - g * p.heads);
   int64_t before = 0;
   int parts_before = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
-    const Request r = b0 == 0 ? r0 : load_request<StatsTiling>(p, lengths, cu, b0 + lane);
-    const int parts = r.tiles ? (int)(((int64_t)r.n * p.group + kColumnRows - 1) / kColumnRows) : 0;
-    const int per = SUM ? (parts > 1 ? 1 : 0) : parts, keys = SUM ? kSumKeys : kColumnKeys;
-    const int items = r.tiles ? (r.len + keys - 1) / keys * per : 0;
-    const int items_to = wave_incl_sum(items, lane), parts_to = wave_incl_sum(parts, lane);
-    const int64_t at = g64 - before - (items_to - items);
-    const uint64_t hit = __ballot(at >= 0 && at < items);
+    const ColumnRequest x = b0 == 0 ? x0 : column_request<SUM>(p, lengths, cu, b0 + lane);
+    const int items_to = wave_incl_sum(x.items, lane), parts_to = wave_incl_sum(x.parts, lane);
+    const int64_t at = g - before - (items_to - x.items);
+    const uint64_t hit = __ballot(at >= 0 && at < x.items);
     if (hit) {
       const int l = __builtin_ctzll(hit);
-      auto pick = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+      auto pick = [&](int y) { return __builtin_amdgcn_readlane(y, l); };
       it.b = b0 + l;
-      it.first = pick(r.first);
-      it.n = pick(r.n);
-      it.len = pick(r.len);
-      it.from = pick(r.from);
-      it.parts = pick(parts);
-      it.part0 = parts_before + pick(parts_to - parts);
-      const int place = pick((int)at), step = SUM ? 1 : it.parts;
-      it.block = (int)((u32)place / (u32)step);
-      it.part = place - it.block * step;
-      return true;
+      it.first = pick(x.r.first);
+      it.n = pick(x.r.n);
+      it.len = pick(x.r.len);
+      it.from = pick(x.r.from);
+      it.parts = pick(x.parts);
+      it.part0 = parts_before + pick(parts_to - x.parts);
+      it.block = pick((int)at);
+      it.part = 0;
+      if (SUM || it.parts == 1) return true;
+      for (int c0 = 0; c0 < it.parts; c0 += 64) {  // the part: one to a lane
+        const int c = it.parts - 1 - c0 - lane, n = c >= 0 ? blocks_seen(p, it.n, it.len, c) : 0;
+        const int to = wave_incl_sum(n, lane);
+        const uint64_t here = __ballot(it.block < to);
+        if (here) {
+          const int k = __builtin_ctzll(here);
+          it.part = it.parts - 1 - c0 - k;
+          it.block -= __builtin_amdgcn_readlane(to - n, k);
+          return true;
+        }
+        it.block -= __builtin_amdgcn_readlane(to, 63);
+      }
+      return false;
     }
     before += __builtin_amdgcn_readlane(items_to, 63);
     parts_before += __builtin_amdgcn_readlane(parts_to, 63);
@@ -374,54 +483,61 @@ __device__ __forceinline__ int first_row(const WeightParams& p, const Column& it
 }
 
 template <class C>
-__global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 2 : 3) void weights_columns_kernel(
+__global__ __launch_bounds__(C::THREADS, kWaveSimd) void weights_columns_kernel(
     WeightParams p, const int32_t* __restrict__ table, const int32_t* __restrict__ lengths, const int32_t* __restrict__ cu) {
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[C::STAGES * C::STEP_BYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[C::STAGES * C::TILE_BYTES];
   __shared__ __attribute__((aligned(16))) float slse[kColumnRows + 64];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int il = lane & 31, hh = lane >> 5;
   const u32 lds = lds_address(smem);
   const Lanes<C> ln(lane);
-  const Request r0 = load_request<StatsTiling>(p, lengths, cu, lane);
+  const ColumnRequest r0 = column_request<false>(p, lengths, cu, lane);
   const int64_t row_bytes = (int64_t)p.heads * p.dim * 2;
   Column it;
   for (int64_t w = blockIdx.x; find_column<false>(p, lengths, cu, w, lane, r0, it); w += gridDim.x) {
-    const int rows = it.n * p.group, key0 = it.block * kColumnKeys;
+    const int rows = it.n * p.group, key0 = it.block * kColumnKeys + wave * C::ROWS_WAVE;  // keys of this wave
     const int end = rows - it.part * kColumnRows < kColumnRows ? rows : (it.part + 1) * kColumnRows;
-    // (Steps of 64 rows from the part's first row.)
-    const int part0 = it.part * kColumnRows, seen0 = first_row(p, it, key0);
+    // (Tiles of 64 rows from the part's first row.)
+    const int part0 = it.part * kColumnRows, seen0 = first_row(p, it, it.block * kColumnKeys);
     if (seen0 >= end) continue;
-    const int begin = seen0 > part0 ? part0 + (seen0 - part0) / 64 * 64 : part0, steps = (end - begin + 63) / 64;
+    const int begin = seen0 > part0 ? part0 + (seen0 - part0) / 64 * 64 : part0, tiles = (end - begin + 63) / 64;
 
-    // K of the lane's key, from its page.
-    const int key = key0 + wave * 32 + il;
-    const u32 pg = key < it.len ? div_page((u32)key, p.page_magic, p.page_shift) : 0u;
-    const int64_t krow = (int64_t)table[(int64_t)it.b * p.width + pg] * p.page_size + ((u32)key - pg * (u32)p.page_size);
-    const bool live = key < it.len && krow >= 0 && krow < p.pool_rows;
-    const char* const kp = static_cast<const char*>(p.k) + (int64_t)it.head * p.dim * 2 + (live ? krow * row_bytes : 0);
-    u32x4 kf[C::KK];
+    // K of the lane's keys, from their pages.
+    u32x4 kf[C::NR][C::KK];
+    int mine[C::NR], all[C::NR];  // the first row that sees the lane's key, all of the wave's 32
 #pragma unroll
-    for (int kk = 0; kk < C::KK; ++kk) {
-      const int d = 16 * kk + 8 * hh;
-      u32x4 x = {0u, 0u, 0u, 0u};
-      if (live && d < p.dim) x = *reinterpret_cast<const u32x4*>(kp + 2 * d);
-      kf[kk] = x;
+    for (int r = 0; r < C::NR; ++r) {
+      const int key = key0 + 32 * r + il;
+      const u32 pg = key < it.len ? div_page((u32)key, p.page_magic, p.page_shift) : 0u;
+      const int64_t krow = (int64_t)table[(int64_t)it.b * p.width + pg] * p.page_size + ((u32)key - pg * (u32)p.page_size);
+      const bool live = key < it.len && krow >= 0 && krow < p.pool_rows;
+      const char* const kp = static_cast<const char*>(p.k) + (int64_t)it.head * p.dim * 2 + (live ? krow * row_bytes : 0);
+#pragma unroll
+      for (int kk = 0; kk < C::KK; ++kk) {
+        const int d = 16 * kk + 8 * hh;
+        u32x4 x = {0u, 0u, 0u, 0u};
+        if (live && d < p.dim) x = *reinterpret_cast<const u32x4*>(kp + 2 * d);
+        kf[r][kk] = x;
+      }
+      mine[r] = first_row(p, it, key);
+      all[r] = first_row(p, it, key0 + 32 * r + 31);
     }
     // L of the part's rows, from their splits.
     __syncthreads();  // the item before is done with slse and the stages
     const WeightNote note = reinterpret_cast<const WeightNote*>(p.request_notes)[it.b];
-    for (int r = begin + tid; r < begin + 64 * steps; r += C::THREADS) {
+    for (int r = begin + tid; r < begin + 64 * tiles; r += C::THREADS) {
       float lse = INFINITY;  // rows that are none weigh nothing
       if (r < end) {
-        const int tile = r / C::ROWS_TILE, last = (tile + 1) * C::ROWS_TILE < rows ? (tile + 1) * C::ROWS_TILE : rows;
-        int hi = it.len - it.n + (last - 1) / p.group + 1;
+        typedef StatsTiling T;
+        const int tile = r / T::ROWS, last = (tile + 1) * T::ROWS < rows ? (tile + 1) * T::ROWS : rows;
+        int hi = it.len - it.n + (int)((u32)(last - 1) / (u32)p.group) + 1;
         hi = hi < 0 ? 0 : hi;
-        const int most = splits_of(p, (hi + StatsTiling::KEYS - 1) / StatsTiling::KEYS, note.chunk);
+        const int most = splits_of(p, (hi + T::KEYS - 1) / T::KEYS, note.chunk);
         const int splits = most < note.splits ? most : note.splits;
         const int64_t slot = (int64_t)(note.base + (note.tiles - 1 - tile) * note.splits) * p.heads + it.head;
         float m = kNegBig, l = 0.0f;
         for (int s = 0; s < splits && slot + (int64_t)s * p.heads < p.work && slot >= 0; ++s) {
-          const float x = p.lse[(slot + (int64_t)s * p.heads) * C::ROWS_TILE + (r - tile * C::ROWS_TILE)], top = fmaxf(m, x);
+          const float x = p.lse[(slot + (int64_t)s * p.heads) * T::ROWS + (r - tile * T::ROWS)], top = fmaxf(m, x);
           l = l * __builtin_amdgcn_exp2f(m - top) + __builtin_amdgcn_exp2f(x - top);
           m = top;
         }
@@ -430,58 +546,80 @@ __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 2 : 3) void weights_co
       slse[r - begin] = lse;
     }
 #pragma unroll
-    for (int kk = 0; kk < C::KK; ++kk) asm volatile("" ::"v"(kf[kk]));
+    for (int r = 0; r < C::NR; ++r)
+#pragma unroll
+      for (int kk = 0; kk < C::KK; ++kk) asm volatile("" ::"v"(kf[r][kk]));
     __syncthreads();
 
-    // 32 rows of Q into LDS, a K tile's layout.
-    auto issue_tile = [&](int row0, u32 dst) {
+    // 64 rows of Q into LDS, a K tile's layout, tile after tile: a lane's rows are 64 apart, so their places
+    // move on by whole tokens and a few heads.
+    constexpr int U = C::INSTR_PER_WAVE;
+    const int hop = C::BN / p.group, skip = C::BN - hop * p.group;  // tokens and heads of 64 rows
+    const int64_t hop_bytes = hop * p.q_token + skip * p.q_head, wrap_bytes = p.q_token - p.group * p.q_head;
+    const char* src[U];
+    int src_head[U], next_row = begin + C::RPI * wave + lane / C::CPR;  // (of instruction 0)
+    constexpr int kApart = C::RPI * C::NWQ;                             // rows between instructions
+    u32 live_dims = 0;  // instruction q's chunk lies below D
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      const int i = q * C::NWQ + wave, r = C::RPI * i + lane / C::CPR, row = begin + r, c = lane % C::CPR ^ (r % C::KSW);
+      const int token = (int)((u32)row / (u32)p.group);
+      src_head[q] = row - token * p.group;
+      live_dims |= c * 8 < p.dim ? 1u << q : 0u;
+      src[q] = static_cast<const char*>(p.q) + (int64_t)(it.first + token) * p.q_token +
+               (int64_t)(it.head * p.group + src_head[q]) * p.q_head + c * 16;
+    }
+    auto issue_tile = [&](int, int at) {
       const char* zero = reinterpret_cast<const char*>(kZeroChunk);
-      const int at = lane % C::CPR;
 #pragma unroll
-      for (int q = 0; q < C::INSTR_PER_WAVE; ++q) {
-        const int i = q * C::NWQ + wave, r = C::RPI * i + lane / C::CPR, row = row0 + r, c = at ^ (r % C::KSW);
-        const int token = (int)((u32)row / (u32)p.group), head = row - token * p.group;
-        const char* src = static_cast<const char*>(p.q) + (int64_t)(it.first + token) * p.q_token +
-                          (int64_t)(it.head * p.group + head) * p.q_head + c * 16;
-        dma_flat(row < end && c * 8 < p.dim ? src : zero, dst + 1024u * (u32)i);
+      for (int q = 0; q < U; ++q) {
+        const bool live = next_row < end - q * kApart && (p.dim == C::DPAD || (live_dims >> q & 1u));
+        dma_flat(live ? src[q] : zero, lds + (u32)at + 1024u * (u32)(q * C::NWQ + wave));
+        src_head[q] += skip;
+        const bool wrap = src_head[q] >= p.group;
+        src_head[q] -= wrap ? p.group : 0;
+        src[q] += hop_bytes + (wrap ? wrap_bytes : 0);
       }
+      next_row += C::BN;
     };
-    const int mine = first_row(p, it, key), all = first_row(p, it, key0 + wave * 32 + 31);
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    stream_steps<C>(
-        steps,
-        [&](int j, int stage) {
-          issue_tile(begin + 64 * j, lds + (u32)(stage * C::STEP_BYTES));
-          issue_tile(begin + 64 * j + 32, lds + (u32)(stage * C::STEP_BYTES + C::TILE_BYTES));
-        },
-        [&](int j, int stage) {
+    float acc[C::NR][4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int at = 64 * j + 32 * h;
-            f32x16 s[1];
-            qk_block<C>(smem + stage * C::STEP_BYTES + h * C::TILE_BYTES, ln, kf, s);
-            f32x4 lse[4];
+    for (int r = 0; r < C::NR; ++r)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) lse[g] = *reinterpret_cast<const f32x4*>(slse + at + 8 * g + 4 * hh);
-            if (begin + at >= all) {
+      for (int k = 0; k < 4; ++k) acc[r][k] = 0.0f;
+    f32x4 lse[4];  // of the lane's rows of a phase
+    int row0 = 0;  // of the phase, in the part
+    stream_tiles<C>(
+        tiles, lds, ln, kf, issue_tile,
+        [&](int j, f32x16(&)[1], int t, int r) {
+          row0 = C::BN * j + 32 * t;
+          if (r == 0) {
 #pragma unroll
-              for (int v = 0; v < 16; ++v)
-                acc[v % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][v], p.scale_log2, -lse[v / 4][v % 4]));
-            } else {
-#pragma unroll
-              for (int v = 0; v < 16; ++v) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][v], p.scale_log2, -lse[v / 4][v % 4]));
-                acc[v % 4] += begin + at + 8 * (v / 4) + 4 * hh + v % 4 >= mine ? e : 0.0f;
-              }
-            }
+            for (int g = 0; g < 4; ++g) lse[g] = *reinterpret_cast<const f32x4*>(slse + row0 + 8 * g + 4 * hh);
           }
-        });
-    const float sum = pair_sum((acc[0] + acc[1]) + (acc[2] + acc[3]));
-    if (hh == 0 && key < it.len) {
-      if (it.parts == 1)
-        add_score(p, p.scores + ((int64_t)it.b * p.heads + it.head) * p.stride, key, it.from, sum);
-      else if (it.part0 + it.part < p.parts_most)
-        p.sums[((int64_t)(it.part0 + it.part) * p.heads + it.head) * p.keys_pad + key] = sum;
+          return begin + row0 >= all[r];
+        },
+        [&](const f32x16& s, int, int r, int e) {
+          acc[r][e % 4] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], p.scale_log2, -lse[e / 4][e % 4]));
+        },
+        [&](const f32x16& s, int, int r) {  // some of the wave's keys lie behind rows of the phase
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], p.scale_log2, -lse[e / 4][e % 4]));
+            acc[r][e % 4] += begin + row0 + 8 * (e / 4) + 4 * hh + e % 4 >= mine[r] ? x : 0.0f;
+          }
+        },
+        [](const f32x16(&)[1], int, int) {});
+#pragma unroll
+    for (int r = 0; r < C::NR; ++r) {
+      const int key = key0 + 32 * r + il;
+      const float sum = pair_sum((acc[r][0] + acc[r][1]) + (acc[r][2] + acc[r][3]));
+      if (hh == 0 && key < it.len) {
+        if (it.parts == 1)
+          add_score(p, p.scores + ((int64_t)it.b * p.heads + it.head) * p.stride, key, it.from, sum);
+        else if (it.part0 + it.part < p.parts_most)
+          p.sums[((int64_t)(it.part0 + it.part) * p.heads + it.head) * p.keys_pad + key] = sum;
+      }
     }
   }
 }
@@ -489,7 +627,7 @@ __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 2 : 3) void weights_co
 static __global__ __launch_bounds__(kFinishThreads) void weights_sum_kernel(WeightParams p, const int32_t* __restrict__ lengths,
                                                                            const int32_t* __restrict__ cu) {
   const int tid = threadIdx.x, lane = tid & 63;
-  const Request r0 = load_request<StatsTiling>(p, lengths, cu, lane);
+  const ColumnRequest r0 = column_request<true>(p, lengths, cu, lane);
   Column it;
   for (int64_t w = blockIdx.x; find_column<true>(p, lengths, cu, w, lane, r0, it); w += gridDim.x) {
     const int end = it.len < (it.block + 1) * kSumKeys ? it.len : (it.block + 1) * kSumKeys;
@@ -497,8 +635,18 @@ static __global__ __launch_bounds__(kFinishThreads) void weights_sum_kernel(Weig
     for (int key = it.block * kSumKeys + tid; key < end; key += kFinishThreads) {
       // Parts whose rows all come before the key's block left nothing.
       float sum = 0.0f;
-      for (int c = first_row(p, it, key / kColumnKeys * kColumnKeys) / kColumnRows; c < it.parts; ++c)
-        if (it.part0 + c < p.parts_most) sum += p.sums[((int64_t)(it.part0 + c) * p.heads + it.head) * p.keys_pad + key];
+      const int last = it.part0 + it.parts < p.parts_most ? it.part0 + it.parts : p.parts_most;
+      const float* const at = p.sums + (int64_t)it.head * p.keys_pad + key;
+      const int64_t step = (int64_t)p.heads * p.keys_pad;
+      int c = it.part0 + first_row(p, it, key / kColumnKeys * kColumnKeys) / kColumnRows;
+      for (; c + 4 <= last; c += 4) {
+        float x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = at[(c + k) * step];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum += x[k];
+      }
+      for (; c < last; ++c) sum += at[c * step];
       add_score(p, row, key, it.from, sum);
     }
   }

@@ -14,6 +14,9 @@ FGW_KV_EXTERN_WEIGHTS(false, 64) FGW_KV_EXTERN_WEIGHTS(false, 128) FGW_KV_EXTERN
 
 namespace {
 
+// Items of weights_stats_kernel, two to a CU, where its tiles are fewer.
+constexpr int kStatsItems = 512;
+
 struct WeightPlan {
   bool many;       // rows of a request and K/V head, at most, past kKeptRows
   Launch launch;   // of the first pass
@@ -70,12 +73,18 @@ WeightPlan plan_weights(const fgw_kv_weights_args& a) {
     p.launch.min_chunk = kLongMinChunk;
     p.launch.many = 1 << 20;
     p.launch.tiles = blocks(StatsTiling::ROWS);
-    plan_items<StatsTiling>(p.launch, e, true);
+    p.launch.items = p.launch.tiles * a.kv_heads;
+    // (Statistics of a split are a number a row: as many splits as even out the causal tiles.)
+    const int64_t most = most_splits<StatsTiling>(e, p.launch.min_chunk, 0);
+    if (most > 1) {
+      p.launch.target = kStatsItems;
+      p.launch.items = std::max(p.launch.items, std::min<int64_t>(p.launch.target, p.launch.items * most));
+    }
     p.launch.slots = p.launch.items;  // every item leaves statistics
     p.lse = p.launch.slots * StatsTiling::ROWS;
     p.notes = (int64_t)a.batch * (int64_t)sizeof(WeightNote) / 4;
     const int64_t parts = blocks(kColumnRows), keys = p.keys_pad / kColumnKeys;
-    p.columns = persistent(parts * keys * a.kv_heads, e.num_cus, 3);
+    p.columns = persistent(parts * keys * a.kv_heads, e.num_cus, a.dim > 128 ? 1 : 2);
     if (rows > kColumnRows) {
       p.parts = parts;
       p.kept = parts * a.kv_heads * p.keys_pad;
