@@ -56,6 +56,7 @@ struct SharedParams : ExtendParams {
   const float* prefix_parts;
   const float* prefix_lse;
   int32_t* group_notes;     // [n_groups] GroupNote
+  int32_t share_from;       // units of 64 KB that sharing has to save (Requests::pays); 0: it always pays
 };
 struct PrefixParams : SharedParams {};
 struct SuffixParams : SharedParams {};
@@ -71,6 +72,7 @@ constexpr bool kPicksFrom = kIsSuffix<P>;  // items with Request::from
 struct GroupNote {
   int32_t base, splits, tiles, first;
 };
+constexpr int kShareRows = 128;  // of a request, on average over its group, up to which sharing may pay
 
 // Tiles of ROWS rows, keys in blocks of BN, splits in units of UNIT blocks.
 template <int ROWS_, int BN_, int UNIT_>
@@ -118,78 +120,6 @@ __device__ __forceinline__ Request load_request(const ExtendParams& p, const int
   return r;
 }
 
-// Requests [f0, f1) of group g and the keys that they share: as many as the first of them, whose table
-// row holds them, has before its new tokens (none for a request alone: it reads its keys itself).
-struct Group {
-  int f0, f1, keys;
-};
-__device__ __forceinline__ Group load_group(const SharedParams& p, const int32_t* lengths, const int32_t* cu, int g) {
-  Group x{0, 0, 0};
-  if (g >= p.n_groups) return x;
-  const int f0 = p.groups[g], f1 = p.groups[g + 1], wanted = p.prefixes[g];
-  if (f0 < 0 || f1 > p.batch || f1 <= f0 + 1) return x;
-  const int n = cu[f0 + 1] - cu[f0], capacity = p.width * p.page_size;
-  int len = lengths[f0];
-  len = len < 0 ? 0 : (len > capacity ? capacity : len);
-  const int before = n >= 0 && n < len ? len - n : 0;
-  x.f0 = f0;
-  x.f1 = f1;
-  x.keys = wanted < before ? wanted : before;
-  x.keys = x.keys < 0 ? 0 : x.keys;
-  return x;
-}
-
-template <class T>
-__device__ __forceinline__ Request load_request(const PrefixParams& p, const int32_t* lengths, const int32_t* cu, int g) {
-  Request r{0, 0, 0, 0, 0, 0, 0, -1};
-  const Group x = load_group(p, lengths, cu, g);
-  if (x.keys == 0) return r;
-  const int first = cu[x.f0], next = cu[x.f1];
-  r.row = x.f0;
-  r.len = x.keys;
-  r.first = first;
-  if (first < 0 || next > p.tokens || next <= first) return r;
-  r.n = next - first;
-  r.tiles = (int)(((int64_t)r.n * p.group + T::ROWS - 1) / T::ROWS);
-  r.units = (r.len + T::KEYS - 1) / T::KEYS;
-  return r;
-}
-
-// The group of each lane's request: up to 64 groups are held one to a lane and passed around, more are
-// searched for in memory (their first requests never fall).
-template <class T>
-__device__ __forceinline__ Request load_request(const SuffixParams& p, const int32_t* lengths, const int32_t* cu, int b) {
-  Group x{0, 0, 0};
-  int group = -1;
-  if (p.n_groups <= 64) {
-    const Group mine = load_group(p, lengths, cu, (int)(threadIdx.x & 63u));
-    for (int g = 0; g < p.n_groups; ++g) {
-      const int f0 = __builtin_amdgcn_readlane(mine.f0, g), f1 = __builtin_amdgcn_readlane(mine.f1, g);
-      const int keys = __builtin_amdgcn_readlane(mine.keys, g);
-      if (b >= f0 && b < f1) {
-        x.keys = keys;
-        group = g;
-      }
-    }
-  } else {
-    int lo = 0, hi = p.n_groups;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (p.groups[mid] <= b) lo = mid; else hi = mid;
-    }
-    x = load_group(p, lengths, cu, lo);
-    group = lo;
-    if (b < x.f0 || b >= x.f1) x.keys = 0;
-  }
-  Request r = load_request<T>(static_cast<const ExtendParams&>(p), lengths, cu, b);
-  if (x.keys > 0 && r.n > 0 && r.len - r.n >= x.keys) {
-    r.from = x.keys;
-    r.group = group;
-    r.units -= r.units > 0 ? r.from / T::KEYS : 0;
-  }
-  return r;
-}
-
 // Inclusive sums over the wave's lanes: by DPP within rows of 16 (shifts by 1, 2, 4, 8), then each
 // row's last lane onto the rows behind it.
 __device__ __forceinline__ int wave_incl_sum(int x, int lane) {
@@ -205,6 +135,140 @@ __device__ __forceinline__ int wave_sum(int x, int lane) {
   return __builtin_amdgcn_readlane(wave_incl_sum(x, lane), 63);
 }
 
+// Requests [f0, f1) of group g, its tokens [first, next) and the keys that its requests share: as many as the
+// first of them, whose table row holds them, has before its new tokens (none for a request alone: it reads
+// its keys itself). Two rounds of reads; every place is read within the arrays.
+struct Group {
+  int f0, f1, keys, first, next;
+};
+__device__ __forceinline__ Group load_group(const SharedParams& p, const int32_t* lengths, const int32_t* cu, int g) {
+  Group x{0, 0, 0, 0, 0};
+  const int at = g < p.n_groups ? g : p.n_groups - 1;
+  const int f0 = p.groups[at], f1 = p.groups[at + 1], wanted = p.prefixes[at];
+  const bool good = g < p.n_groups && f0 >= 0 && f1 <= p.batch && f1 > f0 + 1;
+  const int a = good ? f0 : 0, b = good ? f1 : 0, capacity = p.width * p.page_size;
+  x.first = cu[a];
+  x.next = cu[b];
+  const int n = cu[a + 1] - x.first;
+  int len = lengths[a];
+  len = len < 0 ? 0 : (len > capacity ? capacity : len);
+  const int before = n >= 0 && n < len ? len - n : 0;
+  x.f0 = a;
+  x.f1 = b;
+  x.keys = good ? (wanted < before ? wanted : before) : 0;
+  x.keys = x.keys < 0 ? 0 : x.keys;
+  // (Requests of whole long tiles are bound by their products, which sharing does not save: kv_shared.hip.)
+  if (p.share_from > 0 && (int64_t)(x.next - x.first) * p.group > (int64_t)kShareRows * (x.f1 - x.f0)) x.keys = 0;
+  return x;
+}
+// What the requests of a group would read of the prefix each on its own, in units of 64 KB: once for every
+// 32 rows, in tiles of 128 or 256 dims (a tile of 64 takes the kernel about as long as one of 128).
+__host__ __device__ __forceinline__ int shared_dims(int dim) { return dim <= 128 ? 128 : 256; }
+__device__ __forceinline__ int group_saves(const SharedParams& p, const Group& x) {
+  if (x.keys <= 0) return 0;
+  const float members = (float)(x.f1 - x.f0), rows = (float)(x.next - x.first) * (float)p.group / members;
+  const float bytes = members * ceilf(rows * 0.03125f) * (float)x.keys * (float)p.heads * (float)shared_dims(p.dim) * 4.0f;
+  return (int)fminf(bytes * (1.0f / 65536.0f), 16777216.0f);
+}
+
+template <class T>
+__device__ __forceinline__ Request group_request(const PrefixParams& p, const Group& x) {
+  Request r{0, 0, 0, 0, 0, 0, 0, -1};
+  if (x.keys == 0) return r;
+  r.row = x.f0;
+  r.len = x.keys;
+  r.first = x.first;
+  if (x.first < 0 || x.next > p.tokens || x.next <= x.first) return r;
+  r.n = x.next - x.first;
+  r.tiles = (int)(((int64_t)r.n * p.group + T::ROWS - 1) / T::ROWS);
+  r.units = (r.len + T::KEYS - 1) / T::KEYS;
+  return r;
+}
+
+// The group of each lane's request: up to 64 groups are held one to a lane (`mine`, loaded once) and passed
+// around, more are searched for in memory (their first requests never fall).
+template <class T>
+__device__ __forceinline__ Request load_request(const SuffixParams& p, const int32_t* lengths, const int32_t* cu, int b,
+                                                const Group& mine, bool share) {
+  Request r = load_request<T>(static_cast<const ExtendParams&>(p), lengths, cu, b);
+  int keys = 0, group = -1;
+  if (!share) return r;
+  if (p.n_groups <= 64) {
+    for (int g = 0; g < p.n_groups; ++g) {
+      const int f0 = __builtin_amdgcn_readlane(mine.f0, g), f1 = __builtin_amdgcn_readlane(mine.f1, g);
+      const int shared = __builtin_amdgcn_readlane(mine.keys, g);
+      if (b >= f0 && b < f1) {
+        keys = shared;
+        group = g;
+      }
+    }
+  } else {
+    int lo = 0, hi = p.n_groups;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (p.groups[mid] <= b) lo = mid; else hi = mid;
+    }
+    const Group x = load_group(p, lengths, cu, lo);
+    group = lo;
+    keys = b >= x.f0 && b < x.f1 ? x.keys : 0;
+  }
+  if (keys > 0 && r.n > 0 && r.len - r.n >= keys) {
+    r.from = keys;
+    r.group = group;
+    r.units -= r.units > 0 ? r.from / T::KEYS : 0;
+  }
+  return r;
+}
+
+// The requests of a launch, 64 at a time, one to a lane: the first kHeld times 64 are read once and held.
+template <class T, class P>
+struct Requests {
+  static constexpr int kHeld = kIsSuffix<P> ? 4 : 1;
+  const P& p;
+  const int32_t* const lengths;
+  const int32_t* const cu;
+  const int lane;
+  Group mine{0, 0, 0, 0, 0};  // of the first 64, one to a lane
+  bool share = true;
+  Request held[kHeld];
+  __device__ __forceinline__ Request load(int b) const {
+    if constexpr (kIsSuffix<P>) return load_request<T>(p, lengths, cu, b, mine, share);
+    else if constexpr (kIsPrefix<P>) return share ? group_request<T>(p, b < 64 ? mine : load_group(p, lengths, cu, b)) : Request{0, 0, 0, 0, 0, 0, 0, -1};
+    else return load_request<T>(p, lengths, cu, b);
+  }
+  // Whether the groups' prefixes are worth the two passes and the partials between them; the same in every
+  // program of both.
+  __device__ __forceinline__ bool pays() const {
+    if (p.share_from <= 0) return true;
+    int total = wave_sum(group_saves(p, mine), lane);
+    for (int g = 64; g < p.n_groups && total < p.share_from; g += 64)
+      total += wave_sum(group_saves(p, load_group(p, lengths, cu, g + lane)), lane);
+    return total >= p.share_from;
+  }
+  __device__ __forceinline__ Requests(const P& p_, const int32_t* lengths_, const int32_t* cu_, int lane_)
+      : p(p_), lengths(lengths_), cu(cu_), lane(lane_) {
+    if constexpr (kIsSuffix<P> || kIsPrefix<P>) {
+      if (p.n_groups > 0) {
+        mine = load_group(p, lengths, cu, lane);
+        share = pays();
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k)
+      if (k == 0 || 64 * k < requests_of(p)) held[k] = load(64 * k + lane);
+  }
+  // f(first request, the lane's) for every 64, until one is true.
+  template <class F>
+  __device__ __forceinline__ bool each(F&& f) const {
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k)
+      if (64 * k < requests_of(p) && f(64 * k, held[k])) return true;
+    for (int b0 = 64 * kHeld; b0 < requests_of(p); b0 += 64)
+      if (f(b0, load(b0 + lane))) return true;
+    return false;
+  }
+};
+
 __device__ __forceinline__ int splits_of(const ExtendParams& p, int units, int chunk) {
   return units > chunk && units > p.whole ? (units + chunk - 1) / chunk : 1;
 }
@@ -219,18 +283,17 @@ __device__ __forceinline__ int splits_of(const ExtendParams& p, int units, int c
 // saturate (kMany) so that they stay in 32 bits; the same in every program.
 constexpr int kWhole = 0x40000000, kMany = 1 << 24;
 template <class T, class P>
-__device__ __forceinline__ int best_chunk(const P& p, const int32_t* lengths, const int32_t* cu,
-                                          const Request& r0, int lane) {
+__device__ __forceinline__ int best_chunk(const P& p, const Requests<T, P>& all) {
   const int limit = (int)((u32)p.target / (u32)p.heads);
   if (limit <= 1) return kWhole;
   auto sum = [&](auto&& count) {
     int total = 0;
-    for (int b0 = 0; b0 < requests_of(p); b0 += 64) {
-      const Request r = b0 == 0 ? r0 : load_request<T>(p, lengths, cu, b0 + lane);
+    all.each([&](int, const Request& r) {
       const int64_t x = r.tiles ? count(r) : 0;
-      total += wave_sum((int)(x < kMany ? x : kMany), lane);
+      total += wave_sum((int)(x < kMany ? x : kMany), all.lane);
       total = total < kMany ? total : kMany;
-    }
+      return false;
+    });
     return total;
   };
   const int tiles = sum([](const Request& r) { return (int64_t)r.tiles; });
@@ -264,14 +327,14 @@ template <class T, class P>
 __device__ __forceinline__ bool find_item(const P& p, const int32_t* lengths,
                                           const int32_t* cu, int w, int lane, Item& it,
                                           int* used_chunk = nullptr) {
-  const Request r0 = load_request<T>(p, lengths, cu, lane);
-  const int chunk = p.target > 0 ? best_chunk<T>(p, lengths, cu, r0, lane) : kWhole;
+  const Requests<T, P> all(p, lengths, cu, lane);
+  const int chunk = p.target > 0 ? best_chunk<T>(p, all) : kWhole;
   if (used_chunk) *used_chunk = chunk;
   const int g = (int)((u32)w / (u32)p.heads);
   it.head = w - g * p.heads;
   int items_before = 0;
-  for (int b0 = 0; b0 < requests_of(p); b0 += 64) {
-    const Request r = b0 == 0 ? r0 : load_request<T>(p, lengths, cu, b0 + lane);
+  bool found = false;
+  all.each([&](int b0, const Request& r) {
     const int splits = splits_of(p, r.units, chunk);
     const int items = r.tiles * splits;
     const int items_to = wave_incl_sum(items, lane);
@@ -316,11 +379,13 @@ __device__ __forceinline__ bool find_item(const P& p, const int32_t* lengths,
       it.blk_end = (from + split_bound(units, it.split + 1, it.splits)) * T::UNIT;
       it.blk_end = it.blk_end < end ? it.blk_end : end;
       // (Offsets that fall and rise again make more items than there are places for partials.)
-      return it.split < it.splits && ((it.splits == 1 && !kIsPrefix<P>) || it.slot0 + (it.splits - 1) * it.slot_step < p.work);
+      found = it.split < it.splits && ((it.splits == 1 && !kIsPrefix<P>) || it.slot0 + (it.splits - 1) * it.slot_step < p.work);
+      return true;
     }
     items_before += __builtin_amdgcn_readlane(items_to, 63);
-  }
-  return false;
+    return false;
+  });
+  return found;
 }
 
 // The keys that row R of an item's tile sees.
@@ -801,11 +866,10 @@ __device__ __forceinline__ float softmax_exp_two(const f32x16& s, float m, float
 // The rows of an unsplit tile of a request with a prefix: the four waves' states (cm, cl, co of
 // extend_tile) and the prefix's partials. Threads that rows times dims leave over share a row's partials.
 template <class C>
-__device__ __forceinline__ void finish_shared(const SuffixParams& p, const Item& it, const float* cm, const float* cl,
+__device__ __forceinline__ void finish_shared(const SuffixParams& p, const Item& it, const GroupNote& note, const float* cm, const float* cl,
                                               const float* co, unsigned char* lds, int tid) {
   using E = Elem<C::BF16>;
   constexpr int threads = C::THREADS;
-  const GroupNote note = group_note(p, it.group);
   const int d4n = p.dim / 4, pairs = it.rows * d4n;
   const int share = pairs < threads ? threads / pairs : 1;
   for (int base = 0; base < pairs; base += threads) {
@@ -871,6 +935,9 @@ __device__ __forceinline__ void extend_tile(const P& p, const int32_t* table, co
   const int lane = tid & 63;
   const int il = lane & 31, hh = lane >> 5;
   const Lanes<C> ln(lane);
+  GroupNote note = {};
+  if constexpr (kIsSuffix<P>)
+    if (it.group >= 0) note = group_note(p, it.group);
   constexpr int S = kStages<C::DPAD>;
   unsigned char* const stages = smem + wave * S * C::STAGE_BYTES;
   const u32 stages_lds = lds_address(stages);
@@ -995,7 +1062,7 @@ __device__ __forceinline__ void extend_tile(const P& p, const int32_t* table, co
   using E = Elem<C::BF16>;
   if constexpr (kIsSuffix<P>) {
     if (it.splits == 1 && it.group >= 0) {
-      finish_shared<C>(p, it, cm, cl, co, smem, tid);
+      finish_shared<C>(p, it, note, cm, cl, co, smem, tid);
       return;
     }
   }

@@ -11,8 +11,8 @@ namespace fgw_kv {
   extern template hipError_t launch_extend_long<BF, DP, kRowsBlock, ExtendParams>(const ExtendParams&, int, hipStream_t); \
   extern template hipError_t launch_extend_long<BF, DP, kRowsGroup, ExtendParams>(const ExtendParams&, int, hipStream_t); \
   extern template hipError_t launch_extend_long<BF, DP, kRowsPadded, ExtendParams>(const ExtendParams&, int, hipStream_t);
-extern template hipError_t launch_extend_wide<true, ExtendParams>(const ExtendParams&, int, hipStream_t);
-extern template hipError_t launch_extend_wide<false, ExtendParams>(const ExtendParams&, int, hipStream_t);
+extern template hipError_t launch_extend_wide<true, 256, ExtendParams>(const ExtendParams&, int, hipStream_t);
+extern template hipError_t launch_extend_wide<false, 256, ExtendParams>(const ExtendParams&, int, hipStream_t);
 FGW_KV_EXTERN_LONG(true, 64) FGW_KV_EXTERN_LONG(true, 128)
 FGW_KV_EXTERN_LONG(false, 64) FGW_KV_EXTERN_LONG(false, 128)
 

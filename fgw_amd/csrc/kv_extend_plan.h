@@ -47,7 +47,7 @@ inline ExtendLaunch<P> rows_entry(int dim) {
 // Keys of one DMA instruction: 1024 bytes / (2 * head-dim tile).
 template <bool BF16, class P>
 inline ExtendLaunch<P> long_entry(int dim, int page) {
-  if (dim > 128) return &launch_extend_wide<BF16, P>;
+  if (dim > 128) return &launch_extend_wide<BF16, 256, P>;
   if (dim == 128)
     return page % LongTiling::BN == 0 ? &launch_extend_long<BF16, 128, kRowsBlock, P>
            : page % 4 == 0        ? &launch_extend_long<BF16, 128, kRowsGroup, P>

@@ -104,9 +104,9 @@ __global__ __launch_bounds__(C::THREADS) void extend_wide_kernel(P p, const int3
     store_wave_rows<C>(p, it, wq * C::ROWS_WAVE, smem + wq * 32 * kStagedRowBytes<C>, lane, o, m, l);
 }
 
-template <bool BF16, class P>
+template <bool BF16, int DPAD, class P>
 hipError_t launch_extend_wide(const P& p, int grid, hipStream_t stream) {
-  using C = Cfg<BF16, 256, kLayoutQuery, 0, kDual>;
+  using C = Cfg<BF16, DPAD, kLayoutQuery, 0, kDual>;
   extend_wide_kernel<C, P><<<dim3(grid), dim3(C::THREADS), 0, stream>>>(p, p.table, p.lengths, p.cu);
   return hipGetLastError();
 }

@@ -10,6 +10,15 @@
 //      end and writes the output, a split one's join takes them with its own.
 // A request that does not reach past the prefix with all its new tokens, or is alone in its group, reads
 // all its keys itself in the second pass.
+//
+// Where sharing pays. The passes cost a second launch, and partials of every row and split written and read; what
+// they save is reading: requests of few rows read their keys once for every 32 of them. Requests of more
+// than kShareRows rows are bound by products, of which there are as many either way. Shared / each on its own,
+// us (requests x tokens, Hq 32, Hkv 8, D 128, reads saved): 16x1 prefix 1000 (66 MB) 22.6 / 18.0, 8x1 4000
+// (131 MB) 23.0 / 23.0, 16x1 4000 (262 MB) 23.3 / 34.8, 32x1 8000 (1 GB) 31.9 / 105; 32x32 1000 (0.5 GB) 78 /
+// 56, 4096 (2.1 GB) 118 / 160; 8x64 16000 190 / 148, 8x512 4096 342 / 294. Hence 160 MB, and as much for the
+// partials as 96 bytes for every dim of every row. The device knows the lengths and decides; where the table's
+// capacity rules it out, or tokens and requests do on average, the host leaves the first pass away.
 #include <hip/hip_runtime.h>
 
 #include "kv_extend_plan.h"
@@ -27,18 +36,33 @@ namespace fgw_kv {
   extern template hipError_t launch_extend_long<BF, 128, kRowsBlock, P>(const P&, int, hipStream_t);  \
   extern template hipError_t launch_extend_long<BF, 128, kRowsGroup, P>(const P&, int, hipStream_t);  \
   extern template hipError_t launch_extend_long<BF, 128, kRowsPadded, P>(const P&, int, hipStream_t); \
-  extern template hipError_t launch_extend_wide<BF, P>(const P&, int, hipStream_t);
+  extern template hipError_t launch_extend_wide<BF, 256, P>(const P&, int, hipStream_t);
 FGW_KV_EXTERN(true, PrefixParams) FGW_KV_EXTERN(true, SuffixParams)
 FGW_KV_EXTERN(false, PrefixParams) FGW_KV_EXTERN(false, SuffixParams)
+#define FGW_KV_EXTERN_WIDE(BF, DP) \
+  extern template hipError_t launch_extend_wide<BF, DP, PrefixParams>(const PrefixParams&, int, hipStream_t);
+FGW_KV_EXTERN_WIDE(true, 64) FGW_KV_EXTERN_WIDE(true, 128) FGW_KV_EXTERN_WIDE(false, 64) FGW_KV_EXTERN_WIDE(false, 128)
 
 namespace {
+
+// The kernel of the first pass by the rows of a group: a short tile reads the keys for 32 of them, a wide one
+// for 128, a long one for 256, whose partials are the most. Short / wide / long, us (Hq 32, Hkv 8, D 128): 48
+// rows, four prefixes of 4096 keys 35.2 / 32.8 / -, one of 8192 64 rows 26.8 / 28.0 / -; 128 rows, four of
+// 4096 60.8 / 48.1 / 58.1, 256 rows, one of 8192 - / 48.7 / 54.0, 2048 rows of 4096 keys - / 80.5 / 91.7, 4096 rows
+// - / 111.8 / 109.5.
+constexpr int kWideFrom = 64, kLongPrefixFrom = 2048;
+constexpr int kPrefixMinChunk = 2;  // blocks of 64 keys
+constexpr int64_t kShareBytes = 160 << 20;
+
+enum Tiles { kShort, kWide, kLong };
 
 struct SharedPlan {
   Launch prefix;
   int prefix_rows;  // of a place
-  bool longs;       // long tiles in the first pass
+  Tiles tiles;      // of the first pass
   int64_t notes;    // floats of the groups' notes
   Plan suffix;
+  int share_from;   // SharedParams
 };
 
 template <class T>
@@ -53,18 +77,26 @@ void plan_prefix(SharedPlan& s, const fgw_kv_extend_args& a, int64_t groups) {
   l.floats = l.slots * T::ROWS * (a.dim + 1);
 }
 
-// The kernel of the first pass: long tiles where a group has more than kLongFrom rows on average.
 SharedPlan plan_shared(const fgw_kv_shared_args& args) {
   fgw_kv_extend_args a = args.attend;
   SharedPlan s = {};
   s.suffix = plan(a);
   if (args.groups == 0) return s;
   a.num_cus = std::min(a.num_cus, kMostCus);
-  s.longs = (int64_t)a.tokens * (a.heads / a.kv_heads) > (int64_t)kLongFrom * args.groups;
-  s.prefix.min_chunk = s.longs ? kLongMinChunk : kRowsMinChunk;
-  if (!s.longs)
+  const int64_t total = (int64_t)a.tokens * (a.heads / a.kv_heads);
+  if (!args.always) {
+    const int64_t from = kShareBytes + 96 * (int64_t)a.dim * a.heads * a.tokens;
+    const int64_t requests = std::min(a.batch, a.tokens), key_bytes = 4 * (int64_t)a.kv_heads * shared_dims(a.dim);
+    const double most = (double)(total / 32 + requests) * ((double)a.width * a.page_size) * (double)key_bytes;
+    if (most < (double)from || total > (int64_t)kShareRows * requests) return s;
+    s.share_from = (int)std::min<int64_t>(from >> 16, 1 << 28);
+  }
+  const int64_t rows = total / args.groups;  // of a group, on average
+  s.tiles = rows <= kWideFrom ? kShort : rows <= kLongPrefixFrom || a.dim > 128 ? kWide : kLong;
+  s.prefix.min_chunk = s.tiles == kShort ? kRowsMinChunk : kPrefixMinChunk;
+  if (s.tiles == kShort)
     plan_prefix<ShortTiling>(s, a, args.groups);
-  else if (a.dim > 128)
+  else if (s.tiles == kWide)
     plan_prefix<WideTiling>(s, a, args.groups);
   else
     plan_prefix<LongTiling>(s, a, args.groups);
@@ -88,7 +120,8 @@ int run_shared(const fgw_kv_shared_args& args, const SharedPlan& s, hipStream_t 
   float* work = a.workspace;
   own.groups = args.cu_groups;
   own.prefixes = args.prefix_lens;
-  own.n_groups = args.groups;
+  own.n_groups = s.prefix.items > 0 ? args.groups : 0;
+  own.share_from = s.share_from;
   if (s.prefix.items > 0) {
     PrefixParams p = params_of<PrefixParams>(a);
     static_cast<SharedParams&>(p) = own;
@@ -108,7 +141,11 @@ int run_shared(const fgw_kv_shared_args& args, const SharedPlan& s, hipStream_t 
     own.prefix_slots = p.work;
     own.prefix_rows = s.prefix_rows;
     work = p.parts + s.prefix.floats;
-    const auto entry = s.longs ? long_entry<BF16, PrefixParams>(a.dim, a.page_size) : rows_entry<BF16, PrefixParams>(a.dim);
+    const auto entry = s.tiles == kShort ? rows_entry<BF16, PrefixParams>(a.dim)
+                       : s.tiles == kLong ? long_entry<BF16, PrefixParams>(a.dim, a.page_size)
+                       : a.dim <= 64      ? &launch_extend_wide<BF16, 64, PrefixParams>
+                       : a.dim <= 128     ? &launch_extend_wide<BF16, 128, PrefixParams>
+                                          : &launch_extend_wide<BF16, 256, PrefixParams>;
     const hipError_t e = entry(p, (int)s.prefix.items, stream);
     if (e != hipSuccess) return fail(FGW_MHA_EHIP, "fgw_kv_shared: %s", hipGetErrorString(e));
   }

@@ -9,5 +9,7 @@ template hipError_t launch_extend_long<true, 64, fgw_mha::kRowsPadded, PrefixPar
 template hipError_t launch_extend_long<true, 128, fgw_mha::kRowsBlock, PrefixParams>(const PrefixParams&, int, hipStream_t);
 template hipError_t launch_extend_long<true, 128, fgw_mha::kRowsGroup, PrefixParams>(const PrefixParams&, int, hipStream_t);
 template hipError_t launch_extend_long<true, 128, fgw_mha::kRowsPadded, PrefixParams>(const PrefixParams&, int, hipStream_t);
-template hipError_t launch_extend_wide<true, PrefixParams>(const PrefixParams&, int, hipStream_t);
+template hipError_t launch_extend_wide<true, 64, PrefixParams>(const PrefixParams&, int, hipStream_t);
+template hipError_t launch_extend_wide<true, 128, PrefixParams>(const PrefixParams&, int, hipStream_t);
+template hipError_t launch_extend_wide<true, 256, PrefixParams>(const PrefixParams&, int, hipStream_t);
 }  // namespace fgw_kv

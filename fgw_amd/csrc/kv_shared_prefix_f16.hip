@@ -9,5 +9,7 @@ template hipError_t launch_extend_long<false, 64, fgw_mha::kRowsPadded, PrefixPa
 template hipError_t launch_extend_long<false, 128, fgw_mha::kRowsBlock, PrefixParams>(const PrefixParams&, int, hipStream_t);
 template hipError_t launch_extend_long<false, 128, fgw_mha::kRowsGroup, PrefixParams>(const PrefixParams&, int, hipStream_t);
 template hipError_t launch_extend_long<false, 128, fgw_mha::kRowsPadded, PrefixParams>(const PrefixParams&, int, hipStream_t);
-template hipError_t launch_extend_wide<false, PrefixParams>(const PrefixParams&, int, hipStream_t);
+template hipError_t launch_extend_wide<false, 64, PrefixParams>(const PrefixParams&, int, hipStream_t);
+template hipError_t launch_extend_wide<false, 128, PrefixParams>(const PrefixParams&, int, hipStream_t);
+template hipError_t launch_extend_wide<false, 256, PrefixParams>(const PrefixParams&, int, hipStream_t);
 }  // namespace fgw_kv

@@ -9,5 +9,5 @@ template hipError_t launch_extend_long<true, 64, fgw_mha::kRowsPadded, SuffixPar
 template hipError_t launch_extend_long<true, 128, fgw_mha::kRowsBlock, SuffixParams>(const SuffixParams&, int, hipStream_t);
 template hipError_t launch_extend_long<true, 128, fgw_mha::kRowsGroup, SuffixParams>(const SuffixParams&, int, hipStream_t);
 template hipError_t launch_extend_long<true, 128, fgw_mha::kRowsPadded, SuffixParams>(const SuffixParams&, int, hipStream_t);
-template hipError_t launch_extend_wide<true, SuffixParams>(const SuffixParams&, int, hipStream_t);
+template hipError_t launch_extend_wide<true, 256, SuffixParams>(const SuffixParams&, int, hipStream_t);
 }  // namespace fgw_kv

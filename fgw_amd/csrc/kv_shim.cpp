@@ -483,12 +483,13 @@ PyObject* extend(Args& a) {
   return THPVariable_Wrap(std::move(out));
 }
 
-// (q, k_cache, v_cache, table, lens, cu, cu_groups, prefix_lens, max_new, ... as extend) -> out
+// (q, k_cache, v_cache, table, lens, cu, cu_groups, prefix_lens, always, max_new, ... as extend) -> out
 PyObject* shared(Args& a) {
   Attention x(a);
   const at::Tensor groups = a.tensor(), prefixes = a.tensor();
-  x.parse(a);
   fgw_kv_shared_args r = {};
+  r.always = a.int32();
+  x.parse(a);
   r.cu_groups = metadata(groups, {-1}, x.device);
   need(groups.size(0) > 0, "metadata shape mismatch");
   r.groups = size32(groups.size(0) - 1);

@@ -29,7 +29,8 @@ _kv = _lib.load_kv_module()
 class _SharedKernel:
     """Launch callable of build_shared_kernel."""
 
-    def __init__(self, extend):
+    def __init__(self, extend, always):
+        self.always = always
         self.heads, self.kv_heads, self.dim, self.page_size = (extend.heads, extend.kv_heads, extend.dim,
                                                                extend.page_size)
         self.dtype, self.softmax_scale = extend.dtype, extend.softmax_scale
@@ -40,18 +41,21 @@ class _SharedKernel:
         """O [T, Hq, D] (a new tensor, or `out`, contiguous and apart from all inputs). max_new: as in
         build_extend_kernel's callable."""
         return _kv.shared(q, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens, cu_groups, prefix_lens,
-                          max_new, *self._tail, out)
+                          self.always, max_new, *self._tail, out)
 
 
 @lru_cache(maxsize=128)
-def _planned(extend):
-    return _SharedKernel(extend)
+def _planned(extend, always):
+    return _SharedKernel(extend, always)
 
 
-def build_shared_kernel(heads, kv_heads, dim, page_size, dtype, device_index=None, *, softmax_scale=None):
+def build_shared_kernel(heads, kv_heads, dim, page_size, dtype, device_index=None, *, softmax_scale=None,
+                        always=False):
     """Launch callable of the causal attention of new tokens where requests share prefixes.
 
-    Heads, head dims, types and scale are those of build_extend_kernel. The callable takes (q, k_cache,
+    Heads, head dims, types and scale are those of build_extend_kernel. Sharing takes a second pass: a call
+    whose prefixes are too short for that, by their lengths on the device, or whose requests have too many
+    new tokens each, reads every request's keys itself, unless always is set. The callable takes (q, k_cache,
     v_cache, block_table, cache_seqlens, cu_seqlens, cu_groups, prefix_lens, max_new, out=None), shapes
     free from call to call, and reads nothing back: it can be captured into a HIP graph and replayed after
     lengths, groups and tables were changed in place. What build_extend_kernel says of lengths out of
@@ -59,11 +63,11 @@ def build_shared_kernel(heads, kv_heads, dim, page_size, dtype, device_index=Non
     place of those of a request.
     """
     return _planned(build_extend_kernel(heads, kv_heads, dim, page_size, dtype, device_index,
-                                        softmax_scale=softmax_scale))
+                                        softmax_scale=softmax_scale), bool(always))
 
 
 def mha_paged_shared(q, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens, cu_groups, prefix_lens,
-                     page_size, *, softmax_scale=None, out=None):
+                     page_size, *, softmax_scale=None, always=False, out=None):
     """Attention of new tokens with shared prefixes in one call, with its metadata checked.
 
     As build_shared_kernel's callable, after one copy of lengths and offsets to the host:
@@ -83,7 +87,7 @@ def mha_paged_shared(q, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens
     if q.device.type != "cuda" or any(x.device != q.device for x in (k_cache, v_cache, block_table, *meta)):
         raise ValueError("contiguous inputs on the same GPU required")
     kernel = build_shared_kernel(q.shape[1], k_cache.shape[1], q.shape[2], page_size, q.dtype, q.device.index,
-                                 softmax_scale=softmax_scale)
+                                 softmax_scale=softmax_scale, always=always)
     host = torch.cat(meta).tolist()
     lengths, host = host[:batch], host[batch:]
     cu, host = host[:batch + 1], host[batch + 1:]

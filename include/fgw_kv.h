@@ -136,6 +136,7 @@ typedef struct {
   const int32_t* cu_groups;   /* [groups + 1], device */
   const int32_t* prefix_lens; /* [groups], device */
   int32_t groups;             /* 0: nothing is shared */
+  int32_t always;             /* 0: prefixes are shared where that is faster, by the lengths on the device */
 } fgw_kv_shared_args;
 
 int fgw_kv_shared_workspace(const fgw_kv_shared_args* args, int64_t* floats, int64_t* counters);

@@ -101,9 +101,35 @@ def test_matches_the_64_bit_form(name, dtype):
     cache = _cache(members, prefixes, news, keys, hk, d, page, dtype)
     q = _queries(sum(news), hq, d, dtype)
     print(name, dtype, flush=True)
-    kernel = S.build_shared_kernel(hq, hk, d, page, dtype, 0)
+    kernel = S.build_shared_kernel(hq, hk, d, page, dtype, 0, always=True)
     got = kernel(q.cuda(), *[x.cuda() for x in cache], _offsets(members).cuda(),
                  torch.tensor(prefixes, dtype=torch.int32).cuda(), max(news))
+    _compare(got, q, cache, page, name)
+
+
+# (members, prefixes, new tokens, keys behind, heads, K/V heads, D, page): what is read without sharing, on both
+# sides of the rule.
+SIZES = {
+    "short": ([4], [200], [1] * 4, [1, 2, 3, 4], 8, 2, 128, 16),
+    "long_enough": ([40], [3000], [1] * 40, [1 + i for i in range(40)], 16, 8, 128, 64),
+    "together_long_enough": ([14] * 3, [2900] * 3, [1] * 42, [1 + i for i in range(42)], 8, 8, 128, 16),
+    "too_short_for_the_capacity": ([40], [90], [1] * 40, [1] * 39 + [4000], 16, 8, 128, 64),
+    "many_groups": ([2] * 70, [900] * 70, [1] * 140, [1 + i % 9 for i in range(140)], 8, 8, 64, 16),
+    "many_groups_long_enough": ([2] * 70, [1900] * 70, [1] * 140, [1 + i % 9 for i in range(140)], 8, 8, 64, 64),
+    "many_rows": ([3], [1500], [200, 190, 180], [200, 190, 180], 4, 1, 128, 64),
+    "many_rows_in_one_group": ([2, 40], [1500, 3000], [150, 140] + [1] * 40, [150, 140] + [1] * 40, 8, 8, 128, 64),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", SIZES)
+def test_shared_where_that_is_faster_gives_the_same(name):
+    members, prefixes, news, keys, hq, hk, d, page = SIZES[name]
+    cache = _cache(members, prefixes, news, keys, hk, d, page, torch.bfloat16)
+    q = _queries(sum(news), hq, d, torch.bfloat16)
+    print(name, flush=True)
+    got = S.build_shared_kernel(hq, hk, d, page, "bfloat16", 0)(
+        q.cuda(), *[x.cuda() for x in cache], _offsets(members).cuda(), torch.tensor(prefixes, dtype=torch.int32).cuda(), max(news))
     _compare(got, q, cache, page, name)
 
 
@@ -114,7 +140,7 @@ def test_the_prefix_is_read_through_the_first_request():
     q = _queries(4, 8, 128, torch.bfloat16)
     broken = [x.clone() for x in cache]
     broken[2][1:, :20] = -1
-    kernel = S.build_shared_kernel(8, 2, 128, 16, "bfloat16", 0)
+    kernel = S.build_shared_kernel(8, 2, 128, 16, "bfloat16", 0, always=True)
     got = kernel(q.cuda(), *[x.cuda() for x in broken], _offsets([4]).cuda(), torch.tensor([320], dtype=torch.int32).cuda(), 1)
     _compare(got, q, cache, 16, "first row")
 
@@ -126,7 +152,7 @@ def test_prefixes_that_not_every_request_reaches(prefix):
     members, news, keys = [4], [2, 1, 60, 3], [30, 1, 70, -20]
     cache = _cache(members, [100], news, keys, 2, 64, 16, torch.float16)
     q = _queries(sum(news), 8, 64, torch.float16)
-    kernel = S.build_shared_kernel(8, 2, 64, 16, "float16", 0)
+    kernel = S.build_shared_kernel(8, 2, 64, 16, "float16", 0, always=True)
     got = kernel(q.cuda(), *[x.cuda() for x in cache], _offsets(members).cuda(),
                  torch.tensor([prefix], dtype=torch.int32).cuda(), max(news))
     _compare(got, q, cache, 16, prefix)
@@ -137,7 +163,7 @@ def test_a_first_request_that_ends_early_shares_less():
     """The first request has 37 keys before its token: the others share those alone."""
     cache = _cache([3], [37], [1, 1, 1], [1, 80, 200], 2, 128, 16, torch.bfloat16)
     q = _queries(3, 8, 128, torch.bfloat16)
-    kernel = S.build_shared_kernel(8, 2, 128, 16, "bfloat16", 0)
+    kernel = S.build_shared_kernel(8, 2, 128, 16, "bfloat16", 0, always=True)
     got = kernel(q.cuda(), *[x.cuda() for x in cache], _offsets([3]).cuda(), torch.tensor([64], dtype=torch.int32).cuda(), 1)
     _compare(got, q, cache, 16, "early")
 
@@ -148,7 +174,7 @@ def test_offsets_of_groups_that_say_nothing():
     cache = _cache([2], [90], [1, 2], [5, 6], 2, 64, 16, torch.bfloat16)
     dev = [x.cuda() for x in cache]
     q = _queries(3, 4, 64, torch.bfloat16)
-    kernel = S.build_shared_kernel(4, 2, 64, 16, "bfloat16", 0)
+    kernel = S.build_shared_kernel(4, 2, 64, 16, "bfloat16", 0, always=True)
     for first, prefixes in (([0], []), ([0, 3], [90]), ([2, 0], [90]), ([-1, 2], [90]), ([0, 0, 0], [90, 90]), ([0, 1, 2], [90, 90])):
         print(first, flush=True)
         got = kernel(q.cuda(), *dev, torch.tensor(first, dtype=torch.int32).cuda(),
@@ -163,7 +189,7 @@ def test_rows_behind_the_last_request_are_left_and_strides_are_taken():
     fused[4:] = math.nan
     q = fused.cuda()[:, 2:10]
     out = torch.full((7, 8, 128), 7.0, dtype=torch.bfloat16, device="cuda")
-    kernel = S.build_shared_kernel(8, 2, 128, 16, "bfloat16", 0, softmax_scale=0.25)
+    kernel = S.build_shared_kernel(8, 2, 128, 16, "bfloat16", 0, softmax_scale=0.25, always=True)
     got = kernel(q, *[x.cuda() for x in cache], _offsets([3]).cuda(), torch.tensor([200], dtype=torch.int32).cuda(), 2, out)
     assert got.data_ptr() == out.data_ptr() and bool((out[4:] == 7.0).all())
     _compare(out, fused[:4, 2:10], cache, 16, "padded", scale=0.25)
@@ -174,7 +200,7 @@ def test_pages_outside_the_pool_read_as_zeros():
     k, v, table, lens, cu = _cache([2], [128], [1, 1], [40, 9], 2, 64, 16, torch.bfloat16)
     table[:, 3], table[0, 9] = -1, 10**6
     q = _queries(2, 4, 64, torch.bfloat16)
-    kernel = S.build_shared_kernel(4, 2, 64, 16, "bfloat16", 0)
+    kernel = S.build_shared_kernel(4, 2, 64, 16, "bfloat16", 0, always=True)
     got = kernel(q.cuda(), *[x.cuda() for x in (k, v, table, lens, cu)], _offsets([2]).cuda(),
                  torch.tensor([128], dtype=torch.int32).cuda(), 1)
     _compare(got, q, (k, v, table, lens, cu), 16, "outside")
@@ -188,7 +214,7 @@ def test_nan_of_a_key_reaches_the_rows_that_see_it():
         pos, b = (130, 0) if where == "prefix" else (310, 1)
         k[int(table[b, pos // 16]) * 16 + pos % 16, 0, 5] = math.nan
         q = _queries(3, 4, 128, torch.bfloat16)
-        kernel = S.build_shared_kernel(4, 2, 128, 16, "bfloat16", 0)
+        kernel = S.build_shared_kernel(4, 2, 128, 16, "bfloat16", 0, always=True)
         got = kernel(q.cuda(), *[x.cuda() for x in (k, v, table, lens, cu)], _offsets([3]).cuda(),
                      torch.tensor([300], dtype=torch.int32).cuda(), 1)
         bad = torch.isnan(got).all(-1).cpu()
@@ -204,7 +230,7 @@ def test_captured_and_replayed_after_groups_changed():
     layouts = [([4, 4], [500, 90], [1] * 8, [1, 2, 70, 4, 300, 6, 7, 8]),
                ([6, 2], [300, 200], [1] * 8, [9, 8, 7, 6, 5, 4, 3, 200]),
                ([1, 7], [30, 450], [1] * 8, [1, 1, 1, 1, 60, 61, 62, 63])]
-    kernel = S.build_shared_kernel(hq, hk, d, page, "bfloat16", 0)
+    kernel = S.build_shared_kernel(hq, hk, d, page, "bfloat16", 0, always=True)
     caches = [_cache(*x, hk, d, page, torch.bfloat16, seed=i) for i, x in enumerate(layouts)]
     width = max(c[2].shape[1] for c in caches)
     rows = max(c[0].shape[0] for c in caches)
@@ -242,7 +268,7 @@ def test_two_calls_at_once_on_two_streams():
     cache = _cache([6], [3000], [1] * 6, [1 + 40 * i for i in range(6)], 1, 128, 16, torch.bfloat16)
     dev = [x.cuda() for x in cache]
     meta = [_offsets([6]).cuda(), torch.tensor([3000], dtype=torch.int32).cuda()]
-    kernel = S.build_shared_kernel(8, 1, 128, 16, "bfloat16", 0)
+    kernel = S.build_shared_kernel(8, 1, 128, 16, "bfloat16", 0, always=True)
     qs = [_queries(6, 8, 128, torch.bfloat16, seed=s) for s in (1, 2)]
     qd = [x.cuda() for x in qs]
     streams = [torch.cuda.Stream() for _ in qs]
@@ -262,7 +288,7 @@ def test_one_call_checks_its_metadata():
     cache = [x.cuda() for x in _cache([2], [40], [1, 1], [3, 9], 2, 64, 16, torch.bfloat16)]
     q = _queries(2, 4, 64, torch.bfloat16)
     groups, prefixes = _offsets([2]).cuda(), torch.tensor([40], dtype=torch.int32).cuda()
-    got = S.mha_paged_shared(q.cuda(), *cache, groups, prefixes, 16)
+    got = S.mha_paged_shared(q.cuda(), *cache, groups, prefixes, 16, always=True)
     _compare(got, q, [x.cpu() for x in cache], 16, "one call")
     k, v, table, lens, cu = cache
 
@@ -287,7 +313,7 @@ def test_tensor_refusals():
     k, v, table, lens, cu = cache
     q = _queries(2, 4, 64, torch.bfloat16).cuda()
     groups, prefixes = _offsets([2]).cuda(), torch.tensor([40], dtype=torch.int32).cuda()
-    kernel = S.build_shared_kernel(4, 2, 64, 16, "bfloat16", 0)
+    kernel = S.build_shared_kernel(4, 2, 64, 16, "bfloat16", 0, always=True)
     whole = torch.zeros(2 * 4 * 64 + 16, dtype=torch.bfloat16, device="cuda")
     out, inside = whole[:512].view(2, 4, 64), whole[508:512].view(torch.int32)[:1]
     for args, message in [
@@ -328,15 +354,15 @@ class _Extend(ctypes.Structure):
 
 class _Shared(ctypes.Structure):
     _fields_ = [("attend", _Extend), ("cu_groups", ctypes.c_void_p), ("prefix_lens", ctypes.c_void_p),
-                ("groups", ctypes.c_int32)]
+                ("groups", ctypes.c_int32), ("always", ctypes.c_int32)]
 
 
-def _args(groups=1, **changes):
+def _args(groups=1, always=1, **changes):
     a = _Extend(pool_rows=1024, tokens=4, batch=2, heads=8, kv_heads=2, dim=64, width=8, page_size=16, max_new=3,
                 causal=1, window=0, dtype=1, num_cus=256, scale=0.125)
     for name, value in changes.items():
         setattr(a, name, value)
-    return _Shared(attend=a, groups=groups)
+    return _Shared(attend=a, groups=groups, always=always)
 
 
 @pytest.mark.parametrize("changes,message", [
@@ -361,6 +387,7 @@ def test_workspace_is_bounded_by_the_sizes():
 
     assert need(tokens=0) == 0
     assert need(groups=0) == 0
+    assert need(always=0) == 0    # 128 keys of two requests: nothing to save, each reads its own
     assert 0 < need() < 1 << 20
     # 512 rows of K/V head 0 .. 7 and as many splits as fill the card: below 64 MB.
     assert need(width=4096, tokens=64, batch=64, heads=64, kv_heads=8, dim=128, max_new=1) < 16 << 20
