@@ -22,19 +22,23 @@ struct Books {
 };
 
 // Exclusive sum over the workgroup, and the total in every thread. Two barriers.
+template <int THREADS = kPlanThreads>
 __device__ __forceinline__ int block_scan(int x, int* lds, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // By DPP within rows of 16 lanes (shifts by 1, 2, 4, 8), then each row's last lane onto those behind it.
   int incl = x;
-  for (int off = 1; off < 64; off <<= 1) {
-    const int up = __shfl_up(incl, off, 64);
-    incl += lane >= off ? up : 0;
-  }
+  incl += __builtin_amdgcn_update_dpp(0, incl, 0x111, 0xf, 0xf, false);
+  incl += __builtin_amdgcn_update_dpp(0, incl, 0x112, 0xf, 0xf, false);
+  incl += __builtin_amdgcn_update_dpp(0, incl, 0x114, 0xf, 0xf, false);
+  incl += __builtin_amdgcn_update_dpp(0, incl, 0x118, 0xf, 0xf, false);
+  const int r0 = __builtin_amdgcn_readlane(incl, 15), r1 = __builtin_amdgcn_readlane(incl, 31), r2 = __builtin_amdgcn_readlane(incl, 47);
+  incl += (lane >= 16 ? r0 : 0) + (lane >= 32 ? r1 : 0) + (lane >= 48 ? r2 : 0);
   __syncthreads();  // lds of the scan before is no longer read
   if (lane == 63) lds[wave] = incl;
   __syncthreads();
   int before = 0;
   total = 0;
-  for (int w = 0; w < kPlanWaves; ++w) {
+  for (int w = 0; w < THREADS / 64; ++w) {
     before += w < wave ? lds[w] : 0;
     total += lds[w];
   }
@@ -63,12 +67,14 @@ __device__ __forceinline__ u32 page_bits(int pages, int base) {  // pages that e
 }
 
 // The free pages in order of id, up to `want`: list[0 .. want); returns how many there are of them.
-__device__ __forceinline__ int rank_free(const Books& b, int want, int32_t* list, int* lds) {
+// `first`: held_bits at page 0, if the caller has read them ahead.
+template <int THREADS = kPlanThreads>
+__device__ __forceinline__ int rank_free(const Books& b, int want, int32_t* list, int* lds, const u32* first = nullptr) {
   int found = 0;
-  for (int base = 0; base < b.pages && found < want; base += kSlab) {
-    u32 free = ~held_bits(b.refs, b.pages, base) & page_bits(b.pages, base);
+  for (int base = 0; base < b.pages && found < want; base += THREADS * kSlabPer) {
+    u32 free = ~(first && base == 0 ? *first : held_bits(b.refs, b.pages, base)) & page_bits(b.pages, base);
     int total;
-    int rank = found + block_scan(__popc(free), lds, total);
+    int rank = found + block_scan<THREADS>(__popc(free), lds, total);
     for (; free && rank < want; free &= free - 1u, ++rank)
       list[rank] = base + (int)threadIdx.x * kSlabPer + __ffs(free) - 1;
     found += total;

@@ -29,12 +29,15 @@ typedef u32 u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxLayers = 16;           // of one pair of launches
 constexpr int kPer = 16;                 // sums of a thread in registers
-constexpr int kHeld = kPlanThreads * kPer;
-constexpr int kBins = 2048;
+constexpr int kFewThreads = 256;         // of a program where capacities fit its registers; else kPlanThreads
+constexpr int kBins = 2048, kCopies = 4;
+constexpr int kDirect = 256;             // keys that are compared with each other
 constexpr int kMoveThreads = 256;
-constexpr int kMoveLoads = 2;            // 16-byte chunks of a thread
-constexpr int kMovers = 8192;            // workgroups of a launch that count their work on the device
+constexpr int kMoveLoads = 8;            // 16-byte chunks of a thread at once
+constexpr int kMovers = 4096;            // workgroups of a launch that count their work on the device
 constexpr int kSumLoads = 8;
+constexpr int kLeastPart = 4, kMostPart = 32;  // tokens of a part
+constexpr int kSpread = 2048;            // parts that all rows at their capacity make, or more
 
 struct Layers {
   const float* scores[kMaxLayers];
@@ -42,13 +45,16 @@ struct Layers {
   int32_t head_bytes[2 * kMaxLayers];
 };
 
-// What the plan leaves: rows that shrink, in order, with the work of each; their old lengths and tables.
+// A row that shrinks: its number, old length, budget, and where its fresh pages begin in the list.
+struct Shrunk {
+  int32_t row, len, keep, place;
+};
+// What the plan leaves.
 struct EvictPlan {
-  int32_t* count;    // rows that shrink
-  int32_t* active;   // [rows] which
-  int32_t* base;     // [rows + 1] parts of tokens before, by place in `active`
-  int32_t* place;    // [rows] of a row's fresh pages in the list
-  int32_t* old_len;  // [rows]
+  Shrunk* rows;      // [rows], in order
+  int32_t* count;    // of them
+  int32_t* base;     // [rows + 1] parts of tokens before each, and all parts
+  int32_t* need;     // [rows] of rows past the first THREADS
   int32_t* list;     // fresh pages
   int32_t* table;    // [rows, width] as it was
   int32_t* kept;     // [layers, rows, heads, capacity] positions
@@ -57,81 +63,85 @@ struct EvictPlan {
 struct EvictArgs {
   Books b;
   const int32_t* keep;
-  int32_t first, recent, heads, layers, tokens_part;
-  int64_t stride;  // of a head's sums
+  int32_t first, recent, heads, layers, part;  // tokens of a part
+  int64_t stride;                              // of a head's sums
   int64_t capacity;
   EvictPlan plan;
 };
 
 // Whether row r shrinks, if pages are left; `bad`: its count is below what has to stay.
-__device__ __forceinline__ bool shrinks(const EvictArgs& a, int r, int& len, int& keep, bool& bad) {
-  len = clamp_len(a.b, a.b.lens[r]);
-  keep = a.keep[r];
+__device__ __forceinline__ bool shrinks(const EvictArgs& a, int length, int keep, int& len, bool& bad) {
+  len = clamp_len(a.b, length);
   const bool wanted = keep >= 0 && keep < len;
   bad = wanted && (int64_t)a.first + a.recent > keep;
   return wanted && !bad;
 }
 
+// Free pages to rows in order, as a reservation does. What a thread knows of its first row stays with it: the
+// plan is bound by its round trips to memory.
+template <int THREADS>
 __device__ __forceinline__ void plan_rows(const EvictArgs& a, int32_t* status) {
-  __shared__ int lds[kPlanWaves];
-  __shared__ int short_rows, bad_rows;
+  __shared__ int lds[THREADS / 64];
+  __shared__ int short_rows, bad_rows, given;
   const Books& b = a.b;
-  if (threadIdx.x == 0) short_rows = bad_rows = 0;
-  const int still = a.first / b.page;
-  int want = 0;
-  for (int base = 0; base < b.rows; base += kPlanThreads) {
-    const int r = base + (int)threadIdx.x;
-    int len = 0, keep = 0;
-    bool bad = false;
-    const bool ok = r < b.rows && shrinks(a, r, len, keep, bad);
-    const int need = ok ? (int)(((int64_t)keep + b.page - 1) / b.page) - still : 0;
+  const int tid = threadIdx.x, still = a.first / b.page;
+  if (tid == 0) short_rows = bad_rows = given = 0;
+  struct Row {
+    int len, keep, need;  // need -1: the row stays
+  };
+  auto load = [&](int r) {
+    Row x{0, -1, -1};
+    if (r >= b.rows) return x;
+    x.keep = a.keep[r];
+    bool bad;
+    if (shrinks(a, b.lens[r], x.keep, x.len, bad)) x.need = (int)(((int64_t)x.keep + b.page - 1) / b.page) - still;
+    return x;
+  };
+  const u32 held = held_bits(b.refs, b.pages, 0);  // (beside the lengths)
+  const Row mine = load(tid);
+  __syncthreads();
+  int want = 0, at0 = 0;
+  for (int base = 0; base < b.rows; base += THREADS) {
+    const Row x = base == 0 ? mine : load(base + tid);
     int total;
-    const int before = want + block_scan(need > b.pages ? b.pages + 1 : need, lds, total);
-    if (r < b.rows) {
-      a.plan.place[r] = before;
-      a.plan.old_len[r] = ok ? len : -1;
-    }
-    if (bad) atomicAdd(&bad_rows, 1);
+    const int need = x.need < 0 ? 0 : (x.need > b.pages ? b.pages + 1 : x.need);
+    const int before = want + block_scan<THREADS>(need, lds, total);
+    if (base == 0)
+      at0 = before;
+    else if (base + tid < b.rows)
+      a.plan.need[base + tid] = before;
     want = want + total > b.pages ? b.pages + 1 : want + total;
   }
-  const int found = rank_free(b, want < b.pages ? want : b.pages, a.plan.list, lds);
+  const int found = rank_free<THREADS>(b, want < b.pages ? want : b.pages, a.plan.list, lds, &held);
   int count = 0, parts = 0;
-  for (int base = 0; base < b.rows; base += kPlanThreads) {
-    const int r = base + (int)threadIdx.x;
-    bool go = false;
-    int part = 0;
-    if (r < b.rows && a.plan.old_len[r] >= 0) {
-      const int keep = a.keep[r], at = a.plan.place[r];
-      const int need = (int)(((int64_t)keep + b.page - 1) / b.page) - still;
-      go = need <= 0 || (at <= found && need <= found - at);
-      if (!go) atomicAdd(&short_rows, 1);
-      part = go ? (keep - still * b.page + a.tokens_part - 1) / a.tokens_part : 0;
-    }
+  for (int base = 0; base < b.rows; base += THREADS) {
+    const int r = base + tid;
+    const Row x = base == 0 ? mine : load(r);
+    const int at = base == 0 ? at0 : (r < b.rows ? a.plan.need[r] : 0);
+    const bool go = x.need == 0 || (x.need > 0 && at <= found && x.need <= found - at);
+    if (x.need < 0 && x.keep >= 0 && x.keep < x.len) atomicAdd(&bad_rows, 1);  // (it is below what has to stay)
+    if (x.need > 0 && !go) atomicAdd(&short_rows, 1);
+    if (x.need > 0 && go) atomicMax(&given, at + x.need);
+    const int part = go ? (x.keep - still * b.page + a.part - 1) / a.part : 0;
     int rows_here, parts_here;
-    const int rank = count + block_scan(go ? 1 : 0, lds, rows_here);
-    const int before = parts + block_scan(part, lds, parts_here);
+    const int rank = count + block_scan<THREADS>(go ? 1 : 0, lds, rows_here);
+    const int before = parts + block_scan<THREADS>(part, lds, parts_here);
     if (go) {
-      a.plan.active[rank] = r;
+      a.plan.rows[rank] = Shrunk{r, x.len, x.keep, at};
       a.plan.base[rank] = before;
     }
     count += rows_here;
     parts += parts_here;
   }
-  // Fresh pages that no refused row stands in front of: held from now on.
+  // (Rows in order: the pages that are given are the first ones of the list.)
   __threadfence_block();
   __syncthreads();
-  for (int i = threadIdx.x; i < count; i += kPlanThreads) {
-    const int r = a.plan.active[i], at = a.plan.place[r];
-    const int need = (int)(((int64_t)a.keep[r] + b.page - 1) / b.page) - still;
-    for (int k = 0; k < need; ++k) b.refs[a.plan.list[at + k]] = 1;
-  }
-  if (threadIdx.x == 0) {
+  for (int i = tid; i < given; i += THREADS) b.refs[a.plan.list[i]] = 1;
+  if (tid == 0) {
     *a.plan.count = count;
     a.plan.base[count] = parts;
-    if (status) {
-      status[0] = short_rows;
-      status[1] = bad_rows;
-    }
+    status[0] = short_rows;
+    status[1] = bad_rows;
   }
 }
 
@@ -142,89 +152,144 @@ __device__ __forceinline__ u32 sort_key(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// blockIdx.x 0: the plan (status: in the call's first launch; else none). Others: one (layer, row, head).
-__global__ __launch_bounds__(kPlanThreads) void evict_select_kernel(EvictArgs a, Layers layers, int32_t* status, int plan) {
-  __shared__ int lds[kPlanWaves], bins[kBins], picked[2];
-  __shared__ int counts[kPer * kPlanWaves];
+// blockIdx.x 0: the plan (in the call's first launch). Others: one (layer, row, head).
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictArgs a, Layers layers, int32_t* status, int plan) {
+  constexpr int kWaves = THREADS / 64, kHeld = THREADS * kPer;
+  __shared__ __attribute__((aligned(16))) int bins[kBins * kCopies];
+  __shared__ __attribute__((aligned(16))) u32 few[kDirect];
+  __shared__ int lds[kWaves], picked[3], counts[kPer * kWaves], few_count;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (blockIdx.x == 0) {
-    if (plan) plan_rows(a, status);
+    if (plan) plan_rows<THREADS>(a, status);
     return;
   }
   const int w = (int)blockIdx.x - 1, head = w % a.heads, rest = w / a.heads, r = rest % a.b.rows, layer = rest / a.b.rows;
-  int len, keep;
+  const float* const x = layers.scores[layer] + ((int64_t)r * a.heads + head) * a.stride + a.first;
+  const int most = a.capacity > a.first ? (int)a.capacity - a.first : 0;  // sums that there are from `first` on
+  const int length = a.b.lens[r], keep = a.keep[r];
+  float raw[kPer];
+  auto read = [&](int base) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int i = base + k * THREADS + tid;
+      raw[k] = i < most ? x[i] : 0.0f;
+    }
+  };
+  if (most <= kHeld) read(0);  // (on the way beside the length)
+  int len;
   bool bad;
-  if (!shrinks(a, r, len, keep, bad)) return;
+  if (!shrinks(a, length, keep, len, bad)) return;
   if (plan && layer == 0 && head == 0) {
     const int live = (int)(((int64_t)len + a.b.page - 1) / a.b.page);
-    for (int j = tid; j < live; j += kPlanThreads) a.plan.table[(int64_t)r * a.b.width + j] = a.b.table[(int64_t)r * a.b.width + j];
+    for (int j = tid; j < live; j += THREADS) a.plan.table[(int64_t)r * a.b.width + j] = a.b.table[(int64_t)r * a.b.width + j];
   }
   const int n = len - a.first - a.recent, want = keep - a.first - a.recent;
-  const float* const x = layers.scores[layer] + ((int64_t)r * a.heads + head) * a.stride + a.first;
   int32_t* const kept = a.plan.kept + (((int64_t)layer * a.b.rows + r) * a.heads + head) * a.capacity + a.first;
   if (want == 0) return;
   u32 held[kPer];
   auto load = [&](int base) {
+    if (most > kHeld) read(base);
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int i = base + k * kPlanThreads + tid;
-      held[k] = i < n ? sort_key(x[i]) : 0u;  // (no sum's key is 0: that of minus infinity is 0x007fffff)
-    }
+    for (int k = 0; k < kPer; ++k)
+      held[k] = base + k * THREADS + tid < n ? sort_key(raw[k]) : 0u;  // (no sum's key is 0: that of minus infinity is 0x007fffff)
   };
-  // The digits of the want-th largest key, from the top.
+  // The digits of the want-th largest key, from the top, until the keys that share them are few: those are
+  // compared with each other. Equal sums meet in one bin: lanes take turns at its
+  // kCopies counters, which lie in different banks.
   u32 prefix = 0;
   int left = want;
-  if (n <= kHeld) load(0);
-  constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
-#pragma unroll
-  for (int pass = 0; pass < 3; ++pass) {
-    for (int i = tid; i < kBins; i += kPlanThreads) bins[i] = 0;
+  const int steps = (n + THREADS - 1) / THREADS < kPer ? (n + THREADS - 1) / THREADS : kPer;
+  if (most <= kHeld) load(0);
+  bool done = false;
+  for (int pass = 0; pass < 3 && !done; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    for (int i = tid; i < kBins * kCopies / 4; i += THREADS) reinterpret_cast<int4*>(bins)[i] = int4{0, 0, 0, 0};
     __syncthreads();
     for (int base = 0; base < n; base += kHeld) {
-      if (n > kHeld) load(base);
+      if (most > kHeld) load(base);
 #pragma unroll
       for (int k = 0; k < kPer; ++k) {
-        const bool in = held[k] != 0u && (pass == 0 || held[k] >> (kShift[pass] + kBits[pass]) == prefix);
-        if (in) atomicAdd(&bins[held[k] >> kShift[pass] & ((1u << kBits[pass]) - 1u)], 1);
+        const bool in = k < steps && held[k] != 0u && (pass == 0 || held[k] >> (shift + bits) == prefix);
+        if (in) atomicAdd(&bins[(held[k] >> shift & ((1u << bits) - 1u)) * kCopies + (lane & (kCopies - 1))], 1);
       }
     }
     __syncthreads();
-    const int hi = bins[kBins - 1 - 2 * tid], lo = bins[kBins - 2 - 2 * tid];
+    // Each thread has kBins / THREADS bins, from the highest down.
+    constexpr int kMine = kBins / THREADS;
+    int mine[kMine], sum = 0;
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      const int4 c = reinterpret_cast<const int4*>(bins)[kBins - 1 - (kMine * tid + k)];
+      mine[k] = c.x + c.y + c.z + c.w;
+      sum += mine[k];
+    }
     int total;
-    const int before = block_scan(hi + lo, lds, total);
-    if (before < left && left <= before + hi + lo) {
-      const bool upper = left <= before + hi;
-      picked[0] = kBins - (upper ? 1 : 2) - 2 * tid;
-      picked[1] = left - before - (upper ? 0 : hi);
+    int before = block_scan<THREADS>(sum, lds, total);
+    if (before < left && left <= before + sum) {
+#pragma unroll
+      for (int k = 0; k < kMine; ++k) {
+        if (before < left && left <= before + mine[k]) {
+          picked[0] = kBins - 1 - (kMine * tid + k);
+          picked[1] = left - before;
+          picked[2] = mine[k];
+        }
+        before += mine[k];
+      }
     }
     __syncthreads();
-    prefix = prefix << kBits[pass] | (u32)picked[0];
+    prefix = prefix << bits | (u32)picked[0];
+    left = picked[1];
+    const int share = picked[2];
+    if (pass == 2 || share > kDirect || most > kHeld) continue;
+    done = true;
+    if (tid == 0) few_count = 0;
+    for (int i = tid; i < kDirect; i += THREADS) few[i] = 0u;  // (below every key)
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      if (held[k] != 0u && held[k] >> shift == prefix) few[atomicAdd(&few_count, 1)] = held[k];
+    __syncthreads();
+    const u32 own = tid < kDirect ? few[tid] : 0u;
+    int above = 0, equal = 0;
+    for (int i = 0; i < share; i += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(few + i);
+      above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
+      equal += (o.x == own) + (o.y == own) + (o.z == own) + (o.w == own);
+    }
+    if (own != 0u && above < left && left <= above + equal) {  // (all equal ones write the same)
+      picked[0] = (int)own;
+      picked[1] = left - above;
+    }
+    __syncthreads();
+    prefix = (u32)picked[0];
     left = picked[1];
   }
   // All keys above `prefix` and the first `left` of those that equal it, by position.
   int above_before = 0, equal_before = 0;
   for (int base = 0; base < n; base += kHeld) {
-    if (n > kHeld) load(base);
+    if (most > kHeld) load(base);
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
       const int above = __popcll(__ballot(held[k] > prefix)), equal = __popcll(__ballot(held[k] == prefix));
-      if (lane == 0) counts[k * kPlanWaves + wave] = above | equal << 16;
+      if (lane == 0) counts[k * kWaves + wave] = above | equal << 16;
     }
     __syncthreads();
     int total;
-    const int mine = tid < kPer * kPlanWaves ? counts[tid] : 0;
-    const int sum = block_scan(mine, lds, total);  // (at most 16384 of each kind: no carry from the low half)
-    if (tid < kPer * kPlanWaves) counts[tid] = sum;
+    const int mine = tid < kPer * kWaves ? counts[tid] : 0;
+    const int sum = block_scan<THREADS>(mine, lds, total);  // (at most 16384 of each kind: no carry from the low half)
+    if (tid < kPer * kWaves) counts[tid] = sum;
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
+      if (k >= steps) continue;
       const bool above = held[k] > prefix, equal = held[k] == prefix;
       const uint64_t below = (1ull << lane) - 1ull;
-      const int c = counts[k * kPlanWaves + wave];
+      const int c = counts[k * kWaves + wave];
       const int na = above_before + (c & 0xffff) + __popcll(__ballot(above) & below);
       const int ne = equal_before + (c >> 16) + __popcll(__ballot(equal) & below);
-      if (above || (equal && ne < left)) kept[na + (ne < left ? ne : left)] = a.first + base + k * kPlanThreads + tid;
+      if (above || (equal && ne < left)) kept[na + (ne < left ? ne : left)] = a.first + base + k * THREADS + tid;
     }
     above_before += total & 0xffff;
     equal_before += total >> 16;
@@ -236,16 +301,16 @@ __device__ __forceinline__ int source(const EvictArgs& a, const int32_t* kept, i
   return d < a.first ? d : d >= keep - a.recent ? d + (len - keep) : kept[d];
 }
 
-// blockIdx.y < 2 layers: K or V of a layer, blockIdx.x over parts of tokens; < 3 layers: a layer's sums, over
-// (row, head); then the books, over rows.
+// blockIdx.y < layers: K and V of a layer, blockIdx.x over parts of tokens; < 2 layers: a layer's sums, over
+// (row, head); then the books, over rows. A part: each thread finds the pool rows of one (token, head), then
+// all copy, 16 bytes to a lane, whole tokens written.
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, Layers layers) {
+  __shared__ int64_t from_row[kMoveThreads], to_row[kMoveThreads];  // of a (token, head), of a token
   const Books& b = a.b;
   const int tid = threadIdx.x, lane = tid & 63, count = *a.plan.count, page = b.page, still = a.first / page;
   const int y = (int)blockIdx.y;
-  if (y < 2 * a.layers) {
-    const int head_bytes = layers.head_bytes[y], token_bytes = a.heads * head_bytes, layer = y < a.layers ? y : y - a.layers;
-    char* const pool = layers.data[y];
-    const int chunks = head_bytes / 16, per_token = token_bytes / 16, parts = a.plan.base[count];
+  if (y < a.layers) {
+    const int parts = a.plan.base[count];
     for (int w = blockIdx.x; w < parts; w += gridDim.x) {
       // The row: the last one whose parts begin at w or before.
       int at = 0;
@@ -255,52 +320,66 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, L
         if (n > 0) at = base + n - 1;
         if (n < 64) break;
       }
-      const int r = a.plan.active[at], len = a.plan.old_len[r], keep = a.keep[r];
-      const int d0 = still * page + (w - a.plan.base[at]) * a.tokens_part;
-      const int tokens = keep - d0 < a.tokens_part ? keep - d0 : a.tokens_part;
-      const int32_t* const old_table = a.plan.table + (int64_t)r * b.width;
-      const int32_t* const fresh = a.plan.list + a.plan.place[r];
-      const int32_t* const kept = a.plan.kept + ((int64_t)layer * b.rows + r) * a.heads * a.capacity;
-      for (int u0 = 0; u0 < tokens * per_token; u0 += kMoveThreads * kMoveLoads) {
-        u32x4 x[kMoveLoads];
-        char* to[kMoveLoads];
-#pragma unroll
-        for (int k = 0; k < kMoveLoads; ++k) {
-          const int u = u0 + k * kMoveThreads + tid;
-          to[k] = nullptr;
-          if (u < tokens * per_token) {
-            const int t = (int)((u32)u / (u32)per_token), in_token = u - t * per_token;
-            const int head = (int)((u32)in_token / (u32)chunks), d = d0 + t;
-            const int s = source(a, kept + (int64_t)head * a.capacity, d, keep, len);
-            const int sp = (int)((u32)s / (u32)page), dp = (int)((u32)d / (u32)page);
-            const int from = old_table[sp], into = fresh[dp - still];
-            if (from >= 0 && from < b.pages) {
-              const int64_t row = (int64_t)from * page + (s - sp * page), dst = (int64_t)into * page + (d - dp * page);
-              x[k] = *reinterpret_cast<const u32x4*>(pool + row * token_bytes + in_token * 16);
-              to[k] = pool + dst * token_bytes + in_token * 16;
-            }
+      const Shrunk row = a.plan.rows[at];
+      const int d0 = still * page + (w - a.plan.base[at]) * a.part, tokens = row.keep - d0 < a.part ? row.keep - d0 : a.part;
+      __syncthreads();  // the part before is copied
+      {
+        const int head = (int)((u32)tid / (u32)a.part), t = tid - head * a.part, d = d0 + t;
+        if (head < a.heads && t < tokens) {
+          const int32_t* const kept = a.plan.kept + (((int64_t)y * b.rows + row.row) * a.heads + head) * a.capacity;
+          const int s = source(a, kept, d, row.keep, row.len), sp = (int)((u32)s / (u32)page);
+          const int id = a.plan.table[(int64_t)row.row * b.width + sp];
+          from_row[t * a.heads + head] = id >= 0 && id < b.pages ? (int64_t)id * page + (s - sp * page) : -1;
+          if (head == 0) {
+            const int dp = (int)((u32)d / (u32)page);
+            to_row[t] = (int64_t)a.plan.list[row.place + dp - still] * page + (d - dp * page);
           }
         }
+      }
+      __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kMoveLoads; ++k)
-          if (to[k]) *reinterpret_cast<u32x4*>(to[k]) = x[k];
+      for (int v = 0; v < 2; ++v) {
+        const int which = v ? a.layers + y : y, chunks = layers.head_bytes[which] / 16, per_token = a.heads * chunks;
+        char* const pool = layers.data[which];
+        const int64_t token_bytes = (int64_t)per_token * 16;
+        for (int u0 = 0; u0 < tokens * per_token; u0 += kMoveThreads * kMoveLoads) {
+          u32x4 x[kMoveLoads];
+          char* to[kMoveLoads];
+#pragma unroll
+          for (int k = 0; k < kMoveLoads; ++k) {
+            const int u = u0 + k * kMoveThreads + tid;
+            to[k] = nullptr;
+            if (u < tokens * per_token) {
+              const int pair = (int)((u32)u / (u32)chunks), t = (int)((u32)pair / (u32)a.heads);
+              const int64_t in_token = (int64_t)(u - t * per_token) * 16, from = from_row[pair];
+              if (from >= 0) {
+                x[k] = *reinterpret_cast<const u32x4*>(pool + from * token_bytes + in_token);
+                to[k] = pool + to_row[t] * token_bytes + in_token;
+              }
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < kMoveLoads; ++k)
+            if (to[k]) __builtin_nontemporal_store(x[k], reinterpret_cast<u32x4*>(to[k]));
+        }
       }
     }
     return;
   }
-  if (y < 3 * a.layers) {
-    const int layer = y - 2 * a.layers;
+  if (y < 2 * a.layers) {
+    const int layer = y - a.layers;
     for (int w = blockIdx.x; w < count * a.heads; w += gridDim.x) {
-      const int r = a.plan.active[w / a.heads], head = w % a.heads, len = a.plan.old_len[r], keep = a.keep[r];
-      const int64_t place = ((int64_t)layer * b.rows + r) * a.heads + head;
+      const Shrunk s = a.plan.rows[w / a.heads];
+      const int head = w % a.heads;
+      const int64_t place = ((int64_t)layer * b.rows + s.row) * a.heads + head;
       const int32_t* const kept = a.plan.kept + place * a.capacity;
-      float* const row = const_cast<float*>(layers.scores[layer]) + ((int64_t)r * a.heads + head) * a.stride;
-      for (int base = a.first; base < keep; base += kMoveThreads * kSumLoads) {
+      float* const row = const_cast<float*>(layers.scores[layer]) + ((int64_t)s.row * a.heads + head) * a.stride;
+      for (int base = a.first; base < s.keep; base += kMoveThreads * kSumLoads) {
         float x[kSumLoads];
 #pragma unroll
         for (int k = 0; k < kSumLoads; ++k) {
           const int d = base + k * kMoveThreads + tid;
-          x[k] = d < keep ? row[source(a, kept, d, keep, len)] : 0.0f;
+          x[k] = d < s.keep ? row[source(a, kept, d, s.keep, s.len)] : 0.0f;
         }
 #pragma unroll
         for (int k = 0; k < kSumLoads; ++k) asm volatile("" ::"v"(x[k]));  // read before any wave writes
@@ -308,23 +387,23 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, L
 #pragma unroll
         for (int k = 0; k < kSumLoads; ++k) {
           const int d = base + k * kMoveThreads + tid;
-          if (d < keep) row[d] = x[k];
+          if (d < s.keep) row[d] = x[k];
         }
       }
     }
     return;
   }
   for (int w = blockIdx.x; w < count; w += gridDim.x) {
-    const int r = a.plan.active[w], len = a.plan.old_len[r], keep = a.keep[r];
-    const int live = (int)(((int64_t)len + page - 1) / page), pages = (int)(((int64_t)keep + page - 1) / page);
-    const int32_t* const fresh = a.plan.list + a.plan.place[r];
-    int32_t* const row = b.table + (int64_t)r * b.width;
+    const Shrunk s = a.plan.rows[w];
+    const int live = (int)(((int64_t)s.len + page - 1) / page), pages = (int)(((int64_t)s.keep + page - 1) / page);
+    const int32_t* const fresh = a.plan.list + s.place;
+    int32_t* const row = b.table + (int64_t)s.row * b.width;
     for (int j = still + tid; j < b.width; j += kMoveThreads) {
       const int id = row[j];
       if (j < live && id >= 0 && id < b.pages) atomicSub(&b.refs[id], 1);
       row[j] = j < pages ? fresh[j - still] : -1;
     }
-    if (tid == 0) b.lens[r] = keep;
+    if (tid == 0) b.lens[s.row] = s.keep;
   }
 }
 
@@ -338,6 +417,7 @@ static int check_evict(const fgw_pages_books* books, const fgw_evict_args* a, Bo
   if (int rc = check_books(books, b)) return rc;
   if (!a) return fail(FGW_MHA_EINVAL, "arguments are missing");
   if (a->layers <= 0 || a->heads <= 0) return fail(FGW_MHA_EINVAL, "positive layers and heads required");
+  if (a->heads > kMoveThreads) return fail(FGW_MHA_EUNSUPPORTED, "at most %d K/V heads", kMoveThreads);
   if (a->first < 0 || a->recent < 0) return fail(FGW_MHA_EINVAL, "the tokens that always stay must not be negative");
   if (a->scores_stride < (int64_t)b.width * b.page)
     return fail(FGW_MHA_EINVAL, "the scores must have a place for every key of the table");
@@ -355,7 +435,7 @@ int64_t fgw_pages_evict_workspace(const fgw_pages_books* books, const fgw_evict_
   Books b;
   if (int rc = check_evict(books, args, b)) return rc;
   const int64_t capacity = (int64_t)b.width * b.page;
-  return 2 + 4 * (int64_t)b.rows + b.pages + (int64_t)b.rows * b.width +
+  return 8 + 6 * (int64_t)b.rows + b.pages + (int64_t)b.rows * b.width +
          layers_of_launch(b.rows, args->heads, capacity, args->layers) * b.rows * args->heads * capacity;
 }
 
@@ -364,6 +444,7 @@ int fgw_pages_evict(const fgw_pages_books* books, const fgw_evict_args* args, in
   Books b;
   if (int rc = check_evict(books, args, b)) return rc;
   const fgw_evict_args& a = *args;
+  if (!aligned16(workspace)) return fail(FGW_MHA_EINVAL, "the workspace must be 16-byte aligned");
   if (!a.keep || !a.k_pools || !a.v_pools || !a.scores || !a.k_head_bytes || !a.v_head_bytes || !status || !workspace)
     return fail(FGW_MHA_EINVAL, "tensors are missing");
   for (int i = 0; i < a.layers; ++i) {
@@ -381,16 +462,15 @@ int fgw_pages_evict(const fgw_pages_books* books, const fgw_evict_args* args, in
   e.heads = a.heads;
   e.stride = a.scores_stride;
   e.capacity = (int64_t)b.width * b.page;
-  // A part fills a workgroup's loads about once.
-  const int64_t token_bytes = a.k_head_bytes[0] * a.heads;
-  e.tokens_part = (int32_t)std::min<int64_t>(64, std::max<int64_t>(1, kMoveThreads * kMoveLoads * 16 / token_bytes));
+  // A thread for each (token, head); smaller parts where there are few tokens at most.
+  const int64_t spread = e.capacity * b.rows * a.layers / kSpread;
+  e.part = (int32_t)std::min<int64_t>(std::min(kMostPart, kMoveThreads / a.heads), std::max<int64_t>(spread, kLeastPart));
   EvictPlan& p = e.plan;
-  p.count = workspace;
-  p.active = p.count + 1;
-  p.base = p.active + b.rows;
-  p.place = p.base + b.rows + 1;
-  p.old_len = p.place + b.rows;
-  p.list = p.old_len + b.rows;
+  p.rows = reinterpret_cast<Shrunk*>(workspace);
+  p.count = workspace + 4 * (int64_t)b.rows;
+  p.base = p.count + 1;
+  p.need = p.base + b.rows + 1;
+  p.list = p.need + b.rows;
   p.table = p.list + b.pages;
   p.kept = p.table + (int64_t)b.rows * b.width;
   const int step = (int)layers_of_launch(b.rows, a.heads, e.capacity, a.layers);
@@ -404,11 +484,14 @@ int fgw_pages_evict(const fgw_pages_books* books, const fgw_evict_args* args, in
       layers.head_bytes[i] = (int32_t)a.k_head_bytes[done + i];
       layers.head_bytes[e.layers + i] = (int32_t)a.v_head_bytes[done + i];
     }
-    evict_select_kernel<<<dim3((unsigned)(1 + e.layers * b.rows * a.heads)), dim3(kPlanThreads), 0, stream>>>(
-        e, layers, status, done == 0);
+    const dim3 programs((unsigned)(1 + e.layers * b.rows * a.heads));
+    if (e.capacity <= kFewThreads * kPer)
+      evict_select_kernel<kFewThreads><<<programs, dim3(kFewThreads), 0, stream>>>(e, layers, status, done == 0);
+    else
+      evict_select_kernel<kPlanThreads><<<programs, dim3(kPlanThreads), 0, stream>>>(e, layers, status, done == 0);
     if (int rc = launched("fgw_pages_evict")) return rc;
     const bool last = done + step >= a.layers;
-    const int y = 3 * e.layers + (last ? 1 : 0);
+    const int y = 2 * e.layers + (last ? 1 : 0);
     evict_move_kernel<<<dim3((unsigned)std::max(64, kMovers / y), (unsigned)y), dim3(kMoveThreads), 0, stream>>>(e, layers);
     if (int rc = launched("fgw_pages_evict")) return rc;
   }
