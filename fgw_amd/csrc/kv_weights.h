@@ -93,23 +93,46 @@ __device__ __forceinline__ void add_score(const WeightParams& p, float* row, int
 
 // ---- few rows -----------------------------------------------------------------------------------
 
+// Tiles of a wave on the way. One leaves room for three programs on a CU; one / two, us: 256 requests of up to
+// 512 keys 61 / 70, 32 of 4096 D 256 112 / 120, one of 32768 22.7 / 23.6.
 template <int DPAD>
-constexpr int kWeightStages = DPAD >= 128 ? 2 : 4;
+constexpr int kWeightStages = DPAD >= 128 ? 1 : 2;
 
-// Keys [from, to) of an item's tile: the kept scores of its rows against their L.
+// Keys [from, to) of an item's tile, from a multiple of 4: the kept scores of its rows against their L, four
+// keys to a thread and four rows on the way at a time.
 __device__ __forceinline__ void finish_keys(const WeightParams& p, const Item& it, const float* lse2, int from, int to,
                                             int tid, int threads) {
   const int64_t place = (int64_t)it.b * p.heads + it.head;
   const float* const kept = p.kept + place * p.kept_rows * p.keys_pad;
   float* const row = p.scores + place * p.stride;
-  for (int key = from + tid; key < to; key += threads) {
-    float sum = 0.0f;
-    for (int r = 0; r < it.rows; ++r) {
-      const float s = kept[(int64_t)r * p.keys_pad + key];
-      sum += s == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s - lse2[r]);
+  for (int key = from + 4 * tid; key < to; key += 4 * threads) {
+    float old[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) old[i] = p.decay != 0.0f && key + i < to && key + i < it.from ? row[key + i] : 0.0f;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int r0 = 0; r0 < it.rows; r0 += 4) {
+      f32x4 s[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)  // (the last row again where there are fewer: not added)
+        s[k] = *reinterpret_cast<const f32x4*>(kept + (int64_t)(r0 + k < it.rows ? r0 + k : it.rows - 1) * p.keys_pad + key);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float lse = lse2[r0 + k < it.rows ? r0 + k : 0];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          sum[i] += r0 + k >= it.rows || s[k][i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s[k][i] - lse);
+      }
     }
-    add_score(p, row, key, it.from, sum);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (key + i < to) row[key + i] = (p.decay != 0.0f ? old[i] * p.decay : 0.0f) + sum[i];
   }
+}
+
+// LDS writes and reads of one wave keep their order (the hardware does; this is for the compiler).
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 template <class C>
@@ -117,6 +140,11 @@ __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void weights_ro
     WeightParams p, const int32_t* __restrict__ table, const int32_t* __restrict__ lengths, const int32_t* __restrict__ cu) {
   constexpr int S = kWeightStages<C::DPAD>;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[C::NWK * S * C::TILE_BYTES];
+  // The scores of a wave's last tile, row by row: written to the workspace from here a tile later, whole
+  // rows of 128 bytes (straight from the lanes that hold them, 16 bytes each, the stores took a fifth of the
+  // time: 32 requests of 4096 keys 78 us, without any of them 64).
+  constexpr int kRow = 36;
+  __shared__ __attribute__((aligned(16))) float out[C::NWK][kKeptRows * kRow];
   __shared__ float cm[C::NWK * kKeptRows], cl[C::NWK * kKeptRows], clse[kKeptRows];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int il = lane & 31, hh = lane >> 5;
@@ -138,7 +166,12 @@ __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void weights_ro
   load_q<C>(p, it, il, il < it.rows, hh, qf);
   const Seen seen = row_seen(p, it, il / p.group);
   const int hi_min = row_seen(p, it, 0).hi;
-  float* const kept = p.kept + (((int64_t)it.b * p.heads + it.head) * p.kept_rows + il) * p.keys_pad;
+  float* const kept = p.kept + ((int64_t)it.b * p.heads + it.head) * p.kept_rows * p.keys_pad;
+  auto store_kept = [&](int pos0) {  // 8 rows at a time, 8 lanes to a row
+    for (int r = lane / 8; r < it.rows; r += 8)
+      *reinterpret_cast<f32x4*>(kept + (int64_t)r * p.keys_pad + pos0 + 4 * (lane % 8)) =
+          *reinterpret_cast<const f32x4*>(&out[wave][r * kRow + 4 * (lane % 8)]);
+  };
 
   float m = kNegBig, l = 0.0f;
   keys.ids_ready();
@@ -148,13 +181,15 @@ __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void weights_ro
   for (int n = 0; n < my_n; ++n) {
     const int pos0 = first_pos + kStep * n, rem = my_n - 1 - n;
     const unsigned char* stage = stages + n % S * C::TILE_BYTES;
-    // (Stores of kept scores may be in flight behind the tile too: that only makes the wait stricter.)
-    if (rem >= S - 1)
+    // Behind the tile are those of the next S - 1, and from iteration S + 1 on the stores of S iterations
+    // (memory instructions retire in order): a wait that left those out would be one for the next tile. The
+    // last and the first iterations wait for more than they need.
+    if (rem >= S - 1 && n > S && it.rows <= 8)
+      wait_vm<(S - 1) * C::INSTR + S>();
+    else if (rem >= S - 1 && n > S)
+      wait_vm<(S - 1) * C::INSTR + 2 * S>();
+    else if (rem >= S - 1)
       wait_vm<(S - 1) * C::INSTR>();
-    else if (S > 2 && rem == 2)
-      wait_vm<(S > 2 ? 2 : 0) * C::INSTR>();
-    else if (S > 2 && rem == 1)
-      wait_vm<(S > 2 ? 1 : 0) * C::INSTR>();
     else
       wait_vm<0>();
     asm volatile("" ::: "memory");
@@ -182,13 +217,17 @@ __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void weights_ro
       sum = exp_sum(s[0], m, p.scale_log2);
     }
     l += sum;
+    if (n > 0) store_kept(pos0 - kStep);
+    wave_fence();
     if (il < it.rows) {
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(kept + pos0 + 8 * g + 4 * hh) =
+        *reinterpret_cast<f32x4*>(&out[wave][il * kRow + 8 * g + 4 * hh]) =
             f32x4{s[0][4 * g], s[0][4 * g + 1], s[0][4 * g + 2], s[0][4 * g + 3]} * p.scale_log2;
     }
+    wave_fence();
   }
+  if (my_n > 0) store_kept(first_pos + kStep * (my_n - 1));
 
   const float tot = pair_sum(l);
   if (hh == 0 && il < it.rows) {
@@ -269,8 +308,12 @@ struct OneTile {  // of mask_seen and row_max: 32 rows
 // by side only where their instructions come by turns (16 products 222 ns, the 32 exponentials of a lane with
 // their sums 221 ns; by turns 277 to 333, one after the other 443), so between a phase's products stand the
 // exponentials of the phase before: use(s, t, r, e) takes element e of it; begin(j, s, t, r) and end(s, t, r)
-// come before and after. issue(j, lds offset) starts tile j's DMA. begin says whether the phase takes the
+// come before and after. issue(j, lds offset) starts tile j's DMA (start_tiles: that of the first ones). begin says whether the phase takes the
 // common path; if not, rare(s, t, r) stands for all its elements.
+template <class C, class Issue>
+__device__ __forceinline__ void start_tiles(int tiles, Issue&& issue) {
+  for (int j = 0; j < C::STAGES - 1 && j < tiles; ++j) issue(j, j * C::TILE_BYTES);
+}
 template <class C, class Issue, class Begin, class Use, class Rare, class End>
 __device__ __forceinline__ void stream_tiles(int tiles, u32 lds, const Lanes<C>& ln, const u32x4 (&held)[C::NR][C::KK],
                                              Issue&& issue, Begin&& begin, Use&& use, Rare&& rare, End&& end) {
@@ -286,7 +329,6 @@ __device__ __forceinline__ void stream_tiles(int tiles, u32 lds, const Lanes<C>&
     constexpr int T = decltype(t)::value, K = decltype(kk)::value;
     a[K] = *(const __attribute__((address_space(3))) u32x4*)(lds_at(addr[K]) + at + T * 32 * C::ROW_BYTES);
   };
-  for (int j = 0; j < kAhead && j < tiles; ++j) issue(j, j * C::TILE_BYTES);
   int stage = 0;
   for (int j = 0; j < tiles; ++j) {
     if (kAhead > 1 && j + 1 < tiles)
@@ -306,11 +348,13 @@ __device__ __forceinline__ void stream_tiles(int tiles, u32 lds, const Lanes<C>&
         for (int v = 0; v < 16; ++v) next[0][v] = 0.0f;
         static_for<C::KK>([&](auto kk) {
           constexpr int K = decltype(kk)::value;
-          between(K);
           next[0] = E::mma(a[K], held[R][K], next[0]);
           if constexpr (R == C::NR - 1 && T + 1 < C::ST) read(std::integral_constant<int, T + 1>{}, kk, at);
+          if constexpr (K > 0) between(K - 1);  // (the phase before's last product is through by then)
           __builtin_amdgcn_sched_barrier(0);
         });
+        between(C::KK - 1);
+        __builtin_amdgcn_sched_barrier(0);
       };
       if (P > 0 || j > 0) {
         if (begin(P > 0 ? j : j - 1, cur, QT, QR)) {
@@ -371,12 +415,14 @@ __global__ __launch_bounds__(C::THREADS, kWaveSimd) void weights_stats_kernel(
     l[r] = 0.0f;
   }
   keys.ids_ready();
+  auto issue_tile = [&](int j, int at) { keys.template issue<false>(dl, j, lds + (u32)at); };
+  start_tiles<C>(tiles, issue_tile);
 #pragma unroll
   for (int r = 0; r < C::NR; ++r)
 #pragma unroll
     for (int kk = 0; kk < C::KK; ++kk) asm volatile("" ::"v"(qf[r][kk]));
   stream_tiles<C>(
-      tiles, lds, ln, qf, [&](int j, int at) { keys.template issue<false>(dl, j, lds + (u32)at); },
+      tiles, lds, ln, qf, issue_tile,
       [&](int j, f32x16(&s)[1], int t, int r) {
         const int pos0 = first_pos + C::BN * j + 32 * t;
         if (pos0 + 32 > hi_min[r]) mask_seen<OneTile<C>>(s, pos0, seen[r], hh);
@@ -502,55 +548,7 @@ __global__ __launch_bounds__(C::THREADS, kWaveSimd) void weights_columns_kernel(
     if (seen0 >= end) continue;
     const int begin = seen0 > part0 ? part0 + (seen0 - part0) / 64 * 64 : part0, tiles = (end - begin + 63) / 64;
 
-    // K of the lane's keys, from their pages.
-    u32x4 kf[C::NR][C::KK];
-    int mine[C::NR], all[C::NR];  // the first row that sees the lane's key, all of the wave's 32
-#pragma unroll
-    for (int r = 0; r < C::NR; ++r) {
-      const int key = key0 + 32 * r + il;
-      const u32 pg = key < it.len ? div_page((u32)key, p.page_magic, p.page_shift) : 0u;
-      const int64_t krow = (int64_t)table[(int64_t)it.b * p.width + pg] * p.page_size + ((u32)key - pg * (u32)p.page_size);
-      const bool live = key < it.len && krow >= 0 && krow < p.pool_rows;
-      const char* const kp = static_cast<const char*>(p.k) + (int64_t)it.head * p.dim * 2 + (live ? krow * row_bytes : 0);
-#pragma unroll
-      for (int kk = 0; kk < C::KK; ++kk) {
-        const int d = 16 * kk + 8 * hh;
-        u32x4 x = {0u, 0u, 0u, 0u};
-        if (live && d < p.dim) x = *reinterpret_cast<const u32x4*>(kp + 2 * d);
-        kf[r][kk] = x;
-      }
-      mine[r] = first_row(p, it, key);
-      all[r] = first_row(p, it, key0 + 32 * r + 31);
-    }
-    // L of the part's rows, from their splits.
     __syncthreads();  // the item before is done with slse and the stages
-    const WeightNote note = reinterpret_cast<const WeightNote*>(p.request_notes)[it.b];
-    for (int r = begin + tid; r < begin + 64 * tiles; r += C::THREADS) {
-      float lse = INFINITY;  // rows that are none weigh nothing
-      if (r < end) {
-        typedef StatsTiling T;
-        const int tile = r / T::ROWS, last = (tile + 1) * T::ROWS < rows ? (tile + 1) * T::ROWS : rows;
-        int hi = it.len - it.n + (int)((u32)(last - 1) / (u32)p.group) + 1;
-        hi = hi < 0 ? 0 : hi;
-        const int most = splits_of(p, (hi + T::KEYS - 1) / T::KEYS, note.chunk);
-        const int splits = most < note.splits ? most : note.splits;
-        const int64_t slot = (int64_t)(note.base + (note.tiles - 1 - tile) * note.splits) * p.heads + it.head;
-        float m = kNegBig, l = 0.0f;
-        for (int s = 0; s < splits && slot + (int64_t)s * p.heads < p.work && slot >= 0; ++s) {
-          const float x = p.lse[(slot + (int64_t)s * p.heads) * T::ROWS + (r - tile * T::ROWS)], top = fmaxf(m, x);
-          l = l * __builtin_amdgcn_exp2f(m - top) + __builtin_amdgcn_exp2f(x - top);
-          m = top;
-        }
-        lse = m > 0.5f * kNegBig || l != l ? lse2_of(m, l) : INFINITY;
-      }
-      slse[r - begin] = lse;
-    }
-#pragma unroll
-    for (int r = 0; r < C::NR; ++r)
-#pragma unroll
-      for (int kk = 0; kk < C::KK; ++kk) asm volatile("" ::"v"(kf[r][kk]));
-    __syncthreads();
-
     // 64 rows of Q into LDS, a K tile's layout, tile after tile: a lane's rows are 64 apart, so their places
     // move on by whole tokens and a few heads.
     constexpr int U = C::INSTR_PER_WAVE;
@@ -582,6 +580,81 @@ __global__ __launch_bounds__(C::THREADS, kWaveSimd) void weights_columns_kernel(
       }
       next_row += C::BN;
     };
+    start_tiles<C>(tiles, issue_tile);
+
+    // K of the lane's keys, from their pages.
+    u32x4 kf[C::NR][C::KK];
+    int mine[C::NR], all[C::NR];  // the first row that sees the lane's key, all of the wave's 32
+#pragma unroll
+    for (int r = 0; r < C::NR; ++r) {
+      const int key = key0 + 32 * r + il;
+      const u32 pg = key < it.len ? div_page((u32)key, p.page_magic, p.page_shift) : 0u;
+      const int64_t krow = (int64_t)table[(int64_t)it.b * p.width + pg] * p.page_size + ((u32)key - pg * (u32)p.page_size);
+      const bool live = key < it.len && krow >= 0 && krow < p.pool_rows;
+      const char* const kp = static_cast<const char*>(p.k) + (int64_t)it.head * p.dim * 2 + (live ? krow * row_bytes : 0);
+#pragma unroll
+      for (int kk = 0; kk < C::KK; ++kk) {
+        const int d = 16 * kk + 8 * hh;
+        u32x4 x = {0u, 0u, 0u, 0u};
+        if (live && d < p.dim) x = *reinterpret_cast<const u32x4*>(kp + 2 * d);
+        kf[r][kk] = x;
+      }
+      mine[r] = first_row(p, it, key);
+      all[r] = first_row(p, it, key0 + 32 * r + 31);
+    }
+    // L of the part's rows, from their splits.
+    const WeightNote note = reinterpret_cast<const WeightNote*>(p.request_notes)[it.b];
+    // (Threads that the rows leave over share a row's splits.)
+    const int padded = C::BN * tiles, share = padded < C::THREADS ? C::THREADS / padded : 1;
+    for (int base = 0; base < padded; base += C::THREADS) {
+      const int in_part = share > 1 ? tid % padded : base + tid, g = share > 1 ? tid / padded : 0, r = begin + in_part;
+      float m = kNegBig, l = 0.0f;
+      if (r < end && g < share) {
+        typedef StatsTiling T;
+        const int tile = r / T::ROWS, last = (tile + 1) * T::ROWS < rows ? (tile + 1) * T::ROWS : rows;
+        int hi = it.len - it.n + (int)((u32)(last - 1) / (u32)p.group) + 1;
+        hi = hi < 0 ? 0 : hi;
+        const int most = splits_of(p, (hi + T::KEYS - 1) / T::KEYS, note.chunk);
+        const int64_t slot = (int64_t)(note.base + (note.tiles - 1 - tile) * note.splits) * p.heads + it.head;
+        int splits = most < note.splits ? most : note.splits;
+        splits = slot >= 0 && slot + (int64_t)(splits - 1) * p.heads < p.work ? splits : 0;
+        const float* const lse = p.lse + slot * T::ROWS + (r - tile * T::ROWS);
+        const int64_t step = (int64_t)p.heads * T::ROWS;
+        for (int s0 = g; s0 < splits; s0 += 8 * share) {
+          float x[8], top = m;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] = s0 + k * share < splits ? lse[(s0 + k * share) * step] : kNegBig;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) top = fmaxf(top, x[k]);
+          l *= __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) l += s0 + k * share < splits ? __builtin_amdgcn_exp2f(x[k] - top) : 0.0f;
+          m = top;
+        }
+      }
+      if (share > 1) {  // uniform; one pass
+        slse[tid] = m;
+        slse[C::THREADS + tid] = l;
+        __syncthreads();
+        if (g == 0) {
+          float top = m;
+          for (int k = 1; k < share; ++k) top = fmaxf(top, slse[k * padded + in_part]);
+          l *= __builtin_amdgcn_exp2f(m - top);
+          for (int k = 1; k < share; ++k)
+            l += slse[C::THREADS + k * padded + in_part] * __builtin_amdgcn_exp2f(slse[k * padded + in_part] - top);
+          m = top;
+        }
+        __syncthreads();
+      }
+      // (Rows that are none, or see nothing, weigh nothing.)
+      if (g == 0 && in_part < padded) slse[in_part] = r < end && (m > 0.5f * kNegBig || l != l) ? lse2_of(m, l) : INFINITY;
+    }
+#pragma unroll
+    for (int r = 0; r < C::NR; ++r)
+#pragma unroll
+      for (int kk = 0; kk < C::KK; ++kk) asm volatile("" ::"v"(kf[r][kk]));
+    __syncthreads();
+
     float acc[C::NR][4];
 #pragma unroll
     for (int r = 0; r < C::NR; ++r)

@@ -17,6 +17,8 @@ namespace {
 // Items of weights_stats_kernel, two to a CU, where its tiles are fewer.
 constexpr int kStatsItems = 512;
 
+constexpr int kFewItems = 512, kManyItems = 1024;
+
 struct WeightPlan {
   bool many;       // rows of a request and K/V head, at most, past kKeptRows
   Launch launch;   // of the first pass
@@ -65,7 +67,9 @@ WeightPlan plan_weights(const fgw_kv_weights_args& a) {
     p.launch.whole = a.dim <= 64 ? kRowsWholeNarrow : kRowsWhole;
     p.launch.many = rows <= 8 ? kRowsMany : kRowsManyTall;
     p.launch.tiles = requests;
-    plan_items<ShortTiling>(p.launch, e, true);
+    fgw_kv_extend_args rounds = e;
+    rounds.num_cus = p.launch.tiles * a.kv_heads >= e.num_cus ? kManyItems : kFewItems;
+    plan_items<ShortTiling>(p.launch, rounds, true);
     p.kept_rows = rows;
     p.kept = (int64_t)a.batch * a.kv_heads * rows * p.keys_pad;
     p.lse = p.launch.slots * kKeptRows;
