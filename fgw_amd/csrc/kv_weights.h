@@ -25,7 +25,7 @@
 namespace fgw_kv {
 
 constexpr int kKeptRows = 16;
-constexpr int kColumnRows = 1024;  // rows of a part
+constexpr int kColumnRows = 1024;  // rows of a part at most
 constexpr int kSumKeys = 256;
 constexpr int kColumnKeys = 256;   // keys of an item
 constexpr int kWaveSimd = 2;       // waves to a SIMD
@@ -37,6 +37,7 @@ struct WeightParams : ExtendParams {
   float* sums;      // more rows: [parts, heads, keys_pad]
   int32_t* request_notes;  // more rows: [batch] WeightNote
   int32_t last, kept_rows, keys_pad, parts_most;
+  int32_t part_rows, part_shift;  // rows of a part: kColumnRows or a half or a quarter of it; their log2
   float decay;
 };
 template <>
@@ -318,16 +319,19 @@ template <class C, class Issue, class Begin, class Use, class Rare, class End>
 __device__ __forceinline__ void stream_tiles(int tiles, u32 lds, const Lanes<C>& ln, const u32x4 (&held)[C::NR][C::KK],
                                              Issue&& issue, Begin&& begin, Use&& use, Rare&& rare, End&& end) {
   using E = Elem<C::BF16>;
-  constexpr int kAhead = C::STAGES - 1, PH = C::ST * C::NR;
+  // (Operands: those of all 32 rows up to D 128, where the NR phases share them; at D 256, where all would leave
+  // too few registers, eight ahead.)
+  constexpr int kAhead = C::STAGES - 1, PH = C::ST * C::NR, RING = C::KK < 8 ? C::KK : 8;
+  static_assert(C::NR == 1 || RING == C::KK, "phases share their operands");
   if (tiles <= 0) return;
   u32 addr[C::KK];
 #pragma unroll
   for (int kk = 0; kk < C::KK; ++kk) addr[kk] = lds + (u32)(ln.k_base + 32 * (kk ^ ln.ky));
-  u32x4 a[C::KK];
+  u32x4 a[RING];
   f32x16 s[2][1];
   auto read = [&](auto t, auto kk, u32 at) {
     constexpr int T = decltype(t)::value, K = decltype(kk)::value;
-    a[K] = *(const __attribute__((address_space(3))) u32x4*)(lds_at(addr[K]) + at + T * 32 * C::ROW_BYTES);
+    a[K % RING] = *(const __attribute__((address_space(3))) u32x4*)(lds_at(addr[K]) + at + T * 32 * C::ROW_BYTES);
   };
   int stage = 0;
   for (int j = 0; j < tiles; ++j) {
@@ -337,7 +341,7 @@ __device__ __forceinline__ void stream_tiles(int tiles, u32 lds, const Lanes<C>&
       wait_vm<0>();
     __syncthreads();  // tile j has landed for all waves, tile j - 1 is read
     const u32 at = (u32)(stage * C::TILE_BYTES);
-    static_for<C::KK>([&](auto kk) { read(std::integral_constant<int, 0>{}, kk, at); });
+    static_for<RING>([&](auto kk) { read(std::integral_constant<int, 0>{}, kk, at); });
     if (j + kAhead < tiles) issue(j + kAhead, (stage == 0 ? C::STAGES - 1 : stage - 1) * C::TILE_BYTES);
     static_for<PH>([&](auto ph) {
       constexpr int P = decltype(ph)::value, T = P / C::NR, R = P % C::NR, Q = (P + PH - 1) % PH, QT = Q / C::NR, QR = Q % C::NR;
@@ -348,8 +352,11 @@ __device__ __forceinline__ void stream_tiles(int tiles, u32 lds, const Lanes<C>&
         for (int v = 0; v < 16; ++v) next[0][v] = 0.0f;
         static_for<C::KK>([&](auto kk) {
           constexpr int K = decltype(kk)::value;
-          next[0] = E::mma(a[K], held[R][K], next[0]);
-          if constexpr (R == C::NR - 1 && T + 1 < C::ST) read(std::integral_constant<int, T + 1>{}, kk, at);
+          next[0] = E::mma(a[K % RING], held[R][K], next[0]);
+          if constexpr (K + RING < C::KK)
+            read(std::integral_constant<int, T>{}, std::integral_constant<int, K + RING>{}, at);
+          else if constexpr (R == C::NR - 1 && T + 1 < C::ST)
+            read(std::integral_constant<int, T + 1>{}, std::integral_constant<int, K + RING - C::KK>{}, at);
           if constexpr (K > 0) between(K - 1);  // (the phase before's last product is through by then)
           __builtin_amdgcn_sched_barrier(0);
         });
@@ -458,7 +465,7 @@ struct Column {
 };
 // Blocks of kColumnKeys keys that the rows of a part see: up to its last row's token.
 __device__ __forceinline__ int blocks_seen(const WeightParams& p, int n, int len, int part) {
-  const int64_t rows = (int64_t)n * p.group, end = (int64_t)(part + 1) * kColumnRows;
+  const int64_t rows = (int64_t)n * p.group, end = (int64_t)(part + 1) * p.part_rows;
   const int last = (int)((u32)((end < rows ? end : rows) - 1) / (u32)p.group), hi = len - n + last + 1;
   return hi > 0 ? (hi + kColumnKeys - 1) / kColumnKeys : 0;
 }
@@ -470,7 +477,7 @@ template <bool SUM>
 __device__ __forceinline__ ColumnRequest column_request(const WeightParams& p, const int32_t* lengths, const int32_t* cu, int b) {
   ColumnRequest x;
   x.r = load_request<StatsTiling>(p, lengths, cu, b);
-  x.parts = x.r.tiles ? (int)(((int64_t)x.r.n * p.group + kColumnRows - 1) / kColumnRows) : 0;
+  x.parts = x.r.tiles ? (int)(((int64_t)x.r.n * p.group + p.part_rows - 1) >> p.part_shift) : 0;
   x.items = 0;
   if (SUM)
     x.items = x.parts > 1 ? (x.r.len + kSumKeys - 1) / kSumKeys : 0;
@@ -542,9 +549,9 @@ __global__ __launch_bounds__(C::THREADS, kWaveSimd) void weights_columns_kernel(
   Column it;
   for (int64_t w = blockIdx.x; find_column<false>(p, lengths, cu, w, lane, r0, it); w += gridDim.x) {
     const int rows = it.n * p.group, key0 = it.block * kColumnKeys + wave * C::ROWS_WAVE;  // keys of this wave
-    const int end = rows - it.part * kColumnRows < kColumnRows ? rows : (it.part + 1) * kColumnRows;
+    const int end = rows - it.part * p.part_rows < p.part_rows ? rows : (it.part + 1) * p.part_rows;
     // (Tiles of 64 rows from the part's first row.)
-    const int part0 = it.part * kColumnRows, seen0 = first_row(p, it, it.block * kColumnKeys);
+    const int part0 = it.part * p.part_rows, seen0 = first_row(p, it, it.block * kColumnKeys);
     if (seen0 >= end) continue;
     const int begin = seen0 > part0 ? part0 + (seen0 - part0) / 64 * 64 : part0, tiles = (end - begin + 63) / 64;
 
@@ -711,7 +718,7 @@ static __global__ __launch_bounds__(kFinishThreads) void weights_sum_kernel(Weig
       const int last = it.part0 + it.parts < p.parts_most ? it.part0 + it.parts : p.parts_most;
       const float* const at = p.sums + (int64_t)it.head * p.keys_pad + key;
       const int64_t step = (int64_t)p.heads * p.keys_pad;
-      int c = it.part0 + first_row(p, it, key / kColumnKeys * kColumnKeys) / kColumnRows;
+      int c = it.part0 + (first_row(p, it, key / kColumnKeys * kColumnKeys) >> p.part_shift);
       for (; c + 4 <= last; c += 4) {
         float x[4];
 #pragma unroll

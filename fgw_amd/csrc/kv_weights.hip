@@ -14,14 +14,20 @@ FGW_KV_EXTERN_WEIGHTS(false, 64) FGW_KV_EXTERN_WEIGHTS(false, 128) FGW_KV_EXTERN
 
 namespace {
 
-// Items of weights_stats_kernel, two to a CU, where its tiles are fewer.
+// Items of weights_stats_kernel, two to a CU, where its tiles are fewer. 256 / 512 / 1024 items, us of a call:
+// 2000 tokens of 2 K/V heads of 8 rows 75.0 / 74.3 / 81.0, 64 requests of 17 tokens 92.9 / 93.0 / 97.8.
 constexpr int kStatsItems = 512;
 
-constexpr int kFewItems = 512, kManyItems = 1024;
+// Items of weights_rows_kernel: two to a CU, and the three that it holds where the requests alone fill the card,
+// so that ragged ones even out. 512 / 768 / 1024 items, us: 32 requests of 8 K/V heads, 1 to 8192 keys 92.8 /
+// 86.0 / 93.0, all of 8192 keys 124.6 / 125.0 / 131.8, 64 of 2048 63.8 / 66.0 / 72.6; 8 of 8192, of few
+// requests, 37.8 at 512 and 42.5 at 1024 (256: 40.3).
+constexpr int kFewItems = 512, kManyItems = 768;
 
 struct WeightPlan {
   bool many;       // rows of a request and K/V head, at most, past kKeptRows
   Launch launch;   // of the first pass
+  int part_rows;
   int columns, sums;  // grids of the persistent kernels; 0: no launch
   int64_t keys_pad, kept_rows, parts;
   int64_t kept, lse, notes, floats;  // of workspace
@@ -87,9 +93,17 @@ WeightPlan plan_weights(const fgw_kv_weights_args& a) {
     p.launch.slots = p.launch.items;  // every item leaves statistics
     p.lse = p.launch.slots * StatsTiling::ROWS;
     p.notes = (int64_t)a.batch * (int64_t)sizeof(WeightNote) / 4;
-    const int64_t parts = blocks(kColumnRows), keys = p.keys_pad / kColumnKeys;
+    // Parts of the rows: smaller ones where the items would not fill the card (half of them: causal), down to
+    // what a program of its own is worth. Parts of 1024 rows always / by this rule, us of a call: 512 tokens of
+    // one K/V head of 8 rows 55.5 / 35.9, 4 requests of 300 tokens 53.4 / 35.8, 2000 tokens of 2 heads 77.4 / 74.3.
+    const int64_t keys = p.keys_pad / kColumnKeys;
+    p.part_rows = kColumnRows;
+    while (p.part_rows > kColumnRows / 4 && rows > p.part_rows / 2 &&
+           total / p.part_rows * keys * a.kv_heads < 4 * (int64_t)e.num_cus)
+      p.part_rows /= 2;
+    const int64_t parts = blocks(p.part_rows);
     p.columns = persistent(parts * keys * a.kv_heads, e.num_cus, a.dim > 128 ? 1 : 2);
-    if (rows > kColumnRows) {
+    if (rows > p.part_rows) {
       p.parts = parts;
       p.kept = parts * a.kv_heads * p.keys_pad;
       p.sums = persistent(requests * ((p.keys_pad + kSumKeys - 1) / kSumKeys) * a.kv_heads, e.num_cus, 4);
@@ -110,7 +124,7 @@ int check_weights(const fgw_kv_weights_args* args) {
     return fail(FGW_MHA_EINVAL, "the scores must have a place for every key of the table");
   const int64_t rows = (int64_t)args->tokens * (args->heads / args->kv_heads);
   const int64_t keys = (int64_t)args->width * args->page_size / kColumnKeys + 1;
-  if ((rows / kColumnRows + args->batch) * keys > 0x3fffffff)
+  if ((rows / (kColumnRows / 4) + args->batch) * keys > 0x3fffffff)
     return fail(FGW_MHA_EUNSUPPORTED, "too many rows for one call");
   return FGW_MHA_OK;
 }
@@ -152,6 +166,8 @@ int fgw_kv_weights(const fgw_kv_weights_args* args, hipStream_t stream) {
   w.stride = a.scores_stride;
   w.last = a.last;
   w.decay = a.decay;
+  w.part_rows = p.part_rows;
+  for (w.part_shift = 0; w.part_rows > 1 << w.part_shift;) ++w.part_shift;
   w.keys_pad = (int32_t)p.keys_pad;
   w.kept_rows = (int32_t)p.kept_rows;
   w.parts_most = (int32_t)p.parts;
