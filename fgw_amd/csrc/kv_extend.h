@@ -156,7 +156,8 @@ __device__ __forceinline__ Group load_group(const SharedParams& p, const int32_t
   x.f0 = a;
   x.f1 = b;
   x.keys = good ? (wanted < before ? wanted : before) : 0;
-  x.keys = x.keys < 0 ? 0 : x.keys;
+  // (Offsets that run out of q leave the group no items in the first pass: its requests read their keys themselves.)
+  if (x.keys < 0 || x.first < 0 || x.next > p.tokens || x.next <= x.first) x.keys = 0;
   // (Requests of whole long tiles are bound by their products, which sharing does not save: kv_shared.hip.)
   if (p.share_from > 0 && (int64_t)(x.next - x.first) * p.group > (int64_t)kShareRows * (x.f1 - x.f0)) x.keys = 0;
   return x;
@@ -178,7 +179,6 @@ __device__ __forceinline__ Request group_request(const PrefixParams& p, const Gr
   r.row = x.f0;
   r.len = x.keys;
   r.first = x.first;
-  if (x.first < 0 || x.next > p.tokens || x.next <= x.first) return r;
   r.n = x.next - x.first;
   r.tiles = (int)(((int64_t)r.n * p.group + T::ROWS - 1) / T::ROWS);
   r.units = (r.len + T::KEYS - 1) / T::KEYS;

@@ -183,6 +183,24 @@ def test_offsets_of_groups_that_say_nothing():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("always", [True, False])
+def test_a_group_whose_offsets_run_out_of_q(always):
+    """Its requests within q read their keys themselves, as without groups; other groups share."""
+    news = [1, 2, 1, 1]
+    cache = _cache([2, 2], [300, 90], news, [4, 6, 7, 9], 2, 64, 16, torch.bfloat16)
+    q = _queries(5, 4, 64, torch.bfloat16)
+    dev = [x.cuda() for x in cache]
+    first, prefixes = _offsets([2, 2]).cuda(), torch.tensor([300, 90], dtype=torch.int32).cuda()
+    kernel = S.build_shared_kernel(4, 2, 64, 16, "bfloat16", 0, always=always)
+    want, bound = K.extend_exact(q, *cache, 16)
+    for cu, rows in (([0, 1, 3, 4, 9], 4), ([0, 1, 9, 9, 9], 1)):
+        print(cu, flush=True)
+        dev[4] = torch.tensor(cu, dtype=torch.int32).cuda()
+        got = kernel(q.cuda(), *dev, first, prefixes, 2).cpu().double()
+        assert bool(((got - want).abs()[:rows] <= bound[:rows]).all()), cu
+
+
+@pytest.mark.gpu
 def test_rows_behind_the_last_request_are_left_and_strides_are_taken():
     cache = _cache([3], [200], [1, 2, 1], [1, 2, 50], 2, 128, 16, torch.bfloat16)
     fused = _queries(7, 12, 128, torch.bfloat16)
