@@ -419,6 +419,8 @@ static int check_evict(const fgw_pages_books* books, const fgw_evict_args* a, Bo
   if (a->layers <= 0 || a->heads <= 0) return fail(FGW_MHA_EINVAL, "positive layers and heads required");
   if (a->heads > kMoveThreads) return fail(FGW_MHA_EUNSUPPORTED, "at most %d K/V heads", kMoveThreads);
   if (a->first < 0 || a->recent < 0) return fail(FGW_MHA_EINVAL, "the tokens that always stay must not be negative");
+  if ((int64_t)b.width * b.page > 0x7fffffff - 0x10000)  // (positions run on by a program's reads past the last)
+    return fail(FGW_MHA_EUNSUPPORTED, "table capacity must fit in 31 bits");
   if (a->scores_stride < (int64_t)b.width * b.page)
     return fail(FGW_MHA_EINVAL, "the scores must have a place for every key of the table");
   if ((int64_t)b.rows * a->heads > 0x7fffffff / (4 * kMaxLayers)) return fail(FGW_MHA_EUNSUPPORTED, "too many rows for one call");

@@ -307,6 +307,7 @@ class _Evict(ctypes.Structure):
     (dict(refs=0), {}, "books are missing"), (dict(pages=0), {}, "positive pages"), (dict(pages=1 << 21), {}, "at most"),
     ({}, dict(layers=0), "positive layers"), ({}, dict(heads=0), "positive layers"), ({}, dict(first=-1), "negative"),
     ({}, dict(scores_stride=127), "place for every key"), (dict(rows=1 << 24, width=1), dict(heads=64), "too many rows"),
+    (dict(width=(1 << 24) - 1, page_size=128, rows=1), dict(scores_stride=1 << 31), "31 bits"),
     ({}, {}, "tensors are missing")])
 def test_c_entry_refusals(books, changes, message):
     """Refused on the host before any launch: these run where there is no GPU."""
