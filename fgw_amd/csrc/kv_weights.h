@@ -529,10 +529,11 @@ __device__ __forceinline__ bool find_column(const WeightParams& p, const int32_t
   }
   return false;
 }
-// The first row of a request that sees the key (rows see their token's own position and all before it).
+// The first row of a request that sees the key (rows see their token's own position and all before it); past
+// the last row, where none does.
 __device__ __forceinline__ int first_row(const WeightParams& p, const Column& it, int key) {
   const int token = key - (it.len - it.n);
-  return token > 0 ? token * p.group : 0;
+  return token > 0 ? (token < it.n ? token : it.n) * p.group : 0;
 }
 
 template <class C>

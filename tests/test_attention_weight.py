@@ -88,6 +88,10 @@ CASES = {
     "prompt_parts": ([700, 600, 3], [700, 900, 40], 4, 1, 64, 16, 10**9, 1.0),
     "prompt_parts_large_group": ([150, 260], [2100, 260], 24, 3, 128, 16, 260, 0.25),
     "prompt_parts_dim_256": ([530], [600], 4, 2, 256, 64, 530, 1.0),
+    "parts_of_256": ([700, 260, 257], [700, 900, 300], 2, 2, 128, 16, 700, 1.0),
+    "parts_of_512": ([1400] * 3, [1400, 3000 + 200, 1500], 4, 2, 64, 64, 1400, 1.0),
+    "many_requests_rows": ([17 + i % 60 for i in range(130)], [17 + i % 60 + (41 * i) % 700 for i in range(130)], 8, 1, 64, 16, 70, 0.5),
+    "dim_160_rows": ([90, 300], [1300, 300], 6, 2, 160, 32, 200, 1.0),
     "longer_than_cache": ([300, 20], [100, 7], 4, 2, 128, 16, 300, 1.0),
     "parts_longer_than_cache": ([1500], [700], 2, 1, 64, 16, 1500, 1.0),
 }
