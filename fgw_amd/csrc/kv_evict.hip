@@ -10,13 +10,17 @@
 // independent of every other. Two launches for up to kMaxLayers layers:
 //   evict_select_kernel  program 0 plans: free pages to rows in order (as a reservation), and the list of
 //                        rows that shrink. Beside it one program for each (layer, row, head) finds the
-//                        smallest kept sum by counting digits of 11 bits from the top (three passes over
+//                        smallest kept sum by counting digits of 11 bits from the top, until the sums that
+//                        share them are few enough to compare with each other (at most three passes over
 //                        the sums, which stay in registers up to 16384 of them), then writes the kept
 //                        positions in order, by counts of each wave's part and one scan over them.
-//   evict_move_kernel    K and V, 16 bytes to a lane, read by head and written in whole tokens; the sums, in
-//                        place (one program a head: it reads a stretch, then writes it; kept tokens only move
-//                        down); the books, with the last layers.
-// Program 0 is bound by its chain of reads, the moves by memory.
+//   evict_move_kernel    K and V in parts of some tokens: a thread finds the place of one (token, head), then
+//                        all copy, 16 bytes to a lane, and write whole tokens; the sums, in place (one program
+//                        a head: it reads a stretch, then writes it; kept tokens only move down); the books,
+//                        with the last layers.
+// Measured (BF16, D 128, 8 K/V heads): 16 rows of up to 4096 keys, 12 of them cut to 1000, four layers: select
+// 13 us, as long as a program's chain of passes and scans takes, moves 73 us, 5.3 TB/s of the 393 MB that they
+// read and write, at memory's rate. One row of 381 keys (FP16, D 64) cut to 200: 8 and 6 us, chains of reads.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -29,15 +33,26 @@ typedef u32 u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxLayers = 16;           // of one pair of launches
 constexpr int kPer = 16;                 // sums of a thread in registers
-constexpr int kFewThreads = 256;         // of a program where capacities fit its registers; else kPlanThreads
+// Threads of a program where capacities fit its registers (else kPlanThreads): its scans and barriers are those of
+// four waves, and eight programs share a CU. 256 / 1024 threads, us of a call: 64 rows of 2048 keys, four layers
+// 352 / 400, one row of 1024 16.8 / 19.4.
+constexpr int kFewThreads = 256;
+// Counters of a bin: lanes with equal sums meet in it. One / four, us of a call that moves nothing: 16 rows of 16384
+// equal sums 111 / 50, of 4096 33 / 21, of random ones 15.5 / 17.0.
 constexpr int kBins = 2048, kCopies = 4;
-constexpr int kDirect = 256;             // keys that are compared with each other
+// Keys that are compared with each other in place of the passes that are left. With / without, us: 64 rows of 2048
+// 352 / 362, one of 1024 16.8 / 19.9.
+constexpr int kDirect = 256;
 constexpr int kMoveThreads = 256;
-constexpr int kMoveLoads = 8;            // 16-byte chunks of a thread at once
+constexpr int kMoveLoads = 8;            // 16-byte chunks of a thread at once (4 / 8, us: 64 rows of 2048 383 / 342)
 constexpr int kMovers = 4096;            // workgroups of a launch that count their work on the device
 constexpr int kSumLoads = 8;
-constexpr int kLeastPart = 4, kMostPart = 32;  // tokens of a part
-constexpr int kSpread = 2048;            // parts that all rows at their capacity make, or more
+// Tokens of a part: as many as make kPartBytes of K or V, fewer where all rows at their capacity would be less than
+// kSpread parts. 8 / 16 / 32 KB, us: 12 of 16 rows to 1000 keys, four layers 111 / 101 / 106, 8 rows of 16384 keys to
+// 8000, 4 heads 120 / 106 / 108, 8 heads of D 256 179 / 179 / 183; at least 4 / 16 tokens: one row 15.2 / 17.0.
+constexpr int kLeastPart = 4;
+constexpr int64_t kPartBytes = 16384;
+constexpr int kSpread = 2048;
 
 struct Layers {
   const float* scores[kMaxLayers];
@@ -195,8 +210,7 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictArgs a, Laye
       held[k] = base + k * THREADS + tid < n ? sort_key(raw[k]) : 0u;  // (no sum's key is 0: that of minus infinity is 0x007fffff)
   };
   // The digits of the want-th largest key, from the top, until the keys that share them are few: those are
-  // compared with each other. Equal sums meet in one bin: lanes take turns at its
-  // kCopies counters, which lie in different banks.
+  // compared with each other. Lanes take turns at the kCopies counters of a bin, which lie in different banks.
   u32 prefix = 0;
   int left = want;
   const int steps = (n + THREADS - 1) / THREADS < kPer ? (n + THREADS - 1) / THREADS : kPer;
@@ -464,9 +478,12 @@ int fgw_pages_evict(const fgw_pages_books* books, const fgw_evict_args* args, in
   e.heads = a.heads;
   e.stride = a.scores_stride;
   e.capacity = (int64_t)b.width * b.page;
-  // A thread for each (token, head); smaller parts where there are few tokens at most.
+  // Parts of kPartBytes, with a thread for each (token, head); smaller ones where there are few tokens at most.
+  int64_t widest = 0;
+  for (int i = 0; i < a.layers; ++i) widest = std::max(widest, std::max(a.k_head_bytes[i], a.v_head_bytes[i]));
+  const int64_t tokens = std::max<int64_t>(kPartBytes / (widest * a.heads), kLeastPart);
   const int64_t spread = e.capacity * b.rows * a.layers / kSpread;
-  e.part = (int32_t)std::min<int64_t>(std::min(kMostPart, kMoveThreads / a.heads), std::max<int64_t>(spread, kLeastPart));
+  e.part = (int32_t)std::min(std::min<int64_t>(tokens, kMoveThreads / a.heads), std::max<int64_t>(spread, kLeastPart));
   EvictPlan& p = e.plan;
   p.rows = reinterpret_cast<Shrunk*>(workspace);
   p.count = workspace + 4 * (int64_t)b.rows;

@@ -51,7 +51,7 @@ namespace {
 // 4096 60.8 / 48.1 / 58.1, 256 rows, one of 8192 - / 48.7 / 54.0, 2048 rows of 4096 keys - / 80.5 / 91.7, 4096 rows
 // - / 111.8 / 109.5.
 constexpr int kWideFrom = 64, kLongPrefixFrom = 2048;
-constexpr int kPrefixMinChunk = 2;  // blocks of 64 keys
+constexpr int kPrefixMinChunk = 2;  // blocks of 64 keys; 1 / 2 / 4, us: 64 rows of 8192 keys 44.1 / 43.1 / 44.1
 constexpr int64_t kShareBytes = 160 << 20;
 
 enum Tiles { kShort, kWide, kLong };
