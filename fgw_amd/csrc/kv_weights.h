@@ -17,6 +17,13 @@
 //   weights_columns_kernel the other way round: four waves hold 64 keys each, and up to kColumnRows rows of
 //                          Q go past them, so a lane adds up its own key's weights;
 //   weights_sum_kernel     where a request has more rows than that: the parts' sums.
+//
+// Measured (BF16, 8 K/V heads of 4 rows a token, D 128): one new token of each of 32 requests of up to 4096 keys 45
+// us without the copy of the sums, 3.9 TB/s of K, bound by the longest item's reads (38 us; then 7 for the splits);
+// two prompts of 4096 tokens 359 us, 383 TFLOP/s of the products that the weights need and twice that of those
+// done (stats 191, columns 218 when profiled), bound by exponentials and products in turn: two for a visible pair
+// of either kind, and masked halves of the diagonal's tiles. The last 32 tokens of three prompts of up to 12288
+// keys (FP16, D 96): 34 us, two kernels of one wave of programs, 17 each, most of it their starts and ends.
 #pragma once
 #include "kv_extend.h"
 
@@ -24,7 +31,10 @@
 
 namespace fgw_kv {
 
-constexpr int kKeptRows = 16;
+// Rows of a request and K/V head whose scores are kept: those of one tile. Two passes over K / one with the scores
+// kept, us: 20 rows, 32 requests of 4096 keys 165 / 89 (D 64, 16 requests: 63 / 41), 32 rows, 8 of 4096 50 / 38, one
+// of 32768 52 / 40, 17 rows of 512 keys 21.8 / 16.1.
+constexpr int kKeptRows = ShortTiling::ROWS;
 constexpr int kColumnRows = 1024;  // rows of a part at most
 constexpr int kSumKeys = 256;
 constexpr int kColumnKeys = 256;   // keys of an item
@@ -184,11 +194,13 @@ __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void weights_ro
     const unsigned char* stage = stages + n % S * C::TILE_BYTES;
     // Behind the tile are those of the next S - 1, and from iteration S + 1 on the stores of S iterations
     // (memory instructions retire in order): a wait that left those out would be one for the next tile. The
-    // last and the first iterations wait for more than they need.
+    // last and the first iterations wait for more than they need, and those of more than 24 rows.
     if (rem >= S - 1 && n > S && it.rows <= 8)
       wait_vm<(S - 1) * C::INSTR + S>();
-    else if (rem >= S - 1 && n > S)
+    else if (rem >= S - 1 && n > S && it.rows <= 16)
       wait_vm<(S - 1) * C::INSTR + 2 * S>();
+    else if (rem >= S - 1 && n > S)
+      wait_vm<(S - 1) * C::INSTR + 3 * S>();
     else if (rem >= S - 1)
       wait_vm<(S - 1) * C::INSTR>();
     else
