@@ -404,6 +404,21 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, L
           if (d < s.keep) row[d] = x[k];
         }
       }
+      // Tokens of pages outside the pool, which no part copied: zeros, as such pages read to the attention. (Here,
+      // since the copies have no registers left for it: 120 of 128.)
+      for (int d = still * page + tid; d < s.keep; d += kMoveThreads) {
+        const int at = (int)((u32)source(a, kept, d, s.keep, s.len) / (u32)page), id = a.plan.table[(int64_t)s.row * b.width + at];
+        if (id >= 0 && id < b.pages) continue;
+        const int dp = (int)((u32)d / (u32)page);
+        const int64_t token = (int64_t)a.plan.list[s.place + dp - still] * page + (d - dp * page);
+#pragma unroll 1
+        for (int which = layer; which < 2 * a.layers; which += a.layers) {
+          const int64_t bytes = layers.head_bytes[which];
+          char* const to = layers.data[which] + (token * a.heads + head) * bytes;
+#pragma unroll 1
+          for (int64_t c = 0; c < bytes; c += 16) *reinterpret_cast<u32x4*>(to + c) = u32x4{0u, 0u, 0u, 0u};
+        }
+      }
     }
     return;
   }

@@ -63,6 +63,7 @@ def evict_rows(k_pools, v_pools, scores, refs, table, lens, keep, page_size, *, 
     `first` on; whole pages before that stay, shared or not, and the pages that a row leaves lose a holder.
     Returns int32 [2]: rows refused for want of pages (that call for more, with the rows before them, than
     are free: what this call gives back is free for the next one), rows refused because keep is less than
-    first + recent. Every decision is made on the GPU, the same on every run; nothing is read back.
+    first + recent. Tokens of page ids outside the pools move as zeros. Every decision is made on the GPU, the
+    same on every run; nothing is read back.
     """
     return _kv.evict(k_pools, v_pools, scores, refs, table, lens, keep, page_size, first, recent)

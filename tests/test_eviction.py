@@ -133,6 +133,52 @@ def test_counts_below_what_has_to_stay():
 
 
 @pytest.mark.gpu
+def test_pages_outside_the_pool_move_as_zeros():
+    page, zeros = 16, 39
+    bad = _state([90, 70], page, 8, 40, 2, (64, 32), torch.bfloat16, kind="")
+    bad[3][zeros] = 3  # held, and all zeros
+    for x in bad[0] + bad[1]:
+        x[zeros * page:] = 0.0
+    assert not (bad[4] == zeros).any()
+    good = [[x.clone() for x in part] for part in bad[:3]] + [x.clone() for x in bad[3:]]
+    for r, j, value in ((0, 1, -1), (0, 4, 40), (1, 0, 2**31 - 1)):
+        bad[3][int(bad[4][r, j])] -= 1
+        good[3][int(good[4][r, j])] -= 1
+        bad[4][r, j], good[4][r, j] = value, zeros
+    keep = torch.tensor([50, 33], dtype=torch.int32)
+    dev = [[x.cuda() for x in part] for part in bad[:3]] + [x.cuda() for x in bad[3:]]
+    assert E.evict_rows(*dev, keep.cuda(), page, first=2, recent=7).tolist() == [0, 0]
+    assert X.evict_exact(*good, keep, page, first=2, recent=7) == [0, 0]
+    good[3][zeros] = 3
+    for x, y in zip(dev[0] + dev[1] + dev[2] + dev[3:], good[0] + good[1] + good[2] + good[3:]):
+        assert torch.equal(_bits(x.cpu()), _bits(y))
+
+
+@pytest.mark.gpu
+def test_pools_past_four_gib():
+    """Rows whose offsets pass 32 bits: the same bits as in a small pool."""
+    page, small, large = 64, 30, 50000  # pages of 128 KB
+    state = _state([700, 512], page, 12, small, 8, (128, 128), torch.bfloat16)
+    keep = torch.tensor([300, 512 - 65], dtype=torch.int32).cuda()
+    near = [[x.cuda() for x in part] for part in state[:3]] + [x.cuda() for x in state[3:]]
+    want = E.evict_rows(*near, keep, page, first=70, recent=9)
+    far = [[torch.zeros(large * page, 8, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2)]]
+    for x, y in zip(far[0], (state[0][0], state[1][0])):
+        x[(large - small) * page:] = y.cuda()
+    scores = [state[2][0].cuda()]
+    refs = torch.ones(large, dtype=torch.int32, device="cuda")
+    refs[large - small:] = state[3].cuda()
+    table, lens = torch.where(state[4] < 0, -1, state[4] + large - small).to(torch.int32).cuda(), state[5].cuda()
+    got = E.evict_rows(far[0][:1], far[0][1:], scores, refs, table, lens, keep, page, first=70, recent=9)
+    assert got.tolist() == want.tolist() == [0, 0]
+    assert torch.equal(refs[large - small:], near[3]) and torch.equal(lens, near[5])
+    assert torch.equal(table, torch.where(near[4] < 0, -1, near[4] + large - small))
+    assert torch.equal(scores[0], near[2][0])
+    for x, y in zip(far[0], (near[0][0], near[1][0])):
+        assert torch.equal(x[(large - small) * page:], y)
+
+
+@pytest.mark.gpu
 def test_captured_and_replayed():
     """One graph, with eager calls between its replays, from other books each time."""
     page, width, heads = 16, 8, 2
