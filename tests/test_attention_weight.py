@@ -199,6 +199,22 @@ def test_captured_and_replayed(new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("new", [2, 60])
+def test_a_pool_past_four_gib(new):
+    """Rows whose offsets pass 32 bits: the same bits as in a small pool."""
+    page, large = 64, 50000  # pages of 128 KB
+    k, table, lens, cu = [x.cuda() for x in _cache([new, 1], [700, 90], 8, 128, page, torch.bfloat16)]
+    q = _queries(new + 1, 16, 128, torch.bfloat16).cuda()
+    start = torch.rand(2, 8, table.shape[1] * page, device="cuda")
+    near, far = start.clone(), start.clone()
+    E.add_weights(near, q, k, table, lens, cu, page, new)
+    pool = torch.zeros(large * page, 8, 128, dtype=torch.bfloat16, device="cuda")
+    pool[-k.shape[0]:] = k
+    E.add_weights(far, q, pool, table + (large - k.shape[0] // page), lens, cu, page, new)
+    assert torch.equal(near, far)
+
+
+@pytest.mark.gpu
 def test_two_streams_at_once():
     cache = _cache([1] * 4, [3000, 5, 900, 2], 2, 128, 16, torch.bfloat16)
     dev = [x.cuda() for x in cache]

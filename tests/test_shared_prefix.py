@@ -225,6 +225,24 @@ def test_pages_outside_the_pool_read_as_zeros():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("news", [[1, 1, 2], [40, 50, 30]])
+def test_pools_past_four_gib(news):
+    """Rows whose offsets pass 32 bits: the same bits as in small pools."""
+    page, large = 64, 50000  # pages of 128 KB
+    k, v, table, lens, cu = [x.cuda() for x in _cache([3], [700], news, [n + 70 for n in news], 8, 128, page, torch.bfloat16)]
+    q = _queries(sum(news), 16, 128, torch.bfloat16).cuda()
+    first, prefixes = _offsets([3]).cuda(), torch.tensor([700], dtype=torch.int32).cuda()
+    kernel = S.build_shared_kernel(16, 8, 128, page, "bfloat16", 0, always=True)
+    near = kernel(q, k, v, table, lens, cu, first, prefixes, max(news))
+    pools = [torch.zeros(large * page, 8, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for x, y in zip(pools, (k, v)):
+        x[-y.shape[0]:] = y
+    far = kernel(q, *pools, torch.where(table < 0, -1, table + large - k.shape[0] // page).to(torch.int32), lens, cu, first,
+                 prefixes, max(news))
+    assert torch.equal(near, far)
+
+
+@pytest.mark.gpu
 def test_nan_of_a_key_reaches_the_rows_that_see_it():
     """A NaN among the shared keys: every row of the group is NaN; among one request's own: its rows."""
     for where in ("prefix", "own"):
