@@ -7,7 +7,7 @@
 // L_R needs all keys of a row before the first weight is known, and keys come in splits, so there are
 // two passes. Scores, statistics and sums are fp32; no sum's order hangs on the order of programs.
 //
-// Few rows (up to kKeptRows of a request and K/V head: a decode step). Memory bounds it, so K is read once:
+// Few rows (up to kKeptRows of a request and K/V head: decode, draft tokens). Memory bounds it, so K is read once:
 //   weights_rows_kernel    s = Q K^T as the kernel of few rows of fgw_kv_extend has it (four waves, each
 //                          with 32-key tiles of its own on the way through LDS), kept in the workspace;
 //                          the split's L. A tile of one split is finished at once.
@@ -31,10 +31,14 @@
 
 namespace fgw_kv {
 
-// Rows of a request and K/V head whose scores are kept: those of one tile. Two passes over K / one with the scores
-// kept, us: 20 rows, 32 requests of 4096 keys 165 / 89 (D 64, 16 requests: 63 / 41), 32 rows, 8 of 4096 50 / 38, one
-// of 32768 52 / 40, 17 rows of 512 keys 21.8 / 16.1.
-constexpr int kKeptRows = ShortTiling::ROWS;
+// Rows of a request and K/V head whose scores are kept, in tiles of 32 or 64. The more they are, the more the kept
+// scores weigh against a second reading of K. Two passes over K / one with the scores kept, us, requests of 4096
+// keys, 8 K/V heads: 20 rows, 32 of them 165 / 89, 36 rows 168 / 120, 48 rows 170 / 134, 64 rows 165 / 164 (8
+// requests 50.8 / 49.5, one of 32768 keys 53 / 56); D 64, 16 requests, 20 rows 63 / 41, 48 rows 64 / 58; D 256, 36
+// rows of 4 heads 98 / 62, 64 rows of 8 182 / 118.
+constexpr int kKeptRows = 48, kKeptRowsWide = 64;  // (D > 128)
+template <int NR>
+using KeptTiling = Tiling<32 * NR, ShortTiling::BN, ShortTiling::UNIT>;
 constexpr int kColumnRows = 1024;  // rows of a part at most
 constexpr int kSumKeys = 256;
 constexpr int kColumnKeys = 256;   // keys of an item
@@ -146,21 +150,21 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-template <class C>
+template <class C, int NR>
 __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void weights_rows_kernel(
     WeightParams p, const int32_t* __restrict__ table, const int32_t* __restrict__ lengths, const int32_t* __restrict__ cu) {
-  constexpr int S = kWeightStages<C::DPAD>;
+  constexpr int S = kWeightStages<C::DPAD>, ROWS = 32 * NR;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[C::NWK * S * C::TILE_BYTES];
   // The scores of a wave's last tile, row by row: written to the workspace from here a tile later, whole
   // rows of 128 bytes (straight from the lanes that hold them, 16 bytes each, the stores took a fifth of the
   // time: 32 requests of 4096 keys 78 us, without any of them 64).
   constexpr int kRow = 36;
-  __shared__ __attribute__((aligned(16))) float out[C::NWK][kKeptRows * kRow];
-  __shared__ float cm[C::NWK * kKeptRows], cl[C::NWK * kKeptRows], clse[kKeptRows];
+  __shared__ __attribute__((aligned(16))) float out[C::NWK][ROWS * kRow];
+  __shared__ float cm[C::NWK * ROWS], cl[C::NWK * ROWS], clse[ROWS];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int il = lane & 31, hh = lane >> 5;
   Item it;
-  if (!find_item<ShortTiling>(p, lengths, cu, (int)blockIdx.x, lane, it)) return;
+  if (!find_item<KeptTiling<NR>>(p, lengths, cu, (int)blockIdx.x, lane, it)) return;
   const Lanes<C> ln(lane);
   unsigned char* const stages = smem + wave * S * C::TILE_BYTES;
   const u32 stages_lds = lds_address(stages);
@@ -173,9 +177,17 @@ __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void weights_ro
   const DmaLanes<C> dl(lane, 0, keys.row_bytes);
   auto issue = [&](int n) { keys.template issue<false>(dl, n, stages_lds + (u32)(n % S * C::TILE_BYTES)); };
 
-  u32x4 qf[C::KK];
-  load_q<C>(p, it, il, il < it.rows, hh, qf);
-  const Seen seen = row_seen(p, it, il / p.group);
+  u32x4 qf[NR][C::KK];
+  Seen seen[NR];
+  float m[NR], l[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int row = 32 * r + il;
+    load_q<C>(p, it, row < it.rows ? row : 0, row < it.rows, hh, qf[r]);
+    seen[r] = row_seen(p, it, row / p.group);
+    m[r] = kNegBig;
+    l[r] = 0.0f;
+  }
   const int hi_min = row_seen(p, it, 0).hi;
   float* const kept = p.kept + ((int64_t)it.b * p.heads + it.head) * p.kept_rows * p.keys_pad;
   auto store_kept = [&](int pos0) {  // 8 rows at a time, 8 lanes to a row
@@ -184,23 +196,26 @@ __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void weights_ro
           *reinterpret_cast<const f32x4*>(&out[wave][r * kRow + 4 * (lane % 8)]);
   };
 
-  float m = kNegBig, l = 0.0f;
   keys.ids_ready();
   for (int n = 0; n < S && n < my_n; ++n) issue(n);
 #pragma unroll
-  for (int kk = 0; kk < C::KK; ++kk) asm volatile("" ::"v"(qf[kk]));
+  for (int r = 0; r < NR; ++r)
+#pragma unroll
+    for (int kk = 0; kk < C::KK; ++kk) asm volatile("" ::"v"(qf[r][kk]));
   for (int n = 0; n < my_n; ++n) {
     const int pos0 = first_pos + kStep * n, rem = my_n - 1 - n;
     const unsigned char* stage = stages + n % S * C::TILE_BYTES;
     // Behind the tile are those of the next S - 1, and from iteration S + 1 on the stores of S iterations
     // (memory instructions retire in order): a wait that left those out would be one for the next tile. The
-    // last and the first iterations wait for more than they need, and those of more than 24 rows.
+    // last and the first iterations wait for more than they need, and those of more rows than the count says.
     if (rem >= S - 1 && n > S && it.rows <= 8)
       wait_vm<(S - 1) * C::INSTR + S>();
     else if (rem >= S - 1 && n > S && it.rows <= 16)
       wait_vm<(S - 1) * C::INSTR + 2 * S>();
-    else if (rem >= S - 1 && n > S)
+    else if (rem >= S - 1 && n > S && (NR == 1 || it.rows <= 32))
       wait_vm<(S - 1) * C::INSTR + 3 * S>();
+    else if (rem >= S - 1 && n > S)
+      wait_vm<(S - 1) * C::INSTR + 5 * S>();
     else if (rem >= S - 1)
       wait_vm<(S - 1) * C::INSTR>();
     else
@@ -212,52 +227,62 @@ __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void weights_ro
     wait_lds();
     __builtin_amdgcn_sched_barrier(0);
     if (rem >= S) issue(n + S);
-    f32x16 s[1], t;
+    f32x16 s[NR][1];
 #pragma unroll
-    for (int v = 0; v < 16; ++v) s[0][v] = t[v] = 0.0f;
+    for (int r = 0; r < NR; ++r) {
+      f32x16 t;
 #pragma unroll
-    for (int kk = 0; kk < C::KK; kk += 2) {
-      s[0] = Elem<C::BF16>::mma(ka[kk], qf[kk], s[0]);
-      t = Elem<C::BF16>::mma(ka[kk + 1], qf[kk + 1], t);
+      for (int v = 0; v < 16; ++v) s[r][0][v] = t[v] = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < C::KK; kk += 2) {
+        s[r][0] = Elem<C::BF16>::mma(ka[kk], qf[r][kk], s[r][0]);
+        t = Elem<C::BF16>::mma(ka[kk + 1], qf[r][kk + 1], t);
+      }
+      s[r][0] += t;
+      if (pos0 + C::BN > hi_min) mask_seen<C>(s[r], pos0, seen[r], hh);
+      float sum = exp_sum(s[r][0], m[r], p.scale_log2);
+      if (__ballot(!(sum <= kSoftmaxSumBound))) {
+        const float top = fmaxf(m[r], row_max<C>(s[r], p.scale_log2));
+        l[r] *= __builtin_amdgcn_exp2f(m[r] - top);
+        m[r] = top;
+        sum = exp_sum(s[r][0], top, p.scale_log2);
+      }
+      l[r] += sum;
     }
-    s[0] += t;
-    if (pos0 + C::BN > hi_min) mask_seen<C>(s, pos0, seen, hh);
-    float sum = exp_sum(s[0], m, p.scale_log2);
-    if (__ballot(!(sum <= kSoftmaxSumBound))) {
-      const float top = fmaxf(m, row_max<C>(s, p.scale_log2));
-      l *= __builtin_amdgcn_exp2f(m - top);
-      m = top;
-      sum = exp_sum(s[0], m, p.scale_log2);
-    }
-    l += sum;
     if (n > 0) store_kept(pos0 - kStep);
     wave_fence();
-    if (il < it.rows) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(&out[wave][il * kRow + 8 * g + 4 * hh]) =
-            f32x4{s[0][4 * g], s[0][4 * g + 1], s[0][4 * g + 2], s[0][4 * g + 3]} * p.scale_log2;
+    for (int r = 0; r < NR; ++r) {
+      if (32 * r + il < it.rows) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(&out[wave][(32 * r + il) * kRow + 8 * g + 4 * hh]) =
+              f32x4{s[r][0][4 * g], s[r][0][4 * g + 1], s[r][0][4 * g + 2], s[r][0][4 * g + 3]} * p.scale_log2;
+      }
     }
     wave_fence();
   }
   if (my_n > 0) store_kept(first_pos + kStep * (my_n - 1));
 
-  const float tot = pair_sum(l);
-  if (hh == 0 && il < it.rows) {
-    cm[wave * kKeptRows + il] = m;
-    cl[wave * kKeptRows + il] = tot;
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const float tot = pair_sum(l[r]);
+    if (hh == 0 && 32 * r + il < it.rows) {
+      cm[wave * ROWS + 32 * r + il] = m[r];
+      cl[wave * ROWS + 32 * r + il] = tot;
+    }
   }
   wait_vm<0>();  // the kept scores of every wave
   __syncthreads();
   if (tid < it.rows) {
     float mm = kNegBig, t2 = 0.0f;
 #pragma unroll
-    for (int k = 0; k < C::NWK; ++k) mm = fmaxf(mm, cm[k * kKeptRows + tid]);
+    for (int k = 0; k < C::NWK; ++k) mm = fmaxf(mm, cm[k * ROWS + tid]);
 #pragma unroll
-    for (int k = 0; k < C::NWK; ++k) t2 += cl[k * kKeptRows + tid] * __builtin_amdgcn_exp2f(cm[k * kKeptRows + tid] - mm);
+    for (int k = 0; k < C::NWK; ++k) t2 += cl[k * ROWS + tid] * __builtin_amdgcn_exp2f(cm[k * ROWS + tid] - mm);
     const float lse = lse2_of(mm, t2);
     clse[tid] = lse;
-    if (it.splits > 1) p.lse[(int64_t)it.slot * kKeptRows + tid] = lse;
+    if (it.splits > 1) p.lse[(int64_t)it.slot * ROWS + tid] = lse;
   }
   if (it.splits > 1) return;
   __syncthreads();
@@ -266,20 +291,20 @@ __global__ __launch_bounds__(C::THREADS, C::DPAD == 256 ? 1 : 2) void weights_ro
 
 // The items of weights_rows_kernel again, those of split tiles.
 constexpr int kFinishThreads = 256;
-static __global__ __launch_bounds__(kFinishThreads) void weights_finish_kernel(WeightParams p,
-                                                                              const int32_t* __restrict__ lengths,
-                                                                              const int32_t* __restrict__ cu) {
-  __shared__ float part[kFinishThreads], clse[kKeptRows];
+template <int NR>
+__global__ __launch_bounds__(kFinishThreads) void weights_finish_kernel(WeightParams p, const int32_t* __restrict__ lengths,
+                                                                       const int32_t* __restrict__ cu) {
+  constexpr int ROWS = 32 * NR, kShare = kFinishThreads / ROWS;
+  __shared__ float part[kFinishThreads], clse[ROWS];
   const int tid = threadIdx.x;
   Item it;
-  if (!find_item<ShortTiling>(p, lengths, cu, (int)blockIdx.x, tid & 63, it) || it.splits == 1) return;
-  // 16 threads to a row, then its first one.
-  const int r = tid % kKeptRows, g = tid / kKeptRows;
-  constexpr int kShare = kFinishThreads / kKeptRows;
+  if (!find_item<KeptTiling<NR>>(p, lengths, cu, (int)blockIdx.x, tid & 63, it) || it.splits == 1) return;
+  // kShare threads to a row, then its first one.
+  const int r = tid % ROWS, g = tid / ROWS;
   float m = kNegBig, l = 0.0f;
   if (r < it.rows) {
     for (int s = g; s < it.splits; s += kShare) {
-      const float x = p.lse[(int64_t)(it.slot0 + s * it.slot_step) * kKeptRows + r], top = fmaxf(m, x);
+      const float x = p.lse[(int64_t)(it.slot0 + s * it.slot_step) * ROWS + r], top = fmaxf(m, x);
       l = l * __builtin_amdgcn_exp2f(m - top) + __builtin_amdgcn_exp2f(x - top);
       m = top;
     }
@@ -288,12 +313,12 @@ static __global__ __launch_bounds__(kFinishThreads) void weights_finish_kernel(W
   __syncthreads();
   if (tid < it.rows) {
     float top = kNegBig, sum = 0.0f;
-    for (int k = 0; k < kShare; ++k) top = fmaxf(top, part[k * kKeptRows + tid]);
-    for (int k = 0; k < kShare; ++k) sum += __builtin_amdgcn_exp2f(part[k * kKeptRows + tid] - top);
+    for (int k = 0; k < kShare; ++k) top = fmaxf(top, part[k * ROWS + tid]);
+    for (int k = 0; k < kShare; ++k) sum += __builtin_amdgcn_exp2f(part[k * ROWS + tid] - top);
     clse[tid] = lse2_of(top, sum);
   }
   __syncthreads();
-  const int from = it.blk_begin * ShortTiling::BN, to = it.blk_end * ShortTiling::BN;
+  const int from = it.blk_begin * KeptTiling<NR>::BN, to = it.blk_end * KeptTiling<NR>::BN;
   finish_keys(p, it, clse, from, to < it.len ? to : it.len, tid, kFinishThreads);
 }
 
@@ -749,7 +774,10 @@ template <bool BF16, int DPAD>
 hipError_t launch_weights(const WeightParams& p, bool many, int grid, int columns, hipStream_t stream) {
   if (!many) {
     using C = Cfg<BF16, DPAD, kLayoutKey, DPAD == 128 ? 1 : 0>;
-    weights_rows_kernel<C><<<dim3(grid), dim3(C::THREADS), 0, stream>>>(p, p.table, p.lengths, p.cu);
+    if (p.kept_rows <= 32)
+      weights_rows_kernel<C, 1><<<dim3(grid), dim3(C::THREADS), 0, stream>>>(p, p.table, p.lengths, p.cu);
+    else
+      weights_rows_kernel<C, 2><<<dim3(grid), dim3(C::THREADS), 0, stream>>>(p, p.table, p.lengths, p.cu);
   } else {
     using C = WCfg<BF16, DPAD>;
     weights_stats_kernel<C><<<dim3(grid), dim3(C::THREADS), 0, stream>>>(p, p.table, p.lengths, p.cu);

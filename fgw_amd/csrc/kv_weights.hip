@@ -67,7 +67,7 @@ WeightPlan plan_weights(const fgw_kv_weights_args& a) {
   const int64_t rows = std::min(a.last, a.tokens) * group, requests = std::min(a.batch, a.tokens);
   auto blocks = [&](int64_t size) { return std::min(requests * ((rows + size - 1) / size), total / size + requests); };
   p.keys_pad = (capacity + kColumnKeys - 1) / kColumnKeys * kColumnKeys;
-  p.many = rows > kKeptRows;
+  p.many = rows > (a.dim <= 128 ? kKeptRows : kKeptRowsWide);
   if (!p.many) {
     p.launch.min_chunk = kRowsMinChunk;
     p.launch.whole = a.dim <= 64 ? kRowsWholeNarrow : kRowsWhole;
@@ -75,10 +75,10 @@ WeightPlan plan_weights(const fgw_kv_weights_args& a) {
     p.launch.tiles = requests;
     fgw_kv_extend_args rounds = e;
     rounds.num_cus = p.launch.tiles * a.kv_heads >= e.num_cus ? kManyItems : kFewItems;
-    plan_items<ShortTiling>(p.launch, rounds, true);
+    plan_items<KeptTiling<1>>(p.launch, rounds, true);  // (the same for tiles of 64 rows)
     p.kept_rows = rows;
     p.kept = (int64_t)a.batch * a.kv_heads * rows * p.keys_pad;
-    p.lse = p.launch.slots * kKeptRows;
+    p.lse = p.launch.slots * (rows <= 32 ? 32 : 64);
   } else {
     p.launch.min_chunk = kLongMinChunk;
     p.launch.many = 1 << 20;
@@ -181,8 +181,12 @@ int fgw_kv_weights(const fgw_kv_weights_args* args, hipStream_t stream) {
   w.request_notes = reinterpret_cast<int32_t*>(w.lse + (p.lse + 3) / 4 * 4);
   const hipError_t e = a.dtype == FGW_KV_BFLOAT16 ? launch<true>(w, p, stream) : launch<false>(w, p, stream);
   if (e != hipSuccess) return fail(FGW_MHA_EHIP, "fgw_kv_weights: %s", hipGetErrorString(e));
-  if (!p.many && p.launch.target > 0)
-    weights_finish_kernel<<<dim3((unsigned)p.launch.items), dim3(kFinishThreads), 0, stream>>>(w, w.lengths, w.cu);
+  if (!p.many && p.launch.target > 0) {
+    if (w.kept_rows <= 32)
+      weights_finish_kernel<1><<<dim3((unsigned)p.launch.items), dim3(kFinishThreads), 0, stream>>>(w, w.lengths, w.cu);
+    else
+      weights_finish_kernel<2><<<dim3((unsigned)p.launch.items), dim3(kFinishThreads), 0, stream>>>(w, w.lengths, w.cu);
+  }
   if (p.sums > 0)
     weights_sum_kernel<<<dim3((unsigned)p.sums), dim3(kFinishThreads), 0, stream>>>(w, w.lengths, w.cu);
   return launched("fgw_kv_weights");

@@ -92,6 +92,11 @@ CASES = {
     "parts_of_512": ([1400] * 3, [1400, 3000 + 200, 1500], 4, 2, 64, 64, 1400, 1.0),
     "many_requests_rows": ([17 + i % 60 for i in range(130)], [17 + i % 60 + (41 * i) % 700 for i in range(130)], 8, 1, 64, 16, 70, 0.5),
     "dim_160_rows": ([90, 300], [1300, 300], 6, 2, 160, 32, 200, 1.0),
+    "kept_33_rows": ([33, 40, 1, 32], [33, 3000, 50, 700], 4, 4, 128, 16, 40, 0.5),
+    "kept_48_rows": ([12, 3, 12], [5000, 90, 12], 8, 2, 64, 64, 12, 1.0),
+    "kept_49_rows": ([49, 7], [900, 90], 2, 2, 96, 48, 49, 1.0),
+    "kept_64_rows_wide": ([16, 2, 9], [2500, 90, 9], 8, 2, 256, 64, 16, 1.0),
+    "kept_65_rows_wide": ([65, 3], [300, 90], 2, 2, 160, 16, 65, 1.0),
     "longer_than_cache": ([300, 20], [100, 7], 4, 2, 128, 16, 300, 1.0),
     "parts_longer_than_cache": ([1500], [700], 2, 1, 64, 16, 1500, 1.0),
 }
