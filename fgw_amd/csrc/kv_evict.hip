@@ -19,8 +19,8 @@
 //                        a head: it reads a stretch, then writes it; kept tokens only move down); the books,
 //                        with the last layers.
 // Measured (BF16, D 128, 8 K/V heads): 16 rows of up to 4096 keys, 12 of them cut to 1000, four layers: select
-// 13 us, as long as a program's chain of passes and scans takes, moves 73 us, 5.3 TB/s of the 393 MB that they
-// read and write, at memory's rate. One row of 381 keys (FP16, D 64) cut to 200: 8 and 6 us, chains of reads.
+// 13 us, as long as a program's chain of passes and scans takes, moves 78 us (profiled), 5.0 TB/s of the 393 MB
+// that they read and write, at memory's rate. One row of 381 keys (FP16, D 64) cut to 200: 8 and 6 us, chains of reads.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
