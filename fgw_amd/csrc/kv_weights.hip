@@ -24,8 +24,10 @@ constexpr int kStatsItems = 512;
 // requests, 37.8 at 512 and 42.5 at 1024 (256: 40.3).
 constexpr int kFewItems = 512, kManyItems = 768;
 
+constexpr int64_t kKeptBytes = 256 << 20;
+
 struct WeightPlan {
-  bool many;       // rows of a request and K/V head, at most, past kKeptRows
+  bool many;       // rows of a request and K/V head, at most, past kKeptRows, or too many scores to keep
   Launch launch;   // of the first pass
   int part_rows;
   int columns, sums;  // grids of the persistent kernels; 0: no launch
@@ -67,7 +69,10 @@ WeightPlan plan_weights(const fgw_kv_weights_args& a) {
   const int64_t rows = std::min(a.last, a.tokens) * group, requests = std::min(a.batch, a.tokens);
   auto blocks = [&](int64_t size) { return std::min(requests * ((rows + size - 1) / size), total / size + requests); };
   p.keys_pad = (capacity + kColumnKeys - 1) / kColumnKeys * kColumnKeys;
-  p.many = rows > (a.dim <= 128 ? kKeptRows : kKeptRowsWide);
+  // (Kept scores have a place for every key that the table could hold: no more of them than the pool has bytes.)
+  const int64_t kept = (int64_t)a.batch * a.kv_heads * rows * p.keys_pad;
+  const int64_t bound = std::max<int64_t>(kKeptBytes, a.pool_rows * a.kv_heads * a.dim * 2);
+  p.many = rows > (a.dim <= 128 ? kKeptRows : kKeptRowsWide) || kept * 4 > bound;
   if (!p.many) {
     p.launch.min_chunk = kRowsMinChunk;
     p.launch.whole = a.dim <= 64 ? kRowsWholeNarrow : kRowsWhole;
@@ -77,7 +82,7 @@ WeightPlan plan_weights(const fgw_kv_weights_args& a) {
     rounds.num_cus = p.launch.tiles * a.kv_heads >= e.num_cus ? kManyItems : kFewItems;
     plan_items<KeptTiling<1>>(p.launch, rounds, true);  // (the same for tiles of 64 rows)
     p.kept_rows = rows;
-    p.kept = (int64_t)a.batch * a.kv_heads * rows * p.keys_pad;
+    p.kept = kept;
     p.lse = p.launch.slots * (rows <= 32 ? 32 : 64);
   } else {
     p.launch.min_chunk = kLongMinChunk;

@@ -226,7 +226,8 @@ int fgw_pages_copy(const fgw_pages_pools* pools, int32_t pages, const int32_t* s
  * with them, and lens[r] = keep[r]. The tokens from the page of token `first` on go to fresh pages, lowest id
  * first, rows in order; the old pages lose a holder. A row is left where keep[r] < first + recent
  * (status[1]), and where its pages, with those of the rows before it, are more than the free ones
- * (status[0]): the pages that a call gives back are free for the next one. */
+ * (status[0]): the pages that a call gives back are free for the next one. Tokens of page ids outside the pools
+ * move as zeros. */
 typedef struct {
   const int32_t* keep;        /* [rows], device; negative: the row stays */
   void* const* k_pools;       /* [layers], host; each [pages * page_size, heads, head bytes] */

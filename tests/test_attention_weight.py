@@ -204,6 +204,17 @@ def test_captured_and_replayed(new):
 
 
 @pytest.mark.gpu
+def test_a_table_far_wider_than_the_pool():
+    """Few rows, and places for more scores than the pool has bytes."""
+    k, table, lens, cu = _cache([2, 1, 2, 0], [700, 90, 2, 40], 2, 64, 64, torch.bfloat16)
+    wide = torch.full((4, 17000), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    cache, q = (k, wide, lens, cu), _queries(5, 8, 64, torch.bfloat16)
+    scores = _scores(cache, 2, 64)
+    _check(_run(scores, q, cache, 64, 2, decay=0.5), scores, q, cache, 64, 2, "wide", decay=0.5)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [2, 60])
 def test_a_pool_past_four_gib(new):
     """Rows whose offsets pass 32 bits: the same bits as in a small pool."""
@@ -312,5 +323,8 @@ def test_workspace_follows_the_sizes():
     # A decode step keeps the scores of its rows, and little beside them.
     kept = 64 * 8 * 4 * 4096
     assert kept <= need(tokens=64, batch=64, heads=32, kv_heads=8, last=1, width=256, scores_stride=4096) < kept * 1.02
+    # A table with places for more scores than the pool has bytes: two passes, which keep none.
+    wide = dict(tokens=64, batch=64, heads=32, kv_heads=8, last=1, width=8192, scores_stride=131072, page_size=16)
+    assert need(**wide, pool_rows=1 << 22) > 64 * 8 * 4 * 131072 > (64 << 20) > need(**wide, pool_rows=1 << 16)
     # Prompts: statistics of every row, and sums of each part of 1024 of them for each key.
     assert need(tokens=8192, batch=2, heads=32, kv_heads=8, last=4096, width=256, scores_stride=4096) < 2 * 34 * 8 * 4096
