@@ -612,12 +612,19 @@ __global__ __launch_bounds__(C::THREADS, kWaveSimd) void weights_columns_kernel(
       src[q] = static_cast<const char*>(p.q) + (int64_t)(it.first + token) * p.q_token +
                (int64_t)(it.head * p.group + src_head[q]) * p.q_head + c * 16;
     }
+    // Places behind the part's rows take its last row again, which weighs nothing there (its L is infinite): zeros
+    // would give NaN beside a key that holds an infinity. They are in a request's last part alone, and its
+    // last row sees every key, so what is NaN with it is NaN in any case.
+    static_assert(kApart % C::KSW == 0 && kColumnRows / 4 % C::BN == 0, "a lane's chunk is the same in all its rows");
+    const char* const last_row = static_cast<const char*>(p.q) + (int64_t)(it.first + it.n - 1) * p.q_token +
+                                 (int64_t)(it.head * p.group + p.group - 1) * p.q_head +
+                                 (lane % C::CPR ^ (C::RPI * wave + lane / C::CPR) % C::KSW) * 16;
     auto issue_tile = [&](int, int at) {
       const char* zero = reinterpret_cast<const char*>(kZeroChunk);
 #pragma unroll
       for (int q = 0; q < U; ++q) {
-        const bool live = next_row < end - q * kApart && (p.dim == C::DPAD || (live_dims >> q & 1u));
-        dma_flat(live ? src[q] : zero, lds + (u32)at + 1024u * (u32)(q * C::NWQ + wave));
+        const char* const row = next_row < end - q * kApart ? src[q] : last_row;
+        dma_flat(p.dim == C::DPAD || (live_dims >> q & 1u) ? row : zero, lds + (u32)at + 1024u * (u32)(q * C::NWQ + wave));
         src_head[q] += skip;
         const bool wrap = src_head[q] >= p.group;
         src_head[q] -= wrap ? p.group : 0;
