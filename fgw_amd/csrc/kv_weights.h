@@ -133,9 +133,12 @@ __device__ __forceinline__ void finish_keys(const WeightParams& p, const Item& i
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float lse = lse2[r0 + k < it.rows ? r0 + k : 0];
+        // Keys that the row sees: its own are NaN where L is, also one whose score is minus infinity, as those
+        // that it does not see are kept. (Those weigh nothing beside any other L.)
+        int hi = r0 + k < it.rows ? to : 0;
+        if (lse != lse && r0 + k < it.rows) hi = row_seen(p, it, (r0 + k) / p.group).hi;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          sum[i] += r0 + k >= it.rows || s[k][i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s[k][i] - lse);
+        for (int i = 0; i < 4; ++i) sum[i] += key + i < hi ? __builtin_amdgcn_exp2f(s[k][i] - lse) : 0.0f;
       }
     }
 #pragma unroll

@@ -17,9 +17,11 @@ def _relative(q, k, used, g, length, scale):
     return unit * (2 * (d + 8) * s + length / 32 + 16 + 4 * (s + math.log(length) + 1) + g * used / 8 + 34) + 2.0 ** -20
 
 
-# (new tokens, keys before them, query heads, K/V heads, D, page): rows that leave a tile part empty and ones that
-# fill it, split, in parts, at D 256.
-SHAPES = {"rows_50": (50, 300, 1, 1, 64, 16), "rows_99": (33, 1000, 3, 1, 96, 48), "full_tiles": (64, 500, 2, 2, 128, 64), "parts": (1100, 40, 1, 1, 64, 16),
+# (new tokens, keys before them, query heads, K/V heads, D, page): scores kept, whole and split, 32 rows and 64;
+# two passes with rows that leave a tile part empty, split, in parts, at D 256.
+SHAPES = {"one": (1, 90, 1, 1, 64, 16), "kept": (3, 300, 4, 1, 64, 16), "kept_split": (2, 9000, 8, 2, 128, 64),
+          "kept_tall": (11, 700, 8, 2, 128, 16), "kept_wide": (16, 700, 4, 1, 256, 16), "rows_50": (50, 300, 1, 1, 64, 16),
+          "rows_99": (33, 1000, 3, 1, 96, 48), "full_tiles": (64, 500, 2, 2, 128, 64), "parts": (1100, 40, 1, 1, 64, 16),
           "rows_wide": (67, 400, 1, 1, 256, 16)}
 
 
