@@ -865,13 +865,16 @@ __device__ __forceinline__ float lse_of(float m_log2, float total) {
   return total > 0.0f ? (m_log2 + log2f(total)) * kLn2 : kNegBig;
 }
 
-// floor(nblk * s / splits): the first key block of split s (0 <= s <= splits
-// <= 256). 32-bit arithmetic whenever the product fits, which avoids the
-// 64-bit division routine.
-__device__ __forceinline__ int split_bound(int nblk, int s, int splits) {
-  if (nblk < (1 << 24)) return (int)(((u32)nblk * (u32)s) / (u32)splits);
+// floor(nblk * s / splits): the first key block of split s (0 <= s <= splits <= kMostSplits). 32-bit
+// arithmetic whenever the product fits, which avoids the 64-bit division routine.
+constexpr int kMostSplits = 1024, kBlocksIn32 = 1 << 22;
+__host__ __device__ constexpr __forceinline__ int split_bound(int nblk, int s, int splits) {
+  if (nblk < kBlocksIn32) return (int)(((u32)nblk * (u32)s) / (u32)splits);
   return (int)((int64_t)nblk * s / splits);
 }
+static_assert((uint64_t)(kBlocksIn32 - 1) * kMostSplits <= 0xffffffffu, "the products that are taken in 32 bits fit");
+static_assert(split_bound(1 << 23, 512, 512) == 1 << 23 && split_bound(9000000, 767, 768) == 8988281 &&
+              split_bound((1 << 24) - 1, 1024, 1024) == (1 << 24) - 1, "bounds of long tables");
 
 // Splits of a request of len live keys in a length-balanced plan: enough
 // that none holds more than split_keys keys, at least 1, at most splits.

@@ -29,9 +29,10 @@ constexpr int kRowsWhole = 3, kRowsWholeNarrow = 4;  // (D <= 64)
 constexpr int kRowsMany = 16, kRowsManyTall = 8;  // (requests of more than 8 rows)
 
 // Compute units that a call fills at most: those of the card. They bound splits and workspace (256
-// places of 132 KB), so that offsets of partials and the products of split_bound stay in 32 bits
-// whatever num_cus a caller gives.
+// places of 132 KB), so that offsets of partials that a launch joins itself and the products of split_bound
+// stay in 32 bits whatever num_cus a caller gives.
 constexpr int kMostCus = 256;
+static_assert(kMostCus <= fgw_mha::kMostSplits, "split_bound");
 
 template <class P>
 using ExtendLaunch = hipError_t (*)(const P&, int, hipStream_t);

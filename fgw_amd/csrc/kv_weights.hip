@@ -23,6 +23,7 @@ constexpr int kStatsItems = 512;
 // 86.0 / 93.0, all of 8192 keys 124.6 / 125.0 / 131.8, 64 of 2048 63.8 / 66.0 / 72.6; 8 of 8192, of few
 // requests, 37.8 at 512 and 42.5 at 1024 (256: 40.3).
 constexpr int kFewItems = 512, kManyItems = 768;
+static_assert(std::max({kStatsItems, kFewItems, kManyItems}) <= fgw_mha::kMostSplits, "split_bound");
 
 constexpr int64_t kKeptBytes = 256 << 20;
 
