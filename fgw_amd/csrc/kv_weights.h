@@ -17,6 +17,8 @@
 //   weights_columns_kernel the other way round: four waves hold 64 keys each, and up to kColumnRows rows of
 //                          Q go past them, so a lane adds up its own key's weights;
 //   weights_sum_kernel     where a request has more rows than that: the parts' sums.
+// The last two go over a range of keys at a time, where the partial sums of all of them would be too many
+// (kv_weights.hip).
 //
 // Measured (BF16, 8 K/V heads of 4 rows a token, D 128): one new token of each of 32 requests of up to 4096 keys 45
 // us without the copy of the sums, 3.9 TB/s of K, bound by the longest item's reads (38 us; then 7 for the splits);
@@ -40,18 +42,18 @@ constexpr int kKeptRows = 48, kKeptRowsWide = 64;  // (D > 128)
 template <int NR>
 using KeptTiling = Tiling<32 * NR, ShortTiling::BN, ShortTiling::UNIT>;
 constexpr int kColumnRows = 1024;  // rows of a part at most
-constexpr int kSumKeys = 256;
-constexpr int kColumnKeys = 256;   // keys of an item
+constexpr int kColumnKeys = 256;   // keys of an item, of its sums too
 constexpr int kWaveSimd = 2;       // waves to a SIMD
 
 struct WeightParams : ExtendParams {
   float* scores;    // [batch, heads, stride]
   int64_t stride;
   float* kept;      // few rows: [batch, heads, kept_rows, keys_pad] scores in log2 units
-  float* sums;      // more rows: [parts, heads, keys_pad]
+  float* sums;      // more rows: [parts, heads, keys_pad], of the keys of a launch
   int32_t* request_notes;  // more rows: [batch] WeightNote
   int32_t last, kept_rows, keys_pad, parts_most;
   int32_t part_rows, part_shift;  // rows of a part: kColumnRows or a half or a quarter of it; their log2
+  int32_t block_from, block_to;   // blocks of kColumnKeys keys of a launch
   float decay;
 };
 template <>
@@ -509,20 +511,27 @@ __device__ __forceinline__ int blocks_seen(const WeightParams& p, int n, int len
   const int last = (int)((u32)((end < rows ? end : rows) - 1) / (u32)p.group), hi = len - n + last + 1;
   return hi > 0 ? (hi + kColumnKeys - 1) / kColumnKeys : 0;
 }
+// Those of a launch among the first `blocks`.
+__device__ __forceinline__ int blocks_here(const WeightParams& p, int blocks) {
+  const int to = blocks < p.block_to ? blocks : p.block_to;
+  return to > p.block_from ? to - p.block_from : 0;
+}
 struct ColumnRequest {
   Request r;
   int parts, items;
+  int places;  // for partial sums: none where one part has all rows
 };
 template <bool SUM>
 __device__ __forceinline__ ColumnRequest column_request(const WeightParams& p, const int32_t* lengths, const int32_t* cu, int b) {
   ColumnRequest x;
   x.r = load_request<StatsTiling>(p, lengths, cu, b);
   x.parts = x.r.tiles ? (int)(((int64_t)x.r.n * p.group + p.part_rows - 1) >> p.part_shift) : 0;
+  x.places = x.parts > 1 ? x.parts : 0;
   x.items = 0;
   if (SUM)
-    x.items = x.parts > 1 ? (x.r.len + kSumKeys - 1) / kSumKeys : 0;
+    x.items = x.parts > 1 ? blocks_here(p, (x.r.len + kColumnKeys - 1) / kColumnKeys) : 0;
   else
-    for (int c = 0; c < x.parts; ++c) x.items += blocks_seen(p, x.r.n, x.r.len, c);
+    for (int c = 0; c < x.parts; ++c) x.items += blocks_here(p, blocks_seen(p, x.r.n, x.r.len, c));
   return x;
 }
 template <bool SUM>
@@ -531,10 +540,10 @@ __device__ __forceinline__ bool find_column(const WeightParams& p, const int32_t
   const int64_t g = w / p.heads;
   it.head = (int)(w - g * p.heads);
   int64_t before = 0;
-  int parts_before = 0;
+  int places_before = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
     const ColumnRequest x = b0 == 0 ? x0 : column_request<SUM>(p, lengths, cu, b0 + lane);
-    const int items_to = wave_incl_sum(x.items, lane), parts_to = wave_incl_sum(x.parts, lane);
+    const int items_to = wave_incl_sum(x.items, lane), places_to = wave_incl_sum(x.places, lane);
     const int64_t at = g - before - (items_to - x.items);
     const uint64_t hit = __ballot(at >= 0 && at < x.items);
     if (hit) {
@@ -546,14 +555,14 @@ __device__ __forceinline__ bool find_column(const WeightParams& p, const int32_t
       it.len = pick(x.r.len);
       it.from = pick(x.r.from);
       it.parts = pick(x.parts);
-      it.part0 = parts_before + pick(parts_to - x.parts);
-      it.block = pick((int)at);
+      it.part0 = places_before + pick(places_to - x.places);
+      it.block = p.block_from + pick((int)at);
       it.part = 0;
       if (SUM || it.parts == 1) return true;
       for (int c0 = 0; c0 < it.parts; c0 += 64) {  // the part: one to a lane
-        const int c = it.parts - 1 - c0 - lane, n = c >= 0 ? blocks_seen(p, it.n, it.len, c) : 0;
+        const int c = it.parts - 1 - c0 - lane, n = c >= 0 ? blocks_here(p, blocks_seen(p, it.n, it.len, c)) : 0;
         const int to = wave_incl_sum(n, lane);
-        const uint64_t here = __ballot(it.block < to);
+        const uint64_t here = __ballot(it.block - p.block_from < to);
         if (here) {
           const int k = __builtin_ctzll(here);
           it.part = it.parts - 1 - c0 - k;
@@ -565,7 +574,7 @@ __device__ __forceinline__ bool find_column(const WeightParams& p, const int32_t
       return false;
     }
     before += __builtin_amdgcn_readlane(items_to, 63);
-    parts_before += __builtin_amdgcn_readlane(parts_to, 63);
+    places_before += __builtin_amdgcn_readlane(places_to, 63);
   }
   return false;
 }
@@ -746,7 +755,7 @@ __global__ __launch_bounds__(C::THREADS, kWaveSimd) void weights_columns_kernel(
         if (it.parts == 1)
           add_score(p, p.scores + ((int64_t)it.b * p.heads + it.head) * p.stride, key, it.from, sum);
         else if (it.part0 + it.part < p.parts_most)
-          p.sums[((int64_t)(it.part0 + it.part) * p.heads + it.head) * p.keys_pad + key] = sum;
+          p.sums[((int64_t)(it.part0 + it.part) * p.heads + it.head) * p.keys_pad + (key - p.block_from * kColumnKeys)] = sum;
       }
     }
   }
@@ -758,13 +767,13 @@ static __global__ __launch_bounds__(kFinishThreads) void weights_sum_kernel(Weig
   const ColumnRequest r0 = column_request<true>(p, lengths, cu, lane);
   Column it;
   for (int64_t w = blockIdx.x; find_column<true>(p, lengths, cu, w, lane, r0, it); w += gridDim.x) {
-    const int end = it.len < (it.block + 1) * kSumKeys ? it.len : (it.block + 1) * kSumKeys;
+    const int end = it.len < (it.block + 1) * kColumnKeys ? it.len : (it.block + 1) * kColumnKeys;
     float* const row = p.scores + ((int64_t)it.b * p.heads + it.head) * p.stride;
-    for (int key = it.block * kSumKeys + tid; key < end; key += kFinishThreads) {
+    for (int key = it.block * kColumnKeys + tid; key < end; key += kFinishThreads) {
       // Parts whose rows all come before the key's block left nothing.
       float sum = 0.0f;
       const int last = it.part0 + it.parts < p.parts_most ? it.part0 + it.parts : p.parts_most;
-      const float* const at = p.sums + (int64_t)it.head * p.keys_pad + key;
+      const float* const at = p.sums + (int64_t)it.head * p.keys_pad + (key - p.block_from * kColumnKeys);
       const int64_t step = (int64_t)p.heads * p.keys_pad;
       int c = it.part0 + (first_row(p, it, key / kColumnKeys * kColumnKeys) >> p.part_shift);
       for (; c + 4 <= last; c += 4) {
@@ -781,7 +790,7 @@ static __global__ __launch_bounds__(kFinishThreads) void weights_sum_kernel(Weig
 }
 
 template <bool BF16, int DPAD>
-hipError_t launch_weights(const WeightParams& p, bool many, int grid, int columns, hipStream_t stream) {
+hipError_t launch_weights(const WeightParams& p, bool many, int grid, hipStream_t stream) {
   if (!many) {
     using C = Cfg<BF16, DPAD, kLayoutKey, DPAD == 128 ? 1 : 0>;
     if (p.kept_rows <= 32)
@@ -791,8 +800,13 @@ hipError_t launch_weights(const WeightParams& p, bool many, int grid, int column
   } else {
     using C = WCfg<BF16, DPAD>;
     weights_stats_kernel<C><<<dim3(grid), dim3(C::THREADS), 0, stream>>>(p, p.table, p.lengths, p.cu);
-    weights_columns_kernel<C><<<dim3(columns), dim3(C::THREADS), 0, stream>>>(p, p.table, p.lengths, p.cu);
   }
+  return hipGetLastError();
+}
+template <bool BF16, int DPAD>
+hipError_t launch_weights_columns(const WeightParams& p, int grid, hipStream_t stream) {
+  using C = WCfg<BF16, DPAD>;
+  weights_columns_kernel<C><<<dim3(grid), dim3(C::THREADS), 0, stream>>>(p, p.table, p.lengths, p.cu);
   return hipGetLastError();
 }
 

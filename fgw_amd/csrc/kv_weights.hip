@@ -7,8 +7,9 @@
 
 namespace fgw_kv {
 
-#define FGW_KV_EXTERN_WEIGHTS(BF, DP) \
-  extern template hipError_t launch_weights<BF, DP>(const WeightParams&, bool, int, int, hipStream_t);
+#define FGW_KV_EXTERN_WEIGHTS(BF, DP)                                                              \
+  extern template hipError_t launch_weights<BF, DP>(const WeightParams&, bool, int, hipStream_t); \
+  extern template hipError_t launch_weights_columns<BF, DP>(const WeightParams&, int, hipStream_t);
 FGW_KV_EXTERN_WEIGHTS(true, 64) FGW_KV_EXTERN_WEIGHTS(true, 128) FGW_KV_EXTERN_WEIGHTS(true, 256)
 FGW_KV_EXTERN_WEIGHTS(false, 64) FGW_KV_EXTERN_WEIGHTS(false, 128) FGW_KV_EXTERN_WEIGHTS(false, 256)
 
@@ -25,6 +26,7 @@ constexpr int kStatsItems = 512;
 constexpr int kFewItems = 512, kManyItems = 768;
 static_assert(std::max({kStatsItems, kFewItems, kManyItems}) <= fgw_mha::kMostSplits, "split_bound");
 
+// Bytes of kept scores, or of partial sums, that a call may always ask for; else as many as the pool has.
 constexpr int64_t kKeptBytes = 256 << 20;
 
 struct WeightPlan {
@@ -32,6 +34,7 @@ struct WeightPlan {
   Launch launch;   // of the first pass
   int part_rows;
   int columns, sums;  // grids of the persistent kernels; 0: no launch
+  int blocks, step;   // of kColumnKeys keys: of the table, of one launch of those kernels
   int64_t keys_pad, kept_rows, parts;
   int64_t kept, lse, notes, floats;  // of workspace
 };
@@ -69,7 +72,8 @@ WeightPlan plan_weights(const fgw_kv_weights_args& a) {
   const int64_t group = a.heads / a.kv_heads, total = a.tokens * group, capacity = (int64_t)a.width * a.page_size;
   const int64_t rows = std::min(a.last, a.tokens) * group, requests = std::min(a.batch, a.tokens);
   auto blocks = [&](int64_t size) { return std::min(requests * ((rows + size - 1) / size), total / size + requests); };
-  p.keys_pad = (capacity + kColumnKeys - 1) / kColumnKeys * kColumnKeys;
+  p.blocks = p.step = (int)((capacity + kColumnKeys - 1) / kColumnKeys);
+  p.keys_pad = (int64_t)p.blocks * kColumnKeys;
   // (Kept scores have a place for every key that the table could hold: no more of them than the pool has bytes.)
   const int64_t kept = (int64_t)a.batch * a.kv_heads * rows * p.keys_pad;
   const int64_t bound = std::max<int64_t>(kKeptBytes, a.pool_rows * a.kv_heads * a.dim * 2);
@@ -102,18 +106,22 @@ WeightPlan plan_weights(const fgw_kv_weights_args& a) {
     // Parts of the rows: smaller ones where the items would not fill the card (half of them: causal), down to
     // what a program of its own is worth. Parts of 1024 rows always / by this rule, us of a call: 512 tokens of
     // one K/V head of 8 rows 55.5 / 35.9, 4 requests of 300 tokens 53.4 / 35.8, 2000 tokens of 2 heads 77.4 / 74.3.
-    const int64_t keys = p.keys_pad / kColumnKeys;
     p.part_rows = kColumnRows;
     while (p.part_rows > kColumnRows / 4 && rows > p.part_rows / 2 &&
-           total / p.part_rows * keys * a.kv_heads < 4 * (int64_t)e.num_cus)
+           total / p.part_rows * p.blocks * a.kv_heads < 4 * (int64_t)e.num_cus)
       p.part_rows /= 2;
-    const int64_t parts = blocks(p.part_rows);
-    p.columns = persistent(parts * keys * a.kv_heads, e.num_cus, a.dim > 128 ? 1 : 2);
     if (rows > p.part_rows) {
-      p.parts = parts;
-      p.kept = parts * a.kv_heads * p.keys_pad;
-      p.sums = persistent(requests * ((p.keys_pad + kSumKeys - 1) / kSumKeys) * a.kv_heads, e.num_cus, 4);
+      // Places for the sums of every part (of requests with several) and key, by the table's capacity: where those
+      // are too many, the keys are taken a range at a time, with the same sums.
+      p.parts = std::min(requests * ((rows + p.part_rows - 1) / p.part_rows),
+                         total / p.part_rows + std::min(requests, total / p.part_rows));
+      const int64_t block = p.parts * a.kv_heads * kColumnKeys;
+      p.step = (int)std::max<int64_t>(1, std::min<int64_t>(p.blocks, bound / (4 * block)));
+      p.keys_pad = (int64_t)p.step * kColumnKeys;
+      p.kept = p.step * block;
+      p.sums = persistent(requests * p.step * a.kv_heads, e.num_cus, 4);
     }
+    p.columns = persistent(blocks(p.part_rows) * p.step * a.kv_heads, e.num_cus, a.dim > 128 ? 1 : 2);
   }
   p.floats = p.kept + (p.lse + 3) / 4 * 4 + p.notes;
   return p;
@@ -137,9 +145,15 @@ int check_weights(const fgw_kv_weights_args* args) {
 
 template <bool BF16>
 hipError_t launch(const WeightParams& w, const WeightPlan& p, hipStream_t stream) {
-  return w.dim <= 64    ? launch_weights<BF16, 64>(w, p.many, (int)p.launch.items, p.columns, stream)
-         : w.dim <= 128 ? launch_weights<BF16, 128>(w, p.many, (int)p.launch.items, p.columns, stream)
-                        : launch_weights<BF16, 256>(w, p.many, (int)p.launch.items, p.columns, stream);
+  return w.dim <= 64    ? launch_weights<BF16, 64>(w, p.many, (int)p.launch.items, stream)
+         : w.dim <= 128 ? launch_weights<BF16, 128>(w, p.many, (int)p.launch.items, stream)
+                        : launch_weights<BF16, 256>(w, p.many, (int)p.launch.items, stream);
+}
+template <bool BF16>
+hipError_t launch_columns(const WeightParams& w, const WeightPlan& p, hipStream_t stream) {
+  return w.dim <= 64    ? launch_weights_columns<BF16, 64>(w, p.columns, stream)
+         : w.dim <= 128 ? launch_weights_columns<BF16, 128>(w, p.columns, stream)
+                        : launch_weights_columns<BF16, 256>(w, p.columns, stream);
 }
 
 }  // namespace
@@ -193,8 +207,14 @@ int fgw_kv_weights(const fgw_kv_weights_args* args, hipStream_t stream) {
     else
       weights_finish_kernel<2><<<dim3((unsigned)p.launch.items), dim3(kFinishThreads), 0, stream>>>(w, w.lengths, w.cu);
   }
-  if (p.sums > 0)
-    weights_sum_kernel<<<dim3((unsigned)p.sums), dim3(kFinishThreads), 0, stream>>>(w, w.lengths, w.cu);
+  for (int from = 0; p.many && from < p.blocks; from += p.step) {
+    w.block_from = from;
+    w.block_to = std::min(from + p.step, p.blocks);
+    const hipError_t c = a.dtype == FGW_KV_BFLOAT16 ? launch_columns<true>(w, p, stream) : launch_columns<false>(w, p, stream);
+    if (c != hipSuccess) return fail(FGW_MHA_EHIP, "fgw_kv_weights: %s", hipGetErrorString(c));
+    if (p.sums > 0)
+      weights_sum_kernel<<<dim3((unsigned)p.sums), dim3(kFinishThreads), 0, stream>>>(w, w.lengths, w.cu);
+  }
   return launched("fgw_kv_weights");
 }
 
