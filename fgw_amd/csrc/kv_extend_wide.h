@@ -14,6 +14,28 @@
 
 namespace fgw_kv {
 
+// O^T += V^T (hi + lo)^T for one tile of 32 keys: operands of up to four row tiles of V^T, the next ones on the way.
+template <class C>
+__device__ __forceinline__ void pv_block_two(const unsigned char* vt, const Lanes<C>& ln, const u32x4 (&hi)[C::KS],
+                                             const u32x4 (&lo)[C::KS], f32x16 (&o)[C::DT]) {
+  using E = Elem<C::BF16>;
+  constexpr int G = C::DT < 4 ? C::DT : 4, PER = C::DT / G, NG = PER * C::KS;
+  u32x4 va[2][G];
+  auto read = [&](int g) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) va[g & 1][i] = read_vt<C>(vt, ln, g % PER * G + i, g / PER);
+  };
+  read(0);
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    if (g + 1 < NG) read(g + 1);
+#pragma unroll
+    for (int i = 0; i < G; ++i) o[g % PER * G + i] = E::mma(va[g & 1][i], hi[g / PER], o[g % PER * G + i]);
+#pragma unroll
+    for (int i = 0; i < G; ++i) o[g % PER * G + i] = E::mma(va[g & 1][i], lo[g / PER], o[g % PER * G + i]);
+  }
+}
+
 template <class C, class P>
 __global__ __launch_bounds__(C::THREADS) void extend_wide_kernel(P p, const int32_t* __restrict__ table,
                                                                  const int32_t* __restrict__ lengths,
@@ -70,8 +92,24 @@ __global__ __launch_bounds__(C::THREADS) void extend_wide_kernel(P p, const int3
     u32x4 pf[C::KS];
     qk_block<C>(stage, ln, qf, s);
     if (pos0 + C::BN > hi_min || pos0 < lo_max) mask_seen<C>(s, pos0, seen, hh);
-    online_softmax<C>(s, m, l, o, p.scale_log2, pf);
-    pv_block<C>(stage + C::TILE_BYTES, ln, pf, o);
+    if constexpr (kIsPrefix<P>) {
+      u32x4 pl[C::KS];
+      float sum = softmax_exp_two<C>(s[0], m, p.scale_log2, pf, pl);
+      if (__ballot(!(sum <= kSoftmaxSumBound))) {
+        const float top = fmaxf(m, row_max<C>(s, p.scale_log2));
+        const float keep = __builtin_amdgcn_exp2f(m - top);
+        l *= keep;
+#pragma unroll
+        for (int dt = 0; dt < C::DT; ++dt) o[dt] *= keep;
+        m = top;
+        sum = softmax_exp_two<C>(s[0], m, p.scale_log2, pf, pl);
+      }
+      l += sum;
+      pv_block_two<C>(stage + C::TILE_BYTES, ln, pf, pl, o);
+    } else {
+      online_softmax<C>(s, m, l, o, p.scale_log2, pf);
+      pv_block<C>(stage + C::TILE_BYTES, ln, pf, o);
+    }
   }
   // The second set's state to the first through LDS, lane to lane.
   __syncthreads();

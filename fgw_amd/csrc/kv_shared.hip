@@ -25,23 +25,23 @@
 
 namespace fgw_kv {
 
-#define FGW_KV_EXTERN(BF, P)                                                                       \
-  extern template hipError_t launch_extend_rows<BF, 32, P>(const P&, int, hipStream_t);            \
-  extern template hipError_t launch_extend_rows<BF, 64, P>(const P&, int, hipStream_t);            \
-  extern template hipError_t launch_extend_rows<BF, 128, P>(const P&, int, hipStream_t);           \
-  extern template hipError_t launch_extend_rows<BF, 256, P>(const P&, int, hipStream_t);           \
-  extern template hipError_t launch_extend_long<BF, 64, kRowsBlock, P>(const P&, int, hipStream_t);   \
-  extern template hipError_t launch_extend_long<BF, 64, kRowsGroup, P>(const P&, int, hipStream_t);   \
-  extern template hipError_t launch_extend_long<BF, 64, kRowsPadded, P>(const P&, int, hipStream_t);  \
-  extern template hipError_t launch_extend_long<BF, 128, kRowsBlock, P>(const P&, int, hipStream_t);  \
-  extern template hipError_t launch_extend_long<BF, 128, kRowsGroup, P>(const P&, int, hipStream_t);  \
-  extern template hipError_t launch_extend_long<BF, 128, kRowsPadded, P>(const P&, int, hipStream_t); \
+#define FGW_KV_EXTERN(BF, P)                                                             \
+  extern template hipError_t launch_extend_rows<BF, 32, P>(const P&, int, hipStream_t);  \
+  extern template hipError_t launch_extend_rows<BF, 64, P>(const P&, int, hipStream_t);  \
+  extern template hipError_t launch_extend_rows<BF, 128, P>(const P&, int, hipStream_t); \
+  extern template hipError_t launch_extend_rows<BF, 256, P>(const P&, int, hipStream_t); \
   extern template hipError_t launch_extend_wide<BF, 256, P>(const P&, int, hipStream_t);
 FGW_KV_EXTERN(true, PrefixParams) FGW_KV_EXTERN(true, SuffixParams)
 FGW_KV_EXTERN(false, PrefixParams) FGW_KV_EXTERN(false, SuffixParams)
 #define FGW_KV_EXTERN_WIDE(BF, DP) \
   extern template hipError_t launch_extend_wide<BF, DP, PrefixParams>(const PrefixParams&, int, hipStream_t);
 FGW_KV_EXTERN_WIDE(true, 64) FGW_KV_EXTERN_WIDE(true, 128) FGW_KV_EXTERN_WIDE(false, 64) FGW_KV_EXTERN_WIDE(false, 128)
+#define FGW_KV_EXTERN_LONG(BF, DP, R) \
+  extern template hipError_t launch_extend_long<BF, DP, R, SuffixParams>(const SuffixParams&, int, hipStream_t);
+#define FGW_KV_EXTERN_LONGS(BF)                                                                               \
+  FGW_KV_EXTERN_LONG(BF, 64, kRowsBlock) FGW_KV_EXTERN_LONG(BF, 64, kRowsGroup) FGW_KV_EXTERN_LONG(BF, 64, kRowsPadded) \
+  FGW_KV_EXTERN_LONG(BF, 128, kRowsBlock) FGW_KV_EXTERN_LONG(BF, 128, kRowsGroup) FGW_KV_EXTERN_LONG(BF, 128, kRowsPadded)
+FGW_KV_EXTERN_LONGS(true) FGW_KV_EXTERN_LONGS(false)
 
 namespace {
 
@@ -50,16 +50,14 @@ namespace {
 // rows, four prefixes of 4096 keys 35.2 / 32.8 / -, one of 8192 64 rows 26.8 / 28.0 / -; 128 rows, four of
 // 4096 60.8 / 48.1 / 58.1, 256 rows, one of 8192 - / 48.7 / 54.0, 2048 rows of 4096 keys - / 80.5 / 91.7, 4096 rows
 // - / 111.8 / 109.5.
-constexpr int kWideFrom = 64, kLongPrefixFrom = 2048;
+constexpr int kWideFrom = 64;
 constexpr int kPrefixMinChunk = 2;  // blocks of 64 keys; 1 / 2 / 4, us: 64 rows of 8192 keys 44.1 / 43.1 / 44.1
 constexpr int64_t kShareBytes = 160 << 20;
-
-enum Tiles { kShort, kWide, kLong };
 
 struct SharedPlan {
   Launch prefix;
   int prefix_rows;  // of a place
-  Tiles tiles;      // of the first pass
+  bool wide;        // the first pass's kernel
   int64_t notes;    // floats of the groups' notes
   Plan suffix;
   int share_from;   // SharedParams
@@ -92,14 +90,12 @@ SharedPlan plan_shared(const fgw_kv_shared_args& args) {
     s.share_from = (int)std::min<int64_t>(from >> 16, 1 << 28);
   }
   const int64_t rows = total / args.groups;  // of a group, on average
-  s.tiles = rows <= kWideFrom ? kShort : rows <= kLongPrefixFrom || a.dim > 128 ? kWide : kLong;
-  s.prefix.min_chunk = s.tiles == kShort ? kRowsMinChunk : kPrefixMinChunk;
-  if (s.tiles == kShort)
-    plan_prefix<ShortTiling>(s, a, args.groups);
-  else if (s.tiles == kWide)
+  s.wide = rows > kWideFrom;
+  s.prefix.min_chunk = s.wide ? kPrefixMinChunk : kRowsMinChunk;
+  if (s.wide)
     plan_prefix<WideTiling>(s, a, args.groups);
   else
-    plan_prefix<LongTiling>(s, a, args.groups);
+    plan_prefix<ShortTiling>(s, a, args.groups);
   s.notes = (int64_t)args.groups * (int64_t)sizeof(GroupNote) / 4;
   return s;
 }
@@ -141,11 +137,10 @@ int run_shared(const fgw_kv_shared_args& args, const SharedPlan& s, hipStream_t 
     own.prefix_slots = p.work;
     own.prefix_rows = s.prefix_rows;
     work = p.parts + s.prefix.floats;
-    const auto entry = s.tiles == kShort ? rows_entry<BF16, PrefixParams>(a.dim)
-                       : s.tiles == kLong ? long_entry<BF16, PrefixParams>(a.dim, a.page_size)
-                       : a.dim <= 64      ? &launch_extend_wide<BF16, 64, PrefixParams>
-                       : a.dim <= 128     ? &launch_extend_wide<BF16, 128, PrefixParams>
-                                          : &launch_extend_wide<BF16, 256, PrefixParams>;
+    const auto entry = !s.wide        ? rows_entry<BF16, PrefixParams>(a.dim)
+                       : a.dim <= 64  ? &launch_extend_wide<BF16, 64, PrefixParams>
+                       : a.dim <= 128 ? &launch_extend_wide<BF16, 128, PrefixParams>
+                                      : &launch_extend_wide<BF16, 256, PrefixParams>;
     const hipError_t e = entry(p, (int)s.prefix.items, stream);
     if (e != hipSuccess) return fail(FGW_MHA_EHIP, "fgw_kv_shared: %s", hipGetErrorString(e));
   }

@@ -1,14 +1,7 @@
-// Instantiations of kv_extend_long.h and kv_extend_wide.h for the first pass over shared prefixes, F16.
-#include "kv_extend_long.h"
+// Instantiations of kv_extend_wide.h for the first pass over shared prefixes, F16.
 #include "kv_extend_wide.h"
 
 namespace fgw_kv {
-template hipError_t launch_extend_long<false, 64, fgw_mha::kRowsBlock, PrefixParams>(const PrefixParams&, int, hipStream_t);
-template hipError_t launch_extend_long<false, 64, fgw_mha::kRowsGroup, PrefixParams>(const PrefixParams&, int, hipStream_t);
-template hipError_t launch_extend_long<false, 64, fgw_mha::kRowsPadded, PrefixParams>(const PrefixParams&, int, hipStream_t);
-template hipError_t launch_extend_long<false, 128, fgw_mha::kRowsBlock, PrefixParams>(const PrefixParams&, int, hipStream_t);
-template hipError_t launch_extend_long<false, 128, fgw_mha::kRowsGroup, PrefixParams>(const PrefixParams&, int, hipStream_t);
-template hipError_t launch_extend_long<false, 128, fgw_mha::kRowsPadded, PrefixParams>(const PrefixParams&, int, hipStream_t);
 template hipError_t launch_extend_wide<false, 64, PrefixParams>(const PrefixParams&, int, hipStream_t);
 template hipError_t launch_extend_wide<false, 128, PrefixParams>(const PrefixParams&, int, hipStream_t);
 template hipError_t launch_extend_wide<false, 256, PrefixParams>(const PrefixParams&, int, hipStream_t);
