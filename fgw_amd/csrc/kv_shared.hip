@@ -14,11 +14,13 @@
 // Where sharing pays. The passes cost a second launch, and partials of every row and split written and read; what
 // they save is reading: requests of few rows read their keys once for every 32 of them. Requests of more
 // than kShareRows rows are bound by products, of which there are as many either way. Shared / each on its own,
-// us (requests x tokens, Hq 32, Hkv 8, D 128, reads saved): 16x1 prefix 1000 (66 MB) 22.6 / 18.0, 8x1 4000
-// (131 MB) 23.0 / 23.0, 16x1 4000 (262 MB) 23.3 / 34.8, 32x1 8000 (1 GB) 31.9 / 105; 32x32 1000 (0.5 GB) 78 /
-// 56, 4096 (2.1 GB) 118 / 160; 8x64 16000 190 / 148, 8x512 4096 342 / 294. Hence 160 MB, and as much for the
-// partials as 96 bytes for every dim of every row. The device knows the lengths and decides; where the table's
-// capacity rules it out, or tokens and requests do on average, the host leaves the first pass away.
+// us (requests x tokens, Hq 32, Hkv 8, D 128, reads saved): 8x1 prefix 3000 (98 MB) 23.4 / 19.7, 4096 (134 MB)
+// 24.1 / 24.5, 16x1 2000 (131 MB) 24.7 / 24.6, 4096 (268 MB) 24.0 / 37.0, 32x1 8000 (1 GB) 35.1 / 106; 32x4 2000
+// (262 MB) 37.2 / 35.2, 3000 (393 MB) 37.9 / 45.9; 32x8 3000 (393 MB) 49.6 / 46.8, 4096 (537 MB) 55.4 / 60.4; 64x8
+// 4096 (1.1 GB) 79.5 / 77.4; 32x32 2000 (1 GB) 100.6 / 90.1, 3000 (1.6 GB) 119.1 / 120.1, 8192 (4.3 GB) 238 / 296;
+// 8x64 16000 231 / 136, 8x512 4096 481 / 269. Hence 100 MB, and as much for the partials as 340 bytes for every dim
+// of every row. The device knows the lengths and decides; where the table's capacity rules it out, or tokens and
+// requests do on average, the host leaves the first pass away.
 #include <hip/hip_runtime.h>
 
 #include "kv_extend_plan.h"
@@ -46,13 +48,14 @@ FGW_KV_EXTERN_LONGS(true) FGW_KV_EXTERN_LONGS(false)
 namespace {
 
 // The kernel of the first pass by the rows of a group: a short tile reads the keys for 32 of them, a wide one
-// for 128, a long one for 256, whose partials are the most. Short / wide / long, us (Hq 32, Hkv 8, D 128): 48
-// rows, four prefixes of 4096 keys 35.2 / 32.8 / -, one of 8192 64 rows 26.8 / 28.0 / -; 128 rows, four of
-// 4096 60.8 / 48.1 / 58.1, 256 rows, one of 8192 - / 48.7 / 54.0, 2048 rows of 4096 keys - / 80.5 / 91.7, 4096 rows
-// - / 111.8 / 109.5.
+// for 128. Both hold the weights of the PV product in two numbers of the input type, as few rows have them
+// alone, so that what a token gets does not hang on who shares its prefix. Short / wide, us (Hq 32, Hkv 8, D
+// 128): 48 rows, four prefixes of 4096 keys 36.0 / 36.6, one of 8192 64 rows 27.4 / 30.0; 80 rows, four of 4096
+// 56.2 / 47.6, 128 rows 59.8 / 51.0. Wide with one number, two: 256 rows, one of 8192 36.0 / 38.6, 2048 of 4096
+// 77 / 89, 4096 111 / 143. (Tiles of 256 rows with one number took 109.5 for the last.)
 constexpr int kWideFrom = 64;
-constexpr int kPrefixMinChunk = 2;  // blocks of 64 keys; 1 / 2 / 4, us: 64 rows of 8192 keys 44.1 / 43.1 / 44.1
-constexpr int64_t kShareBytes = 160 << 20;
+constexpr int kPrefixMinChunk = 2;  // blocks of 64 keys; 1 / 2 / 4, us: four prefixes of 1000 keys, 128 rows each 46.1 / 46.1 / 48.1
+constexpr int64_t kShareBytes = 100 << 20, kShareDimBytes = 340;
 
 struct SharedPlan {
   Launch prefix;
@@ -83,7 +86,7 @@ SharedPlan plan_shared(const fgw_kv_shared_args& args) {
   a.num_cus = std::min(a.num_cus, kMostCus);
   const int64_t total = (int64_t)a.tokens * (a.heads / a.kv_heads);
   if (!args.always) {
-    const int64_t from = kShareBytes + 96 * (int64_t)a.dim * a.heads * a.tokens;
+    const int64_t from = kShareBytes + kShareDimBytes * a.dim * a.heads * a.tokens;
     const int64_t requests = std::min(a.batch, a.tokens), key_bytes = 4 * (int64_t)a.kv_heads * shared_dims(a.dim);
     const double most = (double)(total / 32 + requests) * ((double)a.width * a.page_size) * (double)key_bytes;
     if (most < (double)from || total > (int64_t)kShareRows * requests) return s;
