@@ -56,7 +56,7 @@ struct SharedParams : ExtendParams {
   const float* prefix_parts;
   const float* prefix_lse;
   int32_t* group_notes;     // [n_groups] GroupNote
-  int32_t share_from;       // units of 64 KB that sharing has to save (Requests::pays); 0: it always pays
+  int32_t share_from;       // units of 64 KB that sharing has to gain (Requests::pays); 0: it always pays
 };
 struct PrefixParams : SharedParams {};
 struct SuffixParams : SharedParams {};
@@ -73,6 +73,8 @@ struct GroupNote {
   int32_t base, splits, tiles, first;
 };
 constexpr int kShareRows = 128;  // of a request, on average over its group, up to which sharing may pay
+// What the first pass costs for a row that shares, as bytes of reading for each of its dims (kv_shared.hip).
+constexpr int kShareDimBytes = 340;
 
 // Tiles of ROWS rows, keys in blocks of BN, splits in units of UNIT blocks.
 template <int ROWS_, int BN_, int UNIT_>
@@ -162,14 +164,16 @@ __device__ __forceinline__ Group load_group(const SharedParams& p, const int32_t
   if (p.share_from > 0 && (int64_t)(x.next - x.first) * p.group > (int64_t)kShareRows * (x.f1 - x.f0)) x.keys = 0;
   return x;
 }
-// What the requests of a group would read of the prefix each on its own, in units of 64 KB: once for every
-// 32 rows, in tiles of 128 or 256 dims (a tile of 64 takes the kernel about as long as one of 128).
+// What the requests of a group would read of the prefix each on its own, less what the first pass takes for their
+// rows, in units of 64 KB: once for every 32 rows, in tiles of 128 or 256 dims (a tile of 64 takes the kernel
+// about as long as one of 128). (Rounded to integers before they are compared: the same in every kernel.)
 __host__ __device__ __forceinline__ int shared_dims(int dim) { return dim <= 128 ? 128 : 256; }
-__device__ __forceinline__ int group_saves(const SharedParams& p, const Group& x) {
+__device__ __forceinline__ int group_gain(const SharedParams& p, const Group& x) {
   if (x.keys <= 0) return 0;
+  const int64_t cost = (int64_t)(x.next - x.first) * p.q_heads * p.dim * kShareDimBytes >> 16;
   const float members = (float)(x.f1 - x.f0), rows = (float)(x.next - x.first) * (float)p.group / members;
   const float bytes = members * ceilf(rows * 0.03125f) * (float)x.keys * (float)p.heads * (float)shared_dims(p.dim) * 4.0f;
-  return (int)fminf(bytes * (1.0f / 65536.0f), 16777216.0f);
+  return (int)fminf(bytes * (1.0f / 65536.0f), 16777216.0f) - (int)(cost < 16777216 ? cost : 16777216);
 }
 
 template <class T>
@@ -240,9 +244,9 @@ struct Requests {
   // program of both.
   __device__ __forceinline__ bool pays() const {
     if (p.share_from <= 0) return true;
-    int total = wave_sum(group_saves(p, mine), lane);
+    int total = wave_sum(group_gain(p, mine), lane);
     for (int g = 64; g < p.n_groups && total < p.share_from; g += 64)
-      total += wave_sum(group_saves(p, load_group(p, lengths, cu, g + lane)), lane);
+      total += wave_sum(group_gain(p, load_group(p, lengths, cu, g + lane)), lane);
     return total >= p.share_from;
   }
   __device__ __forceinline__ Requests(const P& p_, const int32_t* lengths_, const int32_t* cu_, int lane_)

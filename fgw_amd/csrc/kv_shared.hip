@@ -19,8 +19,9 @@
 // (262 MB) 37.2 / 35.2, 3000 (393 MB) 37.9 / 45.9; 32x8 3000 (393 MB) 49.6 / 46.8, 4096 (537 MB) 55.4 / 60.4; 64x8
 // 4096 (1.1 GB) 79.5 / 77.4; 32x32 2000 (1 GB) 100.6 / 90.1, 3000 (1.6 GB) 119.1 / 120.1, 8192 (4.3 GB) 238 / 296;
 // 8x64 16000 231 / 136, 8x512 4096 481 / 269. Hence 100 MB, and as much for the partials as 340 bytes for every dim
-// of every row. The device knows the lengths and decides; where the table's capacity rules it out, or tokens and
-// requests do on average, the host leaves the first pass away.
+// of every row that shares. The device knows lengths and groups and decides; where the table's capacity rules it
+// out, or tokens and requests do on average, the host leaves the first pass away (which costs 5 us where it is empty;
+// how many of the call's rows share is not known there, and it counts 96 bytes for each).
 #include <hip/hip_runtime.h>
 
 #include "kv_extend_plan.h"
@@ -55,7 +56,7 @@ namespace {
 // 77 / 89, 4096 111 / 143. (Tiles of 256 rows with one number took 109.5 for the last.)
 constexpr int kWideFrom = 64;
 constexpr int kPrefixMinChunk = 2;  // blocks of 64 keys; 1 / 2 / 4, us: four prefixes of 1000 keys, 128 rows each 46.1 / 46.1 / 48.1
-constexpr int64_t kShareBytes = 100 << 20, kShareDimBytes = 340;
+constexpr int64_t kShareBytes = 100 << 20, kHostDimBytes = 96;
 
 struct SharedPlan {
   Launch prefix;
@@ -86,11 +87,11 @@ SharedPlan plan_shared(const fgw_kv_shared_args& args) {
   a.num_cus = std::min(a.num_cus, kMostCus);
   const int64_t total = (int64_t)a.tokens * (a.heads / a.kv_heads);
   if (!args.always) {
-    const int64_t from = kShareBytes + kShareDimBytes * a.dim * a.heads * a.tokens;
+    const int64_t from = kShareBytes + kHostDimBytes * a.dim * a.heads * a.tokens;
     const int64_t requests = std::min(a.batch, a.tokens), key_bytes = 4 * (int64_t)a.kv_heads * shared_dims(a.dim);
     const double most = (double)(total / 32 + requests) * ((double)a.width * a.page_size) * (double)key_bytes;
     if (most < (double)from || total > (int64_t)kShareRows * requests) return s;
-    s.share_from = (int)std::min<int64_t>(from >> 16, 1 << 28);
+    s.share_from = (int)(kShareBytes >> 16);
   }
   const int64_t rows = total / args.groups;  // of a group, on average
   s.wide = rows > kWideFrom;
