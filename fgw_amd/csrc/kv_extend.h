@@ -425,8 +425,9 @@ __device__ __forceinline__ int64_t out_row(const ExtendParams& p, const Item& it
 }
 
 // Partials that this launch joins itself go through buffer loads and stores at device scope (sc1,
-// 16 bytes to a lane): they pass by the L2s of the XCDs, which are not coherent with each other. A
-// launch's partials are below 2^31 bytes (kMostCus in kv_extend.hip: 9 MB).
+// 16 bytes to a lane): they pass by the L2s of the XCDs, which are not coherent with each other. Such a
+// launch's partials are below 2^31 bytes (kMostCus in kv_extend_plan.h: 9 MB); those of a first pass over
+// shared prefixes, which may be more, are joined by the next launch.
 constexpr int kDeviceScope = 17;  // sc0 | sc1
 __device__ __forceinline__ f32x4 device_load4(const float* base, u32 bytes) {
   const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), (short)0, 0x7fffffff, 0x00027000);

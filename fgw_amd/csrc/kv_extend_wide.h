@@ -9,6 +9,10 @@
 // SIMD at 256 registers). Hq 32, Hkv 8, 4096 tokens causal: D 256 424 us (649 TFLOP/s), D 192 433;
 // 512 tokens behind 7680 cached ones, D 256, 210. The kernel of few rows takes 787, 841 and 327 for
 // them.
+//
+// It is also the first pass over shared prefixes for groups of many rows (kv_shared.hip), at all head dims, and there
+// holds P in two numbers, as the kernel of few rows does. 256 rows of a K/V head, 8192 keys, D 128: 27 us with
+// two, 24 with one; two launches for 64 samples 38.6 and 36.0.
 #pragma once
 #include "kv_extend_long.h"
 

@@ -27,11 +27,14 @@ def add_weights(scores, q, k_cache, block_table, cache_seqlens, cu_seqlens, page
       scores[b, h, j] = (decay * scores[b, h, j] if j < len - n else 0) + sum of softmax(scale q k^T)_j
 
     over the query heads of h and the last `last` of the new tokens (all, where they are fewer): 1 in a
-    decode step, the prompt's length for all of a prompt, some tens for what its end looks back at. The
+    decode step, the prompt's length for all of a prompt, some tens for what its end looks back at. (No more
+    than the longest request of the call has: the sizes of T and last say which kernels run, and a decode step
+    with a last of some tens takes those of many rows, 2 to 2.5 times as long.) The
     keys of new tokens thus begin at zero without being cleared; decay 0 forgets all that was there.
     Requests without new tokens, and entries from len on, are left. Lengths and page ids out of range are
-    taken as there; rows that see no key add nothing; a NaN in a query or in a key that it sees gives NaN
-    to all keys that it sees. Sums are fp32, in the same order on every run. Nothing is read back: the call
+    taken as there; rows that see no key add nothing; a NaN in a query or in a key that it sees, or a score of plus
+    infinity, gives NaN to all keys that it sees, and a key with a score of minus infinity gets nothing (a row with no
+    other scores adds nothing). Sums are fp32, in the same order on every run. Nothing is read back: the call
     can be captured into a HIP graph. Records no gradient, and scores may require none.
     """
     if last < 1:

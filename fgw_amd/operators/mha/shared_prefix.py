@@ -12,7 +12,8 @@ A group's prefix is read through the table row of its first request, once for al
 rows hold the same keys, in the same pages (as a fork leaves the whole pages) or in copies of them. It
 counts as far as the first request has it before its own new tokens. A request whose new tokens begin
 within the prefix, or that is alone in its group, reads its own keys instead: the result is that of
-paged_extend for any lengths. Inference only, as there.
+paged_extend for any lengths, up to the order of fp32 sums. The prefix's softmax weights are held in two numbers of
+the input type, as those of few new tokens are there. Inference only, as there.
 """
 from __future__ import annotations
 

@@ -146,7 +146,8 @@ int fgw_kv_shared(const fgw_kv_shared_args* args, hipStream_t stream);
  *   scores[b, h, j] = (j < len_b - n_b ? decay * scores[b, h, j] : 0) + sum of softmax(scale q k^T)_j
  * over the query heads of h and the last min(n_b, last) new tokens of b, each of which sees the keys up to
  * its own position. Requests without new tokens, and entries at and behind len_b, are left as they are.
- * decay 0 forgets what was there, whatever it is. Sums are taken in the same order on every run. */
+ * decay 0 forgets what was there, whatever it is. Sums are taken in the same order on every run. A row with a
+ * NaN or plus infinity among its scores is NaN at every key that it sees. */
 typedef struct {
   fgw_kv_rows q;
   float* scores;         /* [batch, kv_heads, scores_stride] */
@@ -164,7 +165,8 @@ typedef struct {
   float scale, decay;
 } fgw_kv_weights_args;
 
-/* fp32 elements of workspace (pointers are not read), or a negative status. */
+/* fp32 elements of workspace (pointers are not read), or a negative status. Kept scores or partial sums take no
+ * more bytes than the pool has, or 256 MB; beside them a few for each row and split. */
 int64_t fgw_kv_weights_workspace(const fgw_kv_weights_args* args);
 int fgw_kv_weights(const fgw_kv_weights_args* args, hipStream_t stream);
 
